@@ -89,6 +89,17 @@ class CardGridWeights(ctypes.Structure):
     ]
 
 
+class AdamWTensor(ctypes.Structure):
+    _fields_ = [
+        ("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("numel", ctypes.c_int64), ("state", ctypes.c_int64),
+        ("group", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class AdamWGroup(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_double) for name in ("lr", "beta1", "beta2", "eps", "weight_decay")]
+
+
 _SIGNATURES: dict[str, tuple[type, list]] = {
     "cg_last_error": (ctypes.c_char_p, []),
     "cg_version": (_i32, []),
@@ -138,6 +149,9 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
     "cg_value_loss": (_i32, [_p, _p, _p, _p, _i64, _i32, _f32, _p, _p, _p, _i64, _p]),
     "cg_seat_values": (_i32, [_p, _i64, _i32, _p, _p, _p, _p, _i64, _i32, _p, _p, _p]),
     "cg_center_zero_sum": (_i32, [_p, _p, _i64, _i32, _p, _p]),
+    "cg_adamw_control_bytes": (_i64, []),
+    "cg_adamw_workspace_bytes": (_i64, [_i32]),
+    "cg_adamw_step": (_i32, [_p, _i32, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p, _f32, _p, _p, _p, _i64, _p]),
 }
 
 

@@ -1,0 +1,474 @@
+// One AdamW step over many tensors: the gradients' global norm, then every parameter and its moments.
+//
+//   g' = g min(1, max_norm / (|g| + 1e-6)),  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2
+//   p  = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// What bounds it is HBM: an fp32 weight moves 28 bytes with 32-bit moments and 16 with 8-bit ones, and the
+// norm reads the gradient once more. So the step is two launches whatever the number of tensors: the table of
+// tensors travels in the kernel's parameters (nothing is uploaded), a block takes one chunk of one tensor,
+// and the norm kernel's last block turns the norm and the step count into the factors of every group on
+// the device, so the host reads nothing back.
+//
+// 8-bit moments: m and sqrt(v) as e4m3, scaled by the largest magnitude of each block of 256 entries of a
+// tensor (fp32). The root halves the exponent range that v needs; a root that is not zero keeps at least the
+// smallest code, so that no entry with history divides by eps alone. A block's scale is exact, so the block
+// follows its largest entry through changes smaller than a code's step. The update itself uses the new fp32
+// moments, before they are rounded. A block is one warp's eight entries a lane, so its maximum is one
+// warp reduction.
+#include <cuda_fp8.h>
+
+#include <algorithm>
+
+#include "common.cuh"
+
+namespace cg {
+namespace {
+
+constexpr int kBlockEntries = 256;  // entries of one scale; every tensor's state starts on a multiple
+constexpr int kPerLane = 8;
+constexpr int kThreads = 256;
+constexpr int kChunk = 8192;  // entries of a thread block: four 256-entry blocks a warp
+constexpr int kMaxGroups = 16;
+constexpr int kNormBlocks = 1184;  // partial sums of the norm: one fixed order of addition
+constexpr float kE4m3Max = 448.f;
+constexpr float kE4m3Least = 0.001953125f;  // 2^-9
+constexpr float kLeastPeak = 3.0e-36f;      // below it 448 / peak is not finite: the block is held as zero
+
+struct Factors {
+  float decay, step, root, eps, beta1, rest1, beta2, rest2;
+};
+
+// Zeroed before the first step; what the norm kernel leaves for the update.
+struct Control {
+  unsigned ticket;
+  int skip;
+  float clip;
+  int reserved;
+  Factors groups[kMaxGroups];
+};
+
+struct Groups {
+  int count;
+  cg_adamw_group g[kMaxGroups];
+};
+
+struct Entry {
+  void* param;
+  const void* grad;
+  int64_t numel;
+  int64_t state;
+  int32_t first_chunk;  // this tensor's first chunk in the launch
+  int32_t group;
+};
+
+template <int kMax>
+struct Table {
+  int count, chunks;
+  Entry e[kMax];
+};
+
+struct States {
+  void* exp_avg;
+  float* exp_avg_scale;
+  void* exp_avg_sq;
+  float* exp_avg_sq_scale;
+  float* master;
+};
+
+template <int kMax>
+__device__ __forceinline__ int find_tensor(const Table<kMax>& table, int chunk) {
+  int lo = 0, hi = table.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (table.e[mid].first_chunk <= chunk)
+      lo = mid;
+    else
+      hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
+__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "f"(v[0]), "f"(v[1]), "f"(v[2]),
+               "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+
+__device__ __forceinline__ void load8(const __half* p, float (&v)[8]) {
+  const uint4 raw = *reinterpret_cast<const uint4*>(p);
+  const __half2* h = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+
+__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
+  uint4 raw;
+  __nv_bfloat162* h = reinterpret_cast<__nv_bfloat162*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = raw;
+}
+
+__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
+  uint4 raw;
+  __half2* h = reinterpret_cast<__half2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) h[i] = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+  *reinterpret_cast<uint4*>(p) = raw;
+}
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ void from_float(float* p, float v) { *p = v; }
+__device__ __forceinline__ void from_float(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// Eight entries of a tensor from `at`; those at or past `numel` read as zero. `whole`: all eight are inside
+// and the address is aligned to eight entries.
+template <typename T>
+__device__ __forceinline__ void load_entries(const T* base, int64_t at, int64_t numel, bool whole, float (&v)[8]) {
+  if (whole) {
+    load8(base + at, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) v[i] = at + i < numel ? to_float(base[at + i]) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ void store_entries(T* base, int64_t at, int64_t numel, bool whole, const float (&v)[8]) {
+  if (whole) {
+    store8(base + at, v);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i)
+    if (at + i < numel) from_float(base + at + i, v[i]);
+}
+
+template <typename T>
+__device__ __forceinline__ bool aligned8(const T* p) {
+  return (reinterpret_cast<uintptr_t>(p) & (sizeof(T) * kPerLane - 1)) == 0;
+}
+
+// ---- 8-bit moments --------------------------------------------------------------------------------
+__device__ __forceinline__ void decode8(const uint8_t* codes, float unit, float (&v)[8]) {
+  const uint2 raw = *reinterpret_cast<const uint2*>(codes);
+  const __nv_fp8x2_storage_t* pairs = reinterpret_cast<const __nv_fp8x2_storage_t*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(pairs[i], __NV_E4M3)));
+    v[2 * i] = f.x * unit, v[2 * i + 1] = f.y * unit;
+  }
+}
+
+__device__ __forceinline__ void encode8(uint8_t* codes, const float (&v)[8]) {
+  uint2 raw;
+  __nv_fp8x2_storage_t* pairs = reinterpret_cast<__nv_fp8x2_storage_t*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    pairs[i] = __nv_cvt_float2_to_fp8x2(make_float2(v[2 * i], v[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
+  *reinterpret_cast<uint2*>(codes) = raw;
+}
+
+// Largest of the warp's non-negative values; a NaN's bits compare above infinity's, so it is kept.
+__device__ __forceinline__ float warp_peak(float v) {
+  return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
+}
+
+// ---- the global norm and the step's factors ----------------------------------------------------------
+// One thread per group, in double: 1 - b2^t loses half its digits in fp32.
+__device__ void make_factors(const Groups& groups, int64_t* steps, bool finite, float clip, Control* control) {
+  const int64_t t = *steps + 1;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    control->clip = clip;
+    control->skip = finite ? 0 : 1;
+    if (finite) *steps = t;
+  }
+  for (int k = threadIdx.x; k < groups.count; k += blockDim.x) {
+    const cg_adamw_group g = groups.g[k];
+    Factors f;
+    f.decay = static_cast<float>(1.0 - g.lr * g.weight_decay);
+    f.step = static_cast<float>(g.lr / (1.0 - pow(g.beta1, static_cast<double>(t))));
+    f.root = static_cast<float>(1.0 / sqrt(1.0 - pow(g.beta2, static_cast<double>(t))));
+    f.eps = static_cast<float>(g.eps);
+    f.beta1 = static_cast<float>(g.beta1);
+    f.rest1 = static_cast<float>(1.0 - g.beta1);
+    f.beta2 = static_cast<float>(g.beta2);
+    f.rest2 = static_cast<float>(1.0 - g.beta2);
+    control->groups[k] = f;
+  }
+}
+
+__global__ void __launch_bounds__(32) adamw_factors_kernel(const __grid_constant__ Groups groups, int64_t* steps,
+                                                           Control* control) {
+  pdl_trigger();
+  make_factors(groups, steps, true, 1.f, control);
+}
+
+// Squares are summed in fp32 over a thread's eight entries and in double from there on.
+template <typename T, int kMax>
+__global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_constant__ Table<kMax> table,
+                                                              const __grid_constant__ Groups groups, float max_norm,
+                                                              int first_partial, int partials, double* partial,
+                                                              int64_t* steps, float* norm_out, Control* control) {
+  __shared__ double s[kThreads / 32];
+  __shared__ bool last;
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  double total = 0;
+  for (int chunk = blockIdx.x; chunk < table.chunks; chunk += gridDim.x) {
+    const Entry& e = table.e[find_tensor(table, chunk)];
+    const T* grad = static_cast<const T*>(e.grad);
+    const bool aligned = aligned8(grad);
+    const int64_t start = static_cast<int64_t>(chunk - e.first_chunk) * kChunk;
+#pragma unroll
+    for (int b = 0; b < kChunk / (kThreads * kPerLane); ++b) {
+      const int64_t at = start + (b * kThreads + threadIdx.x) * kPerLane;
+      float g[8];
+      load_entries(grad, at, e.numel, aligned && at + kPerLane <= e.numel, g);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) sum = fmaf(g[i], g[i], sum);
+      total += sum;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s[warp] = total;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) total += s[w];
+    partial[first_partial + blockIdx.x] = total;
+    __threadfence();
+    last = atomicInc(&control->ticket, partials - 1) == static_cast<unsigned>(partials - 1);
+  }
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  total = 0;
+  for (int i = threadIdx.x; i < partials; i += kThreads) total += __ldcg(partial + i);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  if (lane == 0) s[warp] = total;
+  __syncthreads();
+  total = 0;
+  for (int w = 0; w < kThreads / 32; ++w) total += s[w];
+  const double norm = sqrt(total);
+  if (threadIdx.x == 0) *norm_out = static_cast<float>(norm);
+  make_factors(groups, steps, isfinite(norm), static_cast<float>(fmin(1.0, max_norm / (norm + 1e-6))), control);
+}
+
+// ---- the update -----------------------------------------------------------------------------------------
+template <typename T, int kBits, int kMax>
+__global__ void __launch_bounds__(kThreads) adamw_update_kernel(const __grid_constant__ Table<kMax> table,
+                                                                const States states,
+                                                                const Control* control) {
+  constexpr bool kMaster = sizeof(T) < 4;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const Entry& e = table.e[find_tensor(table, blockIdx.x)];
+  T* param = static_cast<T*>(e.param);
+  const T* grad = static_cast<const T*>(e.grad);
+  const bool aligned = aligned8(param) && aligned8(grad);
+  const int64_t start = static_cast<int64_t>(blockIdx.x - e.first_chunk) * kChunk;
+  pdl_wait();
+  if (control->skip) return;  // a norm that is not finite: nothing moves
+  const float clip = control->clip;
+  const Factors f = control->groups[e.group];
+  for (int64_t block = start + warp * kBlockEntries; block < start + kChunk && block < e.numel; block += kThreads * kPerLane) {
+    const int64_t at = block + lane * kPerLane;
+    const int64_t held = e.state + at;  // the state's arrays are padded: eight entries are always inside
+    const bool whole = aligned && at + kPerLane <= e.numel;
+    float p[8], g[8], m[8], v[8];
+    load_entries(grad, at, e.numel, whole, g);
+    if (kMaster)
+      load8(states.master + held, p);
+    else
+      load_entries(param, at, e.numel, whole, p);
+    float unit_m = 0.f, unit_r = 0.f;
+    if (kBits == 8) {
+      unit_m = states.exp_avg_scale[held / kBlockEntries] * (1.f / kE4m3Max);
+      unit_r = states.exp_avg_sq_scale[held / kBlockEntries] * (1.f / kE4m3Max);
+      decode8(static_cast<uint8_t*>(states.exp_avg) + held, unit_m, m);
+      decode8(static_cast<uint8_t*>(states.exp_avg_sq) + held, unit_r, v);
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) v[i] *= v[i];
+    } else {
+      load8(static_cast<float*>(states.exp_avg) + held, m);
+      load8(static_cast<float*>(states.exp_avg_sq) + held, v);
+    }
+    float peak_m = 0.f, peak_r = 0.f;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      const float gi = g[i] * clip;
+      m[i] = f.beta1 * m[i] + f.rest1 * gi;
+      v[i] = f.beta2 * v[i] + f.rest2 * (gi * gi);
+      const float root = sqrtf(v[i]);
+      p[i] = p[i] * f.decay - f.step * (m[i] / (root * f.root + f.eps));
+      if (kBits == 8) {
+        v[i] = root;
+        // Bits, not fmaxf, which would drop a NaN.
+        peak_m = __uint_as_float(max(__float_as_uint(peak_m), __float_as_uint(fabsf(m[i]))));
+        peak_r = __uint_as_float(max(__float_as_uint(peak_r), __float_as_uint(root)));
+      }
+    }
+    if (kMaster) store8(states.master + held, p);
+    store_entries(param, at, e.numel, whole, p);
+    if (kBits == 8) {
+      peak_m = warp_peak(peak_m);
+      peak_r = warp_peak(peak_r);
+      const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max / peak_m;
+      const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max / peak_r;
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) {
+        m[i] *= to_m;
+        v[i] = v[i] > 0.f ? fmaxf(v[i] * to_r, kE4m3Least) : v[i] * to_r;
+      }
+      encode8(static_cast<uint8_t*>(states.exp_avg) + held, m);
+      encode8(static_cast<uint8_t*>(states.exp_avg_sq) + held, v);
+      if (lane == 0) {
+        states.exp_avg_scale[held / kBlockEntries] = peak_m;
+        states.exp_avg_sq_scale[held / kBlockEntries] = peak_r;
+      }
+    } else {
+      store8(static_cast<float*>(states.exp_avg) + held, m);
+      store8(static_cast<float*>(states.exp_avg_sq) + held, v);
+    }
+  }
+}
+
+constexpr int kFewTensors = 64, kManyTensors = 640;  // 2.6 and 25 KB of kernel parameters (32 KB is the limit)
+
+// The tensors from `next` on that fit one launch; those without a gradient or without entries are left out.
+template <int kMax>
+void fill_table(const cg_adamw_tensor* tensors, int count, int& next, Table<kMax>& table) {
+  table.count = table.chunks = 0;
+  while (next < count && table.count < kMax) {
+    const cg_adamw_tensor& t = tensors[next];
+    if (t.grad && t.numel > 0) {
+      const int64_t chunks = (t.numel + kChunk - 1) / kChunk;
+      if (table.count && table.chunks + chunks > INT32_MAX) break;
+      table.e[table.count++] = {t.param, t.grad, t.numel, t.state, table.chunks, t.group};
+      table.chunks += static_cast<int>(chunks);
+    }
+    ++next;
+  }
+}
+
+template <typename T, int kMax>
+int run_step(const cg_adamw_tensor* tensors, int count, const Groups& groups, int bits, const States& states,
+             int64_t* steps, float max_norm, float* norm_out, Control* control, double* partial, cudaStream_t s) {
+  Table<kMax> table;
+  if (max_norm > 0) {
+    int partials = 0;
+    for (int next = 0; next < count;) {
+      fill_table(tensors, count, next, table);
+      partials += std::min(table.chunks, kNormBlocks);
+    }
+    int first = 0;
+    for (int next = 0; next < count;) {
+      fill_table(tensors, count, next, table);
+      if (!table.chunks) continue;
+      const int blocks = std::min(table.chunks, kNormBlocks);
+      adamw_norm_kernel<T, kMax><<<blocks, kThreads, 0, s>>>(table, groups, max_norm, first, partials, partial, steps,
+                                                             norm_out, control);
+      if (int rc = check_launch("adamw_norm_kernel")) return rc;
+      first += blocks;
+    }
+  } else {
+    adamw_factors_kernel<<<1, 32, 0, s>>>(groups, steps, control);
+    if (int rc = check_launch("adamw_factors_kernel")) return rc;
+  }
+  for (int next = 0; next < count;) {
+    fill_table(tensors, count, next, table);
+    if (!table.chunks) continue;
+    auto kernel = bits == 8 ? adamw_update_kernel<T, 8, kMax> : adamw_update_kernel<T, 32, kMax>;
+    if (int rc = launch_pdl("adamw_update_kernel", kernel, dim3(table.chunks), dim3(kThreads), 0, s, table, states,
+                            static_cast<const Control*>(control)))
+      return rc;
+  }
+  return CG_OK;
+}
+
+}  // namespace
+}  // namespace cg
+
+extern "C" int64_t cg_adamw_control_bytes(void) { return sizeof(cg::Control); }
+
+extern "C" int64_t cg_adamw_workspace_bytes(int count) {
+  if (count < 0) {
+    cg::set_error(CG_ERR_ARGUMENT, "cg_adamw_workspace_bytes: negative count");
+    return -1;
+  }
+  return (static_cast<int64_t>(count) / cg::kFewTensors + 1) * cg::kNormBlocks * static_cast<int64_t>(sizeof(double));
+}
+
+extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtype, const cg_adamw_group* groups,
+                             int group_count, int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq,
+                             float* exp_avg_sq_scale, float* master, int64_t* steps, float max_norm, float* norm_out,
+                             void* control, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace cg;
+  CG_REQUIRE(count >= 0 && (count == 0 || tensors), "cg_adamw_step: bad tensor table");
+  CG_REQUIRE(valid_dtype(dtype), "cg_adamw_step: dtype must be float32, float16 or bfloat16");
+  CG_REQUIRE(state_bits == 8 || state_bits == 32, "cg_adamw_step: state_bits must be 8 or 32");
+  CG_REQUIRE(groups && group_count > 0 && group_count <= kMaxGroups, "cg_adamw_step: 1..%d groups", kMaxGroups);
+  CG_REQUIRE(exp_avg && exp_avg_sq && steps && control, "cg_adamw_step: NULL state");
+  CG_REQUIRE(state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale), "cg_adamw_step: 8-bit states need scales");
+  CG_REQUIRE(dtype == CG_F32 || master, "cg_adamw_step: 16-bit parameters need fp32 master copies");
+  CG_REQUIRE(!(max_norm > 0) || norm_out, "cg_adamw_step: max_norm needs norm_out");
+  if (max_norm > 0 && (!workspace || workspace_bytes < cg_adamw_workspace_bytes(count)))
+    return set_error(CG_ERR_WORKSPACE, "cg_adamw_step: workspace too small");
+  Groups table;
+  table.count = group_count;
+  for (int k = 0; k < group_count; ++k) {
+    const cg_adamw_group& g = groups[k];
+    CG_REQUIRE(g.beta1 >= 0 && g.beta1 < 1 && g.beta2 >= 0 && g.beta2 < 1, "cg_adamw_step: betas must lie in [0, 1)");
+    CG_REQUIRE(g.eps >= 0, "cg_adamw_step: eps must not be negative");
+    table.g[k] = g;
+  }
+  int live = 0;
+  for (int i = 0; i < count; ++i) {
+    const cg_adamw_tensor& t = tensors[i];
+    CG_REQUIRE(t.numel >= 0 && t.state >= 0 && t.state % kBlockEntries == 0, "cg_adamw_step: tensor %d: bad extent", i);
+    CG_REQUIRE(t.numel <= static_cast<int64_t>(INT32_MAX) * kChunk, "cg_adamw_step: tensor %d is too large", i);
+    CG_REQUIRE(t.group >= 0 && t.group < group_count, "cg_adamw_step: tensor %d: no such group", i);
+    CG_REQUIRE(t.numel == 0 || !t.grad || t.param, "cg_adamw_step: tensor %d: NULL parameter", i);
+    live += t.grad && t.numel > 0;
+  }
+  if (!live) return CG_OK;
+  const States states{exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, master};
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  auto* c = static_cast<Control*>(control);
+  auto* partial = static_cast<double*>(workspace);
+  auto run = [&](auto sample) {
+    using T = decltype(sample);
+    return live <= kFewTensors
+               ? run_step<T, kFewTensors>(tensors, count, table, state_bits, states, steps, max_norm, norm_out, c, partial, s)
+               : run_step<T, kManyTensors>(tensors, count, table, state_bits, states, steps, max_norm, norm_out, c, partial, s);
+  };
+  if (dtype == CG_F32) return run(float{});
+  if (dtype == CG_F16) return run(__half{});
+  return run(__nv_bfloat16{});
+}

@@ -392,6 +392,38 @@ int cg_seat_values(const float* values, int64_t value_rows, int seats, const int
  * first players[i] seats, padded seats zero. */
 int cg_center_zero_sum(const float* values, const int64_t* players, int64_t n, int seats, float* out, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * AdamW over many tensors (the update's optimizer step and the clip before it; the
+ * reference runs torch's fused Adam after clip_grad_norm, rl/trainer.py:175-183, 392-401).
+ * One step of `count` tensors of one dtype:
+ *   g' = g * min(1, max_norm / (|g| + 1e-6)), |g| over every tensor (max_norm <= 0: g' = g)
+ *   m = b1 m + (1 - b1) g', v = b2 v + (1 - b2) g'^2
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * The state lives in flat arrays in which tensor i owns numel entries from `state` on, a
+ * multiple of 256, padded with zeros to the next multiple: exp_avg and exp_avg_sq fp32
+ * (state_bits 32), or e4m3 codes of m and of sqrt(v) with one fp32 scale per 256 entries
+ * (the block's largest magnitude, code 448; state_bits 8); master fp32 copies of 16-bit
+ * parameters (NULL for fp32 ones). A tensor with grad NULL is left as it is. steps int64 is
+ * t on the device, shared by all tensors, and counts up by one. With max_norm a norm that is
+ * not finite leaves everything as it is (steps too); norm_out fp32 receives |g|.
+ * control: cg_adamw_control_bytes(), zeroed before its first use and kept with the state.
+ * ------------------------------------------------------------------------------- */
+typedef struct {
+  void* param;
+  const void* grad;
+  int64_t numel, state;
+  int32_t group, reserved;
+} cg_adamw_tensor;
+typedef struct {
+  double lr, beta1, beta2, eps, weight_decay;
+} cg_adamw_group;
+int64_t cg_adamw_control_bytes(void);
+int64_t cg_adamw_workspace_bytes(int count);
+int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtype, const cg_adamw_group* groups, int group_count,
+                  int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale,
+                  float* master, int64_t* steps, float max_norm, float* norm_out, void* control, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
