@@ -206,6 +206,146 @@ def ppo_terms(logits: torch.Tensor, old_probs: torch.Tensor, actions: torch.Tens
     )
 
 
+# -- the anchored objective ------------------------------------------------------------------------
+ANCHORED_KEYS = ("policy_loss", "row_weight", "entropy_raw", "entropy", "entropy_weight", "clip", "behavior_kl",
+                 "reference_kl", "objective")
+
+
+def _rows_of(name: str, tensor: torch.Tensor, rows: int, device: torch.device, dtype: torch.dtype) -> torch.Tensor:
+    if tensor.shape != (rows,) or tensor.device != device:
+        raise ValueError(f"{name} must be [{rows}] on {device}, not {tuple(tensor.shape)} on {tensor.device}")
+    return tensor.to(dtype).contiguous()
+
+
+def _plane_of(name: str, tensor: torch.Tensor, like: torch.Tensor) -> torch.Tensor:
+    if tensor.shape != like.shape or tensor.device != like.device:
+        raise ValueError(f"{name} must be {tuple(like.shape)} on {like.device}, not {tuple(tensor.shape)} on {tensor.device}")
+    return _unit_rows(tensor)
+
+
+def _unit_rows(plane: torch.Tensor) -> torch.Tensor:
+    """The plane with adjacent row entries and rows that do not overlap (a copy only where it has neither)."""
+
+    if plane.shape[1] > 1 and plane.stride(1) != 1 or plane.shape[0] > 1 and plane.stride(0) < plane.shape[1]:
+        return plane.contiguous()
+    return plane
+
+
+def _row_stride(plane: torch.Tensor) -> int:
+    return plane.stride(0) if plane.shape[0] > 1 else plane.shape[1]
+
+
+def _logits_and_mask(logits: torch.Tensor, actions: torch.Tensor, legal: torch.Tensor | None):
+    if logits.dim() != 2 or logits.shape[1] == 0:
+        raise ValueError(f"logits must be [rows, width] with a width, not {tuple(logits.shape)}")
+    if logits.dtype not in nat.DTYPE_CODES:
+        raise ValueError(f"logits must be float32, float16 or bfloat16, not {logits.dtype}")
+    if actions.is_floating_point():
+        raise ValueError("actions must be integers")
+    if legal is not None:
+        if legal.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"legal must be bool or uint8, not {legal.dtype}")
+        legal = _plane_of("legal", legal, logits)
+    nat.ptr(logits)  # refuses CPU tensors
+    return _unit_rows(logits), _rows_of("actions", actions, logits.shape[0], logits.device, torch.int64), legal
+
+
+def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights, clip, beta,
+                  alpha, want_grad: bool = True):
+    rows, width = logits.shape
+    # The gradient takes the logits' row stride where that only pads the row, so that both rows align alike.
+    stride = _row_stride(logits)
+    grad_stride = stride if stride <= width + 64 else width
+    grad = None
+    if want_grad:
+        grad = torch.empty((rows, grad_stride), dtype=logits.dtype, device=logits.device)[:, :width]
+    totals = torch.empty(len(ANCHORED_KEYS), device=logits.device)
+    need = nat.query("cg_anchored_objective_workspace_bytes", rows)
+    with torch.cuda.device(logits.device):
+        workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
+        nat.call("cg_anchored_objective", nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], rows, width, stride,
+                 nat.ptr(reference_logits), 0 if reference_logits is None else _row_stride(reference_logits),
+                 nat.ptr(reference_log_probs), nat.ptr(legal), 0 if legal is None else _row_stride(legal),
+                 nat.ptr(actions), nat.ptr(old), nat.ptr(advantages), nat.ptr(weights), clip, beta, alpha,
+                 nat.ptr(grad), grad_stride, nat.ptr(totals), nat.ptr(workspace), need, nat.stream_handle(logits.device))
+    return grad, totals
+
+
+class _AnchoredObjective(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights, clip,
+                beta, alpha):
+        inputs = (logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights)
+        ctx.scalars = (clip, beta, alpha)
+        ctx.gradient, totals = _run_anchored(*inputs, *ctx.scalars, want_grad=ctx.needs_input_grad[0])
+        ctx.save_for_backward(*inputs)  # a second backward computes the gradient again
+        ctx.mark_non_differentiable(totals)
+        return totals[-1].clone(), totals
+
+    @staticmethod
+    def backward(ctx, grad_objective, _grad_totals):
+        gradient, ctx.gradient = ctx.gradient, None
+        if gradient is None:
+            gradient, _ = _run_anchored(*ctx.saved_tensors, *ctx.scalars)
+        gradient = gradient.mul_(grad_objective)
+        return gradient, None, None, None, None, None, None, None, None, None, None
+
+
+def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_probs: torch.Tensor,
+                       advantages: torch.Tensor, weights: torch.Tensor, *, clip_ratio: float, beta: float,
+                       alpha: float = 0.0, reference_logits: torch.Tensor | None = None,
+                       reference_log_probs: torch.Tensor | None = None, legal: torch.Tensor | None = None):
+    """The clipped policy objective anchored to a reference policy by a KL term, over any vocabulary.
+
+    ``sum w (surrogate + beta KL - alpha normalized_entropy)`` over rows of logits [N, V] (float32, float16 or
+    bfloat16, any row stride), with the taken ``actions`` [N], the behaviour's log-probabilities of them
+    ``old_log_probs`` [N], and ``advantages`` and ``weights`` [N]. The reference is either its logits [N, V]
+    (``reference_logits``, in the logits' dtype: the exact KL(pi || reference) over the legal set) or its log-probability
+    of the action alone (``reference_log_probs`` [N]: the sampled estimate exp(u) - u - 1 with
+    u = reference - log pi). ``legal`` (bool or uint8 [N, V]) masks logits and reference alike; what it hides may hold
+    anything. A row with a negative action, weight 0 or nothing legal counts for nothing.
+
+    Returns (objective, totals): objective is a differentiable fp32 scalar (with respect to the logits; its gradient is
+    computed with it, in the logits' dtype), totals fp32 [9] in ``ANCHORED_KEYS`` order, as ``policy_objective``
+    reports them. An action past the width or outside ``legal`` counts for nothing and sets the fault word
+    (``_native.fault_status``).
+    """
+
+    if beta and (reference_logits is None) == (reference_log_probs is None):
+        raise ValueError("a KL term takes reference_logits or reference_log_probs, one of the two")
+    if reference_logits is not None and reference_log_probs is not None:
+        raise ValueError("give reference_logits or reference_log_probs, not both")
+    if clip_ratio < 0:
+        raise ValueError("clip_ratio must not be negative")
+    logits, actions, legal = _logits_and_mask(logits, actions, legal)
+    rows, device = logits.shape[0], logits.device
+    if reference_logits is not None:
+        if reference_logits.dtype != logits.dtype:
+            raise ValueError(f"reference_logits must be {logits.dtype}, not {reference_logits.dtype}")
+        reference_logits = _plane_of("reference_logits", reference_logits.detach(), logits)
+    if reference_log_probs is not None:
+        reference_log_probs = _rows_of("reference_log_probs", reference_log_probs.detach(), rows, device, torch.float32)
+    rest = [_rows_of(name, value.detach(), rows, device, torch.float32)
+            for name, value in (("old_log_probs", old_log_probs), ("advantages", advantages), ("weights", weights))]
+    return _AnchoredObjective.apply(logits, reference_logits, reference_log_probs, legal, actions, *rest,
+                                    float(clip_ratio), float(beta), float(alpha))
+
+
+def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, legal: torch.Tensor | None = None) -> torch.Tensor:
+    """log pi(action) per row, fp32 [N], over the legal entries: what ``anchored_objective`` takes as the behaviour's or the
+    reference's log-probabilities. Not differentiable. 0 where the action is negative or nothing is legal, minus
+    infinity where the action itself is illegal."""
+
+    logits, actions, legal = _logits_and_mask(logits.detach(), actions, legal)
+    rows, width = logits.shape
+    out = torch.empty(rows, device=logits.device)
+    with torch.cuda.device(logits.device):
+        nat.call("cg_action_log_probs", nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], rows, width,
+                 _row_stride(logits), nat.ptr(legal), 0 if legal is None else _row_stride(legal), nat.ptr(actions),
+                 nat.ptr(out), nat.stream_handle(logits.device))
+    return out
+
+
 # -- value loss ----------------------------------------------------------------------------------
 class _ValueLoss(torch.autograd.Function):
     @staticmethod

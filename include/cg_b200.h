@@ -376,6 +376,31 @@ int cg_value_loss(const float* prediction, const float* targets, const int32_t* 
                   int64_t rows, int players_max, float reward_scale, float* grad, double* totals, void* workspace,
                   int64_t workspace_bytes, void* stream);
 
+/* The anchored objective: the clipped surrogate with a KL term to a reference policy and an
+ * entropy bonus, over a vocabulary of any width, with its gradient. Per row, over its legal set S
+ * (legal uint8 [rows, width], or NULL for every entry), lp = log softmax_S(logits):
+ *   L = sum_i w_i (surr_i + beta KL_i - alpha [|S| > 1] H_i / log |S|)
+ *   surr = -min(ratio A, clip(ratio, 1 -+ clip_ratio) A), ratio = exp(lp[action] - old_log_prob)
+ * KL = sum_S p (lp - log softmax_S(reference_logits)), or exp(u) - u - 1 with
+ * u = reference_log_prob - lp[action], or 0 where both references are NULL. logits and
+ * reference_logits share a dtype; each has its own row stride (entries). grad [rows, width] (or NULL)
+ * has the logits' dtype and receives dL/dlogits (0 at illegal entries); totals fp32 [9] = sums of w times
+ * (surr, 1, H, H / log |S|, [|S| > 1], [|ratio - 1| > clip], ratio - 1 - log ratio, KL) and L, summed in
+ * float64 in a fixed order. A row counts for nothing, with a zero gradient, where its action is negative, its
+ * weight 0 or nothing in it is legal (a mask that is all zero, logits that are all minus infinity).
+ * An action >= width or outside the legal set does the same and sets the fault word (0x420 / 0x421). */
+int64_t cg_anchored_objective_workspace_bytes(int64_t rows);
+int cg_anchored_objective(const void* logits, int dtype, int64_t rows, int width, int64_t stride,
+                          const void* reference_logits, int64_t reference_stride, const float* reference_log_probs,
+                          const uint8_t* legal, int64_t legal_stride, const int64_t* actions,
+                          const float* old_log_probs, const float* advantages, const float* weights, float clip_ratio,
+                          float beta, float alpha, void* grad, int64_t grad_stride, float* totals, void* workspace,
+                          int64_t workspace_bytes, void* stream);
+/* lp[action] alone, fp32 [rows] (the behaviour's or the reference's log-probabilities for the
+ * objective): 0 where the row counts for nothing, minus infinity where the action is illegal. */
+int cg_action_log_probs(const void* logits, int dtype, int64_t rows, int width, int64_t stride, const uint8_t* legal,
+                        int64_t legal_stride, const int64_t* actions, float* log_probs, void* stream);
+
 /* The PPO baseline's seat values (PPOTrainer._baseline / _recorded_values, trainer.py:556-571,
  * 610-632): decision i reads row flat[i] (or i when flat is NULL) of values fp32 [value_rows,
  * seats]; absolute seat s takes column (s - shift[i]) mod players[i], seats >= players[i] zero.
