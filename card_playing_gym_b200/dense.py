@@ -1,0 +1,109 @@
+"""A linear layer with its bias, activation and residual in the product's epilogue, differentiable.
+
+``linear(x, weight, bias, residual, activation=...)`` is ``activation(x @ weight.T + bias) + residual`` in one product
+(csrc/dense.cu), in float32, float16 or bfloat16 with fp32 sums: the shapes of the reference trunk's MLP and projections
+(cardgym/nn/trunk.py:124-157) in training, where gradients flow to every input, and for single tokens.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _native as nat
+
+ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
+
+
+def _unit_rows(matrix: torch.Tensor) -> torch.Tensor:
+    """The matrix with adjacent row entries and rows that do not overlap (a copy only where it has neither)."""
+
+    if matrix.shape[1] > 1 and matrix.stride(1) != 1 or matrix.shape[0] > 1 and matrix.stride(0) < matrix.shape[1]:
+        return matrix.contiguous()
+    return matrix
+
+
+def _row_stride(matrix: torch.Tensor) -> int:
+    return max(matrix.stride(0), matrix.shape[1]) if matrix.shape[0] > 1 else matrix.shape[1]
+
+
+def _workspace(x, weight, dy, activation: int) -> torch.Tensor:
+    need = nat.query("cg_linear_workspace_bytes", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight),
+                     nat.ptr(dy), 0 if dy is None else _row_stride(dy), nat.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1],
+                     weight.shape[0], activation, 0 if dy is None else 1)
+    return torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, activation):
+        rows, inner = x.shape
+        outer = weight.shape[0]
+        trains = any(ctx.needs_input_grad[:3])
+        with torch.cuda.device(x.device):
+            y = torch.empty((rows, outer), dtype=x.dtype, device=x.device)
+            pre = torch.empty_like(y) if trains and activation else None
+            workspace = _workspace(x, weight, None, activation)
+            nat.call("cg_linear_forward", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight),
+                     nat.ptr(bias), nat.ptr(residual), 0 if residual is None else _row_stride(residual),
+                     nat.DTYPE_CODES[x.dtype], rows, inner, outer, activation, nat.ptr(y), nat.ptr(pre),
+                     nat.ptr(workspace), workspace.numel(), nat.stream_handle(x.device))
+        if trains:
+            ctx.save_for_backward(x, weight, pre)
+        ctx.activation = activation
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        dx = dweight = dbias = None
+        needs_x, needs_weight, needs_bias, needs_residual, _ = ctx.needs_input_grad
+        if needs_x or needs_weight or needs_bias:
+            x, weight, pre = ctx.saved_tensors
+            rows, inner = x.shape
+            outer = weight.shape[0]
+            g = _unit_rows(dy)
+            with torch.cuda.device(x.device):
+                dx = torch.empty((rows, inner), dtype=x.dtype, device=x.device) if needs_x else None
+                dweight = torch.empty((outer, inner), dtype=x.dtype, device=x.device) if needs_weight else None
+                dbias = torch.empty(outer, dtype=x.dtype, device=x.device) if needs_bias else None
+                workspace = _workspace(x, weight, g, ctx.activation)
+                nat.call("cg_linear_backward", nat.ptr(g), _row_stride(g), nat.ptr(pre), nat.ptr(x), _row_stride(x),
+                         nat.ptr(weight), _row_stride(weight), nat.DTYPE_CODES[x.dtype], rows, inner, outer,
+                         ctx.activation, nat.ptr(dx), nat.ptr(dweight), nat.ptr(dbias), nat.ptr(workspace),
+                         workspace.numel(), nat.stream_handle(x.device))
+        return dx, dweight, dbias, dy if needs_residual else None, None
+
+
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None,
+           residual: torch.Tensor | None = None, *, activation: str = "none") -> torch.Tensor:
+    """``activation(x @ weight.T + bias) + residual``: x [..., K], weight [N, K], bias [N], residual [..., N] -> [..., N].
+
+    All share one dtype (float32, float16, bfloat16) and one CUDA device; rows may be strided. ``activation``: "none",
+    "relu", "gelu" (exact, by erf) or "silu". Products are summed in fp32 and rounded once, after the residual.
+
+    Differentiable in x, weight, bias and residual. In training the sum before the activation is kept in the inputs'
+    dtype, as is the gradient that enters the two backward products: each a rounding of 2^-8 (bfloat16) or 2^-11
+    (float16) beside the results' own, which halves what the pass reads and writes.
+    """
+
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"activation must be one of {sorted(ACTIVATIONS)}, not {activation!r}")
+    if x.dtype not in nat.DTYPE_CODES:
+        raise ValueError(f"x must be float32, float16 or bfloat16, not {x.dtype}")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"x {tuple(x.shape)} does not multiply a weight of {tuple(weight.shape)}")
+    outer = weight.shape[0]
+    shape = (*x.shape[:-1], outer)
+    if bias is not None and bias.shape != (outer,):
+        raise ValueError(f"bias must be [{outer}], not {tuple(bias.shape)}")
+    if residual is not None and residual.shape != shape:
+        raise ValueError(f"residual must be {shape}, not {tuple(residual.shape)}")
+    for name, tensor in (("weight", weight), ("bias", bias), ("residual", residual)):
+        if tensor is not None and (tensor.dtype != x.dtype or tensor.device != x.device):
+            raise ValueError(f"{name} must be {x.dtype} on {x.device}, as x is, not {tensor.dtype} on {tensor.device}")
+    nat.ptr(x)  # refuses CPU tensors
+    if x.dim() != 2:
+        x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty((shape[:-1].numel(), 0))
+        residual = None if residual is None else residual.reshape(x.shape[0], outer)
+    y = _Linear.apply(_unit_rows(x), _unit_rows(weight), None if bias is None else bias.contiguous(),
+                      None if residual is None else _unit_rows(residual), ACTIVATIONS[activation])
+    return y if len(shape) == 2 else y.view(shape)

@@ -449,6 +449,29 @@ int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtype, const cg
                   float* master, int64_t* steps, float max_norm, float* norm_out, void* control, void* workspace,
                   int64_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * A linear layer with its epilogue (the shapes of cardgym/nn/trunk.py:124-157 in training):
+ *   y = act(x W^T + bias) + residual, x [rows, inner], W [outer, inner], y [rows, outer]
+ * act: 0 none, 1 relu, 2 gelu (erf), 3 silu. x, W and residual have a row stride (entries); bias and
+ * residual may be NULL. One dtype for everything, fp32 sums, one rounding. pre [rows, outer]
+ * (or NULL) receives x W^T + bias for the backward pass:
+ *   dpre = dy act'(pre), dx = dpre W, dweight = dpre^T x, dbias = sum over rows of dpre
+ * (dx, dweight and dbias contiguous, each may be NULL; pre is read unless act is 0; the
+ * residual's gradient is dy itself). The workspace depends on the operands' alignment: the query
+ * takes the pointers and strides of the call it is for (dy NULL for the forward one).
+ * ------------------------------------------------------------------------------- */
+int64_t cg_linear_workspace_bytes(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                  const void* dy, int64_t dy_stride, int dtype, int64_t rows, int64_t inner,
+                                  int64_t outer, int activation, int backward);
+int cg_linear_forward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
+                      const void* residual, int64_t residual_stride, int dtype, int64_t rows, int64_t inner,
+                      int64_t outer, int activation, void* y, void* pre, void* workspace, int64_t workspace_bytes,
+                      void* stream);
+int cg_linear_backward(const void* dy, int64_t dy_stride, const void* pre, const void* x, int64_t x_stride,
+                       const void* weight, int64_t weight_stride, int dtype, int64_t rows, int64_t inner,
+                       int64_t outer, int activation, void* dx, void* dweight, void* dbias, void* workspace,
+                       int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,255 @@
+"""dense.linear against its formula in 64 bits: types, activations, odd sizes from one entry to past a tile, strides,
+missing biases and residuals, empty extents, gradients (the formula's and differences), and its refusals.
+
+Tolerances. A product's sum of K fp32 terms is within 2^-24 sqrt-to-linear of sum |a||b|: 2^-21 of it covers any order of
+addition of exact products up to these depths (the float32 operands' three bfloat16 parts leave 2^-23 of it). The activation's
+derivative is at most 1.13, its curvature at most 1.1. 16-bit results round once (2^-8, 2^-11); the sum kept for the
+backward pass and the gradient entering its products round once more each."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+from card_playing_gym_b200 import dense
+from card_playing_gym_b200 import _native as nat
+
+TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
+HALF_STEP = {torch.float32: 2.0 ** -24, torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}
+ACC = 2.0 ** -21
+LEAST = {torch.float32: 1e-37, torch.bfloat16: 1e-37, torch.float16: 2.0 ** -25}
+
+ACT = {"none": lambda z: z * 1.0, "relu": torch.relu, "gelu": torch.nn.functional.gelu, "silu": torch.nn.functional.silu}
+
+
+def normal(shape, dtype, seed, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (scale * torch.randn(shape, generator=g, device="cuda")).to(dtype)
+
+
+def case(m, k, n, dtype, bias=True, residual=True):
+    return dict(x=normal((m, k), dtype, 1), weight=normal((n, k), dtype, 2, 1 / math.sqrt(max(k, 1))),
+                bias=normal((n,), dtype, 3, 0.5) if bias else None,
+                residual=normal((m, n), dtype, 4) if residual else None, dy=normal((m, n), dtype, 5))
+
+
+def check(data, activation, backward=True):
+    dtype = data["x"].dtype
+    leaves = {name: data[name].detach().requires_grad_(backward) for name in ("x", "weight", "bias", "residual")
+              if data[name] is not None}
+    y = dense.linear(leaves["x"], leaves["weight"], leaves.get("bias"), leaves.get("residual"), activation=activation)
+    wide = {name: value.detach().double().requires_grad_(backward) for name, value in leaves.items()}
+    pre = wide["x"] @ wide["weight"].t()
+    reach = wide["x"].abs().detach() @ wide["weight"].abs().t().detach()
+    if "bias" in wide:
+        pre = pre + wide["bias"]
+        reach = reach + wide["bias"].abs().detach()
+    want = ACT[activation](pre)
+    if "residual" in wide:
+        want = want + wide["residual"]
+    half, least = HALF_STEP[dtype], LEAST[dtype]
+    assert y.dtype == dtype and y.shape == want.shape
+    near = 1.2 * ACC * reach + 2.0 ** -20 * (pre.detach().abs() + want.detach().abs())
+    assert ((y.double() - want).abs() <= near + (half + ACC) * want.abs() + least).all()
+    if not backward:
+        return y
+    grads = dict(zip(leaves, torch.autograd.grad(y, list(leaves.values()), data["dy"])))
+    expected = dict(zip(wide, torch.autograd.grad(want, list(wide.values()), data["dy"].double())))
+    pre, dy = pre.detach(), data["dy"].double()
+    dpre_bound = dy.abs() * 1.2  # |dpre|, and what a rounding of pre and of dpre moves it by
+    off = dy.abs() * (1.2 * half * (activation != "none") + 1.1 * (half * pre.abs() + 1.2 * ACC * reach) * (activation not in ("none", "relu"))
+                      + 2.0 ** -20)
+    if activation == "relu":  # the kink: a sum within its error of zero may fall on either side
+        off = off + dy.abs() * (pre.abs() <= 1.2 * ACC * reach + least)
+    bounds = {"x": off @ wide["weight"].detach().abs() + ACC * (dpre_bound @ wide["weight"].detach().abs()),
+              "weight": off.t() @ wide["x"].detach().abs() + ACC * (dpre_bound.t() @ wide["x"].detach().abs()),
+              "bias": off.sum(0) + ACC * dpre_bound.sum(0), "residual": torch.zeros_like(dy)}
+    for name, grad in grads.items():
+        assert grad.dtype == dtype
+        bound = bounds[name] + (half + ACC) * expected[name].abs() + least
+        assert ((grad.double() - expected[name]).abs() <= bound).all(), name
+    return y
+
+
+SHAPES = [(1, 1, 1), (1, 240, 720), (2, 7, 3), (5, 64, 64), (17, 33, 129), (64, 240, 720), (129, 720, 240), (127, 65, 257),
+          (300, 1001, 515), (257, 128, 1), (1000, 1, 300), (515, 2050, 130), (2048, 256, 512)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", list(ACT))
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", SHAPES)
+def test_forward_and_backward(shape, dtype, activation):
+    check(case(*shape, TYPES[dtype]), activation)
+    assert nat.fault_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 7, 8, 9, 16, 31, 32, 33, 64, 65])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("inner,outer", [(240, 720), (4096, 1000), (77, 33), (3000, 4097)])
+def test_few_tokens(rows, dtype, inner, outer):
+    with torch.no_grad():
+        check(case(rows, inner, outer, TYPES[dtype]), "gelu", backward=False)
+        check(case(rows, inner, outer, TYPES[dtype], bias=False, residual=False), "none", backward=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("bias,residual", [(False, False), (True, False), (False, True)])
+def test_parts_may_be_missing(dtype, bias, residual):
+    check(case(200, 96, 160, TYPES[dtype], bias, residual), "silu")
+    check(case(200, 96, 160, TYPES[dtype], bias, residual), "none")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(4000, 24, 40), (40000, 32, 16), (20000, 240, 720)])
+def test_tall_batches_join_their_slices(dtype, shape):
+    check(case(*shape, TYPES[dtype]), "gelu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("pad", [1, 3, 8])
+def test_strided_and_unaligned_inputs(dtype, pad):
+    """Rows longer than the matrix, matrices that start inside a row, transposed and expanded ones."""
+
+    data = case(150, 72, 136, TYPES[dtype])
+    for name in ("x", "weight", "residual", "dy"):
+        m, k = data[name].shape
+        store = torch.full((m, k + 2 * pad), math.nan, dtype=data[name].dtype, device="cuda")
+        store[:, pad:pad + k] = data[name]
+        data[name] = store[:, pad:pad + k]
+    store = torch.zeros(136 + pad, dtype=TYPES[dtype], device="cuda")
+    store[pad:] = data["bias"]
+    data["bias"] = store[pad:]
+    check(data, "gelu")
+    data = case(150, 72, 136, TYPES[dtype])
+    for name in ("x", "weight", "residual", "dy"):
+        data[name] = data[name].t().contiguous().t()
+    check(data, "gelu")
+    data["dy"] = data["dy"][:1].expand(150, 136)
+    data["x"] = data["x"][:1].expand(150, 72)
+    check(data, "silu")
+
+
+@pytest.mark.gpu
+def test_leading_dimensions():
+    x, weight, bias = normal((3, 5, 48), torch.bfloat16, 1), normal((32, 48), torch.bfloat16, 2), normal((32,), torch.bfloat16, 3)
+    y = dense.linear(x, weight, bias, normal((3, 5, 32), torch.bfloat16, 4), activation="relu")
+    flat = dense.linear(x.view(15, 48), weight, bias, normal((3, 5, 32), torch.bfloat16, 4).view(15, 32), activation="relu")
+    assert y.shape == (3, 5, 32) and torch.equal(y.view(15, 32), flat)
+    one = dense.linear(x[0, 0], weight, bias, activation="relu")
+    assert one.shape == (32,)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(0, 16, 8), (4, 0, 8), (4, 16, 0)])
+def test_empty_extents(dtype, shape):
+    """No rows: nothing; no depth: the epilogue of zero; no outputs: zero gradients."""
+
+    data = case(*shape, TYPES[dtype])
+    leaves = {k: data[k].detach().requires_grad_() for k in ("x", "weight", "bias", "residual")}
+    y = dense.linear(*leaves.values(), activation="gelu")
+    grads = torch.autograd.grad(y, list(leaves.values()), data["dy"])
+    assert all(g.shape == leaf.shape for g, leaf in zip(grads, leaves.values()))
+    if shape[1] == 0:
+        want = torch.nn.functional.gelu(data["bias"].double()) + data["residual"].double()
+        assert ((y.double() - want).abs() <= 2 * HALF_STEP[TYPES[dtype]] * (want.abs() + 1)).all()
+    assert not grads[0].any() and not grads[1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", ["gelu", "silu", "relu"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_infinities_and_nan_stay_in_their_rows(dtype, activation):
+    data = case(140, 64, 96, TYPES[dtype], residual=False)
+    want = dense.linear(data["x"], data["weight"], data["bias"], activation=activation)
+    data["x"][7, 3] = math.nan
+    data["x"][9] = 0.0
+    data["x"][9, 5] = math.inf
+    got = dense.linear(data["x"], data["weight"], data["bias"], activation=activation)
+    assert torch.isnan(got[7]).all()
+    assert not torch.isfinite(got[9]).all() or activation != "none"
+    rest = [i for i in range(140) if i not in (7, 9)]
+    assert torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", list(ACT))
+def test_the_gradient_against_differences(activation):
+    """Central differences of sum(dy * y) in fp32 at h = 2^-5: rounding 2^-22 |L| / h, curvature h^2."""
+
+    data = case(6, 9, 5, torch.float32)
+    if activation == "relu":  # away from the kink
+        data["bias"] = data["bias"].sign() * 4
+    leaves = {k: data[k].detach().requires_grad_() for k in ("x", "weight", "bias", "residual")}
+    grads = dict(zip(leaves, torch.autograd.grad(dense.linear(*leaves.values(), activation=activation), list(leaves.values()),
+                                                 data["dy"])))
+
+    def value(inputs):
+        with torch.no_grad():
+            return float((dense.linear(*inputs.values(), activation=activation).double() * data["dy"].double()).sum())
+
+    h = 2.0 ** -5
+    for name, at in (("x", (2, 3)), ("weight", (4, 8)), ("bias", (1,)), ("residual", (5, 2))):
+        ends = []
+        for sign in (1, -1):
+            moved = {k: v.detach().clone() for k, v in leaves.items()}
+            moved[name][at] += sign * h
+            ends.append(value(moved))
+        assert (ends[0] - ends[1]) / (2 * h) == pytest.approx(float(grads[name][at]), abs=30 * 2.0 ** -22 / h + 30 * h * h)
+
+
+@pytest.mark.gpu
+def test_only_what_needs_a_gradient_gets_one():
+    data = case(64, 48, 32, torch.bfloat16)
+    full = {k: data[k].detach().requires_grad_() for k in ("x", "weight", "bias", "residual")}
+    every = torch.autograd.grad(dense.linear(*full.values(), activation="gelu"), list(full.values()), data["dy"])
+    for name, want in zip(full, every):
+        some = {k: data[k].detach().requires_grad_(k == name) for k in full}
+        (got,) = torch.autograd.grad(dense.linear(*some.values(), activation="gelu"), [some[name]], data["dy"])
+        assert torch.equal(got, want), name
+
+
+@pytest.mark.gpu
+def test_streams_and_repeats_agree():
+    data = case(500, 240, 720, torch.bfloat16)
+    want = check(data, "gelu")
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = check(data, "gelu")
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(want, got)
+
+
+@pytest.mark.gpu
+def test_refusals_on_the_device():
+    x, w = normal((4, 8), torch.float32, 1), normal((6, 8), torch.float32, 2)
+    with pytest.raises(ValueError, match="weight must be"):
+        dense.linear(x, w.bfloat16())
+    with pytest.raises(ValueError, match="bias must be"):
+        dense.linear(x, w, normal((5,), torch.float32, 3))
+    with pytest.raises(ValueError, match="residual must be"):
+        dense.linear(x, w, None, normal((4, 5), torch.float32, 3))
+
+
+def test_refusals_without_a_gpu():
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    with pytest.raises(ValueError, match="CUDA"):
+        dense.linear(x, w)
+    with pytest.raises(ValueError, match="activation"):
+        dense.linear(x, w, activation="tanh")
+    with pytest.raises(ValueError, match="does not multiply"):
+        dense.linear(x, torch.zeros(6, 7))
+    with pytest.raises(ValueError, match="float32, float16 or bfloat16"):
+        dense.linear(x.double(), w.double())
+    with pytest.raises(nat.NativeError, match="activation"):
+        nat.call("cg_linear_forward", None, 8, None, 8, None, None, 0, 0, 4, 8, 6, 9, None, None, None, 0, None)
+    with pytest.raises(nat.NativeError, match="shape"):
+        nat.query("cg_linear_workspace_bytes", None, 8, None, 8, None, 0, 0, -1, 8, 8, 0, 0)
