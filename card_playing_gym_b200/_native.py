@@ -6,6 +6,7 @@ kernel raises. ``lib()`` loads the library once per process.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from functools import lru_cache
 from pathlib import Path
@@ -241,6 +242,15 @@ def ptr(tensor: torch.Tensor | None) -> int | None:
     if not tensor.is_cuda:
         raise ValueError("card_playing_gym_b200 kernels take CUDA tensors only (there is no CPU path)")
     return tensor.data_ptr()
+
+
+_NO_SWITCH = contextlib.nullcontext()
+
+
+def on_device(device: torch.device):
+    """A context in which `device` is current; nothing to enter where it is already."""
+
+    return _NO_SWITCH if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def stream_handle(device: torch.device | None = None) -> int:

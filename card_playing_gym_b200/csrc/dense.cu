@@ -1,192 +1,235 @@
 // A linear layer with its epilogue, and its backward pass:
 //   y = act(x W^T + b) + residual          x [M, K], W [N, K], b [N], residual and y [M, N]
 //   dpre = dy act'(pre), pre = x W^T + b;  dx = dpre W,  dW = dpre^T x,  db = sum over rows of dpre
-// All three products are C[i, j] = sum_k A(i, k) B(j, k) over operands read in place through their strides.
-// Sums are fp32 whatever the operands' type; results are rounded once to it.
+// The products run on the tensor cores (product.cu), which reads 16-bit operands in place in either order; around them:
+//
+//   pack_kernel   float32 operands as three bfloat16 parts; 16-bit operands whose rows do not start on 16 bytes
+//                 as a copy that does
+//   slope_kernel  dpre, in the form the products read, and the column sums of db in the same pass over dy and pre
+//
+// pre and dpre are kept in the operands' type: a 16-bit pre moves act' by its slope times 2^-8 |pre| (bfloat16) and a
+// 16-bit dpre is what the tensor cores multiply; db sums dpre before that rounding.
 #include <algorithm>
 
-#include "common.cuh"
+#include "elements.cuh"
 
 namespace cg {
 namespace {
 
-enum Activation { kNone = 0, kRelu = 1, kGelu = 2, kSilu = 3 };
-
+// ---- operands in the products' form --------------------------------------------------------------------------------
+// Four entries of a T matrix in operand form at `out`: T itself, or a float32's three parts, `part` entries apart.
 template <typename T>
-__device__ __forceinline__ float as_float(T v);
-template <>
-__device__ __forceinline__ float as_float(float v) { return v; }
-template <>
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
-__device__ __forceinline__ float activate(float z, int activation) {
-  if (activation == kRelu) return z < 0.f ? 0.f : z;  // a NaN stays one
-  if (activation == kGelu) return gelu_erf(z);
-  if (activation == kSilu) return z / (1.f + __expf(-z));
-  return z;
-}
-
-__device__ __forceinline__ float activation_slope(float z, int activation) {
-  if (activation == kRelu) return z > 0.f ? 1.f : z == z ? 0.f : z;
-  if (activation == kGelu) {
-    const float cumulative = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-    const float tail = z * z > 200.f ? 0.f : z * 0.3989422804014327f * __expf(-0.5f * z * z);
-    return cumulative + tail;
-  }
-  if (activation == kSilu) {
-    const float gate = 1.f / (1.f + __expf(-z));
-    return gate * (1.f + z * (1.f - gate));
-  }
-  return 1.f;
-}
-
-struct Operand {
-  const void* base;
-  int64_t outer, inner;  // strides over i (or j) and over k
-};
-
-struct Epilogue {
-  const void* bias;      // [J], or null
-  const void* residual;  // [I, J], or null
-  void* pre;             // [I, J] contiguous, or null: the sum before the activation, kept for the backward pass
-  int64_t residual_stride, out_stride;
-  int activation;
-};
-
-// ---- plain tiles: 64 x 64 outputs a block, 4 x 4 a thread, operands through shared memory -------------------
-constexpr int kTile = 64, kDepth = 16;
-
-template <typename T>
-__global__ void __launch_bounds__(256) product_kernel(Operand a, Operand b, int64_t rows, int64_t cols, int64_t depth,
-                                                      Epilogue e, T* out) {
-  __shared__ float sa[kDepth][kTile + 1], sb[kDepth][kTile + 1];
-  const int64_t i0 = static_cast<int64_t>(blockIdx.y) * kTile, j0 = static_cast<int64_t>(blockIdx.x) * kTile;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const T* pa = static_cast<const T*>(a.base);
-  const T* pb = static_cast<const T*>(b.base);
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < depth; k0 += kDepth) {
-    for (int t = threadIdx.x; t < kTile * kDepth; t += 256) {
-      const int i = a.inner == 1 ? t / kDepth : t % kTile, k = a.inner == 1 ? t % kDepth : t / kTile;
-      sa[k][i] = i0 + i < rows && k0 + k < depth ? as_float(pa[(i0 + i) * a.outer + (k0 + k) * a.inner]) : 0.f;
-    }
-    for (int t = threadIdx.x; t < kTile * kDepth; t += 256) {
-      const int j = b.inner == 1 ? t / kDepth : t % kTile, k = b.inner == 1 ? t % kDepth : t / kTile;
-      sb[k][j] = j0 + j < cols && k0 + k < depth ? as_float(pb[(j0 + j) * b.outer + (k0 + k) * b.inner]) : 0.f;
-    }
-    __syncthreads();
+__device__ __forceinline__ void store_operand(typename OperandOf<T>::type* out, int64_t part, const float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+    __nv_bfloat16 p[4][3];
 #pragma unroll
-    for (int k = 0; k < kDepth; ++k)
+    for (int i = 0; i < 4; ++i) three_parts(v[i], p[i]);
 #pragma unroll
-      for (int u = 0; u < 4; ++u)
+    for (int k = 0; k < 3; ++k) {
+      uint2 raw;
+      auto* h = reinterpret_cast<__nv_bfloat16*>(&raw);
 #pragma unroll
-        for (int v = 0; v < 4; ++v) acc[u][v] = fmaf(sa[k][ty + 16 * u], sb[k][tx + 16 * v], acc[u][v]);
-    __syncthreads();
-  }
-  for (int u = 0; u < 4; ++u)
-    for (int v = 0; v < 4; ++v) {
-      const int64_t i = i0 + ty + 16 * u, j = j0 + tx + 16 * v;
-      if (i >= rows || j >= cols) continue;
-      float z = acc[u][v];
-      if (e.bias) z += as_float(static_cast<const T*>(e.bias)[j]);
-      if (e.pre) put(static_cast<T*>(e.pre) + i * cols + j, z);
-      z = activate(z, e.activation);
-      if (e.residual) z += as_float(static_cast<const T*>(e.residual)[i * e.residual_stride + j]);
-      put(out + i * e.out_stride + j, z);
+      for (int i = 0; i < 4; ++i) h[i] = p[i][k];
+      *reinterpret_cast<uint2*>(out + k * part) = raw;
     }
+  } else {
+    store4(out, v);
+  }
 }
 
 template <typename T>
-int run_product(const Operand& a, const Operand& b, int64_t rows, int64_t cols, int64_t depth, const Epilogue& e, void* out,
-                cudaStream_t s) {
-  const dim3 grid(static_cast<unsigned>((cols + kTile - 1) / kTile), static_cast<unsigned>((rows + kTile - 1) / kTile));
-  product_kernel<T><<<grid, 256, 0, s>>>(a, b, rows, cols, depth, e, static_cast<T*>(out));
-  return check_launch("product_kernel");
+__global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t stride, int64_t rows, int64_t cols,
+                                                   typename OperandOf<T>::type* out, int64_t out_stride) {
+  const bool aligned = aligned4<T>(in, stride);
+  const int64_t quads = (cols + 3) / 4, total = rows * quads;
+  for (int64_t index = blockIdx.x * 256ll + threadIdx.x; index < total; index += gridDim.x * 256ll) {
+    const int64_t i = index / quads, j = (index - i * quads) * 4;
+    float v[4];
+    load4(in + i * stride + j, static_cast<int>(min(int64_t{4}, cols - j)), aligned && j + 4 <= cols, v);
+    store_operand<T>(out + i * out_stride + j, rows * out_stride, v);
+  }
 }
 
 // ---- dpre and the bias gradient -----------------------------------------------------------------------------------
-// A block takes 32 columns of one slice of the rows; its warps' column sums join in shared memory, the slices' in
-// order in the second kernel.
-constexpr int kSlices = 64;
-
+// A block takes 128 columns of one slice of the rows, four columns a lane, a row a warp at a time. Its warps' column
+// sums join in shared memory, the slices' in order in bias_sum_kernel.
 template <typename T>
 __global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t rows, int64_t cols,
-                                                    int64_t slice, int activation, T* dpre, float* partial) {
-  __shared__ float s[8][33];
+                                                    int64_t slice, int activation, typename OperandOf<T>::type* dpre,
+                                                    int64_t dpre_stride, float* partial) {
+  __shared__ float4 s[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + lane;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 128 + lane * 4;
   const int64_t lo = blockIdx.y * slice, hi = min(rows, lo + slice);
-  float sum = 0.f;
-  if (j < cols)
+  const bool aligned_dy = aligned4<T>(dy, dy_stride), aligned_pre = aligned4<T>(pre, cols);
+  const int n = static_cast<int>(max(int64_t{0}, min(int64_t{4}, cols - j)));
+  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  if (n > 0) {
+#pragma unroll 4
     for (int64_t i = lo + warp; i < hi; i += 8) {
-      float g = as_float(dy[i * dy_stride + j]);
-      if (pre) g *= activation_slope(as_float(pre[i * cols + j]), activation);
-      if (dpre) put(dpre + i * cols + j, g);
-      sum += g;
+      float g[4], z[4];
+      load4(dy + i * dy_stride + j, n, aligned_dy && n == 4, g);
+      if (activation != kActNone) {
+        load4(pre + i * cols + j, n, aligned_pre && n == 4, z);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) g[k] *= activation_slope(z[k], activation);
+      }
+      if (dpre) store_operand<T>(dpre + i * dpre_stride + j, rows * dpre_stride, g);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) sum[k] += g[k];
     }
-  s[warp][lane] = sum;
-  __syncthreads();
-  if (partial && warp == 0 && j < cols) {
-    for (int w = 1; w < 8; ++w) sum += s[w][lane];
-    partial[blockIdx.y * cols + j] = sum;
   }
+  if (!partial) return;
+  s[warp][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  __syncthreads();
+  if (warp != 0 || n == 0) return;
+  for (int w = 1; w < 8; ++w) {
+    const float4 f = s[w][lane];
+    sum[0] += f.x, sum[1] += f.y, sum[2] += f.z, sum[3] += f.w;
+  }
+  for (int k = 0; k < n; ++k) partial[blockIdx.y * cols + j + k] = sum[k];
 }
 
 template <typename T>
 __global__ void __launch_bounds__(256) bias_sum_kernel(const float* partial, int slices, int64_t cols, T* db) {
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  __shared__ float s[8][33];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t j = static_cast<int64_t>(blockIdx.x) * 32 + lane;
   pdl_wait();
-  if (j >= cols) return;
   float sum = 0.f;
-  for (int k = 0; k < slices; ++k) sum += partial[k * cols + j];
+  if (j < cols)
+    for (int k = warp; k < slices; k += 8) sum += partial[k * cols + j];
+  s[warp][lane] = sum;
+  __syncthreads();
+  if (warp != 0 || j >= cols) return;
+  for (int w = 1; w < 8; ++w) sum += s[w][lane];
   put(db + j, sum);
 }
 
+// ---- plans -----------------------------------------------------------------------------------------------------------
 bool valid_extent(int64_t rows, int64_t cols, int64_t depth) {
-  constexpr int64_t most = int64_t{1} << 31;
+  constexpr int64_t most = (int64_t{1} << 31) - 256;
   return rows >= 0 && cols >= 0 && depth >= 0 && rows < most && cols < most && depth < most;
 }
 
-template <typename T>
-int forward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t rows, int64_t inner,
-            int64_t outer, const Epilogue& e, void* y, cudaStream_t s) {
-  return run_product<T>({x, x_stride, 1}, {weight, weight_stride, 1}, rows, outer, inner, e, y, s);
+int64_t padded(int64_t bytes) { return (bytes + 255) / 256 * 256; }
+int64_t padded_row(int64_t entries) { return (entries + 7) / 8 * 8; }
+
+// Whether an operand has to be packed: every float32 one, and a 16-bit one whose rows do not all start on 16 bytes.
+bool needs_pack(const void* base, int64_t stride, int64_t rows, int dtype) {
+  return dtype == CG_F32 || (reinterpret_cast<uintptr_t>(base) & 15) != 0 || (rows > 1 && stride % 8 != 0);
+}
+
+int64_t packed_bytes(int64_t rows, int64_t cols, int dtype) {
+  return padded(rows * padded_row(cols) * 2 * (dtype == CG_F32 ? 3 : 1));
+}
+
+struct Layout {
+  int64_t sums, dpre, x, weight, partial, bytes;  // byte offsets, -1 where a part is not needed
+  int64_t slice;
+  int slices;
+};
+
+Layout plan_layout(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* dy, int64_t dy_stride,
+                   int dtype, int64_t rows, int64_t inner, int64_t outer, int activation, bool backward) {
+  Layout l = {-1, -1, -1, -1, -1, 0, 1, 0};
+  auto take = [&](int64_t bytes) {
+    const int64_t at = l.bytes;
+    l.bytes += padded(bytes);
+    return at;
+  };
+  if (backward) {
+    // Blocks of 128 columns by slices of the rows: eight blocks an SM, slices of at least 32 rows.
+    const int64_t across = (outer + 127) / 128;
+    int64_t slices = std::max<int64_t>(1, 8 * 148 / std::max<int64_t>(across, 1));
+    slices = std::max<int64_t>(1, std::min(slices, (rows + 31) / 32));
+    l.slice = std::max<int64_t>(1, (rows + slices - 1) / slices);
+    l.slices = static_cast<int>((rows + l.slice - 1) / l.slice);
+    l.sums = take(l.slices * outer * static_cast<int64_t>(sizeof(float)));
+    if (activation != kActNone || needs_pack(dy, dy_stride, rows, dtype)) l.dpre = take(packed_bytes(rows, outer, dtype));
+  }
+  if (!backward && rows <= kFewRows) return l;
+  if (needs_pack(x, x_stride, rows, dtype)) l.x = take(packed_bytes(rows, inner, dtype));
+  if (needs_pack(weight, weight_stride, outer, dtype)) l.weight = take(packed_bytes(outer, inner, dtype));
+  const int64_t partial = backward ? std::max(plan_product(rows, inner, outer, dtype).partial_bytes,
+                                              plan_product(outer, inner, rows, dtype).partial_bytes)
+                                   : plan_product(rows, outer, inner, dtype).partial_bytes;
+  l.partial = take(partial);
+  return l;
 }
 
 template <typename T>
-int backward(const void* dy, int64_t dy_stride, const void* pre, const void* x, int64_t x_stride, const void* weight,
-             int64_t weight_stride, int64_t rows, int64_t inner, int64_t outer, int activation, void* dx, void* dweight,
-             void* dbias, char* workspace, cudaStream_t s) {
-  T* dpre = nullptr;
-  float* partial = reinterpret_cast<float*>(workspace);
-  if (activation != kNone) dpre = reinterpret_cast<T*>(workspace + kSlices * outer * sizeof(float));
-  const int64_t slice = (rows + kSlices - 1) / kSlices;
+int pack(const void* in, int64_t stride, int64_t rows, int64_t cols, void* out, cudaStream_t s) {
+  const int64_t quads = rows * ((cols + 3) / 4);
+  if (quads == 0) return CG_OK;
+  const int blocks = static_cast<int>(std::min<int64_t>((quads + 255) / 256, 16 * sm_count()));
+  pack_kernel<T><<<blocks, 256, 0, s>>>(static_cast<const T*>(in), stride, rows, cols,
+                                        static_cast<typename OperandOf<T>::type*>(out), padded_row(cols));
+  return check_launch("pack_kernel");
+}
+
+// An operand read in place. A single row has no stride to speak of.
+ProductOperand in_place(const void* base, int64_t stride, int64_t rows, int64_t cols) {
+  return {base, rows > 1 ? stride : padded_row(cols), 0, false};
+}
+
+// An operand stored [rows, cols], packed where its layout has a place for it.
+template <typename T>
+int operand(const void* base, int64_t stride, int64_t rows, int64_t cols, char* workspace, int64_t at, ProductOperand* o,
+            cudaStream_t s) {
+  *o = in_place(base, stride, rows, cols);
+  if (at < 0) return CG_OK;
+  *o = {workspace + at, padded_row(cols), rows * padded_row(cols), false};
+  return pack<T>(base, stride, rows, cols, workspace + at, s);
+}
+
+ProductOperand across(ProductOperand o) {
+  o.across = true;
+  return o;
+}
+
+template <typename T>
+int forward(const Layout& l, const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int dtype, int64_t rows,
+            int64_t inner, int64_t outer, const ProductEpilogue& e, char* workspace, cudaStream_t s) {
+  ProductOperand a, b;
+  if (int rc = operand<T>(x, x_stride, rows, inner, workspace, l.x, &a, s)) return rc;
+  if (int rc = operand<T>(weight, weight_stride, outer, inner, workspace, l.weight, &b, s)) return rc;
+  return run_product(a, b, rows, outer, inner, dtype, e, workspace + l.partial, s);
+}
+
+template <typename T>
+int backward(const Layout& l, const void* dy, int64_t dy_stride, const void* pre, const void* x, int64_t x_stride,
+             const void* weight, int64_t weight_stride, int dtype, int64_t rows, int64_t inner, int64_t outer, int activation,
+             void* dx, void* dweight, void* dbias, char* workspace, cudaStream_t s) {
+  using O = typename OperandOf<T>::type;
+  auto* sums = reinterpret_cast<float*>(workspace + l.sums);
+  O* dpre = l.dpre < 0 || !(dx || dweight) ? nullptr : reinterpret_cast<O*>(workspace + l.dpre);
   if ((dpre || dbias) && rows > 0 && outer > 0) {
-    const dim3 grid(static_cast<unsigned>((outer + 31) / 32), static_cast<unsigned>((rows + slice - 1) / slice));
-    slope_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), dy_stride, static_cast<const T*>(pre), rows, outer, slice,
-                                         activation, dpre, dbias ? partial : nullptr);
+    const dim3 grid(static_cast<unsigned>((outer + 127) / 128), static_cast<unsigned>(l.slices));
+    slope_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), dy_stride, static_cast<const T*>(pre), rows, outer, l.slice,
+                                         activation, dpre, padded_row(outer), dbias ? sums : nullptr);
     if (int rc = check_launch("slope_kernel")) return rc;
   }
   if (dbias) {
-    const int slices = rows > 0 ? static_cast<int>((rows + slice - 1) / slice) : 0;
-    if (int rc = launch_pdl("bias_sum_kernel", bias_sum_kernel<T>, dim3(static_cast<unsigned>((outer + 255) / 256)), dim3(256),
-                            0, s, static_cast<const float*>(partial), slices, outer, static_cast<T*>(dbias)))
+    if (int rc = launch_pdl("bias_sum_kernel", bias_sum_kernel<T>, dim3(static_cast<unsigned>((outer + 31) / 32)), dim3(256), 0, s,
+                            static_cast<const float*>(sums), rows > 0 ? l.slices : 0, outer, static_cast<T*>(dbias)))
       return rc;
   }
-  const void* g = dpre ? dpre : dy;
-  const int64_t g_stride = dpre ? outer : dy_stride;
-  if (dx && rows > 0) {
-    const Epilogue e = {nullptr, nullptr, nullptr, 0, inner, kNone};
-    if (int rc = run_product<T>({g, g_stride, 1}, {weight, 1, weight_stride}, rows, inner, outer, e, dx, s)) return rc;
+  const ProductOperand g = dpre ? ProductOperand{dpre, padded_row(outer), rows * padded_row(outer), false}
+                                : in_place(dy, dy_stride, rows, outer);
+  const ProductEpilogue into = {nullptr, nullptr, nullptr, nullptr, 0, inner, kActNone};
+  ProductOperand o;
+  if (dx) {
+    if (int rc = operand<T>(weight, weight_stride, outer, inner, workspace, l.weight, &o, s)) return rc;
+    ProductEpilogue e = into;
+    e.out = dx;
+    if (int rc = run_product(g, across(o), rows, inner, outer, dtype, e, workspace + l.partial, s)) return rc;
   }
   if (dweight) {
-    const Epilogue e = {nullptr, nullptr, nullptr, 0, inner, kNone};
-    if (int rc = run_product<T>({g, 1, g_stride}, {x, 1, x_stride}, outer, inner, rows, e, dweight, s)) return rc;
+    if (int rc = operand<T>(x, x_stride, rows, inner, workspace, l.x, &o, s)) return rc;
+    ProductEpilogue e = into;
+    e.out = dweight;
+    if (int rc = run_product(across(g), across(o), outer, inner, rows, dtype, e, workspace + l.partial, s)) return rc;
   }
   return CG_OK;
 }
@@ -194,22 +237,15 @@ int backward(const void* dy, int64_t dy_stride, const void* pre, const void* x, 
 }  // namespace
 }  // namespace cg
 
-namespace cg {
-namespace {
-int64_t workspace_bytes_of(int dtype, int64_t rows, int64_t outer, bool backward) {
-  return backward ? kSlices * outer * static_cast<int64_t>(sizeof(float)) + rows * outer * dtype_size(dtype) : 0;
-}
-}  // namespace
-}  // namespace cg
-
-extern "C" int64_t cg_linear_workspace_bytes(const void*, int64_t, const void*, int64_t, const void*, int64_t, int dtype,
-                                             int64_t rows, int64_t inner, int64_t outer, int, int backward) {
+extern "C" int64_t cg_linear_workspace_bytes(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride,
+                                             const void* dy, int64_t dy_stride, int dtype, int64_t rows, int64_t inner,
+                                             int64_t outer, int activation, int backward) {
   using namespace cg;
   if (!valid_extent(rows, outer, inner) || !valid_dtype(dtype)) {
     set_error(CG_ERR_ARGUMENT, "cg_linear_workspace_bytes: bad shape or dtype");
     return -1;
   }
-  return workspace_bytes_of(dtype, rows, outer, backward);
+  return plan_layout(x, x_stride, weight, weight_stride, dy, dy_stride, dtype, rows, inner, outer, activation, backward).bytes;
 }
 
 extern "C" int cg_linear_forward(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, const void* bias,
@@ -219,18 +255,21 @@ extern "C" int cg_linear_forward(const void* x, int64_t x_stride, const void* we
   using namespace cg;
   CG_REQUIRE(valid_dtype(dtype), "cg_linear_forward: dtype must be float32, float16 or bfloat16");
   CG_REQUIRE(valid_extent(rows, outer, inner), "cg_linear_forward: bad shape");
-  CG_REQUIRE(activation >= kNone && activation <= kSilu, "cg_linear_forward: unknown activation");
+  CG_REQUIRE(activation >= kActNone && activation <= kActSilu, "cg_linear_forward: unknown activation");
   CG_REQUIRE(x_stride >= inner && weight_stride >= inner && (!residual || residual_stride >= outer),
              "cg_linear_forward: stride smaller than a row");
   if (rows == 0 || outer == 0) return CG_OK;
   CG_REQUIRE(y && (inner == 0 || (x && weight)), "cg_linear_forward: NULL pointer");
-  (void)workspace;
-  (void)workspace_bytes;
-  const Epilogue e = {bias, residual, pre, residual_stride, outer, activation};
+  const Layout l = plan_layout(x, x_stride, weight, weight_stride, nullptr, 0, dtype, rows, inner, outer, activation, false);
+  if (workspace_bytes < l.bytes || (l.bytes && !workspace))
+    return set_error(CG_ERR_WORKSPACE, "cg_linear_forward: workspace too small");
+  const ProductEpilogue e = {bias, residual, pre, y, residual_stride, outer, activation};
+  char* w = static_cast<char*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (dtype == CG_F32) return forward<float>(x, x_stride, weight, weight_stride, rows, inner, outer, e, y, s);
-  if (dtype == CG_F16) return forward<__half>(x, x_stride, weight, weight_stride, rows, inner, outer, e, y, s);
-  return forward<__nv_bfloat16>(x, x_stride, weight, weight_stride, rows, inner, outer, e, y, s);
+  if (rows <= kFewRows) return run_few_rows(x, x_stride, weight, weight_stride, rows, inner, outer, dtype, e, s);
+  if (dtype == CG_F32) return forward<float>(l, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, e, w, s);
+  if (dtype == CG_F16) return forward<__half>(l, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, e, w, s);
+  return forward<__nv_bfloat16>(l, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, e, w, s);
 }
 
 extern "C" int cg_linear_backward(const void* dy, int64_t dy_stride, const void* pre, const void* x, int64_t x_stride,
@@ -240,22 +279,25 @@ extern "C" int cg_linear_backward(const void* dy, int64_t dy_stride, const void*
   using namespace cg;
   CG_REQUIRE(valid_dtype(dtype), "cg_linear_backward: dtype must be float32, float16 or bfloat16");
   CG_REQUIRE(valid_extent(rows, outer, inner), "cg_linear_backward: bad shape");
-  CG_REQUIRE(activation >= kNone && activation <= kSilu, "cg_linear_backward: unknown activation");
+  CG_REQUIRE(activation >= kActNone && activation <= kActSilu, "cg_linear_backward: unknown activation");
   CG_REQUIRE(dy_stride >= outer && x_stride >= inner && weight_stride >= inner,
              "cg_linear_backward: stride smaller than a row");
-  CG_REQUIRE(rows == 0 || outer == 0 || (dy && (activation == kNone || pre)), "cg_linear_backward: NULL pointer");
-  if (!workspace || workspace_bytes < workspace_bytes_of(dtype, rows, outer, true))
+  CG_REQUIRE(rows == 0 || outer == 0 || (dy && (activation == kActNone || pre)), "cg_linear_backward: NULL pointer");
+  const Layout l = plan_layout(x, x_stride, weight, weight_stride, dy, dy_stride, dtype, rows, inner, outer, activation, true);
+  if (workspace_bytes < l.bytes || (l.bytes && !workspace))
     return set_error(CG_ERR_WORKSPACE, "cg_linear_backward: workspace too small");
   char* w = static_cast<char*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (inner == 0) dx = dweight = nullptr;
+  if (rows == 0) dx = nullptr;
   if (outer == 0) dweight = dbias = nullptr;
+  CG_REQUIRE((!dx || weight || outer == 0) && (!dweight || x || rows == 0), "cg_linear_backward: NULL pointer");
   if (dtype == CG_F32)
-    return backward<float>(dy, dy_stride, pre, x, x_stride, weight, weight_stride, rows, inner, outer, activation, dx, dweight,
-                           dbias, w, s);
+    return backward<float>(l, dy, dy_stride, pre, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, activation, dx,
+                           dweight, dbias, w, s);
   if (dtype == CG_F16)
-    return backward<__half>(dy, dy_stride, pre, x, x_stride, weight, weight_stride, rows, inner, outer, activation, dx, dweight,
-                            dbias, w, s);
-  return backward<__nv_bfloat16>(dy, dy_stride, pre, x, x_stride, weight, weight_stride, rows, inner, outer, activation, dx,
-                                 dweight, dbias, w, s);
+    return backward<__half>(l, dy, dy_stride, pre, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, activation, dx,
+                            dweight, dbias, w, s);
+  return backward<__nv_bfloat16>(l, dy, dy_stride, pre, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, activation,
+                                 dx, dweight, dbias, w, s);
 }

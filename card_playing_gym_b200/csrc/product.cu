@@ -1,0 +1,472 @@
+// C[i, j] = sum_k A(i, k) B(j, k) on the tensor cores, with the linear layer's epilogue.
+//
+// Pairs of CTAs on two SMs compute 256 x tile_n outputs: one tcgen05.mma.cta_group::2 (M = 256, K = 16) reads each
+// CTA's own 128 rows of A and its half of B's tile_n rows from its own shared memory, so a stage of 64 k's is 32 KB per
+// SM for 2 x 256 x 256 x 64 FMAs, and each CTA's tensor memory receives its own 128 rows. The kernel is persistent: tensor
+// memory holds two accumulators, and the epilogue of one tile runs while the next is multiplied.
+//   warps 0-7  epilogue: tensor memory -> registers -> a 4 KB shared-memory square per warp -> rows of four columns a lane,
+//              so that bias, residual and results move in whole sectors whatever the strides
+//   warp 8     lane 0 fills the ring of six stages by TMA (128-byte swizzle; both operand orders, so neither product of
+//              the backward pass transposes anything in memory)
+//   warp 9     allocates tensor memory; in the even CTA lane 0 issues the MMAs
+// Loads of both CTAs complete on the even CTA's barriers; MMA completions are committed to both CTAs'.
+//
+// float32 operands are three bfloat16 parts each (8 bits of mantissa apiece, the parts exact): the six products of
+// parts that reach 2^-24 of the result run as one longer sum, the smallest first, at 6/1 of the bfloat16 work. The
+// tensor cores cut their running sum at each step (measured: 1.7e-8 of it, always toward zero), which a long
+// float32 sum would show: after kChunkBlocks blocks of k the epilogue takes the sum into registers, where it is
+// added with rounding, and the next chunk starts from zero in the other accumulator. 16-bit results keep one
+// running sum: at 8192 k's the cut is 9e-6 against their own rounding of 2^-11 or 2^-8.
+//
+// Where the tiles do not fill the chip's pairs, k is split: every split writes fp32 partial sums and
+// product_join_kernel adds them in order and applies the epilogue.
+#include "product.h"
+
+#include <cuda.h>
+
+#include <algorithm>
+
+#include "elements.cuh"
+#include "tcgen05.cuh"
+
+namespace cg {
+namespace {
+
+constexpr int kTileM = 256, kTileK = 64;  // a pair's rows; k's of a stage (128 bytes of 16-bit entries)
+constexpr int kStages = 6;
+constexpr int kHalfBytes = 128 * kTileK * 2;  // one CTA's A (or B at tile_n 256) of a stage
+constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kEpilogueWarps = 8;
+constexpr int kLoadWarp = 8, kMmaWarp = 9;
+constexpr int kThreads = 10 * 32;
+constexpr int kSquareBytes = 32 * 32 * 4;
+constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSquareBytes + 1024;
+constexpr int kAccumulatorColumns = 256;
+constexpr int kBoxRows = 64;          // rows of a box of an operand stored across
+constexpr int kLeastSplitBlocks = 8;  // k blocks a split is worth: its partial tile costs 512 KB of traffic
+constexpr int kChunkBlocks = 4;       // k blocks (256 k's) of one running sum of a float32 product: 16 steps a part
+constexpr int kParts = 6;             // products of parts of a float32 product
+
+// The pairs of parts of a float32 product, smallest first.
+__device__ __constant__ signed char kPartA[kParts] = {2, 0, 1, 1, 0, 0};
+__device__ __constant__ signed char kPartB[kParts] = {0, 2, 1, 0, 1, 0};
+
+struct Params {
+  int64_t rows, cols;
+  int tile_n, tiles_i, tiles_j, blocks, splits, per_split;
+  int chunk;  // blocks of one running sum; for float32 its k blocks times the parts
+  uint32_t instruction;
+  int across_a, across_b;
+  float* partial;
+  int64_t partial_stride;
+  ProductEpilogue e;
+};
+
+struct Item {
+  int i, j, split, first, last;
+};
+
+// Tiles go in groups of eight columns, down the rows inside a group, so that the pairs working at one time share
+// their operands in L2.
+__device__ __forceinline__ Item item_of(const Params& p, int index) {
+  Item t;
+  const int tiles = p.tiles_i * p.tiles_j;
+  t.split = index / tiles;
+  const int tile = index % tiles;
+  const int group = tile / (8 * p.tiles_i);
+  const int width = min(8, p.tiles_j - group * 8);
+  const int inside = tile - group * 8 * p.tiles_i;
+  t.i = inside / width;
+  t.j = group * 8 + inside % width;
+  t.first = t.split * p.per_split;
+  t.last = min(t.first + p.per_split, p.blocks);
+  return t;
+}
+
+// K-major, 128-byte swizzle: eight-row atoms of 1024 bytes; a K = 16 step is 32 bytes along the row.
+// Across (MN-major): 64 i's by 8 k's per atom, k groups 1024 bytes apart, the next 64 i's a box (64 k's) further.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t address, bool across) {
+  uint64_t d = (address >> 4) & 0x3FFFu;
+  d |= static_cast<uint64_t>(across ? (kBoxRows * 128) >> 4 : 1) << 16;
+  d |= static_cast<uint64_t>(1024 >> 4) << 32;
+  d |= static_cast<uint64_t>(1) << 46;
+  d |= static_cast<uint64_t>(2) << 61;
+  return d;
+}
+
+__device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t barrier) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], "
+      "[%5];" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(z), "r"(barrier)
+      : "memory");
+}
+
+// Four columns of one row: the fp32 sums to their place.
+template <typename T>
+__device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int64_t j, int64_t cols, const float (&bias)[4],
+                                        bool aligned, float (&z)[4]) {
+  const int n = static_cast<int>(min(static_cast<int64_t>(4), cols - j));
+  const bool whole = aligned && n == 4;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) z[k] += bias[k];
+  if (e.pre) store4(static_cast<T*>(e.pre) + i * cols + j, n, whole, z);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) z[k] = activate(z[k], e.activation);
+  if (e.residual) {
+    float r[4];
+    load4(static_cast<const T*>(e.residual) + i * e.residual_stride + j, n, whole, r);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) z[k] += r[k];
+  }
+  store4(static_cast<T*>(e.out) + i * e.out_stride + j, n, whole, z);
+}
+
+template <typename T>
+__device__ __forceinline__ void load_bias(const ProductEpilogue& e, int64_t j, int64_t cols, float (&bias)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bias[k] = e.bias && j + k < cols ? as_float(static_cast<const T*>(e.bias)[j + k]) : 0.f;
+}
+
+template <typename T>
+__device__ __forceinline__ bool epilogue_aligned(const ProductEpilogue& e, int64_t cols) {
+  return aligned4<T>(e.out, e.out_stride) && (!e.residual || aligned4<T>(e.residual, e.residual_stride)) &&
+         (!e.pre || aligned4<T>(e.pre, cols));
+}
+
+template <typename T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ Params p) {
+  extern __shared__ unsigned char smem_raw[];
+  __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
+  __shared__ uint32_t tmem_slot;
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = tc::cluster_ctarank();
+  constexpr bool kPromote = sizeof(T) == 4;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      tc::bar_init(&full[s], 1);
+      tc::bar_init(&empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      tc::bar_init(&acc_full[s], 1);
+      tc::bar_init(&acc_empty[s], 2 * kEpilogueWarps);
+    }
+    tc::bar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    tc::tmem_alloc_pair(&tmem_slot, 512);
+    tc::tmem_relinquish_pair();
+  }
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();  // barriers and tensor memory are ready in both CTAs
+  tc::fence_after_sync();
+  const uint32_t tmem = tmem_slot;
+  const int items = p.tiles_i * p.tiles_j * p.splits;
+  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const int half_n = p.tile_n / 2;
+  bool ok = true;
+
+  if (warp == kLoadWarp) {
+    if (lane == 0) {
+      const uint32_t bytes = kHalfBytes + half_n * kTileK * 2;
+      int stage = 0;
+      uint32_t lap = 0;
+      for (int index = pair; index < items && ok; index += pairs) {
+        const Item t = item_of(p, index);
+        const int i0 = t.i * kTileM + static_cast<int>(rank) * 128;
+        const int j0 = t.j * p.tile_n + static_cast<int>(rank) * half_n;
+        for (int b = t.first; b < t.last; ++b) {
+          if (lap > 0 && !(ok = tc::bar_wait(&empty[stage], (lap - 1) & 1u, 0x500))) break;
+          int k0 = b * kTileK, part_a = 0, part_b = 0;
+          if (kPromote) {
+            const int deep = p.chunk / kParts, chunk = b / p.chunk, inside = b - chunk * p.chunk;
+            const int segment = inside / deep;
+            k0 = (chunk * deep + inside - segment * deep) * kTileK;
+            part_a = kPartA[segment], part_b = kPartB[segment];
+          }
+          const uint32_t at = tc::smem_u32(smem + stage * kStageBytes);
+          const uint32_t barrier = tc::map_shared(tc::smem_u32(&full[stage]), 0);
+          if (rank == 0) tc::bar_expect_tx(&full[stage], 2 * bytes);
+          if (p.across_a) {
+            for (int c = 0; c < 2; ++c) load_box(at + c * kBoxRows * 128, &map_a, i0 + c * 64, k0, part_a, barrier);
+          } else {
+            load_box(at, &map_a, k0, i0, part_a, barrier);
+          }
+          if (p.across_b) {
+            for (int c = 0; c < half_n / 64; ++c)
+              load_box(at + kHalfBytes + c * kBoxRows * 128, &map_b, j0 + c * 64, k0, part_b, barrier);
+          } else {
+            load_box(at + kHalfBytes, &map_b, k0, j0, part_b, barrier);
+          }
+          if (++stage == kStages) {
+            stage = 0;
+            ++lap;
+          }
+        }
+      }
+      // Every stage that was filled has been read before this CTA leaves.
+      for (int s = 0; s < kStages && ok; ++s) {
+        const uint32_t fills = lap + (s < stage ? 1 : 0);
+        if (fills > 0) ok = tc::bar_wait(&empty[s], (fills - 1) & 1u, 0x501);
+      }
+    }
+  } else if (warp == kMmaWarp) {
+    if (lane == 0 && rank == 0) {
+      const uint32_t step_a = p.across_a ? (16 * 128) >> 4 : 32 >> 4, step_b = p.across_b ? (16 * 128) >> 4 : 32 >> 4;
+      int stage = 0, done = 0;  // running sums so far: they alternate between the accumulators
+      uint32_t lap = 0;
+      for (int index = pair; index < items && ok; index += pairs) {
+        const Item t = item_of(p, index);
+        for (int first = t.first; first < t.last && ok; first += p.chunk, ++done) {
+          const int s = done & 1, last = min(first + p.chunk, t.last);
+          if (done >= 2 && !(ok = tc::bar_wait_cluster(&acc_empty[s], ((done >> 1) - 1) & 1u, 0x502))) break;
+          tc::fence_after_sync();
+          const uint32_t accumulator = tmem + s * kAccumulatorColumns;
+          for (int b = first; b < last; ++b) {
+            if (!(ok = tc::bar_wait_cluster(&full[stage], lap & 1u, 0x503))) break;
+            tc::fence_after_sync();
+            const uint32_t at = tc::smem_u32(smem + stage * kStageBytes);
+            uint64_t da = operand_desc(at, p.across_a), db = operand_desc(at + kHalfBytes, p.across_b);
+#pragma unroll
+            for (int k = 0; k < kTileK / 16; ++k) {
+              tc::mma_bf16_pair(accumulator, da, db, p.instruction, b > first || k > 0);
+              da += step_a;
+              db += step_b;
+            }
+            tc::mma_commit_pair(&empty[stage]);
+            if (++stage == kStages) {
+              stage = 0;
+              ++lap;
+            }
+          }
+          if (ok) tc::mma_commit_pair(&acc_full[s]);
+        }
+      }
+    }
+  } else {
+    float4* square = reinterpret_cast<float4*>(smem + kStages * kStageBytes + warp * kSquareBytes);
+    const int quarter = warp & 3, half = warp >> 2;
+    const bool aligned = epilogue_aligned<T>(p.e, p.cols);
+    const int chunks = half_n / 32;  // 32-column chunks of this warp's half of the columns
+    int done = 0;
+    // The next running sum is complete; false where the wait ran out.
+    auto wait_sum = [&] {
+      ok = tc::bar_wait(&acc_full[done & 1], (done >> 1) & 1u, 0x504);
+      ok = __all_sync(0xffffffffu, ok);
+      tc::fence_after_sync();
+      return ok;
+    };
+    auto read_sum = [&](int c, float (&v)[32]) {
+      tc::tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (done & 1) * kAccumulatorColumns +
+                        (half * chunks + c) * 32,
+                    v);
+    };
+    // This warp has read all it needs of the running sum: its accumulator may be written again.
+    auto release_sum = [&] {
+      tc::fence_before_sync();
+      __syncwarp();
+      if (lane == 0) tc::bar_arrive_cluster(tc::map_shared(tc::smem_u32(&acc_empty[done & 1]), 0));
+      ++done;
+    };
+    for (int index = pair; index < items && ok; index += pairs) {
+      const Item t = item_of(p, index);
+      const int64_t i0 = static_cast<int64_t>(t.i) * kTileM + rank * 128 + quarter * 32;
+      const int64_t tile_j = static_cast<int64_t>(t.j) * p.tile_n;
+      // 32 rows by 32 columns of sums, a row a lane, to their place.
+      auto store_sums = [&](int c, const float (&v)[32]) {
+        const int column = (half * chunks + c) * 32;
+        const int64_t j = tile_j + column + (lane & 7) * 4;
+        if (i0 >= p.rows || tile_j + column >= p.cols) return;
+#pragma unroll
+        for (int q = 0; q < 8; ++q)
+          square[lane * 8 + (q ^ (lane & 7))] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+        __syncwarp();
+        float bias[4];
+        load_bias<T>(p.e, j, p.cols, bias);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const int row = r * 4 + (lane >> 3);
+          const float4 f = square[row * 8 + ((lane & 7) ^ (row & 7))];
+          float z[4] = {f.x, f.y, f.z, f.w};
+          if (i0 + row >= p.rows || j >= p.cols) continue;
+          if (p.partial)
+            *reinterpret_cast<float4*>(p.partial + (t.split * p.rows + i0 + row) * p.partial_stride + j) = f;
+          else
+            finish4<T>(p.e, i0 + row, j, p.cols, bias, aligned, z);
+        }
+        __syncwarp();
+      };
+      if constexpr (kPromote) {
+        float sums[4][32];
+        for (int first = t.first; first < t.last && ok; first += p.chunk) {
+          if (!wait_sum()) break;
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            if (c >= chunks) continue;
+            float v[32];
+            read_sum(c, v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) sums[c][k] = first == t.first ? v[k] : sums[c][k] + v[k];
+          }
+          release_sum();
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          if (c < chunks) store_sums(c, sums[c]);
+      } else {
+        if (!wait_sum()) break;
+        for (int c = 0; c < chunks; ++c) {
+          float v[32];
+          read_sum(c, v);
+          if (c == chunks - 1) release_sum();
+          store_sums(c, v);
+        }
+      }
+    }
+  }
+  if (!ok) {
+    // A wait ran out: give copies in flight time to land before the shared memory goes.
+    const uint64_t start = tc::now_ns();
+    while (tc::now_ns() - start < 10000000ull) {
+    }
+  }
+  __syncwarp();
+  tc::fence_before_sync();
+  __syncthreads();
+  tc::cluster_sync();
+  tc::fence_after_sync();
+  if (warp == kMmaWarp) tc::tmem_dealloc_pair(tmem, 512);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256) product_join_kernel(const float* partial, int64_t partial_stride, int splits, int64_t rows,
+                                                           int64_t cols, const ProductEpilogue e) {
+  const bool aligned = epilogue_aligned<T>(e, cols);
+  const int64_t quads = (cols + 3) / 4, total = rows * quads;
+  for (int64_t index = blockIdx.x * 256ll + threadIdx.x; index < total; index += gridDim.x * 256ll) {
+    const int64_t i = index / quads, j = (index - i * quads) * 4;
+    float z[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int s = 0; s < splits; ++s) {
+      const float4 f = *reinterpret_cast<const float4*>(partial + (s * rows + i) * partial_stride + j);
+      z[0] += f.x, z[1] += f.y, z[2] += f.z, z[3] += f.w;
+    }
+    float bias[4];
+    load_bias<T>(e, j, cols, bias);
+    finish4<T>(e, i, j, cols, bias, aligned, z);
+  }
+}
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+  static EncodeTiled found = [] {
+    void* entry = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &entry, 12000, cudaEnableDefault, &result) != cudaSuccess ||
+        result != cudaDriverEntryPointSuccess)
+      entry = nullptr;
+    return reinterpret_cast<EncodeTiled>(entry);
+  }();
+  return found;
+}
+
+// The map of an operand: [parts][outer][inner] with boxes of 64 inner entries by `box` rows.
+int make_map(CUtensorMap* map, const ProductOperand& o, int64_t inner, int64_t outer, int parts, int box, bool half) {
+  EncodeTiled encode = encode_tiled();
+  if (!encode) return set_error(CG_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+  CG_REQUIRE((reinterpret_cast<uintptr_t>(o.base) & 15) == 0 && o.stride % 8 == 0 && o.part % 8 == 0,
+             "run_product: operands must be aligned to 16 bytes");
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(inner), static_cast<cuuint64_t>(outer), static_cast<cuuint64_t>(parts)};
+  const cuuint64_t row_bytes = static_cast<cuuint64_t>(std::max(o.stride, inner)) * 2;
+  const cuuint64_t strides[2] = {(row_bytes + 15) & ~cuuint64_t{15},
+                                 parts > 1 ? static_cast<cuuint64_t>(o.part) * 2 : (row_bytes + 15) & ~cuuint64_t{15}};
+  const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
+  const CUresult rc = encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                             const_cast<void*>(o.base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (rc != CUDA_SUCCESS) return set_error(CG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
+  return CG_OK;
+}
+
+template <typename T>
+int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, int64_t cols, int64_t depth, int dtype,
+              const ProductEpilogue& e, float* partial, cudaStream_t stream) {
+  const ProductPlan plan = plan_product(rows, cols, depth, dtype);
+  if (plan.blocks > 0) {
+    const bool half = dtype == CG_F16;
+    const int parts = dtype == CG_F32 ? 3 : 1;
+    CUtensorMap map_a, map_b;
+    if (int rc = make_map(&map_a, a, a.across ? rows : depth, a.across ? depth : rows, parts, a.across ? kBoxRows : 128, half))
+      return rc;
+    if (int rc = make_map(&map_b, b, b.across ? cols : depth, b.across ? depth : cols, parts,
+                          b.across ? kBoxRows : plan.tile_n / 2, half))
+      return rc;
+    Params p;
+    p.rows = rows, p.cols = cols;
+    p.tile_n = plan.tile_n, p.tiles_i = plan.tiles_i, p.tiles_j = plan.tiles_j;
+    p.blocks = plan.blocks, p.splits = plan.splits, p.per_split = plan.per_split, p.chunk = plan.chunk;
+    p.across_a = a.across, p.across_b = b.across;
+    // fp32 accumulator; A and B both float16 or both bfloat16; the transpose bits say "across".
+    p.instruction = (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (a.across ? 1u << 15 : 0u) | (b.across ? 1u << 16 : 0u) |
+                    (static_cast<uint32_t>(plan.tile_n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
+    p.partial = plan.splits > 1 ? partial : nullptr;
+    p.partial_stride = plan.partial_stride;
+    p.e = e;
+    static const cudaError_t configured =
+        cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+    if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel: %s", cudaGetErrorString(configured));
+    const int items = plan.tiles_i * plan.tiles_j * plan.splits;
+    const int pairs = std::min(items, sm_count() / 2);
+    product_kernel<T><<<2 * pairs, kThreads, kSmemBytes, stream>>>(map_a, map_b, p);
+    if (int rc = check_launch("product_kernel")) return rc;
+    if (plan.splits == 1) return CG_OK;
+  }
+  const int64_t quads = rows * ((cols + 3) / 4);
+  const int blocks = static_cast<int>(std::min<int64_t>((quads + 255) / 256, 16 * sm_count()));
+  product_join_kernel<T><<<blocks, 256, 0, stream>>>(partial, plan.partial_stride, plan.blocks > 0 ? plan.splits : 0, rows, cols, e);
+  return check_launch("product_join_kernel");
+}
+
+}  // namespace
+
+ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
+  ProductPlan plan = {};
+  plan.tile_n = cols > 128 ? 256 : 128;
+  plan.tiles_i = static_cast<int>((rows + kTileM - 1) / kTileM);
+  plan.tiles_j = static_cast<int>((cols + plan.tile_n - 1) / plan.tile_n);
+  const int64_t pairs = 74;  // the B200's 148 SMs
+  const int64_t k_blocks = (depth + kTileK - 1) / kTileK, tiles = static_cast<int64_t>(plan.tiles_i) * plan.tiles_j;
+  // A split is a whole number of units: one k block, or a float32 chunk.
+  const int64_t unit_blocks = dtype == CG_F32 ? std::max<int64_t>(1, std::min<int64_t>(kChunkBlocks, k_blocks)) : 1;
+  const int64_t unit = unit_blocks * (dtype == CG_F32 ? kParts : 1), units = (k_blocks + unit_blocks - 1) / unit_blocks;
+  int64_t splits = 1;
+  if (tiles > 0 && 2 * tiles <= pairs) splits = std::min(pairs / tiles, units * unit / kLeastSplitBlocks);
+  splits = std::max<int64_t>(1, std::min(splits, units));
+  const int64_t units_each = units > 0 ? (units + splits - 1) / splits : 1;
+  plan.blocks = static_cast<int>(units * unit);
+  plan.per_split = static_cast<int>(units_each * unit);
+  plan.splits = units > 0 ? static_cast<int>((units + units_each - 1) / units_each) : 1;
+  plan.chunk = dtype == CG_F32 ? static_cast<int>(unit) : std::max(1, plan.per_split);
+  plan.partial_stride = (cols + 3) / 4 * 4;
+  plan.partial_bytes = plan.splits > 1 ? plan.splits * rows * plan.partial_stride * 4 : 0;
+  return plan;
+}
+
+int run_product(const ProductOperand& a, const ProductOperand& b, int64_t rows, int64_t cols, int64_t depth, int dtype,
+                const ProductEpilogue& e, void* partial, cudaStream_t stream) {
+  if (rows == 0 || cols == 0) return CG_OK;
+  auto* sums = static_cast<float*>(partial);
+  if (dtype == CG_F32) return run_typed<float>(a, b, rows, cols, depth, dtype, e, sums, stream);
+  if (dtype == CG_F16) return run_typed<__half>(a, b, rows, cols, depth, dtype, e, sums, stream);
+  return run_typed<__nv_bfloat16>(a, b, rows, cols, depth, dtype, e, sums, stream);
+}
+
+}  // namespace cg

@@ -26,27 +26,34 @@ def _row_stride(matrix: torch.Tensor) -> int:
     return max(matrix.stride(0), matrix.shape[1]) if matrix.shape[0] > 1 else matrix.shape[1]
 
 
-def _workspace(x, weight, dy, activation: int) -> torch.Tensor:
+def _workspace(x, weight, dy, activation: int) -> torch.Tensor | None:
     need = nat.query("cg_linear_workspace_bytes", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight),
                      nat.ptr(dy), 0 if dy is None else _row_stride(dy), nat.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1],
                      weight.shape[0], activation, 0 if dy is None else 1)
-    return torch.empty(max(need, 1), dtype=torch.uint8, device=x.device)
+    return torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+
+
+def _forward(x, weight, bias, residual, activation: int, keep: bool):
+    """(y, the sum before the activation where it is to be kept)."""
+
+    rows, inner = x.shape
+    outer = weight.shape[0]
+    with nat.on_device(x.device):
+        y = torch.empty((rows, outer), dtype=x.dtype, device=x.device)
+        pre = torch.empty_like(y) if keep else None
+        workspace = _workspace(x, weight, None, activation)
+        nat.call("cg_linear_forward", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight), nat.ptr(bias),
+                 nat.ptr(residual), 0 if residual is None else _row_stride(residual), nat.DTYPE_CODES[x.dtype], rows,
+                 inner, outer, activation, nat.ptr(y), nat.ptr(pre), nat.ptr(workspace),
+                 0 if workspace is None else workspace.numel(), nat.stream_handle(x.device))
+    return y, pre
 
 
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation):
-        rows, inner = x.shape
-        outer = weight.shape[0]
         trains = any(ctx.needs_input_grad[:3])
-        with torch.cuda.device(x.device):
-            y = torch.empty((rows, outer), dtype=x.dtype, device=x.device)
-            pre = torch.empty_like(y) if trains and activation else None
-            workspace = _workspace(x, weight, None, activation)
-            nat.call("cg_linear_forward", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight),
-                     nat.ptr(bias), nat.ptr(residual), 0 if residual is None else _row_stride(residual),
-                     nat.DTYPE_CODES[x.dtype], rows, inner, outer, activation, nat.ptr(y), nat.ptr(pre),
-                     nat.ptr(workspace), workspace.numel(), nat.stream_handle(x.device))
+        y, pre = _forward(x, weight, bias, residual, activation, trains and activation != 0)
         if trains:
             ctx.save_for_backward(x, weight, pre)
         ctx.activation = activation
@@ -61,7 +68,7 @@ class _Linear(torch.autograd.Function):
             rows, inner = x.shape
             outer = weight.shape[0]
             g = _unit_rows(dy)
-            with torch.cuda.device(x.device):
+            with nat.on_device(x.device):
                 dx = torch.empty((rows, inner), dtype=x.dtype, device=x.device) if needs_x else None
                 dweight = torch.empty((outer, inner), dtype=x.dtype, device=x.device) if needs_weight else None
                 dbias = torch.empty(outer, dtype=x.dtype, device=x.device) if needs_bias else None
@@ -69,7 +76,7 @@ class _Linear(torch.autograd.Function):
                 nat.call("cg_linear_backward", nat.ptr(g), _row_stride(g), nat.ptr(pre), nat.ptr(x), _row_stride(x),
                          nat.ptr(weight), _row_stride(weight), nat.DTYPE_CODES[x.dtype], rows, inner, outer,
                          ctx.activation, nat.ptr(dx), nat.ptr(dweight), nat.ptr(dbias), nat.ptr(workspace),
-                         workspace.numel(), nat.stream_handle(x.device))
+                         0 if workspace is None else workspace.numel(), nat.stream_handle(x.device))
         return dx, dweight, dbias, dy if needs_residual else None, None
 
 
@@ -104,6 +111,10 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
     if x.dim() != 2:
         x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty((shape[:-1].numel(), 0))
         residual = None if residual is None else residual.reshape(x.shape[0], outer)
-    y = _Linear.apply(_unit_rows(x), _unit_rows(weight), None if bias is None else bias.contiguous(),
-                      None if residual is None else _unit_rows(residual), ACTIVATIONS[activation])
+    inputs = (_unit_rows(x), _unit_rows(weight), None if bias is None else bias.contiguous(),
+              None if residual is None else _unit_rows(residual))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):
+        y = _Linear.apply(*inputs, ACTIVATIONS[activation])
+    else:
+        y, _ = _forward(*inputs, ACTIVATIONS[activation], False)
     return y if len(shape) == 2 else y.view(shape)

@@ -167,7 +167,7 @@ class AdamW(torch.optim.Optimizer):
             entry.beta1, entry.beta2 = group["betas"]
         need = nat.query("cg_adamw_workspace_bytes", len(table)) if self.max_norm else 0
         second = flat["exp_avg_sq" if self.state_bits == 32 else "exp_avg_sq_root"]
-        with torch.cuda.device(device):
+        with nat.on_device(device):
             workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
             nat.call("cg_adamw_step", table, len(table), nat.DTYPE_CODES[dtype], self._groups, len(self._groups),
                      self.state_bits, nat.ptr(flat["exp_avg"]), nat.ptr(flat.get("exp_avg_scale")), nat.ptr(second),

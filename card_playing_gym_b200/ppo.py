@@ -261,7 +261,7 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
         grad = torch.empty((rows, grad_stride), dtype=logits.dtype, device=logits.device)[:, :width]
     totals = torch.empty(len(ANCHORED_KEYS), device=logits.device)
     need = nat.query("cg_anchored_objective_workspace_bytes", rows)
-    with torch.cuda.device(logits.device):
+    with nat.on_device(logits.device):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
         nat.call("cg_anchored_objective", nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], rows, width, stride,
                  nat.ptr(reference_logits), 0 if reference_logits is None else _row_stride(reference_logits),
@@ -339,7 +339,7 @@ def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, legal: torc
     logits, actions, legal = _logits_and_mask(logits.detach(), actions, legal)
     rows, width = logits.shape
     out = torch.empty(rows, device=logits.device)
-    with torch.cuda.device(logits.device):
+    with nat.on_device(logits.device):
         nat.call("cg_action_log_probs", nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], rows, width,
                  _row_stride(logits), nat.ptr(legal), 0 if legal is None else _row_stride(legal), nat.ptr(actions),
                  nat.ptr(out), nat.stream_handle(logits.device))
