@@ -6,17 +6,19 @@
 //   KL = sum p (lp - lr)                       with the reference's logits, or
 //   KL = exp(u) - u - 1, u = lr_a - lp_a       with the reference's log-probability of the action alone
 //   L = sum_i w (surr + beta KL - alpha [|S| > 1] H / log |S|)
-//   dL/dz_j = p_j (K0 + w beta ((z_j - r_j) - (max z - max r)) + w alpha' (z_j - max z)) + [j = a] w c
+//   dL/dz_j = p_j (K0 + w beta (z_j - r_j) + w alpha' (z_j - max z)) + [j = a] w c
 // with c = d surr / d ratio * ratio (+ beta (1 - exp(u))), alpha' = alpha / log |S| and
-//   K0 = w (-c - beta (KL + log s - log t) + alpha' (H - log s)),
+//   K0 = w (-c - beta (KL + log s - log t + max z - max r) + alpha' (H - log s)),
 // s and t the sums of exp(z - max z) and exp(r - max r). The differences from the maxima are what keeps KL and H,
 // sums of small terms, from cancelling against the large log-sum-exps. An illegal entry acts as a logit of minus
 // infinity, whatever it holds.
 //
-// All row arithmetic is fp32; the nine totals are summed in double in a fixed order and rounded once.
+// All row arithmetic is fp32. The totals are summed in fp32 over the rows of one thread (some tens) and in double
+// from there on, in a fixed order.
 #include <algorithm>
 
-#include "common.cuh"
+#include "elements.cuh"
+#include "tcgen05.cuh"
 
 namespace cg {
 namespace {
@@ -55,13 +57,6 @@ __device__ __forceinline__ float max_nan(float x, float y) {
   return m;
 }
 
-__device__ __forceinline__ float as_float(float v) { return v; }
-__device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void put(float* p, float v) { *p = v; }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
 // A row's sums over its legal entries.
 struct RowSums {
   float peak, sum;              // max z, sum e with e = exp(z - max z)
@@ -73,14 +68,14 @@ struct RowSums {
 
 // What the gradient pass needs of a row.
 struct RowGrad {
-  float inv_sum, constant, beta, alpha, shift, action;
+  float inv_sum, constant, beta, alpha, action;
 };
 
 // The row's contribution to the totals (zeros unless it counts) and its gradient's coefficients.
 // z_a: the action's logit, minus infinity where it is illegal.
 __device__ __forceinline__ RowGrad finish_row(const Args& a, int64_t row, const RowSums& s, float z_a, bool counts,
-                                              double (&acc)[kTotals]) {
-  RowGrad g = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+                                              float (&acc)[kTotals]) {
+  RowGrad g = {0.f, 0.f, 0.f, 0.f, 0.f};
   if (!counts) return g;
   const float w = a.weights[row], advantage = a.advantages[row];
   const float log_sum = logf(s.sum);
@@ -101,7 +96,6 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, int64_t row, const 
     log_apart = log_sum - logf(s.reference_sum);
     kl = s.apart * g.inv_sum - log_apart;
     g.beta = w * a.beta;
-    g.shift = s.peak - s.reference_peak;
   } else if (a.reference_action) {
     const float u = a.reference_action[row] - lp;
     kl = expf(u) - u - 1.f;
@@ -109,18 +103,17 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, int64_t row, const 
   }
   g.alpha = w * a.alpha * norm;
   g.action = w * slope;
-  g.constant = -g.action + g.alpha * (entropy - log_sum) - g.beta * (kl + log_apart);
+  g.constant = -g.action + g.alpha * (entropy - log_sum) - g.beta * (kl + log_apart + (s.peak - s.reference_peak));
   const float objective = surrogate + a.beta * kl - a.alpha * norm * entropy;
-  const double wd = w;
-  acc[0] += wd * surrogate;
-  acc[1] += wd;
-  acc[2] += wd * entropy;
-  acc[3] += wd * (norm * entropy);
-  acc[4] += eligible ? wd : 0.0;
-  acc[5] += fabsf(ratio - 1.f) > a.clip ? wd : 0.0;
-  acc[6] += wd * (ratio - 1.f - log_ratio);
-  acc[7] += wd * kl;
-  acc[8] += wd * objective;
+  acc[0] += w * surrogate;
+  acc[1] += w;
+  acc[2] += w * entropy;
+  acc[3] += w * (norm * entropy);
+  acc[4] += eligible ? w : 0.f;
+  acc[5] += fabsf(ratio - 1.f) > a.clip ? w : 0.f;
+  acc[6] += w * (ratio - 1.f - log_ratio);
+  acc[7] += w * kl;
+  acc[8] += w * objective;
   return g;
 }
 
@@ -142,12 +135,523 @@ __device__ __forceinline__ bool row_counts(const Args& a, int64_t row, int64_t a
   return a.weights[row] != 0.f;
 }
 
-__device__ __forceinline__ float gradient_entry(const RowGrad& g, const RowSums& s, float z, float r, bool exact) {
-  const float from_peak = z - s.peak;
+// dL/dz of an entry that is not the action. A probability of zero has a zero gradient whatever it is multiplied by.
+__device__ __forceinline__ float gradient_entry(const RowGrad& g, float peak, float z, float r, bool exact) {
+  const float from_peak = z - peak;
   const float p = exp2_fast(from_peak * kLog2e) * g.inv_sum;
   float k = fmaf(g.alpha, from_peak, g.constant);
-  if (exact) k = fmaf(g.beta, (z - r) - g.shift, k);
-  return p == 0.f ? 0.f : p * k;  // a probability of zero times an infinite difference
+  if (exact) k = fmaf(g.beta, z - r, k);
+  return p == 0.f ? 0.f : p * k;
+}
+
+// One entry's part of a row's sums.
+__device__ __forceinline__ void add_entry(RowSums& s, float z, float r, bool exact) {
+  const float from_peak = z - s.peak;
+  const float e = exp2_fast(from_peak * kLog2e);
+  s.sum += e;
+  if (exact) {
+    const float reference_from_peak = r - s.reference_peak;
+    s.reference_sum += exp2_fast(reference_from_peak * kLog2e);
+    if (e != 0.f) s.apart = fmaf(e, from_peak - reference_from_peak, s.apart);
+  }
+  if (e != 0.f) s.spread = fmaf(e, from_peak, s.spread);
+}
+
+// Sixteen bytes of a row as floats and back.
+template <typename T>
+constexpr int kVector = 16 / static_cast<int>(sizeof(T));
+
+__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[4]) {
+  v[0] = __uint_as_float(raw.x), v[1] = __uint_as_float(raw.y), v[2] = __uint_as_float(raw.z), v[3] = __uint_as_float(raw.w);
+}
+__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[8], __half) {
+  const __half2* h = reinterpret_cast<const __half2*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x, v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[8], __nv_bfloat16) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[2 * i] = __uint_as_float(w[i] << 16), v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+}
+__device__ __forceinline__ void unpack(const uint4& raw, float (&v)[4], float) { unpack(raw, v); }
+__device__ __forceinline__ uint4 repack(const float (&v)[4], float) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+template <typename T>
+__device__ __forceinline__ uint4 repack(const float (&v)[8], T) {
+  uint4 raw;
+  auto* h = reinterpret_cast<typename PairOf<T>::type*>(&raw);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) pair_from(h[i], v[2 * i], v[2 * i + 1]);
+  return raw;
+}
+
+// The largest entry of sixteen-byte units, a NaN if there is one. 16-bit entries are compared in pairs.
+template <typename T>
+struct UnitMax {
+  typename PairOf<T>::type top;
+  __device__ __forceinline__ UnitMax() { pair_from(top, -INFINITY, -INFINITY); }
+  __device__ __forceinline__ void take(const uint4& raw) {
+    const auto* h = reinterpret_cast<const typename PairOf<T>::type*>(&raw);
+    top = __hmax2_nan(top, __hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+  }
+  __device__ __forceinline__ float value() const {
+    const float2 f = pair_float(top);
+    return max_nan(f.x, f.y);
+  }
+};
+template <>
+struct UnitMax<float> {
+  float top = -INFINITY;
+  __device__ __forceinline__ void take(const uint4& raw) {
+    top = max_nan(top, max_nan(max_nan(__uint_as_float(raw.x), __uint_as_float(raw.y)),
+                               max_nan(__uint_as_float(raw.z), __uint_as_float(raw.w))));
+  }
+  __device__ __forceinline__ float value() const { return top; }
+};
+
+// Whether every row of a plane starts on sixteen bytes.
+template <typename T>
+__device__ __forceinline__ bool aligned_rows(const void* base, int64_t stride, int64_t rows) {
+  return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && (rows == 1 || stride * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+}
+
+// ---- up to 1024 entries: a row in the registers of four lanes or of a warp --------------------------------------------
+// A row has some 300 instructions of its own (reductions, logarithms, the ratio) beside 30 an entry, so rows of up to 64
+// entries take four lanes, eight rows a warp. The row is read once and written once,
+// and the grid is one resident wave of warps. Aligned rows move in vectors of sixteen bytes, a lane holding every
+// kLanes-th vector; others entry by entry, a lane holding every kLanes-th entry, so that both are coalesced.
+template <typename T, int kLanes, int kVectors>
+__global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
+  constexpr int kVec = kVector<T>, kPer = kVec * kVectors, kGroups = 32 / kLanes;
+  __shared__ double scratch[8][kTotals];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int group = lane / kLanes, l = lane % kLanes;
+  const uint32_t group_mask = kLanes == 32 ? 0xffffffffu : ((1u << (kLanes & 31)) - 1u) << (group * kLanes);
+  const bool exact = a.reference != nullptr;
+  const bool vectors = aligned_rows<T>(a.logits, a.stride, a.rows) &&
+                       (!exact || aligned_rows<T>(a.reference, a.reference_stride, a.rows)) &&
+                       (!a.grad || aligned_rows<T>(a.grad, a.grad_stride, a.rows)) &&
+                       (!a.legal || ((reinterpret_cast<uintptr_t>(a.legal) & (kVec - 1)) == 0 &&
+                                     (a.rows == 1 || a.legal_stride % kVec == 0)));
+  float acc[kTotals] = {};
+  // The entry of slot (v, e).
+  auto entry = [&](int v, int e) { return vectors ? (l + kLanes * v) * kVec + e : l + kLanes * (v * kVec + e); };
+  auto reduce = [&](float v, bool largest) {
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) {
+      const float other = __shfl_xor_sync(0xffffffffu, v, o);
+      v = largest ? max_nan(v, other) : v + other;
+    }
+    return v;
+  };
+  const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * kGroups;
+  const int64_t warp_first = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * kGroups;
+  // Every group of a warp runs the same iterations, so that the shuffles stay converged.
+  for (int64_t base = warp_first; base < a.rows; base += step) {
+    const int64_t row = base + group;
+    const bool live = row < a.rows;
+    const T* gz = static_cast<const T*>(a.logits) + row * a.stride;
+    const T* gr = exact ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
+    const uint8_t* gl = a.legal ? a.legal + row * a.legal_stride : nullptr;
+    const int64_t action = live ? a.actions[row] : -1;
+    // Illegal entries, and those past the row, are minus infinity.
+    float z[kPer], r[kPer], z_a = 0.f, count = 0.f;
+    bool mine = false;
+    if (vectors) {
+      uint4 raw_z[kVectors], raw_r[kVectors];
+      uint2 raw_l[kVectors];
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) {
+        const int j = (l + kLanes * v) * kVec;
+        raw_z[v] = raw_r[v] = make_uint4(0, 0, 0, 0);
+        raw_l[v] = make_uint2(0x01010101u, 0x01010101u);
+        if (!live || j + kVec > a.width) continue;
+        raw_z[v] = *reinterpret_cast<const uint4*>(gz + j);
+        if (exact) raw_r[v] = *reinterpret_cast<const uint4*>(gr + j);
+        if (gl) {
+          if constexpr (kVec == 4)
+            raw_l[v].x = *reinterpret_cast<const uint32_t*>(gl + j);
+          else
+            raw_l[v] = *reinterpret_cast<const uint2*>(gl + j);
+        }
+      }
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) {
+        const int j = (l + kLanes * v) * kVec;
+        float t[kVec], u[kVec];
+        uint32_t in[kVec];
+        if (live && j < a.width && j + kVec > a.width) {  // the row's last entries, fewer than a vector
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) {
+            const bool inside = j + e < a.width;
+            t[e] = inside ? as_float(gz[j + e]) : 0.f;
+            u[e] = inside && exact ? as_float(gr[j + e]) : 0.f;
+            in[e] = inside ? (gl ? gl[j + e] : 1u) : 0u;
+          }
+        } else {
+          unpack(raw_z[v], t, T());
+          unpack(raw_r[v], u, T());
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            in[e] = live && j < a.width ? (e < 4 ? raw_l[v].x : raw_l[v].y) >> (8 * (e & 3)) & 255u : 0u;
+        }
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const int k = v * kVec + e;
+          z[k] = in[e] ? t[e] : -INFINITY;
+          r[k] = in[e] ? u[e] : -INFINITY;
+          count += in[e] ? 1.f : 0.f;
+          if (in[e] && j + e == action) z_a = z[k], mine = true;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) {
+        const int j = l + kLanes * k;
+        const bool in = live && j < a.width && (!gl || gl[j]);
+        z[k] = in ? as_float(gz[j]) : -INFINITY;
+        r[k] = in && exact ? as_float(gr[j]) : -INFINITY;
+        count += in ? 1.f : 0.f;
+        if (in && j == action) z_a = z[k], mine = true;
+      }
+    }
+    RowSums s = {};
+    float peak = -INFINITY, reference_peak = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) {
+      peak = max_nan(peak, z[k]);
+      if (exact) reference_peak = max_nan(reference_peak, r[k]);
+    }
+    s.peak = reduce(peak, true);
+    if (exact) s.reference_peak = reduce(reference_peak, true);
+    s.count = reduce(count, false);
+    const bool action_legal = (__ballot_sync(0xffffffffu, mine) & group_mask) != 0;
+    z_a = reduce(z_a, false);  // one lane holds it
+    if (!action_legal) z_a = -INFINITY;
+    if (s.peak != -INFINITY) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) add_entry(s, z[k], exact ? r[k] : 0.f, exact);
+    }
+    s.sum = reduce(s.sum, false);
+    if (!a.log_probs) s.spread = reduce(s.spread, false);
+    if (exact) {
+      s.reference_sum = reduce(s.reference_sum, false);
+      s.apart = reduce(s.apart, false);
+    }
+    const bool counts = row_counts(a, row, action, s, z_a, action_legal, l == 0);
+    if (a.log_probs) {
+      if (live && l == 0) a.log_probs[row] = counts ? (z_a - s.peak) - logf(s.sum) : 0.f;
+      continue;
+    }
+    const RowGrad g = finish_row(a, row, s, z_a, counts, acc);  // every lane of the group keeps the same totals
+    if (!a.grad || !live) continue;
+    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+      float t[kVec];
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        const int k = v * kVec + e;
+        t[e] = counts ? gradient_entry(g, s.peak, z[k], exact ? r[k] : 0.f, exact) : 0.f;
+        if (counts && entry(v, e) == action) t[e] += g.action;
+      }
+      const int j = (l + kLanes * v) * kVec;
+      if (vectors && j + kVec <= a.width) {
+        *reinterpret_cast<uint4*>(out + j) = repack(t, T());
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e)
+          if (entry(v, e) < a.width) put(out + entry(v, e), t[e]);
+      }
+    }
+  }
+  if (a.log_probs) return;
+  // The groups' leaders in order, then the warps.
+#pragma unroll
+  for (int k = 0; k < kTotals; ++k) {
+    double total = acc[k];
+#pragma unroll
+    for (int other = 1; other < kGroups; ++other) {
+      total += __shfl_sync(0xffffffffu, acc[k], other * kLanes);
+    }
+    if (lane == 0) scratch[warp][k] = total;
+  }
+  __syncthreads();
+  if (threadIdx.x < kTotals) {
+    double total = 0;
+    for (int w = 0; w < 8; ++w) total += scratch[w][threadIdx.x];
+    a.partial[blockIdx.x * kTotals + threadIdx.x] = total;
+  }
+}
+
+// ---- wider rows: a row in the shared memory of a cluster --------------------------------------------------------------
+// The row is read once, by bulk copies, and stays in shared memory for its maxima, its sums and its gradient. A cluster
+// of C blocks holds it, C the least that leaves room for three blocks an SM (so that one block's copies run under
+// another's arithmetic); the blocks exchange their maxima and sums through each other's shared memory.
+// Slices are copied with the alignment they have in memory: the sixteen-byte units inside by the copy engine, the few
+// bytes at the ends by threads. The arithmetic runs over the same units; planes whose rows are aligned differently
+// from the logits' are read entry by entry from shared memory.
+constexpr int kWideThreads = 256;
+constexpr int kMaxCluster = 16;
+constexpr int kSlots = 4;
+
+// The bytes before the first sixteen-byte boundary of `bytes` bytes at `src`, and those in whole units after it.
+__device__ __forceinline__ uint32_t aligned_part(const void* src, int bytes, int* head) {
+  const int lead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15);
+  *head = min(lead, bytes);
+  return static_cast<uint32_t>((bytes - *head) & ~15);
+}
+
+__device__ __forceinline__ void store_remote(uint32_t address, float v) {
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
+}
+
+template <typename T, bool kExact>
+__global__ void __launch_bounds__(kWideThreads, 4) anchored_wide_kernel(const Args a, int slice, int clusters) {
+  constexpr int kVec = kVector<T>;
+  extern __shared__ __align__(16) unsigned char smem[];
+  __shared__ __align__(8) uint64_t arrived;
+  __shared__ float warp_values[kWideThreads / 32][kSlots], cluster_values[2][kMaxCluster][kSlots];
+  __shared__ float row_peak, row_reference_peak;
+  __shared__ RowGrad row_grad;
+  __shared__ bool row_live;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  uint32_t rank = 0, size = 1;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+  const int plane = slice * static_cast<int>(sizeof(T)) + 32;  // a slice and its misalignment
+  const int lo = static_cast<int>(rank) * slice;
+  const int n = max(0, min(slice, a.width - lo));
+  if (tid == 0) {
+    tc::bar_init(&arrived, 1);
+    tc::bar_fence_init();
+  }
+  __syncthreads();
+  if (size > 1) tc::cluster_sync();
+
+  // Values of every thread reduced over the cluster, the first `maxima` of them by maximum; the result is warp 0's.
+  auto reduce = [&](float (&v)[kSlots], int count, int maxima, int which) {
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+      if (k >= count) continue;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, v[k], o);
+        v[k] = k < maxima ? max_nan(v[k], other) : v[k] + other;
+      }
+      if (lane == 0) warp_values[warp][k] = v[k];
+    }
+    __syncthreads();
+    // Warp 0: lane w takes partial result w; a butterfly joins the first `m` lanes, a power of two.
+    auto join = [&](const float (*values)[kSlots], int m) {
+#pragma unroll
+      for (int k = 0; k < kSlots; ++k) {
+        if (k >= count) continue;
+        v[k] = values[lane & (m - 1)][k];
+        for (int o = m / 2; o > 0; o >>= 1) {
+          const float other = __shfl_xor_sync(0xffffffffu, v[k], o);
+          v[k] = k < maxima ? max_nan(v[k], other) : v[k] + other;
+        }
+      }
+    };
+    if (warp == 0) {
+      join(warp_values, kWideThreads / 32);
+      if (size > 1 && lane < static_cast<int>(size)) {
+#pragma unroll
+        for (int k = 0; k < kSlots; ++k)
+          if (k < count) store_remote(tc::map_shared(tc::smem_u32(&cluster_values[which][rank][k]), lane), v[k]);
+      }
+      __syncwarp();
+    }
+    if (size > 1) {
+      tc::cluster_sync();
+      if (warp == 0) join(cluster_values[which], static_cast<int>(size));
+    }
+  };
+
+  float acc[kTotals] = {};
+  uint32_t phase = 0;
+  for (int64_t row = blockIdx.x / size; row < a.rows; row += clusters) {
+    const T* gz = static_cast<const T*>(a.logits) + row * a.stride + lo;
+    const T* gr = kExact ? static_cast<const T*>(a.reference) + row * a.reference_stride + lo : nullptr;
+    const uint8_t* gl = a.legal ? a.legal + row * a.legal_stride + lo : nullptr;
+    const int64_t action = a.actions[row];
+    // Entry 0 of each plane, at its own misalignment.
+    unsigned char* pz = smem + (reinterpret_cast<uintptr_t>(gz) & 15);
+    unsigned char* pr = smem + plane + (reinterpret_cast<uintptr_t>(gr) & 15);
+    unsigned char* pl = smem + (kExact ? 2 : 1) * plane + (reinterpret_cast<uintptr_t>(gl) & 15);
+    const int bytes = n * static_cast<int>(sizeof(T));
+    int head_z, head_r = 0, head_l = 0;
+    const uint32_t inner_z = aligned_part(gz, bytes, &head_z);
+    const uint32_t inner_r = kExact ? aligned_part(gr, bytes, &head_r) : 0;
+    const uint32_t inner_l = gl ? aligned_part(gl, n, &head_l) : 0;
+    if (tid == 0) {
+      tc::fence_async_smem();  // what this block wrote to and read from the slices is done
+      tc::bar_expect_tx(&arrived, inner_z + inner_r + inner_l);
+      if (inner_z) tc::bulk_g2s(pz + head_z, reinterpret_cast<const unsigned char*>(gz) + head_z, inner_z, &arrived);
+      if (inner_r) tc::bulk_g2s(pr + head_r, reinterpret_cast<const unsigned char*>(gr) + head_r, inner_r, &arrived);
+      if (inner_l) tc::bulk_g2s(pl + head_l, gl + head_l, inner_l, &arrived);
+    }
+    auto copy_ends = [&](unsigned char* dst, const void* src, int total, int head, uint32_t inner) {
+      const unsigned char* from = static_cast<const unsigned char*>(src);
+      const int tail = total - head - static_cast<int>(inner);
+      if (tid < head) dst[tid] = from[tid];
+      if (tid >= 32 && tid < 32 + tail) dst[head + inner + tid - 32] = from[head + inner + tid - 32];
+    };
+    copy_ends(pz, gz, bytes, head_z, inner_z);
+    if (kExact) copy_ends(pr, gr, bytes, head_r, inner_r);
+    if (gl) copy_ends(pl, gl, n, head_l, inner_l);
+    __syncthreads();
+    tc::bar_wait(&arrived, phase, 0x422);
+    phase ^= 1;
+
+    T* z = reinterpret_cast<T*>(pz);
+    T* r = reinterpret_cast<T*>(pr);
+    const int head = head_z / static_cast<int>(sizeof(T));  // entries before the first unit
+    const int units = static_cast<int>(inner_z) / 16;
+    const int ends = n - units * kVec;  // entries outside the units, head first
+    const bool alike = !kExact || (reinterpret_cast<uintptr_t>(gz) & 15) == (reinterpret_cast<uintptr_t>(gr) & 15);
+    auto end_entry = [&](int k) { return k < head ? k : k + units * kVec; };
+    auto load_unit = [&](const T* base, int j, bool whole, float (&v)[kVec]) {
+      if (whole) {
+        unpack(*reinterpret_cast<const uint4*>(base + j), v, T());
+      } else {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) v[e] = as_float(base[j + e]);
+      }
+    };
+
+    // Maxima. An illegal entry becomes a logit of minus infinity, here and in the reference.
+    RowSums s = {};
+    float m[kSlots] = {-INFINITY, -INFINITY, 0.f, 0.f};
+    if (!gl && alike) {
+      UnitMax<T> top_z, top_r;
+#pragma unroll 4
+      for (int u = tid; u < units; u += kWideThreads) {
+        top_z.take(*reinterpret_cast<const uint4*>(z + head + u * kVec));
+        if (kExact) top_r.take(*reinterpret_cast<const uint4*>(r + head + u * kVec));
+      }
+      m[0] = top_z.value();
+      if (kExact) m[1] = top_r.value();
+    }
+    for (int u = !gl && alike ? units : tid; u < units; u += kWideThreads) {
+      const int j = head + u * kVec;
+      float vz[kVec], vr[kVec];
+      load_unit(z, j, true, vz);
+      if (kExact) load_unit(r, j, alike, vr);
+      if (gl) {
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          const bool in = pl[j + e];
+          m[2] += in ? 1.f : 0.f;
+          vz[e] = in ? vz[e] : -INFINITY;
+          if (kExact) vr[e] = in ? vr[e] : -INFINITY;
+          if (!in) {
+            put(z + j + e, -INFINITY);
+            if (kExact) put(r + j + e, -INFINITY);
+          }
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) {
+        m[0] = max_nan(m[0], vz[e]);
+        if (kExact) m[1] = max_nan(m[1], vr[e]);
+      }
+    }
+    if (tid < ends) {
+      const int j = end_entry(tid);
+      const bool in = !gl || pl[j];
+      m[2] += in ? 1.f : 0.f;
+      if (!in) {
+        put(z + j, -INFINITY);
+        if (kExact) put(r + j, -INFINITY);
+      } else {
+        m[0] = max_nan(m[0], as_float(z[j]));
+        if (kExact) m[1] = max_nan(m[1], as_float(r[j]));
+      }
+    }
+    reduce(m, 3, 2, 0);
+    if (tid == 0) row_peak = m[0], row_reference_peak = kExact ? m[1] : 0.f;
+    const float count = gl ? m[2] : static_cast<float>(a.width);  // warp 0's
+    __syncthreads();
+    s.peak = row_peak, s.reference_peak = row_reference_peak;
+
+    // Sums.
+    if (s.peak != -INFINITY) {
+      for (int u = tid; u < units; u += kWideThreads) {
+        const int j = head + u * kVec;
+        float vz[kVec], vr[kVec];
+        load_unit(z, j, true, vz);
+        if (kExact) load_unit(r, j, alike, vr);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) add_entry(s, vz[e], kExact ? vr[e] : 0.f, kExact);
+      }
+      if (tid < ends) {
+        const int j = end_entry(tid);
+        add_entry(s, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact);
+      }
+    }
+    float t[kSlots] = {s.sum, s.spread, s.reference_sum, s.apart};
+    reduce(t, kExact ? 4 : 2, 0, 1);
+    if (warp == 0) {
+      s.sum = t[0], s.spread = t[1], s.reference_sum = t[2], s.apart = t[3], s.count = count;
+      const bool inside = action >= 0 && action < a.width;
+      const bool action_legal = inside && (!gl || a.legal[row * a.legal_stride + action]);
+      const float z_a = action_legal ? as_float(static_cast<const T*>(a.logits)[row * a.stride + action]) : -INFINITY;
+      const bool live = row_counts(a, row, action, s, z_a, action_legal, rank == 0 && lane == 0);
+      if (a.log_probs) {
+        if (rank == 0 && lane == 0) a.log_probs[row] = live ? (z_a - s.peak) - logf(s.sum) : 0.f;
+      } else {
+        const RowGrad grad = finish_row(a, row, s, z_a, live, acc);
+        if (lane == 0) row_grad = grad, row_live = live;
+      }
+    }
+    __syncthreads();
+    if (a.log_probs) continue;
+    const RowGrad g = row_grad;
+    const bool counts = row_live;
+    if (a.grad) {
+      T* out = static_cast<T*>(a.grad) + row * a.grad_stride + lo;
+      const bool alike_out = (reinterpret_cast<uintptr_t>(gz) & 15) == (reinterpret_cast<uintptr_t>(out) & 15);
+      const int64_t at = action - lo;  // the action inside this slice
+      for (int u = tid; u < units; u += kWideThreads) {
+        const int j = head + u * kVec;
+        float vz[kVec], vr[kVec], v[kVec];
+        load_unit(z, j, true, vz);
+        if (kExact) load_unit(r, j, alike, vr);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) {
+          v[e] = counts ? gradient_entry(g, s.peak, vz[e], kExact ? vr[e] : 0.f, kExact) : 0.f;
+        }
+        if (counts && at >= j && at < j + kVec) {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e)
+            if (at == j + e) v[e] += g.action;
+        }
+        if (alike_out) {
+          *reinterpret_cast<uint4*>(out + j) = repack(v, T());
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) put(out + j + e, v[e]);
+        }
+      }
+      if (tid < ends) {
+        const int j = end_entry(tid);
+        float v = counts ? gradient_entry(g, s.peak, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact) : 0.f;
+        if (counts && at == j) v += g.action;
+        put(out + j, v);
+      }
+    }
+    __syncthreads();  // the slices may be overwritten
+  }
+  if (!a.log_probs && rank == 0 && tid == 0)
+    for (int k = 0; k < kTotals; ++k) a.partial[blockIdx.x / size * kTotals + k] = acc[k];
+  if (size > 1) tc::cluster_sync();  // no block leaves while another may still write to its shared memory
 }
 
 // ---- any width: one block per row, the row read once for its maxima, once for its sums, once for its gradient ---
@@ -171,7 +675,7 @@ __device__ __forceinline__ float block_reduce(float v, float* scratch) {
 template <typename T>
 __global__ void __launch_bounds__(kStreamThreads) anchored_stream_kernel(const Args a) {
   __shared__ float scratch[kStreamThreads / 32];
-  double acc[kTotals] = {};
+  float acc[kTotals] = {};
   const bool exact = a.reference != nullptr;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* z = static_cast<const T*>(a.logits) + row * a.stride;
@@ -193,15 +697,7 @@ __global__ void __launch_bounds__(kStreamThreads) anchored_stream_kernel(const A
     const bool any = s.peak != -INFINITY;
     for (int j = threadIdx.x; any && j < a.width; j += kStreamThreads) {
       if (legal && !legal[j]) continue;
-      const float from_peak = as_float(z[j]) - s.peak;
-      const float e = exp2_fast(from_peak * kLog2e);
-      s.sum += e;
-      if (e != 0.f) s.spread = fmaf(e, from_peak, s.spread);
-      if (exact) {
-        const float reference_from_peak = as_float(r[j]) - s.reference_peak;
-        s.reference_sum += exp2_fast(reference_from_peak * kLog2e);
-        if (e != 0.f) s.apart = fmaf(e, from_peak - reference_from_peak, s.apart);
-      }
+      add_entry(s, as_float(z[j]), exact ? as_float(r[j]) : 0.f, exact);
     }
     s.sum = block_reduce<0>(s.sum, scratch);
     s.spread = block_reduce<0>(s.spread, scratch);
@@ -217,14 +713,13 @@ __global__ void __launch_bounds__(kStreamThreads) anchored_stream_kernel(const A
       if (threadIdx.x == 0) a.log_probs[row] = counts ? (z_a - s.peak) - logf(s.sum) : 0.f;
       continue;
     }
-    double ignored[kTotals] = {};
-    const RowGrad g = finish_row(a, row, s, z_a, counts, threadIdx.x == 0 ? acc : ignored);
+    const RowGrad g = finish_row(a, row, s, z_a, counts, acc);
     if (!a.grad) continue;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
     for (int j = threadIdx.x; j < a.width; j += kStreamThreads) {
       float v = 0.f;
       if (counts && !(legal && !legal[j])) {
-        v = gradient_entry(g, s, as_float(z[j]), exact ? as_float(r[j]) : 0.f, exact);
+        v = gradient_entry(g, s.peak, as_float(z[j]), exact ? as_float(r[j]) : 0.f, exact);
         if (j == action) v += g.action;
       }
       put(out + j, v);
@@ -234,26 +729,120 @@ __global__ void __launch_bounds__(kStreamThreads) anchored_stream_kernel(const A
     for (int k = 0; k < kTotals; ++k) a.partial[blockIdx.x * kTotals + k] = acc[k];
 }
 
-// Warp k sums total k over the blocks: lane l the partials l, l + 32, ..., then a butterfly.
+// Warp k sums total k over the blocks: lane l the partials l, l + 32, ..., then a butterfly. The last total, the
+// objective, is written once more after them.
 __global__ void __launch_bounds__(kTotals * 32) anchored_totals_kernel(const double* partial, int count, float* totals) {
   const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
   pdl_wait();
   double total = 0;
+#pragma unroll 8
   for (int b = lane; b < count; b += 32) total += partial[b * kTotals + k];
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
   if (lane == 0) totals[k] = static_cast<float>(total);
+  if (lane == 0 && k == kTotals - 1) totals[kTotals] = static_cast<float>(total);
+}
+
+// A gradient times the gradient of the objective. The usual one is 1, and then there is nothing to do.
+template <typename T>
+__global__ void __launch_bounds__(256) anchored_scale_kernel(T* grad, int64_t rows, int64_t width, int64_t stride,
+                                                             const float* scale) {
+  const float by = *scale;
+  if (by == 1.f) return;
+  for (int64_t row = blockIdx.x; row < rows; row += gridDim.x)
+    for (int64_t j = threadIdx.x; j < width; j += 256) {
+      T* at = grad + row * stride + j;
+      put(at, as_float(*at) * by);
+    }
+}
+
+// The blocks of a kernel that are resident at once.
+template <typename K>
+int resident_blocks(K kernel, int threads) {
+  int per_sm = 0;
+  if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, threads, 0) != cudaSuccess || per_sm < 1) per_sm = 1;
+  return std::min(per_sm * sm_count(), kPartials);
+}
+
+template <typename T, int kLanes, int kVectors>
+int run_narrow(const Args& a, int* blocks, cudaStream_t s) {
+  static const int resident = resident_blocks(anchored_narrow_kernel<T, kLanes, kVectors>, 256);
+  constexpr int kRows = 8 * (32 / kLanes);
+  *blocks = static_cast<int>(std::min<int64_t>((a.rows + kRows - 1) / kRows, resident));
+  anchored_narrow_kernel<T, kLanes, kVectors><<<*blocks, 256, 0, s>>>(a);
+  return check_launch("anchored_narrow_kernel");
+}
+
+constexpr int kSharedPerSm = 227 * 1024;
+constexpr int kSharedPerBlock = 224 * 1024;           // beside the static part
+constexpr int kSliceBytes = kSharedPerSm / 3 - 2048;  // three blocks an SM
+
+template <typename T, bool kExact>
+int run_wide(const Args& a, int* blocks, cudaStream_t s, bool* fits) {
+  auto kernel = anchored_wide_kernel<T, kExact>;
+  static const cudaError_t configured = [&] {
+    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerBlock);
+    return rc != cudaSuccess ? rc : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  }();
+  if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "anchored_wide_kernel: %s", cudaGetErrorString(configured));
+  constexpr int kPlanes = kExact ? 2 : 1;
+  auto shared_of = [&](int slice) { return kPlanes * (slice * static_cast<int>(sizeof(T)) + 32) + (a.legal ? slice + 32 : 0); };
+  int size = 1, slice = 0, shared = 0;
+  for (;; size *= 2) {
+    // Slices of whole units, so that every block's slice is aligned as the row is.
+    const int64_t each = (static_cast<int64_t>(a.width) + size - 1) / size;
+    if (each < (1 << 20)) {
+      slice = static_cast<int>((each + 15) / 16 * 16);
+      shared = shared_of(slice);
+      if (shared <= kSliceBytes) break;
+      if (size == kMaxCluster) break;
+    } else if (size == kMaxCluster) {
+      shared = kSharedPerBlock + 1;
+      break;
+    }
+  }
+  *fits = shared <= kSharedPerBlock;
+  if (!*fits) return CG_OK;
+  const int per_sm = std::max(1, std::min(4, kSharedPerSm / (shared + 2048)));
+  const int clusters = static_cast<int>(std::min<int64_t>(a.rows, std::max(1, per_sm * sm_count() / size)));
+  *blocks = clusters;  // one partial sum a cluster
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(clusters * size));
+  config.blockDim = dim3(kWideThreads);
+  config.dynamicSmemBytes = shared;
+  config.stream = s;
+  cudaLaunchAttribute attribute[1];
+  attribute[0].id = cudaLaunchAttributeClusterDimension;
+  attribute[0].val.clusterDim.x = size;
+  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+  config.attrs = attribute;
+  config.numAttrs = 1;
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, slice, clusters);
+  if (err != cudaSuccess) return set_error(CG_ERR_CUDA, "anchored_wide_kernel launch: %s", cudaGetErrorString(err));
+  return check_launch("anchored_wide_kernel");
+}
+
+// A row goes where it fits: registers of four lanes (64 entries) or of a warp (1024), a cluster's shared memory, or nowhere
+// (it is streamed three times).
+template <typename T>
+int run_typed(const Args& a, int* blocks, cudaStream_t s) {
+  constexpr int kUnit = 8 / kVector<T>;  // vectors of eight entries
+  if (a.width <= 64) return run_narrow<T, 4, 2 * kUnit>(a, blocks, s);
+  if (a.width <= 256) return run_narrow<T, 32, kUnit>(a, blocks, s);
+  if (a.width <= 512) return run_narrow<T, 32, 2 * kUnit>(a, blocks, s);
+  if (a.width <= 1024) return run_narrow<T, 32, 4 * kUnit>(a, blocks, s);
+  bool fits = false;
+  if (int rc = a.reference ? run_wide<T, true>(a, blocks, s, &fits) : run_wide<T, false>(a, blocks, s, &fits)) return rc;
+  if (fits) return CG_OK;
+  *blocks = static_cast<int>(std::min<int64_t>(a.rows, kPartials));
+  anchored_stream_kernel<T><<<*blocks, kStreamThreads, 0, s>>>(a);
+  return check_launch("anchored_stream_kernel");
 }
 
 int run_rows(const Args& a, int dtype, int* blocks, cudaStream_t s) {
-  *blocks = static_cast<int>(std::min<int64_t>(a.rows, kPartials));
-  if (dtype == CG_F32)
-    anchored_stream_kernel<float><<<*blocks, kStreamThreads, 0, s>>>(a);
-  else if (dtype == CG_F16)
-    anchored_stream_kernel<__half><<<*blocks, kStreamThreads, 0, s>>>(a);
-  else
-    anchored_stream_kernel<__nv_bfloat16><<<*blocks, kStreamThreads, 0, s>>>(a);
-  return check_launch("anchored_stream_kernel");
+  if (dtype == CG_F32) return run_typed<float>(a, blocks, s);
+  if (dtype == CG_F16) return run_typed<__half>(a, blocks, s);
+  return run_typed<__nv_bfloat16>(a, blocks, s);
 }
 
 }  // namespace
@@ -294,6 +883,24 @@ extern "C" int cg_anchored_objective(const void* logits, int dtype, int64_t rows
   }
   return launch_pdl("anchored_totals_kernel", anchored_totals_kernel, dim3(1), dim3(kTotals * 32), 0, s,
                     static_cast<const double*>(partial), blocks, totals);
+}
+
+extern "C" int cg_anchored_scale(void* grad, int dtype, int64_t rows, int width, int64_t stride, const float* scale,
+                                 void* stream) {
+  using namespace cg;
+  CG_REQUIRE(valid_dtype(dtype), "cg_anchored_scale: dtype must be float32, float16 or bfloat16");
+  CG_REQUIRE(rows >= 0 && width > 0 && stride >= width, "cg_anchored_scale: bad shape");
+  if (rows == 0) return CG_OK;
+  CG_REQUIRE(grad && scale, "cg_anchored_scale: NULL pointer");
+  const int blocks = static_cast<int>(std::min<int64_t>(rows, 8 * sm_count()));
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == CG_F32)
+    anchored_scale_kernel<<<blocks, 256, 0, s>>>(static_cast<float*>(grad), rows, width, stride, scale);
+  else if (dtype == CG_F16)
+    anchored_scale_kernel<<<blocks, 256, 0, s>>>(static_cast<__half*>(grad), rows, width, stride, scale);
+  else
+    anchored_scale_kernel<<<blocks, 256, 0, s>>>(static_cast<__nv_bfloat16*>(grad), rows, width, stride, scale);
+  return check_launch("anchored_scale_kernel");
 }
 
 extern "C" int cg_action_log_probs(const void* logits, int dtype, int64_t rows, int width, int64_t stride,

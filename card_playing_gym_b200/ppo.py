@@ -259,7 +259,7 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
     grad = None
     if want_grad:
         grad = torch.empty((rows, grad_stride), dtype=logits.dtype, device=logits.device)[:, :width]
-    totals = torch.empty(len(ANCHORED_KEYS), device=logits.device)
+    sums = torch.empty(len(ANCHORED_KEYS) + 1, device=logits.device)  # the totals, and the objective once more
     need = nat.query("cg_anchored_objective_workspace_bytes", rows)
     with nat.on_device(logits.device):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
@@ -267,8 +267,8 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
                  nat.ptr(reference_logits), 0 if reference_logits is None else _row_stride(reference_logits),
                  nat.ptr(reference_log_probs), nat.ptr(legal), 0 if legal is None else _row_stride(legal),
                  nat.ptr(actions), nat.ptr(old), nat.ptr(advantages), nat.ptr(weights), clip, beta, alpha,
-                 nat.ptr(grad), grad_stride, nat.ptr(totals), nat.ptr(workspace), need, nat.stream_handle(logits.device))
-    return grad, totals
+                 nat.ptr(grad), grad_stride, nat.ptr(sums), nat.ptr(workspace), need, nat.stream_handle(logits.device))
+    return grad, sums
 
 
 class _AnchoredObjective(torch.autograd.Function):
@@ -277,17 +277,20 @@ class _AnchoredObjective(torch.autograd.Function):
                 beta, alpha):
         inputs = (logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights)
         ctx.scalars = (clip, beta, alpha)
-        ctx.gradient, totals = _run_anchored(*inputs, *ctx.scalars, want_grad=ctx.needs_input_grad[0])
+        ctx.gradient, sums = _run_anchored(*inputs, *ctx.scalars)
         ctx.save_for_backward(*inputs)  # a second backward computes the gradient again
+        totals = sums[:-1]
         ctx.mark_non_differentiable(totals)
-        return totals[-1].clone(), totals
+        return sums[-1], totals
 
     @staticmethod
     def backward(ctx, grad_objective, _grad_totals):
         gradient, ctx.gradient = ctx.gradient, None
         if gradient is None:
             gradient, _ = _run_anchored(*ctx.saved_tensors, *ctx.scalars)
-        gradient = gradient.mul_(grad_objective)
+        with nat.on_device(gradient.device):
+            nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
+                     _row_stride(gradient), nat.ptr(grad_objective.contiguous()), nat.stream_handle(gradient.device))
         return gradient, None, None, None, None, None, None, None, None, None, None
 
 
@@ -327,8 +330,12 @@ def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_prob
         reference_log_probs = _rows_of("reference_log_probs", reference_log_probs.detach(), rows, device, torch.float32)
     rest = [_rows_of(name, value.detach(), rows, device, torch.float32)
             for name, value in (("old_log_probs", old_log_probs), ("advantages", advantages), ("weights", weights))]
-    return _AnchoredObjective.apply(logits, reference_logits, reference_log_probs, legal, actions, *rest,
-                                    float(clip_ratio), float(beta), float(alpha))
+    inputs = (logits, reference_logits, reference_log_probs, legal, actions, *rest, float(clip_ratio), float(beta),
+              float(alpha))
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return _AnchoredObjective.apply(*inputs)
+    _, sums = _run_anchored(*inputs, want_grad=False)
+    return sums[-1], sums[:-1]
 
 
 def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, legal: torch.Tensor | None = None) -> torch.Tensor:

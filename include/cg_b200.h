@@ -384,9 +384,9 @@ int cg_value_loss(const float* prediction, const float* targets, const int32_t* 
  * KL = sum_S p (lp - log softmax_S(reference_logits)), or exp(u) - u - 1 with
  * u = reference_log_prob - lp[action], or 0 where both references are NULL. logits and
  * reference_logits share a dtype; each has its own row stride (entries). grad [rows, width] (or NULL)
- * has the logits' dtype and receives dL/dlogits (0 at illegal entries); totals fp32 [9] = sums of w times
- * (surr, 1, H, H / log |S|, [|S| > 1], [|ratio - 1| > clip], ratio - 1 - log ratio, KL) and L, summed in
- * float64 in a fixed order. A row counts for nothing, with a zero gradient, where its action is negative, its
+ * has the logits' dtype and receives dL/dlogits (0 at illegal entries); totals fp32 [10] = sums of w times
+ * (surr, 1, H, H / log |S|, [|S| > 1], [|ratio - 1| > clip], ratio - 1 - log ratio, KL), then L twice (one
+ * to keep as the objective), summed in a fixed order. A row counts for nothing, with a zero gradient, where its action is negative, its
  * weight 0 or nothing in it is legal (a mask that is all zero, logits that are all minus infinity).
  * An action >= width or outside the legal set does the same and sets the fault word (0x420 / 0x421). */
 int64_t cg_anchored_objective_workspace_bytes(int64_t rows);
@@ -396,6 +396,9 @@ int cg_anchored_objective(const void* logits, int dtype, int64_t rows, int width
                           const float* old_log_probs, const float* advantages, const float* weights, float clip_ratio,
                           float beta, float alpha, void* grad, int64_t grad_stride, float* totals, void* workspace,
                           int64_t workspace_bytes, void* stream);
+/* grad *= *scale in place (scale on the device): the chain rule for the gradient above; returns at once
+ * where *scale is 1. */
+int cg_anchored_scale(void* grad, int dtype, int64_t rows, int width, int64_t stride, const float* scale, void* stream);
 /* lp[action] alone, fp32 [rows] (the behaviour's or the reference's log-probabilities for the
  * objective): 0 where the row counts for nothing, minus infinity where the action is illegal. */
 int cg_action_log_probs(const void* logits, int dtype, int64_t rows, int width, int64_t stride, const uint8_t* legal,
