@@ -188,8 +188,13 @@ def declared_symbols() -> list[str]:
     return list(_SIGNATURES)
 
 
+@lru_cache(maxsize=None)
+def _function(name: str):
+    return getattr(lib(), name)
+
+
 def call(name: str, *args) -> int:
-    status = getattr(lib(), name)(*args)
+    status = _function(name)(*args)
     if status != 0:
         message = lib().cg_last_error().decode(errors="replace")
         raise NativeError(f"{name} failed ({status}): {message}")
@@ -197,7 +202,7 @@ def call(name: str, *args) -> int:
 
 
 def query(name: str, *args) -> int:
-    value = getattr(lib(), name)(*args)
+    value = _function(name)(*args)
     if value < 0:
         raise NativeError(f"{name} rejected its arguments: {lib().cg_last_error().decode(errors='replace')}")
     return value
@@ -255,7 +260,8 @@ def on_device(device: torch.device):
 
 
 def stream_handle(device: torch.device | None = None) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    index = torch.cuda.current_device() if device is None or device.index is None else device.index
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 class Workspace:

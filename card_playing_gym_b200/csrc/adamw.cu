@@ -192,6 +192,14 @@ __device__ __forceinline__ void encode8(uint8_t* codes, const float (&v)[8]) {
   *reinterpret_cast<uint2*>(codes) = raw;
 }
 
+// Square root and quotient within 2 units in the last place: the update they make is the learning rate's fraction
+// of a weight, and exact ones (some 30 instructions an entry) would cost more than the memory they hide behind.
+__device__ __forceinline__ float root_fast(float v) {
+  float r;
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
+
 // Largest of the warp's non-negative values; a NaN's bits compare above infinity's, so it is kept.
 __device__ __forceinline__ float warp_peak(float v) {
   return __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(v)));
@@ -283,7 +291,7 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
 
 // ---- the update -----------------------------------------------------------------------------------------
 template <typename T, int kBits, int kMax>
-__global__ void __launch_bounds__(kThreads) adamw_update_kernel(const __grid_constant__ Table<kMax> table,
+__global__ void __launch_bounds__(kThreads, 4) adamw_update_kernel(const __grid_constant__ Table<kMax> table,
                                                                 const States states,
                                                                 const Control* control) {
   constexpr bool kMaster = sizeof(T) < 4;
@@ -325,8 +333,8 @@ __global__ void __launch_bounds__(kThreads) adamw_update_kernel(const __grid_con
       const float gi = g[i] * clip;
       m[i] = f.beta1 * m[i] + f.rest1 * gi;
       v[i] = f.beta2 * v[i] + f.rest2 * (gi * gi);
-      const float root = sqrtf(v[i]);
-      p[i] = p[i] * f.decay - f.step * (m[i] / (root * f.root + f.eps));
+      const float root = root_fast(v[i]);
+      p[i] = p[i] * f.decay - f.step * __fdividef(m[i], root * f.root + f.eps);
       if (kBits == 8) {
         v[i] = root;
         // Bits, not fmaxf, which would drop a NaN.

@@ -51,43 +51,78 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t stride, 
 }
 
 // ---- dpre and the bias gradient -----------------------------------------------------------------------------------
-// A block takes 128 columns of one slice of the rows, four columns a lane, a row a warp at a time. Its warps' column
-// sums join in shared memory, the slices' in order in bias_sum_kernel.
+// A block takes 32 sixteen-byte vectors of columns of one slice of the rows, a vector a lane, a row a warp at a time. Its
+// warps' column sums join in shared memory, the slices' in order in bias_sum_kernel. It is bound by memory once the
+// activation's slope costs one exponential: sixteen entries of each input a lane are in flight at a time.
 template <typename T>
-__global__ void __launch_bounds__(256) slope_kernel(const T* dy, int64_t dy_stride, const T* pre, int64_t rows, int64_t cols,
-                                                    int64_t slice, int activation, typename OperandOf<T>::type* dpre,
-                                                    int64_t dpre_stride, float* partial) {
-  __shared__ float4 s[8][32];
+constexpr int kSlopeVector = 16 / static_cast<int>(sizeof(T));
+
+// The first n entries of a vector at `p`; `whole`: all of them, aligned to four.
+template <typename T, int kVec>
+__device__ __forceinline__ void load_vector(const T* __restrict__ p, int n, bool whole, float (&v)[kVec]) {
+#pragma unroll
+  for (int k = 0; k < kVec; k += 4) {
+    float part[4];
+    load4(p + k, n - k, whole, part);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[k + i] = part[i];
+  }
+}
+
+template <typename T, int kActivation>
+__global__ void __launch_bounds__(256, 3) slope_kernel(const T* __restrict__ dy, int64_t dy_stride, const T* __restrict__ pre,
+                                                       int64_t rows, int64_t cols, int64_t slice,
+                                                       typename OperandOf<T>::type* __restrict__ dpre, int64_t dpre_stride,
+                                                       float* __restrict__ partial) {
+  constexpr int kVec = kSlopeVector<T>, kRows = 16 / kVec;
+  __shared__ float s[8][32 * kVec];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t j = static_cast<int64_t>(blockIdx.x) * 128 + lane * 4;
+  const int64_t j = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * kVec;
   const int64_t lo = blockIdx.y * slice, hi = min(rows, lo + slice);
-  const bool aligned_dy = aligned4<T>(dy, dy_stride), aligned_pre = aligned4<T>(pre, cols);
-  const int n = static_cast<int>(max(int64_t{0}, min(int64_t{4}, cols - j)));
-  float sum[4] = {0.f, 0.f, 0.f, 0.f};
+  const int n = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kVec), cols - j)));
+  const bool whole_dy = aligned4<T>(dy, dy_stride) && n == kVec, whole_pre = aligned4<T>(pre, cols) && n == kVec;
+  float sum[kVec] = {};
   if (n > 0) {
-#pragma unroll 4
-    for (int64_t i = lo + warp; i < hi; i += 8) {
-      float g[4], z[4];
-      load4(dy + i * dy_stride + j, n, aligned_dy && n == 4, g);
-      if (activation != kActNone) {
-        load4(pre + i * cols + j, n, aligned_pre && n == 4, z);
+    for (int64_t i0 = lo + warp; i0 < hi; i0 += 8 * kRows) {
+      float g[kRows][kVec], z[kRows][kVec];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) g[k] *= activation_slope(z[k], activation);
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t i = i0 + 8 * r;
+        if (i >= hi) continue;
+        load_vector<T, kVec>(dy + i * dy_stride + j, n, whole_dy, g[r]);
+        if (kActivation != kActNone) load_vector<T, kVec>(pre + i * cols + j, n, whole_pre, z[r]);
       }
-      if (dpre) store_operand<T>(dpre + i * dpre_stride + j, rows * dpre_stride, g);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) sum[k] += g[k];
+      for (int r = 0; r < kRows; ++r) {
+        const int64_t i = i0 + 8 * r;
+        if (i >= hi) continue;
+#pragma unroll
+        for (int k = 0; k < kVec; ++k) {
+          if (kActivation != kActNone) g[r][k] *= activation_slope<T, kActivation>(z[r][k]);
+          sum[k] += g[r][k];
+        }
+        if (dpre) {
+#pragma unroll
+          for (int k = 0; k < kVec; k += 4) {
+            const float part[4] = {g[r][k], g[r][k + 1], g[r][k + 2], g[r][k + 3]};
+            if (k < n) store_operand<T>(dpre + i * dpre_stride + j + k, rows * dpre_stride, part);
+          }
+        }
+      }
     }
   }
   if (!partial) return;
-  s[warp][lane] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+#pragma unroll
+  for (int k = 0; k < kVec; ++k) s[warp][k * 32 + lane] = sum[k];
   __syncthreads();
-  if (warp != 0 || n == 0) return;
-  for (int w = 1; w < 8; ++w) {
-    const float4 f = s[w][lane];
-    sum[0] += f.x, sum[1] += f.y, sum[2] += f.z, sum[3] += f.w;
+  for (int c = threadIdx.x; c < 32 * kVec; c += 256) {
+    const int64_t column = static_cast<int64_t>(blockIdx.x) * 32 * kVec + (c & 31) * kVec + (c >> 5);
+    if (column >= cols) continue;
+    float total = s[0][c];
+#pragma unroll
+    for (int w = 1; w < 8; ++w) total += s[w][c];
+    partial[blockIdx.y * cols + column] = total;
   }
-  for (int k = 0; k < n; ++k) partial[blockIdx.y * cols + j + k] = sum[k];
 }
 
 template <typename T>
@@ -139,9 +174,10 @@ Layout plan_layout(const void* x, int64_t x_stride, const void* weight, int64_t 
     return at;
   };
   if (backward) {
-    // Blocks of 128 columns by slices of the rows: eight blocks an SM, slices of at least 32 rows.
-    const int64_t across = (outer + 127) / 128;
-    int64_t slices = std::max<int64_t>(1, 8 * 148 / std::max<int64_t>(across, 1));
+    // Blocks of 32 vectors of columns by slices of the rows: six blocks an SM, slices of at least 32 rows.
+    const int64_t columns = 32 * (16 / (dtype == CG_F32 ? 4 : 2));
+    const int64_t across = (outer + columns - 1) / columns;
+    int64_t slices = std::max<int64_t>(1, 6 * 148 / std::max<int64_t>(across, 1));
     slices = std::max<int64_t>(1, std::min(slices, (rows + 31) / 32));
     l.slice = std::max<int64_t>(1, (rows + slices - 1) / slices);
     l.slices = static_cast<int>((rows + l.slice - 1) / l.slice);
@@ -205,9 +241,14 @@ int backward(const Layout& l, const void* dy, int64_t dy_stride, const void* pre
   auto* sums = reinterpret_cast<float*>(workspace + l.sums);
   O* dpre = l.dpre < 0 || !(dx || dweight) ? nullptr : reinterpret_cast<O*>(workspace + l.dpre);
   if ((dpre || dbias) && rows > 0 && outer > 0) {
-    const dim3 grid(static_cast<unsigned>((outer + 127) / 128), static_cast<unsigned>(l.slices));
-    slope_kernel<T><<<grid, 256, 0, s>>>(static_cast<const T*>(dy), dy_stride, static_cast<const T*>(pre), rows, outer, l.slice,
-                                         activation, dpre, padded_row(outer), dbias ? sums : nullptr);
+    constexpr int kColumns = 32 * kSlopeVector<T>;
+    const dim3 grid(static_cast<unsigned>((outer + kColumns - 1) / kColumns), static_cast<unsigned>(l.slices));
+    auto kernel = activation == kActRelu   ? slope_kernel<T, kActRelu>
+                  : activation == kActGelu ? slope_kernel<T, kActGelu>
+                  : activation == kActSilu ? slope_kernel<T, kActSilu>
+                                           : slope_kernel<T, kActNone>;
+    kernel<<<grid, 256, 0, s>>>(static_cast<const T*>(dy), dy_stride, static_cast<const T*>(pre), rows, outer, l.slice, dpre,
+                                padded_row(outer), dbias ? sums : nullptr);
     if (int rc = check_launch("slope_kernel")) return rc;
   }
   if (dbias) {

@@ -127,19 +127,21 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const T* x, int64
 #pragma unroll
     for (int k = 0; k < 4; ++k) sums[warp][n * 8 + 2 * t + (k & 1)][g + 8 * (k >> 1)] = c[n][k];
   __syncthreads();
-  for (int index = threadIdx.x; index < kTokens * 8 * kOutputs; index += kWarps * 32) {
-    const int token = index / kOutputs, o = index % kOutputs;
-    const int64_t j = j0 + o;
-    if (token >= rows || j >= outer) continue;
-    float z = 0.f;
+  with_activation(e.activation, [&](auto activation) {
+    for (int index = threadIdx.x; index < kTokens * 8 * kOutputs; index += kWarps * 32) {
+      const int token = index / kOutputs, o = index % kOutputs;
+      const int64_t j = j0 + o;
+      if (token >= rows || j >= outer) continue;
+      float z = 0.f;
 #pragma unroll
-    for (int s = 0; s < kWarps; ++s) z += sums[s][token][o];
-    if (e.bias) z += as_float(static_cast<const T*>(e.bias)[j]);
-    if (e.pre) put(static_cast<T*>(e.pre) + token * outer + j, z);
-    z = activate(z, e.activation);
-    if (e.residual) z += as_float(static_cast<const T*>(e.residual)[token * e.residual_stride + j]);
-    put(static_cast<T*>(e.out) + token * e.out_stride + j, z);
-  }
+      for (int s = 0; s < kWarps; ++s) z += sums[s][token][o];
+      if (e.bias) z += as_float(static_cast<const T*>(e.bias)[j]);
+      if (e.pre) put(static_cast<T*>(e.pre) + token * outer + j, z);
+      z = activate<T, activation>(z);
+      if (e.residual) z += as_float(static_cast<const T*>(e.residual)[token * e.residual_stride + j]);
+      put(static_cast<T*>(e.out) + token * e.out_stride + j, z);
+    }
+  });
 }
 
 template <typename T>

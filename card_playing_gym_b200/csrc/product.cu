@@ -102,8 +102,14 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
       : "memory");
 }
 
-// Four columns of one row: the fp32 sums to their place.
 template <typename T>
+__device__ __forceinline__ void load_bias(const ProductEpilogue& e, int64_t j, int64_t cols, float (&bias)[4]) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bias[k] = e.bias && j + k < cols ? as_float(static_cast<const T*>(e.bias)[j + k]) : 0.f;
+}
+
+// Four columns of one row: the fp32 sums to their place.
+template <typename T, int kActivation>
 __device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int64_t j, int64_t cols, const float (&bias)[4],
                                         bool aligned, float (&z)[4]) {
   const int n = static_cast<int>(min(static_cast<int64_t>(4), cols - j));
@@ -112,7 +118,7 @@ __device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int
   for (int k = 0; k < 4; ++k) z[k] += bias[k];
   if (e.pre) store4(static_cast<T*>(e.pre) + i * cols + j, n, whole, z);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) z[k] = activate(z[k], e.activation);
+  for (int k = 0; k < 4; ++k) z[k] = activate<T, kActivation>(z[k]);
   if (e.residual) {
     float r[4];
     load4(static_cast<const T*>(e.residual) + i * e.residual_stride + j, n, whole, r);
@@ -122,10 +128,53 @@ __device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int
   store4(static_cast<T*>(e.out) + i * e.out_stride + j, n, whole, z);
 }
 
-template <typename T>
-__device__ __forceinline__ void load_bias(const ProductEpilogue& e, int64_t j, int64_t cols, float (&bias)[4]) {
+// A warp's square of 32 x 32 sums in shared memory (a row of eight four-column vectors, vector q of row r at q ^ (r & 7)) to
+// its place: four rows at a time, four columns a lane. 16-bit residual rows are all in flight before the
+// first result is stored (float32 ones would not fit beside a promoted sum).
+template <typename T, int kActivation>
+__device__ __forceinline__ void finish_square(const ProductEpilogue& e, const float4* square, int lane, int64_t i0, int64_t rows,
+                                              int64_t j, int64_t cols, bool aligned) {
+  float bias[4];
+  const int q = lane & 7, first = lane >> 3;
+  if (aligned && i0 + 32 <= rows && j - 4 * q + 32 <= cols) {
+    const int64_t i = i0 + first;
+    T* out = static_cast<T*>(e.out) + i * e.out_stride + j;
+    T* pre = e.pre ? static_cast<T*>(e.pre) + i * cols + j : nullptr;
+    const int64_t out_step = 4 * e.out_stride, pre_step = 4 * cols, residual_step = 4 * e.residual_stride;
+    const T* from = static_cast<const T*>(e.residual) + i * e.residual_stride + j;
+    uint2 residual[8];
+    if (sizeof(T) == 2 && e.residual) {
 #pragma unroll
-  for (int k = 0; k < 4; ++k) bias[k] = e.bias && j + k < cols ? as_float(static_cast<const T*>(e.bias)[j + k]) : 0.f;
+      for (int r = 0; r < 8; ++r) residual[r] = *reinterpret_cast<const uint2*>(from + r * residual_step);
+    }
+    load_bias<T>(e, j, cols, bias);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      const int row = r * 4 + first;
+      const float4 f = square[row * 8 + (q ^ (row & 7))];
+      float z[4] = {f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]};
+      if (pre) store4(pre + r * pre_step, z);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) z[k] = activate<T, kActivation>(z[k]);
+      if (e.residual) {
+        float add[4];
+        load4(sizeof(T) == 2 ? reinterpret_cast<const T*>(&residual[r]) : from + r * residual_step, add);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) z[k] += add[k];
+      }
+      store4(out + r * out_step, z);
+    }
+    return;
+  }
+  if (j >= cols) return;
+  load_bias<T>(e, j, cols, bias);
+  for (int r = 0; r < 8; ++r) {
+    const int row = r * 4 + first;
+    if (i0 + row >= rows) return;
+    const float4 f = square[row * 8 + (q ^ (row & 7))];
+    float z[4] = {f.x, f.y, f.z, f.w};
+    finish4<T, kActivation>(e, i0 + row, j, cols, bias, aligned, z);
+  }
 }
 
 template <typename T>
@@ -285,18 +334,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 8; ++q)
           square[lane * 8 + (q ^ (lane & 7))] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         __syncwarp();
-        float bias[4];
-        load_bias<T>(p.e, j, p.cols, bias);
+        if (p.partial) {
+          float* to = p.partial + (t.split * p.rows + i0 + (lane >> 3)) * p.partial_stride + j;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-          const int row = r * 4 + (lane >> 3);
-          const float4 f = square[row * 8 + ((lane & 7) ^ (row & 7))];
-          float z[4] = {f.x, f.y, f.z, f.w};
-          if (i0 + row >= p.rows || j >= p.cols) continue;
-          if (p.partial)
-            *reinterpret_cast<float4*>(p.partial + (t.split * p.rows + i0 + row) * p.partial_stride + j) = f;
-          else
-            finish4<T>(p.e, i0 + row, j, p.cols, bias, aligned, z);
+          for (int r = 0; r < 8; ++r) {
+            const int row = r * 4 + (lane >> 3);
+            if (i0 + row < p.rows && j < p.cols)
+              *reinterpret_cast<float4*>(to + r * 4 * p.partial_stride) = square[row * 8 + ((lane & 7) ^ (row & 7))];
+          }
+        } else {
+          with_activation(p.e.activation, [&](auto activation) {
+            finish_square<T, activation>(p.e, square, lane, i0, p.rows, j, p.cols, aligned);
+          });
         }
         __syncwarp();
       };
@@ -357,7 +406,7 @@ __global__ void __launch_bounds__(256) product_join_kernel(const float* partial,
     }
     float bias[4];
     load_bias<T>(e, j, cols, bias);
-    finish4<T>(e, i, j, cols, bias, aligned, z);
+    with_activation(e.activation, [&](auto activation) { finish4<T, activation>(e, i, j, cols, bias, aligned, z); });
   }
 }
 

@@ -17,6 +17,8 @@ ACTIVATIONS = {"none": 0, "relu": 1, "gelu": 2, "silu": 3}
 def _unit_rows(matrix: torch.Tensor) -> torch.Tensor:
     """The matrix with adjacent row entries and rows that do not overlap (a copy only where it has neither)."""
 
+    if matrix.is_contiguous():
+        return matrix
     if matrix.shape[1] > 1 and matrix.stride(1) != 1 or matrix.shape[0] > 1 and matrix.stride(0) < matrix.shape[1]:
         return matrix.contiguous()
     return matrix

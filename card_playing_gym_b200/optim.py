@@ -9,9 +9,14 @@ With ``weight_decay=0`` it is Adam. It is a ``torch.optim.Optimizer`` (parameter
 
 from __future__ import annotations
 
+from operator import attrgetter
+
+import numpy as np
 import torch
 
 from . import _native as nat
+
+_dtype_of, _layout_of = attrgetter("dtype"), attrgetter("layout")
 
 BLOCK = 256  # entries of one scale of the 8-bit moments; every parameter's state starts on a multiple of it
 
@@ -106,6 +111,8 @@ class AdamW(torch.optim.Optimizer):
             self.state[p] = views
         # The host table of the step: extents and groups are fixed, addresses are filled in at every step.
         self._table = (nat.AdamWTensor * len(self._parameters))()
+        self._addresses = np.frombuffer(self._table, dtype=np.dtype([("param", "u8"), ("grad", "u8"), ("rest", "V24")]))
+        self._dtype = first.dtype
         self._numels = [p.numel() for p in self._parameters]
         index = 0
         for number, group in enumerate(self.param_groups):
@@ -143,6 +150,21 @@ class AdamW(torch.optim.Optimizer):
         self.steps.copy_(state_dict["steps"])
 
     # -- the step -----------------------------------------------------------------------------------------------------
+    def _check(self, params: list, grads: list, present: list) -> None:
+        """That the table still describes the parameters and gradients: one pass per property, for the host's sake."""
+
+        held = grads if all(present) else [g for g in grads if g is not None]
+        numels = self._numels if all(present) else [n for g, n in zip(grads, self._numels) if g is not None]
+        if (list(map(torch.Tensor.numel, params)) != self._numels or set(map(_dtype_of, params)) != {self._dtype}
+                or set(map(torch.Tensor.get_device, params)) != {self.steps.get_device()}
+                or not all(map(torch.Tensor.is_contiguous, params))):
+            raise ValueError("a parameter has changed its size, dtype, device or layout since the optimizer was built")
+        if set(map(_layout_of, held)) - {torch.strided} or not all(map(torch.Tensor.is_contiguous, held)):
+            raise ValueError("a gradient is not dense and contiguous")
+        if (list(map(torch.Tensor.numel, held)) != numels or set(map(_dtype_of, held)) - {self._dtype}
+                or set(map(torch.Tensor.get_device, held)) - {self.steps.get_device()}):
+            raise ValueError("a gradient has not its parameter's size, dtype or device")
+
     @torch.no_grad()
     def step(self, closure=None):
         loss = None
@@ -150,18 +172,12 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         flat, device = self.flat, self.steps.device
-        table, dtype = self._table, self._parameters[0].dtype
-        for i, p in enumerate(self._parameters):
-            entry, g = table[i], p.grad
-            if g is None:
-                entry.grad = None
-                continue
-            if p.numel() != self._numels[i] or p.dtype is not dtype or not p.is_contiguous():
-                raise ValueError(f"parameter {i} has changed its size, dtype or layout since the optimizer was built")
-            if g.is_sparse or not g.is_contiguous():
-                raise ValueError(f"the gradient of parameter {i} is not dense and contiguous")
-            entry.param = nat.ptr(p)
-            entry.grad = nat.ptr(g)
+        params = self._parameters
+        grads = [p.grad for p in params]
+        self._check(params, grads, [g is not None for g in grads])
+        self._addresses["param"] = list(map(torch.Tensor.data_ptr, params))
+        self._addresses["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+        table = self._table
         for entry, group in zip(self._groups, self.param_groups):
             entry.lr, entry.eps, entry.weight_decay = group["lr"], group["eps"], group["weight_decay"]
             entry.beta1, entry.beta2 = group["betas"]
@@ -169,7 +185,7 @@ class AdamW(torch.optim.Optimizer):
         second = flat["exp_avg_sq" if self.state_bits == 32 else "exp_avg_sq_root"]
         with nat.on_device(device):
             workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-            nat.call("cg_adamw_step", table, len(table), nat.DTYPE_CODES[dtype], self._groups, len(self._groups),
+            nat.call("cg_adamw_step", table, len(table), nat.DTYPE_CODES[self._dtype], self._groups, len(self._groups),
                      self.state_bits, nat.ptr(flat["exp_avg"]), nat.ptr(flat.get("exp_avg_scale")), nat.ptr(second),
                      nat.ptr(flat.get("exp_avg_sq_root_scale")), nat.ptr(flat.get("master")), nat.ptr(self.steps),
                      float(self.max_norm or 0.0), nat.ptr(self.grad_norm), nat.ptr(self._control),

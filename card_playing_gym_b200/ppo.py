@@ -212,6 +212,8 @@ ANCHORED_KEYS = ("policy_loss", "row_weight", "entropy_raw", "entropy", "entropy
 
 
 def _rows_of(name: str, tensor: torch.Tensor, rows: int, device: torch.device, dtype: torch.dtype) -> torch.Tensor:
+    if tensor.dtype is dtype and tensor.shape == (rows,) and tensor.device == device and tensor.is_contiguous():
+        return tensor
     if tensor.shape != (rows,) or tensor.device != device:
         raise ValueError(f"{name} must be [{rows}] on {device}, not {tuple(tensor.shape)} on {tensor.device}")
     return tensor.to(dtype).contiguous()
@@ -226,6 +228,8 @@ def _plane_of(name: str, tensor: torch.Tensor, like: torch.Tensor) -> torch.Tens
 def _unit_rows(plane: torch.Tensor) -> torch.Tensor:
     """The plane with adjacent row entries and rows that do not overlap (a copy only where it has neither)."""
 
+    if plane.is_contiguous():
+        return plane
     if plane.shape[1] > 1 and plane.stride(1) != 1 or plane.shape[0] > 1 and plane.stride(0) < plane.shape[1]:
         return plane.contiguous()
     return plane
@@ -277,6 +281,7 @@ class _AnchoredObjective(torch.autograd.Function):
                 beta, alpha):
         inputs = (logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights)
         ctx.scalars = (clip, beta, alpha)
+        ctx.set_materialize_grads(False)  # the totals have no gradient to make zeros for
         ctx.gradient, sums = _run_anchored(*inputs, *ctx.scalars)
         ctx.save_for_backward(*inputs)  # a second backward computes the gradient again
         totals = sums[:-1]
@@ -285,13 +290,15 @@ class _AnchoredObjective(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, grad_objective, _grad_totals):
+        if grad_objective is None:
+            return (None,) * 11
         gradient, ctx.gradient = ctx.gradient, None
         if gradient is None:
             gradient, _ = _run_anchored(*ctx.saved_tensors, *ctx.scalars)
         with nat.on_device(gradient.device):
             nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
                      _row_stride(gradient), nat.ptr(grad_objective.contiguous()), nat.stream_handle(gradient.device))
-        return gradient, None, None, None, None, None, None, None, None, None, None
+        return (gradient, *(None,) * 10)
 
 
 def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_probs: torch.Tensor,
@@ -325,11 +332,12 @@ def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_prob
     if reference_logits is not None:
         if reference_logits.dtype != logits.dtype:
             raise ValueError(f"reference_logits must be {logits.dtype}, not {reference_logits.dtype}")
-        reference_logits = _plane_of("reference_logits", reference_logits.detach(), logits)
+        reference_logits = _plane_of("reference_logits", reference_logits, logits)
     if reference_log_probs is not None:
-        reference_log_probs = _rows_of("reference_log_probs", reference_log_probs.detach(), rows, device, torch.float32)
-    rest = [_rows_of(name, value.detach(), rows, device, torch.float32)
-            for name, value in (("old_log_probs", old_log_probs), ("advantages", advantages), ("weights", weights))]
+        reference_log_probs = _rows_of("reference_log_probs", reference_log_probs, rows, device, torch.float32)
+    rest = (_rows_of("old_log_probs", old_log_probs, rows, device, torch.float32),
+            _rows_of("advantages", advantages, rows, device, torch.float32),
+            _rows_of("weights", weights, rows, device, torch.float32))
     inputs = (logits, reference_logits, reference_log_probs, legal, actions, *rest, float(clip_ratio), float(beta),
               float(alpha))
     if torch.is_grad_enabled() and logits.requires_grad:
