@@ -27,7 +27,7 @@ namespace {
 constexpr int kBlockEntries = 256;  // entries of one scale; every tensor's state starts on a multiple
 constexpr int kPerLane = 8;
 constexpr int kThreads = 256;
-constexpr int kChunk = 8192;  // entries of a thread block: four 256-entry blocks a warp
+constexpr int kChunk = 16384;  // entries of a thread block: eight 256-entry blocks a warp
 constexpr int kMaxGroups = 16;
 constexpr int kNormBlocks = 1184;  // partial sums of the norm: one fixed order of addition
 constexpr float kE4m3Max = 448.f;
@@ -173,8 +173,7 @@ __device__ __forceinline__ bool aligned8(const T* p) {
 }
 
 // ---- 8-bit moments --------------------------------------------------------------------------------
-__device__ __forceinline__ void decode8(const uint8_t* codes, float unit, float (&v)[8]) {
-  const uint2 raw = *reinterpret_cast<const uint2*>(codes);
+__device__ __forceinline__ void decode8(const uint2& raw, float unit, float (&v)[8]) {
   const __nv_fp8x2_storage_t* pairs = reinterpret_cast<const __nv_fp8x2_storage_t*>(&raw);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -252,12 +251,29 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
     const T* grad = static_cast<const T*>(e.grad);
     const bool aligned = aligned8(grad);
     const int64_t start = static_cast<int64_t>(chunk - e.first_chunk) * kChunk;
+    constexpr int kSteps = kChunk / (kThreads * kPerLane), kAtOnce = sizeof(T) == 2 ? kSteps : kSteps / 2;
+    if (aligned && start + kChunk <= e.numel) {
+      // Loads of 128 bytes a lane are in flight at a time.
 #pragma unroll
-    for (int b = 0; b < kChunk / (kThreads * kPerLane); ++b) {
+      for (int b = 0; b < kSteps; b += kAtOnce) {
+        float g[kAtOnce][8];
+#pragma unroll
+        for (int c = 0; c < kAtOnce; ++c) load8(grad + start + ((b + c) * kThreads + threadIdx.x) * kPerLane, g[c]);
+#pragma unroll
+        for (int c = 0; c < kAtOnce; ++c) {
+          float sum = 0.f;
+#pragma unroll
+          for (int i = 0; i < kPerLane; ++i) sum = fmaf(g[c][i], g[c][i], sum);
+          total += sum;
+        }
+      }
+      continue;
+    }
+    for (int b = 0; b < kSteps; ++b) {
       const int64_t at = start + (b * kThreads + threadIdx.x) * kPerLane;
-      float g[8];
+      if (at >= e.numel) break;
+      float g[8], sum = 0.f;
       load_entries(grad, at, e.numel, aligned && at + kPerLane <= e.numel, g);
-      float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kPerLane; ++i) sum = fmaf(g[i], g[i], sum);
       total += sum;
@@ -290,80 +306,122 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
 }
 
 // ---- the update -----------------------------------------------------------------------------------------
+// What a lane has in flight of one 256-entry block: its eight entries as they are in memory.
+template <typename T, int kBits>
+struct Loaded {
+  float p[8], g[8], m[8], v[8];     // fp32 parts
+  uint4 raw_g;                      // a 16-bit gradient
+  uint2 codes_m, codes_v;           // 8-bit moments
+  float peak_m, peak_r;
+  bool whole;
+};
+
+template <typename T, int kBits>
+__device__ __forceinline__ void load_block(Loaded<T, kBits>& l, const Entry& e, const States& states, int64_t at, bool aligned) {
+  const int64_t held = e.state + at;  // the state's arrays are padded: eight entries are always inside
+  const T* param = static_cast<const T*>(e.param);
+  const T* grad = static_cast<const T*>(e.grad);
+  l.whole = aligned && at + kPerLane <= e.numel;
+  if constexpr (sizeof(T) == 2) {
+    if (l.whole)
+      l.raw_g = *reinterpret_cast<const uint4*>(grad + at);
+    else
+      load_entries(grad, at, e.numel, false, l.g);
+    load8(states.master + held, l.p);
+  } else {
+    load_entries(grad, at, e.numel, l.whole, l.g);
+    load_entries(param, at, e.numel, l.whole, l.p);
+  }
+  if constexpr (kBits == 8) {
+    l.codes_m = *reinterpret_cast<const uint2*>(static_cast<uint8_t*>(states.exp_avg) + held);
+    l.codes_v = *reinterpret_cast<const uint2*>(static_cast<uint8_t*>(states.exp_avg_sq) + held);
+    l.peak_m = states.exp_avg_scale[held / kBlockEntries];
+    l.peak_r = states.exp_avg_sq_scale[held / kBlockEntries];
+  } else {
+    load8(static_cast<float*>(states.exp_avg) + held, l.m);
+    load8(static_cast<float*>(states.exp_avg_sq) + held, l.v);
+  }
+}
+
+template <typename T, int kBits>
+__device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e, const States& states, int64_t at, int lane,
+                                             const Factors& f, float clip) {
+  const int64_t held = e.state + at;
+  if constexpr (sizeof(T) == 2) {
+    if (l.whole) load8(reinterpret_cast<const T*>(&l.raw_g), l.g);
+  }
+  if constexpr (kBits == 8) {
+    decode8(l.codes_m, l.peak_m * (1.f / kE4m3Max), l.m);
+    decode8(l.codes_v, l.peak_r * (1.f / kE4m3Max), l.v);
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) l.v[i] *= l.v[i];
+  }
+  float peak_m = 0.f, peak_r = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) {
+    const float g = l.g[i] * clip;
+    l.m[i] = f.beta1 * l.m[i] + f.rest1 * g;
+    l.v[i] = f.beta2 * l.v[i] + f.rest2 * (g * g);
+    const float root = root_fast(l.v[i]);
+    l.p[i] = l.p[i] * f.decay - f.step * __fdividef(l.m[i], root * f.root + f.eps);
+    if (kBits == 8) {
+      l.v[i] = root;
+      // Bits, not fmaxf, which would drop a NaN.
+      peak_m = __uint_as_float(max(__float_as_uint(peak_m), __float_as_uint(fabsf(l.m[i]))));
+      peak_r = __uint_as_float(max(__float_as_uint(peak_r), __float_as_uint(root)));
+    }
+  }
+  if (sizeof(T) == 2) store8(states.master + held, l.p);
+  store_entries(static_cast<T*>(e.param), at, e.numel, l.whole, l.p);
+  if constexpr (kBits == 8) {
+    peak_m = warp_peak(peak_m);
+    peak_r = warp_peak(peak_r);
+    const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max / peak_m;
+    const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max / peak_r;
+#pragma unroll
+    for (int i = 0; i < kPerLane; ++i) {
+      l.m[i] *= to_m;
+      l.v[i] = l.v[i] > 0.f ? fmaxf(l.v[i] * to_r, kE4m3Least) : l.v[i] * to_r;
+    }
+    encode8(static_cast<uint8_t*>(states.exp_avg) + held, l.m);
+    encode8(static_cast<uint8_t*>(states.exp_avg_sq) + held, l.v);
+    if (lane == 0) {
+      states.exp_avg_scale[held / kBlockEntries] = peak_m;
+      states.exp_avg_sq_scale[held / kBlockEntries] = peak_r;
+    }
+  } else {
+    store8(static_cast<float*>(states.exp_avg) + held, l.m);
+    store8(static_cast<float*>(states.exp_avg_sq) + held, l.v);
+  }
+}
+
+// A warp takes every eighth block of its chunk; the next block's loads are in flight while this one is computed and
+// stored. The first loads go out before the wait for the factors: nothing the kernel before this one writes is among
+// them.
 template <typename T, int kBits, int kMax>
-__global__ void __launch_bounds__(kThreads, 4) adamw_update_kernel(const __grid_constant__ Table<kMax> table,
-                                                                const States states,
-                                                                const Control* control) {
-  constexpr bool kMaster = sizeof(T) < 4;
+__global__ void __launch_bounds__(kThreads, kBits == 8 ? 3 : 2) adamw_update_kernel(const __grid_constant__ Table<kMax> table,
+                                                                                    const States states, const Control* control) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Entry& e = table.e[find_tensor(table, blockIdx.x)];
-  T* param = static_cast<T*>(e.param);
-  const T* grad = static_cast<const T*>(e.grad);
-  const bool aligned = aligned8(param) && aligned8(grad);
+  const bool aligned = aligned8(static_cast<const T*>(e.param)) && aligned8(static_cast<const T*>(e.grad));
   const int64_t start = static_cast<int64_t>(blockIdx.x - e.first_chunk) * kChunk;
+  const int64_t end = min(start + kChunk, e.numel);
+  constexpr int kStride = kThreads / 32 * kBlockEntries;
+  int64_t block = start + warp * kBlockEntries;
+  if (block >= end) return;
+  Loaded<T, kBits> now, next;
+  load_block(now, e, states, block + lane * kPerLane, aligned);
   pdl_wait();
   if (control->skip) return;  // a norm that is not finite: nothing moves
   const float clip = control->clip;
   const Factors f = control->groups[e.group];
-  for (int64_t block = start + warp * kBlockEntries; block < start + kChunk && block < e.numel; block += kThreads * kPerLane) {
-    const int64_t at = block + lane * kPerLane;
-    const int64_t held = e.state + at;  // the state's arrays are padded: eight entries are always inside
-    const bool whole = aligned && at + kPerLane <= e.numel;
-    float p[8], g[8], m[8], v[8];
-    load_entries(grad, at, e.numel, whole, g);
-    if (kMaster)
-      load8(states.master + held, p);
-    else
-      load_entries(param, at, e.numel, whole, p);
-    float unit_m = 0.f, unit_r = 0.f;
-    if (kBits == 8) {
-      unit_m = states.exp_avg_scale[held / kBlockEntries] * (1.f / kE4m3Max);
-      unit_r = states.exp_avg_sq_scale[held / kBlockEntries] * (1.f / kE4m3Max);
-      decode8(static_cast<uint8_t*>(states.exp_avg) + held, unit_m, m);
-      decode8(static_cast<uint8_t*>(states.exp_avg_sq) + held, unit_r, v);
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) v[i] *= v[i];
-    } else {
-      load8(static_cast<float*>(states.exp_avg) + held, m);
-      load8(static_cast<float*>(states.exp_avg_sq) + held, v);
-    }
-    float peak_m = 0.f, peak_r = 0.f;
-#pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      const float gi = g[i] * clip;
-      m[i] = f.beta1 * m[i] + f.rest1 * gi;
-      v[i] = f.beta2 * v[i] + f.rest2 * (gi * gi);
-      const float root = root_fast(v[i]);
-      p[i] = p[i] * f.decay - f.step * __fdividef(m[i], root * f.root + f.eps);
-      if (kBits == 8) {
-        v[i] = root;
-        // Bits, not fmaxf, which would drop a NaN.
-        peak_m = __uint_as_float(max(__float_as_uint(peak_m), __float_as_uint(fabsf(m[i]))));
-        peak_r = __uint_as_float(max(__float_as_uint(peak_r), __float_as_uint(root)));
-      }
-    }
-    if (kMaster) store8(states.master + held, p);
-    store_entries(param, at, e.numel, whole, p);
-    if (kBits == 8) {
-      peak_m = warp_peak(peak_m);
-      peak_r = warp_peak(peak_r);
-      const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max / peak_m;
-      const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max / peak_r;
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) {
-        m[i] *= to_m;
-        v[i] = v[i] > 0.f ? fmaxf(v[i] * to_r, kE4m3Least) : v[i] * to_r;
-      }
-      encode8(static_cast<uint8_t*>(states.exp_avg) + held, m);
-      encode8(static_cast<uint8_t*>(states.exp_avg_sq) + held, v);
-      if (lane == 0) {
-        states.exp_avg_scale[held / kBlockEntries] = peak_m;
-        states.exp_avg_sq_scale[held / kBlockEntries] = peak_r;
-      }
-    } else {
-      store8(static_cast<float*>(states.exp_avg) + held, m);
-      store8(static_cast<float*>(states.exp_avg_sq) + held, v);
-    }
+  for (;;) {
+    const int64_t after = block + kStride;
+    if (after < end) load_block(next, e, states, after + lane * kPerLane, aligned);
+    update_block(now, e, states, block + lane * kPerLane, lane, f, clip);
+    if (after >= end) break;
+    now = next;
+    block = after;
   }
 }
 

@@ -391,14 +391,90 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
 
 // ---- wider rows: a row in the shared memory of a cluster --------------------------------------------------------------
 // The row is read once, by bulk copies, and stays in shared memory for its maxima, its sums and its gradient. A cluster
-// of C blocks holds it, C the least that leaves room for three blocks an SM (so that one block's copies run under
-// another's arithmetic); the blocks exchange their maxima and sums through each other's shared memory.
+// of C blocks holds it, C the least that leaves room for three blocks an SM, so that one block's copies and barriers
+// run under another's arithmetic; narrow slices have two buffers, the next row's copies running under this one's arithmetic.
+// Every thread sums its own entries relative to its own maxima, and the maxima and sums are joined once, over the
+// block and then over the cluster through each other's shared memory: one cluster barrier a row.
+//
+// What bounds it is instruction issue beside HBM: three exponentials an entry and, in pairs of packed fp32
+// arithmetic, some 20 instructions. Entries at minus infinity, which the packed sums turn into NaN, are found by
+// that and summed again with tests.
+//
 // Slices are copied with the alignment they have in memory: the sixteen-byte units inside by the copy engine, the few
 // bytes at the ends by threads. The arithmetic runs over the same units; planes whose rows are aligned differently
 // from the logits' are read entry by entry from shared memory.
 constexpr int kWideThreads = 256;
 constexpr int kMaxCluster = 16;
-constexpr int kSlots = 4;
+
+// Partial results over some entries, each relative to their own maxima.
+struct Part {
+  float peak, reference_peak, sum, spread, reference_sum, apart, count;
+};
+constexpr int kSlots = sizeof(Part) / sizeof(float);
+
+// The parts of 2^steps neighbouring lanes (or of the whole warp) joined; every lane gets the result.
+template <bool kExact>
+__device__ __forceinline__ void join_lanes(Part& p, int lanes) {
+  float peak = p.peak, reference_peak = p.reference_peak;
+  for (int o = lanes / 2; o > 0; o >>= 1) {
+    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
+    if (kExact) reference_peak = max_nan(reference_peak, __shfl_xor_sync(0xffffffffu, reference_peak, o));
+  }
+  const float up = p.peak == -INFINITY ? 0.f : p.peak - peak;
+  const float scale = p.peak == -INFINITY ? 0.f : exp2_fast(up * kLog2e);
+  if (kExact) {
+    const float reference_up = p.reference_peak == -INFINITY ? 0.f : p.reference_peak - reference_peak;
+    p.reference_sum *= p.reference_peak == -INFINITY ? 0.f : exp2_fast(reference_up * kLog2e);
+    // Without a reference entry above minus infinity the part's differences are infinite already.
+    p.apart = scale == 0.f ? 0.f : scale * fmaf(up - reference_up, p.sum, p.apart);
+  }
+  p.spread = scale == 0.f ? 0.f : scale * fmaf(up, p.sum, p.spread);
+  p.sum = scale == 0.f ? 0.f : scale * p.sum;
+  p.peak = peak, p.reference_peak = reference_peak;
+  for (int o = lanes / 2; o > 0; o >>= 1) {
+    p.sum += __shfl_xor_sync(0xffffffffu, p.sum, o);
+    p.spread += __shfl_xor_sync(0xffffffffu, p.spread, o);
+    p.count += __shfl_xor_sync(0xffffffffu, p.count, o);
+    if (kExact) {
+      p.reference_sum += __shfl_xor_sync(0xffffffffu, p.reference_sum, o);
+      p.apart += __shfl_xor_sync(0xffffffffu, p.apart, o);
+    }
+  }
+}
+
+// Two fp32 values in one register pair, added, multiplied and combined in one instruction.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(lo), "f"(hi));
+  return t;
+}
+__device__ __forceinline__ float2 apart_of(Two t) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(t.v));
+  return f;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two t;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+  return t;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two t;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+  return t;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two t;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return t;
+}
+__device__ __forceinline__ Two exp2_two(Two x) {
+  const float2 f = apart_of(x);
+  return two(exp2_fast(f.x), exp2_fast(f.y));
+}
 
 // The bytes before the first sixteen-byte boundary of `bytes` bytes at `src`, and those in whole units after it.
 __device__ __forceinline__ uint32_t aligned_part(const void* src, int bytes, int* head) {
@@ -411,14 +487,37 @@ __device__ __forceinline__ void store_remote(uint32_t address, float v) {
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
 }
 
+// One plane of a row's slice: where it is in memory and where in shared memory, at the same misalignment.
+struct Plane {
+  const unsigned char* from;
+  unsigned char* to;  // entry 0
+  int bytes, head;
+  uint32_t inner;
+  __device__ __forceinline__ Plane(const void* src, unsigned char* base, int size) {
+    from = static_cast<const unsigned char*>(src);
+    to = base + (reinterpret_cast<uintptr_t>(src) & 15);
+    bytes = src ? size : 0;
+    inner = aligned_part(src, bytes, &head);
+  }
+  __device__ __forceinline__ int tail() const { return bytes - head - static_cast<int>(inner); }
+  __device__ __forceinline__ void copy_units(uint64_t* barrier) const {
+    if (inner) tc::bulk_g2s(to + head, from + head, inner, barrier);
+  }
+  __device__ __forceinline__ void copy_ends(int tid) const {
+    if (tid < head) to[tid] = from[tid];
+    if (tid >= 32 && tid < 32 + tail()) to[head + inner + tid - 32] = from[head + inner + tid - 32];
+  }
+};
+
 template <typename T, bool kExact>
-__global__ void __launch_bounds__(kWideThreads, 4) anchored_wide_kernel(const Args a, int slice, int clusters) {
+__global__ void __launch_bounds__(kWideThreads, 3) anchored_wide_kernel(const Args a, int slice, int clusters, int buffer_bytes,
+                                                                        int buffers) {
   constexpr int kVec = kVector<T>;
   extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ __align__(8) uint64_t arrived;
-  __shared__ float warp_values[kWideThreads / 32][kSlots], cluster_values[2][kMaxCluster][kSlots];
-  __shared__ float row_peak, row_reference_peak;
+  __shared__ __align__(8) uint64_t arrived[2];
+  __shared__ float warp_parts[kWideThreads / 32][kSlots], cluster_parts[2][kMaxCluster][kSlots];
   __shared__ RowGrad row_grad;
+  __shared__ float row_peak;
   __shared__ bool row_live;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   uint32_t rank = 0, size = 1;
@@ -428,94 +527,61 @@ __global__ void __launch_bounds__(kWideThreads, 4) anchored_wide_kernel(const Ar
   const int lo = static_cast<int>(rank) * slice;
   const int n = max(0, min(slice, a.width - lo));
   if (tid == 0) {
-    tc::bar_init(&arrived, 1);
+    tc::bar_init(&arrived[0], 1);
+    tc::bar_init(&arrived[1], 1);
     tc::bar_fence_init();
   }
   __syncthreads();
   if (size > 1) tc::cluster_sync();
 
-  // Values of every thread reduced over the cluster, the first `maxima` of them by maximum; the result is warp 0's.
-  auto reduce = [&](float (&v)[kSlots], int count, int maxima, int which) {
-#pragma unroll
-    for (int k = 0; k < kSlots; ++k) {
-      if (k >= count) continue;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const float other = __shfl_xor_sync(0xffffffffu, v[k], o);
-        v[k] = k < maxima ? max_nan(v[k], other) : v[k] + other;
-      }
-      if (lane == 0) warp_values[warp][k] = v[k];
-    }
-    __syncthreads();
-    // Warp 0: lane w takes partial result w; a butterfly joins the first `m` lanes, a power of two.
-    auto join = [&](const float (*values)[kSlots], int m) {
-#pragma unroll
-      for (int k = 0; k < kSlots; ++k) {
-        if (k >= count) continue;
-        v[k] = values[lane & (m - 1)][k];
-        for (int o = m / 2; o > 0; o >>= 1) {
-          const float other = __shfl_xor_sync(0xffffffffu, v[k], o);
-          v[k] = k < maxima ? max_nan(v[k], other) : v[k] + other;
-        }
-      }
-    };
-    if (warp == 0) {
-      join(warp_values, kWideThreads / 32);
-      if (size > 1 && lane < static_cast<int>(size)) {
-#pragma unroll
-        for (int k = 0; k < kSlots; ++k)
-          if (k < count) store_remote(tc::map_shared(tc::smem_u32(&cluster_values[which][rank][k]), lane), v[k]);
-      }
-      __syncwarp();
-    }
-    if (size > 1) {
-      tc::cluster_sync();
-      if (warp == 0) join(cluster_values[which], static_cast<int>(size));
-    }
+  auto plane_z = [&](int64_t row, int buffer) {
+    return Plane(static_cast<const T*>(a.logits) + row * a.stride + lo, smem + buffer * buffer_bytes,
+                 n * static_cast<int>(sizeof(T)));
+  };
+  auto plane_r = [&](int64_t row, int buffer) {
+    return Plane(kExact ? static_cast<const T*>(a.reference) + row * a.reference_stride + lo : nullptr,
+                 smem + buffer * buffer_bytes + plane, n * static_cast<int>(sizeof(T)));
+  };
+  auto plane_l = [&](int64_t row, int buffer) {
+    return Plane(a.legal ? a.legal + row * a.legal_stride + lo : nullptr,
+                 smem + buffer * buffer_bytes + (kExact ? 2 : 1) * plane, n);
+  };
+  // Thread 0 starts a row's copies. Whatever the block read from and wrote to the buffer is done.
+  auto issue = [&](int64_t row, int buffer) {
+    if (tid != 0 || row >= a.rows) return;
+    const Plane pz = plane_z(row, buffer), pr = plane_r(row, buffer), pl = plane_l(row, buffer);
+    tc::fence_async_smem();
+    tc::bar_expect_tx(&arrived[buffer], pz.inner + pr.inner + pl.inner);
+    pz.copy_units(&arrived[buffer]);
+    if (kExact) pr.copy_units(&arrived[buffer]);
+    pl.copy_units(&arrived[buffer]);
   };
 
   float acc[kTotals] = {};
-  uint32_t phase = 0;
-  for (int64_t row = blockIdx.x / size; row < a.rows; row += clusters) {
-    const T* gz = static_cast<const T*>(a.logits) + row * a.stride + lo;
-    const T* gr = kExact ? static_cast<const T*>(a.reference) + row * a.reference_stride + lo : nullptr;
-    const uint8_t* gl = a.legal ? a.legal + row * a.legal_stride + lo : nullptr;
+  uint32_t turn = 0;  // rows done: the buffer and its barrier's phase
+  const int64_t first = blockIdx.x / size;
+  issue(first, 0);
+  for (int64_t row = first; row < a.rows; row += clusters, ++turn) {
+    const int buffer = buffers == 2 ? turn & 1 : 0;
+    if (buffers == 2) issue(row + clusters, buffer ^ 1);
+    const Plane pz = plane_z(row, buffer), pr = plane_r(row, buffer), pl = plane_l(row, buffer);
+    const bool masked = a.legal != nullptr;
     const int64_t action = a.actions[row];
-    // Entry 0 of each plane, at its own misalignment.
-    unsigned char* pz = smem + (reinterpret_cast<uintptr_t>(gz) & 15);
-    unsigned char* pr = smem + plane + (reinterpret_cast<uintptr_t>(gr) & 15);
-    unsigned char* pl = smem + (kExact ? 2 : 1) * plane + (reinterpret_cast<uintptr_t>(gl) & 15);
-    const int bytes = n * static_cast<int>(sizeof(T));
-    int head_z, head_r = 0, head_l = 0;
-    const uint32_t inner_z = aligned_part(gz, bytes, &head_z);
-    const uint32_t inner_r = kExact ? aligned_part(gr, bytes, &head_r) : 0;
-    const uint32_t inner_l = gl ? aligned_part(gl, n, &head_l) : 0;
-    if (tid == 0) {
-      tc::fence_async_smem();  // what this block wrote to and read from the slices is done
-      tc::bar_expect_tx(&arrived, inner_z + inner_r + inner_l);
-      if (inner_z) tc::bulk_g2s(pz + head_z, reinterpret_cast<const unsigned char*>(gz) + head_z, inner_z, &arrived);
-      if (inner_r) tc::bulk_g2s(pr + head_r, reinterpret_cast<const unsigned char*>(gr) + head_r, inner_r, &arrived);
-      if (inner_l) tc::bulk_g2s(pl + head_l, gl + head_l, inner_l, &arrived);
+    if (pz.head | pz.tail() | pr.head | pr.tail() | pl.head | pl.tail()) {
+      pz.copy_ends(tid);
+      if (kExact) pr.copy_ends(tid);
+      pl.copy_ends(tid);
+      __syncthreads();
     }
-    auto copy_ends = [&](unsigned char* dst, const void* src, int total, int head, uint32_t inner) {
-      const unsigned char* from = static_cast<const unsigned char*>(src);
-      const int tail = total - head - static_cast<int>(inner);
-      if (tid < head) dst[tid] = from[tid];
-      if (tid >= 32 && tid < 32 + tail) dst[head + inner + tid - 32] = from[head + inner + tid - 32];
-    };
-    copy_ends(pz, gz, bytes, head_z, inner_z);
-    if (kExact) copy_ends(pr, gr, bytes, head_r, inner_r);
-    if (gl) copy_ends(pl, gl, n, head_l, inner_l);
-    __syncthreads();
-    tc::bar_wait(&arrived, phase, 0x422);
-    phase ^= 1;
+    tc::bar_wait(&arrived[buffer], (buffers == 2 ? turn >> 1 : turn) & 1u, 0x422);
 
-    T* z = reinterpret_cast<T*>(pz);
-    T* r = reinterpret_cast<T*>(pr);
-    const int head = head_z / static_cast<int>(sizeof(T));  // entries before the first unit
-    const int units = static_cast<int>(inner_z) / 16;
+    T* z = reinterpret_cast<T*>(pz.to);
+    T* r = reinterpret_cast<T*>(pr.to);
+    const uint8_t* legal = pl.to;
+    const int head = pz.head / static_cast<int>(sizeof(T));  // entries before the first unit
+    const int units = static_cast<int>(pz.inner) / 16;
     const int ends = n - units * kVec;  // entries outside the units, head first
-    const bool alike = !kExact || (reinterpret_cast<uintptr_t>(gz) & 15) == (reinterpret_cast<uintptr_t>(gr) & 15);
+    const bool alike = !kExact || ((reinterpret_cast<uintptr_t>(pz.from) ^ reinterpret_cast<uintptr_t>(pr.from)) & 15) == 0;
     auto end_entry = [&](int k) { return k < head ? k : k + units * kVec; };
     auto load_unit = [&](const T* base, int j, bool whole, float (&v)[kVec]) {
       if (whole) {
@@ -526,107 +592,180 @@ __global__ void __launch_bounds__(kWideThreads, 4) anchored_wide_kernel(const Ar
       }
     };
 
-    // Maxima. An illegal entry becomes a logit of minus infinity, here and in the reference.
+    // This thread's maxima. An illegal entry becomes a logit of minus infinity, here and in the reference.
     RowSums s = {};
-    float m[kSlots] = {-INFINITY, -INFINITY, 0.f, 0.f};
-    if (!gl && alike) {
+    float count = 0.f;
+    s.peak = s.reference_peak = -INFINITY;
+    if (!masked && alike) {
       UnitMax<T> top_z, top_r;
 #pragma unroll 4
       for (int u = tid; u < units; u += kWideThreads) {
         top_z.take(*reinterpret_cast<const uint4*>(z + head + u * kVec));
         if (kExact) top_r.take(*reinterpret_cast<const uint4*>(r + head + u * kVec));
       }
-      m[0] = top_z.value();
-      if (kExact) m[1] = top_r.value();
-    }
-    for (int u = !gl && alike ? units : tid; u < units; u += kWideThreads) {
-      const int j = head + u * kVec;
-      float vz[kVec], vr[kVec];
-      load_unit(z, j, true, vz);
-      if (kExact) load_unit(r, j, alike, vr);
-      if (gl) {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const bool in = pl[j + e];
-          m[2] += in ? 1.f : 0.f;
-          vz[e] = in ? vz[e] : -INFINITY;
-          if (kExact) vr[e] = in ? vr[e] : -INFINITY;
-          if (!in) {
-            put(z + j + e, -INFINITY);
-            if (kExact) put(r + j + e, -INFINITY);
-          }
-        }
-      }
-#pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        m[0] = max_nan(m[0], vz[e]);
-        if (kExact) m[1] = max_nan(m[1], vr[e]);
-      }
-    }
-    if (tid < ends) {
-      const int j = end_entry(tid);
-      const bool in = !gl || pl[j];
-      m[2] += in ? 1.f : 0.f;
-      if (!in) {
-        put(z + j, -INFINITY);
-        if (kExact) put(r + j, -INFINITY);
-      } else {
-        m[0] = max_nan(m[0], as_float(z[j]));
-        if (kExact) m[1] = max_nan(m[1], as_float(r[j]));
-      }
-    }
-    reduce(m, 3, 2, 0);
-    if (tid == 0) row_peak = m[0], row_reference_peak = kExact ? m[1] : 0.f;
-    const float count = gl ? m[2] : static_cast<float>(a.width);  // warp 0's
-    __syncthreads();
-    s.peak = row_peak, s.reference_peak = row_reference_peak;
-
-    // Sums.
-    if (s.peak != -INFINITY) {
+      s.peak = top_z.value();
+      if (kExact) s.reference_peak = top_r.value();
+    } else {
       for (int u = tid; u < units; u += kWideThreads) {
         const int j = head + u * kVec;
         float vz[kVec], vr[kVec];
         load_unit(z, j, true, vz);
         if (kExact) load_unit(r, j, alike, vr);
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) add_entry(s, vz[e], kExact ? vr[e] : 0.f, kExact);
+        for (int e = 0; e < kVec; ++e) {
+          const bool in = !masked || legal[j + e];
+          if (!in) {
+            put(z + j + e, -INFINITY);
+            if (kExact) put(r + j + e, -INFINITY);
+          } else {
+            count += 1.f;
+            s.peak = max_nan(s.peak, vz[e]);
+            if (kExact) s.reference_peak = max_nan(s.reference_peak, vr[e]);
+          }
+        }
+      }
+    }
+    if (tid < ends) {
+      const int j = end_entry(tid);
+      if (masked && !legal[j]) {
+        put(z + j, -INFINITY);
+        if (kExact) put(r + j, -INFINITY);
+      } else {
+        count += 1.f;
+        s.peak = max_nan(s.peak, as_float(z[j]));
+        if (kExact) s.reference_peak = max_nan(s.reference_peak, as_float(r[j]));
+      }
+    }
+
+    // This thread's sums.
+    const float reference_base = s.reference_peak == -INFINITY ? 0.f : s.reference_peak;
+    auto sum_tested = [&] {
+      RowSums t = s;
+      t.sum = t.spread = t.apart = t.reference_sum = 0.f;
+      t.peak = s.peak == -INFINITY ? 0.f : s.peak;
+      t.reference_peak = reference_base;
+      for (int u = tid; u < units; u += kWideThreads) {
+        const int j = head + u * kVec;
+        float vz[kVec], vr[kVec];
+        load_unit(z, j, true, vz);
+        if (kExact) load_unit(r, j, alike, vr);
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) add_entry(t, vz[e], kExact ? vr[e] : 0.f, kExact);
       }
       if (tid < ends) {
         const int j = end_entry(tid);
-        add_entry(s, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact);
+        add_entry(t, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact);
       }
-    }
-    float t[kSlots] = {s.sum, s.spread, s.reference_sum, s.apart};
-    reduce(t, kExact ? 4 : 2, 0, 1);
-    if (warp == 0) {
-      s.sum = t[0], s.spread = t[1], s.reference_sum = t[2], s.apart = t[3], s.count = count;
-      const bool inside = action >= 0 && action < a.width;
-      const bool action_legal = inside && (!gl || a.legal[row * a.legal_stride + action]);
-      const float z_a = action_legal ? as_float(static_cast<const T*>(a.logits)[row * a.stride + action]) : -INFINITY;
-      const bool live = row_counts(a, row, action, s, z_a, action_legal, rank == 0 && lane == 0);
-      if (a.log_probs) {
-        if (rank == 0 && lane == 0) a.log_probs[row] = live ? (z_a - s.peak) - logf(s.sum) : 0.f;
-      } else {
-        const RowGrad grad = finish_row(a, row, s, z_a, live, acc);
-        if (lane == 0) row_grad = grad, row_live = live;
+      s.sum = t.sum, s.spread = t.spread, s.apart = t.apart, s.reference_sum = t.reference_sum;
+    };
+    bool tested = masked || !alike;  // whether this thread's entries need tests for minus infinity
+    if (s.peak != -INFINITY) {
+      if (!tested) {
+        const Two from = two(-s.peak, -s.peak), reference_from = two(-reference_base, -reference_base);
+        const Two scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
+        Two sum = two(0.f, 0.f), spread = sum, apart = sum, reference_sum = sum;
+#pragma unroll 2
+        for (int u = tid; u < units; u += kWideThreads) {
+          const int j = head + u * kVec;
+          float vz[kVec], vr[kVec];
+          load_unit(z, j, true, vz);
+          if (kExact) load_unit(r, j, true, vr);
+#pragma unroll
+          for (int e = 0; e < kVec; e += 2) {
+            const Two x = two(vz[e], vz[e + 1]) + from;
+            const Two p = exp2_two(x * scale);
+            sum = sum + p;
+            spread = fma(p, x, spread);
+            if (kExact) {
+              const Two y = two(vr[e], vr[e + 1]) + reference_from;
+              reference_sum = reference_sum + exp2_two(y * scale);
+              apart = fma(p, fma(y, minus, x), apart);
+            }
+          }
+        }
+        const float2 fs = apart_of(sum), fd = apart_of(spread), fa = apart_of(apart), fr = apart_of(reference_sum);
+        s.sum = fs.x + fs.y, s.spread = fd.x + fd.y, s.apart = fa.x + fa.y, s.reference_sum = fr.x + fr.y;
+        if (tid < ends) {
+          const int j = end_entry(tid);
+          add_entry(s, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact);
+        }
+        tested = isnan(s.spread) || isnan(s.apart);
       }
+      if (tested) sum_tested();
+    } else {
+      tested = true;
+      if (kExact) sum_tested();  // the reference's sum counts where this thread has no logit above minus infinity
     }
+
+    Part part = {s.peak, s.reference_peak, s.sum, s.spread, s.reference_sum, s.apart, count};
+    join_lanes<kExact>(part, 32);
+    if (lane == 0) *reinterpret_cast<Part*>(warp_parts[warp]) = part;
     __syncthreads();
-    if (a.log_probs) continue;
-    const RowGrad g = row_grad;
-    const bool counts = row_live;
+    if (warp == 0) {
+      part = *reinterpret_cast<const Part*>(warp_parts[lane & (kWideThreads / 32 - 1)]);
+      join_lanes<kExact>(part, kWideThreads / 32);
+      if (size > 1 && lane < static_cast<int>(size)) {
+        const float* value = reinterpret_cast<const float*>(&part);
+        const uint32_t to = tc::map_shared(tc::smem_u32(cluster_parts[turn & 1][rank]), lane);
+#pragma unroll
+        for (int k = 0; k < kSlots; ++k) store_remote(to + 4 * k, value[k]);
+      }
+      __syncwarp();
+    }
+    if (size > 1) tc::cluster_sync();
+    if (warp == 0) {
+      if (size > 1) {
+        part = *reinterpret_cast<const Part*>(cluster_parts[turn & 1][lane & (size - 1)]);
+        join_lanes<kExact>(part, static_cast<int>(size));
+      }
+      const RowSums t = {part.peak, part.sum, part.spread, part.apart, kExact ? part.reference_peak : 0.f, part.reference_sum,
+                         masked ? part.count : static_cast<float>(a.width)};
+      const bool inside = action >= 0 && action < a.width;
+      const bool action_legal = inside && (!masked || a.legal[row * a.legal_stride + action]);
+      const float z_a = action_legal ? as_float(static_cast<const T*>(a.logits)[row * a.stride + action]) : -INFINITY;
+      const bool live = row_counts(a, row, action, t, z_a, action_legal, rank == 0 && lane == 0);
+      if (a.log_probs) {
+        if (rank == 0 && lane == 0) a.log_probs[row] = live ? (z_a - t.peak) - logf(t.sum) : 0.f;
+      } else {
+        const RowGrad grad = finish_row(a, row, t, z_a, live, acc);
+        if (lane == 0) row_grad = grad, row_live = live, row_peak = t.peak;
+      }
+    }
     if (a.grad) {
+      __syncthreads();
+      const RowGrad g = row_grad;
+      const float peak = row_peak;
+      const bool counts = row_live;
+      // Large coefficients could take a finite difference past the largest float: then a probability of zero is tested.
+      tested |= g.alpha > 0.5f || g.beta > 0.5f;
       T* out = static_cast<T*>(a.grad) + row * a.grad_stride + lo;
-      const bool alike_out = (reinterpret_cast<uintptr_t>(gz) & 15) == (reinterpret_cast<uintptr_t>(out) & 15);
+      const bool alike_out = ((reinterpret_cast<uintptr_t>(pz.from) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
       const int64_t at = action - lo;  // the action inside this slice
+      const Two from = two(-peak, -peak), scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
+      const Two inv_sum = two(g.inv_sum, g.inv_sum), alpha = two(g.alpha, g.alpha), beta = two(g.beta, g.beta),
+                constant = two(g.constant, g.constant);
+#pragma unroll 2
       for (int u = tid; u < units; u += kWideThreads) {
         const int j = head + u * kVec;
         float vz[kVec], vr[kVec], v[kVec];
         load_unit(z, j, true, vz);
         if (kExact) load_unit(r, j, alike, vr);
+        if (!counts) {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          v[e] = counts ? gradient_entry(g, s.peak, vz[e], kExact ? vr[e] : 0.f, kExact) : 0.f;
+          for (int e = 0; e < kVec; ++e) v[e] = 0.f;
+        } else if (tested) {
+#pragma unroll
+          for (int e = 0; e < kVec; ++e) v[e] = gradient_entry(g, peak, vz[e], kExact ? vr[e] : 0.f, kExact);
+        } else {
+#pragma unroll
+          for (int e = 0; e < kVec; e += 2) {
+            const Two zz = two(vz[e], vz[e + 1]);
+            const Two x = zz + from;
+            Two k = fma(alpha, x, constant);
+            if (kExact) k = fma(beta, fma(two(vr[e], vr[e + 1]), minus, zz), k);
+            const float2 f = apart_of(exp2_two(x * scale) * inv_sum * k);
+            v[e] = f.x, v[e + 1] = f.y;
+          }
         }
         if (counts && at >= j && at < j + kVec) {
 #pragma unroll
@@ -642,15 +781,17 @@ __global__ void __launch_bounds__(kWideThreads, 4) anchored_wide_kernel(const Ar
       }
       if (tid < ends) {
         const int j = end_entry(tid);
-        float v = counts ? gradient_entry(g, s.peak, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact) : 0.f;
+        float v = counts ? gradient_entry(g, peak, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact) : 0.f;
         if (counts && at == j) v += g.action;
         put(out + j, v);
       }
     }
-    __syncthreads();  // the slices may be overwritten
+    __syncthreads();  // the buffer may be overwritten
+    if (buffers == 1) issue(row + clusters, 0);
   }
   if (!a.log_probs && rank == 0 && tid == 0)
     for (int k = 0; k < kTotals; ++k) a.partial[blockIdx.x / size * kTotals + k] = acc[k];
+  __syncwarp();
   if (size > 1) tc::cluster_sync();  // no block leaves while another may still write to its shared memory
 }
 
@@ -786,7 +927,9 @@ int run_wide(const Args& a, int* blocks, cudaStream_t s, bool* fits) {
   }();
   if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "anchored_wide_kernel: %s", cudaGetErrorString(configured));
   constexpr int kPlanes = kExact ? 2 : 1;
-  auto shared_of = [&](int slice) { return kPlanes * (slice * static_cast<int>(sizeof(T)) + 32) + (a.legal ? slice + 32 : 0); };
+  auto shared_of = [&](int slice) {  // a multiple of 16: slices are
+    return kPlanes * (slice * static_cast<int>(sizeof(T)) + 32) + (a.legal ? slice + 32 : 0);
+  };
   int size = 1, slice = 0, shared = 0;
   for (;; size *= 2) {
     // Slices of whole units, so that every block's slice is aligned as the row is.
@@ -803,13 +946,15 @@ int run_wide(const Args& a, int* blocks, cudaStream_t s, bool* fits) {
   }
   *fits = shared <= kSharedPerBlock;
   if (!*fits) return CG_OK;
-  const int per_sm = std::max(1, std::min(4, kSharedPerSm / (shared + 2048)));
+  // Two buffers where three blocks an SM still fit.
+  const int buffers = 2 * shared <= kSliceBytes ? 2 : 1;
+  const int per_sm = std::max(1, std::min(3, kSharedPerSm / (buffers * shared + 2048)));
   const int clusters = static_cast<int>(std::min<int64_t>(a.rows, std::max(1, per_sm * sm_count() / size)));
   *blocks = clusters;  // one partial sum a cluster
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(clusters * size));
   config.blockDim = dim3(kWideThreads);
-  config.dynamicSmemBytes = shared;
+  config.dynamicSmemBytes = buffers * shared;
   config.stream = s;
   cudaLaunchAttribute attribute[1];
   attribute[0].id = cudaLaunchAttributeClusterDimension;
@@ -817,7 +962,7 @@ int run_wide(const Args& a, int* blocks, cudaStream_t s, bool* fits) {
   attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
   config.attrs = attribute;
   config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, slice, clusters);
+  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, slice, clusters, shared, buffers);
   if (err != cudaSuccess) return set_error(CG_ERR_CUDA, "anchored_wide_kernel launch: %s", cudaGetErrorString(err));
   return check_launch("anchored_wide_kernel");
 }
