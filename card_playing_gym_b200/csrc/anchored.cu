@@ -18,13 +18,12 @@
 #include <algorithm>
 
 #include "elements.cuh"
-#include "tcgen05.cuh"
 
 namespace cg {
 namespace {
 
 constexpr int kTotals = 9;
-constexpr int kPartials = 1184;  // the grid's upper bound: a fixed order of addition for a given row count
+constexpr int kPartials = 4736;  // the grid's upper bound: a fixed order of addition for a given row count
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -57,49 +56,68 @@ __device__ __forceinline__ float max_nan(float x, float y) {
   return m;
 }
 
-// A row's sums over its legal entries.
+// A row's sums over its legal entries, relative to a base near the largest logit (every formula is the same for any
+// base; one within kLazy of the maximum keeps the exponentials in range).
 struct RowSums {
-  float peak, sum;              // max z, sum e with e = exp(z - max z)
-  float spread;                 // sum e (z - max z)
-  float apart;                  // sum e ((z - max z) - (r - max r))
-  float reference_peak, reference_sum;
+  float peak, sum;              // the base m, sum e with e = exp(z - m)
+  float spread;                 // sum e (z - m)
+  float apart;                  // sum e ((z - m) - (r - m_r))
+  float reference_peak, reference_sum;  // m_r, sum exp(r - m_r)
   float count;                  // legal entries
 };
+constexpr float kLazy = 8.f;
 
 // What the gradient pass needs of a row.
 struct RowGrad {
   float inv_sum, constant, beta, alpha, action;
 };
 
+// What a row brings beside its planes, loaded before the planes are waited for.
+struct RowIn {
+  int64_t action;
+  float weight, advantage, old_log_prob, reference_log_prob;
+};
+
+__device__ __forceinline__ RowIn load_row(const Args& a, int64_t row) {
+  RowIn in = {a.actions[row], 1.f, 0.f, 0.f, 0.f};
+  if (!a.log_probs) {
+    in.weight = a.weights[row];
+    in.advantage = a.advantages[row];
+    in.old_log_prob = a.old_log_probs[row];
+    if (a.reference_action) in.reference_log_prob = a.reference_action[row];
+  }
+  return in;
+}
+
 // The row's contribution to the totals (zeros unless it counts) and its gradient's coefficients.
 // z_a: the action's logit, minus infinity where it is illegal.
-__device__ __forceinline__ RowGrad finish_row(const Args& a, int64_t row, const RowSums& s, float z_a, bool counts,
+__device__ __forceinline__ RowGrad finish_row(const Args& a, const RowIn& in, const RowSums& s, float z_a, bool counts,
                                               float (&acc)[kTotals]) {
   RowGrad g = {0.f, 0.f, 0.f, 0.f, 0.f};
   if (!counts) return g;
-  const float w = a.weights[row], advantage = a.advantages[row];
-  const float log_sum = logf(s.sum);
+  const float w = in.weight, advantage = in.advantage;
+  const float log_sum = __logf(s.sum);
   const float lp = (z_a - s.peak) - log_sum;
-  const float log_ratio = lp - a.old_log_probs[row];
-  const float ratio = expf(log_ratio);
+  const float log_ratio = lp - in.old_log_prob;
+  const float ratio = __expf(log_ratio);
   const float free = ratio * advantage;
   const float bounded = fminf(fmaxf(ratio, 1.f - a.clip), 1.f + a.clip) * advantage;
   const bool held = free > bounded;
   const float surrogate = -(held ? bounded : free);
   float slope = held ? 0.f : -advantage * ratio;
-  const float entropy = log_sum - s.spread / s.sum;
+  g.inv_sum = __fdividef(1.f, s.sum);
+  const float entropy = log_sum - s.spread * g.inv_sum;
   const bool eligible = s.count > 1.f;
-  const float norm = eligible ? 1.f / logf(s.count) : 0.f;
+  const float norm = eligible ? __fdividef(1.f, __logf(s.count)) : 0.f;
   float kl = 0.f, log_apart = 0.f;
-  g.inv_sum = 1.f / s.sum;
   if (a.reference) {
-    log_apart = log_sum - logf(s.reference_sum);
+    log_apart = log_sum - __logf(s.reference_sum);
     kl = s.apart * g.inv_sum - log_apart;
     g.beta = w * a.beta;
   } else if (a.reference_action) {
-    const float u = a.reference_action[row] - lp;
-    kl = expf(u) - u - 1.f;
-    slope += a.beta * (1.f - expf(u));
+    const float u = in.reference_log_prob - lp, grown = __expf(u);
+    kl = grown - u - 1.f;
+    slope += a.beta * (1.f - grown);
   }
   g.alpha = w * a.alpha * norm;
   g.action = w * slope;
@@ -119,10 +137,9 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, int64_t row, const 
 
 // Whether a row counts: it has an action inside the vocabulary and something legal, and for the objective its
 // weight is not zero and its action is legal. Bad actions set the fault word.
-__device__ __forceinline__ bool row_counts(const Args& a, int64_t row, int64_t action, const RowSums& s, float z_a,
-                                           bool action_legal, bool report) {
-  if (action < 0) return false;
-  if (action >= a.width) {
+__device__ __forceinline__ bool row_counts(const Args& a, const RowIn& in, const RowSums& s, bool action_legal, bool report) {
+  if (in.action < 0) return false;
+  if (in.action >= a.width) {
     if (report) raise_fault(0x420);
     return false;
   }
@@ -132,7 +149,7 @@ __device__ __forceinline__ bool row_counts(const Args& a, int64_t row, int64_t a
     if (report) raise_fault(0x421);
     return false;
   }
-  return a.weights[row] != 0.f;
+  return in.weight != 0.f;
 }
 
 // dL/dz of an entry that is not the action. A probability of zero has a zero gradient whatever it is multiplied by.
@@ -258,7 +275,9 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
     const T* gz = static_cast<const T*>(a.logits) + row * a.stride;
     const T* gr = exact ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
     const uint8_t* gl = a.legal ? a.legal + row * a.legal_stride : nullptr;
-    const int64_t action = live ? a.actions[row] : -1;
+    RowIn in_row = {-1, 0.f, 0.f, 0.f, 0.f};
+    if (live) in_row = load_row(a, row);
+    const int64_t action = in_row.action;
     // Illegal entries, and those past the row, are minus infinity.
     float z[kPer], r[kPer], z_a = 0.f, count = 0.f;
     bool mine = false;
@@ -343,12 +362,12 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
       s.reference_sum = reduce(s.reference_sum, false);
       s.apart = reduce(s.apart, false);
     }
-    const bool counts = row_counts(a, row, action, s, z_a, action_legal, l == 0);
+    const bool counts = row_counts(a, in_row, s, action_legal, l == 0);
     if (a.log_probs) {
       if (live && l == 0) a.log_probs[row] = counts ? (z_a - s.peak) - logf(s.sum) : 0.f;
       continue;
     }
-    const RowGrad g = finish_row(a, row, s, z_a, counts, acc);  // every lane of the group keeps the same totals
+    const RowGrad g = finish_row(a, in_row, s, z_a, counts, acc);  // every lane of the group keeps the same totals
     if (!a.grad || !live) continue;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
 #pragma unroll
@@ -389,37 +408,27 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
   }
 }
 
-// ---- wider rows: a row in the shared memory of a cluster --------------------------------------------------------------
-// The row is read once, by bulk copies, and stays in shared memory for its maxima, its sums and its gradient. A cluster
-// of C blocks holds it, C the least that leaves room for three blocks an SM, so that one block's copies and barriers
-// run under another's arithmetic; narrow slices have two buffers, the next row's copies running under this one's arithmetic.
-// Every thread sums its own entries relative to its own maxima, and the maxima and sums are joined once, over the
-// block and then over the cluster through each other's shared memory: one cluster barrier a row.
+// ---- wider rows: a block a row ------------------------------------------------------------------------------------------
+// A thread holds its share of the row, or of a batch of it, in registers as it is in memory: up to four units of sixteen
+// bytes of each plane in flight at a time. It sums a batch relative to the batch's own maxima and merges the result into
+// its running sums, so the row's maxima are never waited for; the block joins its threads once a row.
+// A row of one batch (kHeld) is read once and its gradient computed from the registers. A longer one is read again for
+// the gradient, out of L2: the blocks are made so large that the rows in work at one time fit there (see run_wide).
 //
-// What bounds it is instruction issue beside HBM: three exponentials an entry and, in pairs of packed fp32
-// arithmetic, some 20 instructions. Entries at minus infinity, which the packed sums turn into NaN, are found by
-// that and summed again with tests.
-//
-// Slices are copied with the alignment they have in memory: the sixteen-byte units inside by the copy engine, the few
-// bytes at the ends by threads. The arithmetic runs over the same units; planes whose rows are aligned differently
-// from the logits' are read entry by entry from shared memory.
-constexpr int kWideThreads = 256;
-constexpr int kMaxCluster = 16;
+// What bounds it is instruction issue beside memory: three exponentials an entry and, in packed fp32 pairs, some 20
+// instructions. Entries at minus infinity, which the packed sums turn into NaN, are found by that and summed again
+// with tests. Units start where the logits' row is aligned; the few entries before and after them go one a
+// thread, and planes aligned differently from the logits' are read entry by entry.
 
-// Partial results over some entries, each relative to their own maxima.
+// Partial results over some entries, each relative to their own maxima. `tested`: minus infinity was among them.
 struct Part {
-  float peak, reference_peak, sum, spread, reference_sum, apart, count;
+  float peak, reference_peak, sum, spread, reference_sum, apart, count, tested;
 };
-constexpr int kSlots = sizeof(Part) / sizeof(float);
+__device__ __forceinline__ Part no_part() { return {-INFINITY, -INFINITY, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}; }
 
-// The parts of 2^steps neighbouring lanes (or of the whole warp) joined; every lane gets the result.
+// The part relative to larger maxima.
 template <bool kExact>
-__device__ __forceinline__ void join_lanes(Part& p, int lanes) {
-  float peak = p.peak, reference_peak = p.reference_peak;
-  for (int o = lanes / 2; o > 0; o >>= 1) {
-    peak = max_nan(peak, __shfl_xor_sync(0xffffffffu, peak, o));
-    if (kExact) reference_peak = max_nan(reference_peak, __shfl_xor_sync(0xffffffffu, reference_peak, o));
-  }
+__device__ __forceinline__ void rebase(Part& p, float peak, float reference_peak) {
   const float up = p.peak == -INFINITY ? 0.f : p.peak - peak;
   const float scale = p.peak == -INFINITY ? 0.f : exp2_fast(up * kLog2e);
   if (kExact) {
@@ -427,19 +436,45 @@ __device__ __forceinline__ void join_lanes(Part& p, int lanes) {
     p.reference_sum *= p.reference_peak == -INFINITY ? 0.f : exp2_fast(reference_up * kLog2e);
     // Without a reference entry above minus infinity the part's differences are infinite already.
     p.apart = scale == 0.f ? 0.f : scale * fmaf(up - reference_up, p.sum, p.apart);
+    p.reference_peak = reference_peak;
   }
   p.spread = scale == 0.f ? 0.f : scale * fmaf(up, p.sum, p.spread);
   p.sum = scale == 0.f ? 0.f : scale * p.sum;
-  p.peak = peak, p.reference_peak = reference_peak;
-  for (int o = lanes / 2; o > 0; o >>= 1) {
+  p.peak = peak;
+}
+
+// Bases for more entries whose maxima are top and reference_top: the part keeps its own, so that its sums need no scaling,
+// unless an exponential would pass exp(kLazy).
+template <bool kExact>
+__device__ __forceinline__ void lift(Part& p, float top, float reference_top) {
+  if (top <= p.peak + kLazy && (!kExact || reference_top <= p.reference_peak + kLazy) && p.peak != -INFINITY) return;
+  const float peak = top <= p.peak + kLazy ? p.peak : top;
+  const float reference_peak = reference_top <= p.reference_peak + kLazy ? p.reference_peak : reference_top;
+  rebase<kExact>(p, max_nan(p.peak, peak), max_nan(p.reference_peak, reference_peak));
+}
+
+__device__ __forceinline__ float warp_max_nan(float v) {
+  float m;
+  asm("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
+// The parts of the first `lanes` lanes of a warp joined (the others hold no_part()); lane 0 gets the result.
+template <bool kExact>
+__device__ __forceinline__ void join_lanes(Part& p, int lanes, bool masked) {
+  rebase<kExact>(p, warp_max_nan(p.peak), kExact ? warp_max_nan(p.reference_peak) : 0.f);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    if (o >= lanes) continue;
     p.sum += __shfl_xor_sync(0xffffffffu, p.sum, o);
     p.spread += __shfl_xor_sync(0xffffffffu, p.spread, o);
-    p.count += __shfl_xor_sync(0xffffffffu, p.count, o);
     if (kExact) {
       p.reference_sum += __shfl_xor_sync(0xffffffffu, p.reference_sum, o);
       p.apart += __shfl_xor_sync(0xffffffffu, p.apart, o);
     }
+    if (masked) p.count += __shfl_xor_sync(0xffffffffu, p.count, o);
   }
+  p.tested = __any_sync(0xffffffffu, p.tested != 0.f) ? 1.f : 0.f;
 }
 
 // Two fp32 values in one register pair, added, multiplied and combined in one instruction.
@@ -476,412 +511,346 @@ __device__ __forceinline__ Two exp2_two(Two x) {
   return two(exp2_fast(f.x), exp2_fast(f.y));
 }
 
-// The bytes before the first sixteen-byte boundary of `bytes` bytes at `src`, and those in whole units after it.
-__device__ __forceinline__ uint32_t aligned_part(const void* src, int bytes, int* head) {
-  const int lead = static_cast<int>((16 - (reinterpret_cast<uintptr_t>(src) & 15)) & 15);
-  *head = min(lead, bytes);
-  return static_cast<uint32_t>((bytes - *head) & ~15);
-}
-
-__device__ __forceinline__ void store_remote(uint32_t address, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(address), "f"(v) : "memory");
-}
-
-// One plane of a row's slice: where it is in memory and where in shared memory, at the same misalignment.
-struct Plane {
-  const unsigned char* from;
-  unsigned char* to;  // entry 0
-  int bytes, head;
-  uint32_t inner;
-  __device__ __forceinline__ Plane(const void* src, unsigned char* base, int size) {
-    from = static_cast<const unsigned char*>(src);
-    to = base + (reinterpret_cast<uintptr_t>(src) & 15);
-    bytes = src ? size : 0;
-    inner = aligned_part(src, bytes, &head);
+// A row's planes, and where its units and the entries outside them are.
+template <typename T>
+struct Row {
+  const T* z;
+  const T* r;
+  const uint8_t* legal;
+  int width, head, units, ends;
+  bool alike;
+  __device__ __forceinline__ Row(const Args& a, int64_t row) {
+    z = static_cast<const T*>(a.logits) + row * a.stride;
+    r = a.reference ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
+    legal = a.legal ? a.legal + row * a.legal_stride : nullptr;
+    width = a.width;
+    const uintptr_t lead = (16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15;
+    head = min(static_cast<int>(lead / sizeof(T)), width);
+    units = (width - head) / kVector<T>;
+    ends = width - units * kVector<T>;
+    alike = !r || ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(r)) & 15) == 0;
   }
-  __device__ __forceinline__ int tail() const { return bytes - head - static_cast<int>(inner); }
-  __device__ __forceinline__ void copy_units(uint64_t* barrier) const {
-    if (inner) tc::bulk_g2s(to + head, from + head, inner, barrier);
-  }
-  __device__ __forceinline__ void copy_ends(int tid) const {
-    if (tid < head) to[tid] = from[tid];
-    if (tid >= 32 && tid < 32 + tail()) to[head + inner + tid - 32] = from[head + inner + tid - 32];
-  }
+  __device__ __forceinline__ int unit_entry(int unit) const { return head + unit * kVector<T>; }
+  __device__ __forceinline__ int end_entry(int k) const { return k < head ? k : k + units * kVector<T>; }
+  __device__ __forceinline__ bool in(int j) const { return !legal || legal[j]; }
 };
 
-template <typename T, bool kExact>
-__global__ void __launch_bounds__(kWideThreads, 3) anchored_wide_kernel(const Args a, int slice, int clusters, int buffer_bytes,
-                                                                        int buffers) {
-  constexpr int kVec = kVector<T>;
-  extern __shared__ __align__(16) unsigned char smem[];
-  __shared__ __align__(8) uint64_t arrived[2];
-  __shared__ float warp_parts[kWideThreads / 32][kSlots], cluster_parts[2][kMaxCluster][kSlots];
-  __shared__ RowGrad row_grad;
-  __shared__ float row_peak;
-  __shared__ bool row_live;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  uint32_t rank = 0, size = 1;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-  const int plane = slice * static_cast<int>(sizeof(T)) + 32;  // a slice and its misalignment
-  const int lo = static_cast<int>(rank) * slice;
-  const int n = max(0, min(slice, a.width - lo));
-  if (tid == 0) {
-    tc::bar_init(&arrived[0], 1);
-    tc::bar_init(&arrived[1], 1);
-    tc::bar_fence_init();
+// Minus infinity in the entries of a unit whose mask byte is zero.
+template <typename T>
+__device__ __forceinline__ void hide(uint4& unit, uint2 mask) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&unit);
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[e] = mask.x >> (8 * e) & 255u ? w[e] : 0xff800000u;
+  } else {
+    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t bytes = (e < 2 ? mask.x : mask.y) >> (16 * (e & 1));
+      const uint32_t keep = (bytes & 0xffu ? 0x0000ffffu : 0u) | (bytes & 0xff00u ? 0xffff0000u : 0u);
+      w[e] = (w[e] & keep) | (kInf & ~keep);
+    }
   }
-  __syncthreads();
-  if (size > 1) tc::cluster_sync();
-
-  auto plane_z = [&](int64_t row, int buffer) {
-    return Plane(static_cast<const T*>(a.logits) + row * a.stride + lo, smem + buffer * buffer_bytes,
-                 n * static_cast<int>(sizeof(T)));
-  };
-  auto plane_r = [&](int64_t row, int buffer) {
-    return Plane(kExact ? static_cast<const T*>(a.reference) + row * a.reference_stride + lo : nullptr,
-                 smem + buffer * buffer_bytes + plane, n * static_cast<int>(sizeof(T)));
-  };
-  auto plane_l = [&](int64_t row, int buffer) {
-    return Plane(a.legal ? a.legal + row * a.legal_stride + lo : nullptr,
-                 smem + buffer * buffer_bytes + (kExact ? 2 : 1) * plane, n);
-  };
-  // Thread 0 starts a row's copies. Whatever the block read from and wrote to the buffer is done.
-  auto issue = [&](int64_t row, int buffer) {
-    if (tid != 0 || row >= a.rows) return;
-    const Plane pz = plane_z(row, buffer), pr = plane_r(row, buffer), pl = plane_l(row, buffer);
-    tc::fence_async_smem();
-    tc::bar_expect_tx(&arrived[buffer], pz.inner + pr.inner + pl.inner);
-    pz.copy_units(&arrived[buffer]);
-    if (kExact) pr.copy_units(&arrived[buffer]);
-    pl.copy_units(&arrived[buffer]);
-  };
-
-  float acc[kTotals] = {};
-  uint32_t turn = 0;  // rows done: the buffer and its barrier's phase
-  const int64_t first = blockIdx.x / size;
-  issue(first, 0);
-  for (int64_t row = first; row < a.rows; row += clusters, ++turn) {
-    const int buffer = buffers == 2 ? turn & 1 : 0;
-    if (buffers == 2) issue(row + clusters, buffer ^ 1);
-    const Plane pz = plane_z(row, buffer), pr = plane_r(row, buffer), pl = plane_l(row, buffer);
-    const bool masked = a.legal != nullptr;
-    const int64_t action = a.actions[row];
-    if (pz.head | pz.tail() | pr.head | pr.tail() | pl.head | pl.tail()) {
-      pz.copy_ends(tid);
-      if (kExact) pr.copy_ends(tid);
-      pl.copy_ends(tid);
-      __syncthreads();
-    }
-    tc::bar_wait(&arrived[buffer], (buffers == 2 ? turn >> 1 : turn) & 1u, 0x422);
-
-    T* z = reinterpret_cast<T*>(pz.to);
-    T* r = reinterpret_cast<T*>(pr.to);
-    const uint8_t* legal = pl.to;
-    const int head = pz.head / static_cast<int>(sizeof(T));  // entries before the first unit
-    const int units = static_cast<int>(pz.inner) / 16;
-    const int ends = n - units * kVec;  // entries outside the units, head first
-    const bool alike = !kExact || ((reinterpret_cast<uintptr_t>(pz.from) ^ reinterpret_cast<uintptr_t>(pr.from)) & 15) == 0;
-    auto end_entry = [&](int k) { return k < head ? k : k + units * kVec; };
-    auto load_unit = [&](const T* base, int j, bool whole, float (&v)[kVec]) {
-      if (whole) {
-        unpack(*reinterpret_cast<const uint4*>(base + j), v, T());
-      } else {
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) v[e] = as_float(base[j + e]);
-      }
-    };
-
-    // This thread's maxima. An illegal entry becomes a logit of minus infinity, here and in the reference.
-    RowSums s = {};
-    float count = 0.f;
-    s.peak = s.reference_peak = -INFINITY;
-    if (!masked && alike) {
-      UnitMax<T> top_z, top_r;
-#pragma unroll 4
-      for (int u = tid; u < units; u += kWideThreads) {
-        top_z.take(*reinterpret_cast<const uint4*>(z + head + u * kVec));
-        if (kExact) top_r.take(*reinterpret_cast<const uint4*>(r + head + u * kVec));
-      }
-      s.peak = top_z.value();
-      if (kExact) s.reference_peak = top_r.value();
-    } else {
-      for (int u = tid; u < units; u += kWideThreads) {
-        const int j = head + u * kVec;
-        float vz[kVec], vr[kVec];
-        load_unit(z, j, true, vz);
-        if (kExact) load_unit(r, j, alike, vr);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const bool in = !masked || legal[j + e];
-          if (!in) {
-            put(z + j + e, -INFINITY);
-            if (kExact) put(r + j + e, -INFINITY);
-          } else {
-            count += 1.f;
-            s.peak = max_nan(s.peak, vz[e]);
-            if (kExact) s.reference_peak = max_nan(s.reference_peak, vr[e]);
-          }
-        }
-      }
-    }
-    if (tid < ends) {
-      const int j = end_entry(tid);
-      if (masked && !legal[j]) {
-        put(z + j, -INFINITY);
-        if (kExact) put(r + j, -INFINITY);
-      } else {
-        count += 1.f;
-        s.peak = max_nan(s.peak, as_float(z[j]));
-        if (kExact) s.reference_peak = max_nan(s.reference_peak, as_float(r[j]));
-      }
-    }
-
-    // This thread's sums.
-    const float reference_base = s.reference_peak == -INFINITY ? 0.f : s.reference_peak;
-    auto sum_tested = [&] {
-      RowSums t = s;
-      t.sum = t.spread = t.apart = t.reference_sum = 0.f;
-      t.peak = s.peak == -INFINITY ? 0.f : s.peak;
-      t.reference_peak = reference_base;
-      for (int u = tid; u < units; u += kWideThreads) {
-        const int j = head + u * kVec;
-        float vz[kVec], vr[kVec];
-        load_unit(z, j, true, vz);
-        if (kExact) load_unit(r, j, alike, vr);
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) add_entry(t, vz[e], kExact ? vr[e] : 0.f, kExact);
-      }
-      if (tid < ends) {
-        const int j = end_entry(tid);
-        add_entry(t, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact);
-      }
-      s.sum = t.sum, s.spread = t.spread, s.apart = t.apart, s.reference_sum = t.reference_sum;
-    };
-    bool tested = masked || !alike;  // whether this thread's entries need tests for minus infinity
-    if (s.peak != -INFINITY) {
-      if (!tested) {
-        const Two from = two(-s.peak, -s.peak), reference_from = two(-reference_base, -reference_base);
-        const Two scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
-        Two sum = two(0.f, 0.f), spread = sum, apart = sum, reference_sum = sum;
-#pragma unroll 2
-        for (int u = tid; u < units; u += kWideThreads) {
-          const int j = head + u * kVec;
-          float vz[kVec], vr[kVec];
-          load_unit(z, j, true, vz);
-          if (kExact) load_unit(r, j, true, vr);
-#pragma unroll
-          for (int e = 0; e < kVec; e += 2) {
-            const Two x = two(vz[e], vz[e + 1]) + from;
-            const Two p = exp2_two(x * scale);
-            sum = sum + p;
-            spread = fma(p, x, spread);
-            if (kExact) {
-              const Two y = two(vr[e], vr[e + 1]) + reference_from;
-              reference_sum = reference_sum + exp2_two(y * scale);
-              apart = fma(p, fma(y, minus, x), apart);
-            }
-          }
-        }
-        const float2 fs = apart_of(sum), fd = apart_of(spread), fa = apart_of(apart), fr = apart_of(reference_sum);
-        s.sum = fs.x + fs.y, s.spread = fd.x + fd.y, s.apart = fa.x + fa.y, s.reference_sum = fr.x + fr.y;
-        if (tid < ends) {
-          const int j = end_entry(tid);
-          add_entry(s, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact);
-        }
-        tested = isnan(s.spread) || isnan(s.apart);
-      }
-      if (tested) sum_tested();
-    } else {
-      tested = true;
-      if (kExact) sum_tested();  // the reference's sum counts where this thread has no logit above minus infinity
-    }
-
-    Part part = {s.peak, s.reference_peak, s.sum, s.spread, s.reference_sum, s.apart, count};
-    join_lanes<kExact>(part, 32);
-    if (lane == 0) *reinterpret_cast<Part*>(warp_parts[warp]) = part;
-    __syncthreads();
-    if (warp == 0) {
-      part = *reinterpret_cast<const Part*>(warp_parts[lane & (kWideThreads / 32 - 1)]);
-      join_lanes<kExact>(part, kWideThreads / 32);
-      if (size > 1 && lane < static_cast<int>(size)) {
-        const float* value = reinterpret_cast<const float*>(&part);
-        const uint32_t to = tc::map_shared(tc::smem_u32(cluster_parts[turn & 1][rank]), lane);
-#pragma unroll
-        for (int k = 0; k < kSlots; ++k) store_remote(to + 4 * k, value[k]);
-      }
-      __syncwarp();
-    }
-    if (size > 1) tc::cluster_sync();
-    if (warp == 0) {
-      if (size > 1) {
-        part = *reinterpret_cast<const Part*>(cluster_parts[turn & 1][lane & (size - 1)]);
-        join_lanes<kExact>(part, static_cast<int>(size));
-      }
-      const RowSums t = {part.peak, part.sum, part.spread, part.apart, kExact ? part.reference_peak : 0.f, part.reference_sum,
-                         masked ? part.count : static_cast<float>(a.width)};
-      const bool inside = action >= 0 && action < a.width;
-      const bool action_legal = inside && (!masked || a.legal[row * a.legal_stride + action]);
-      const float z_a = action_legal ? as_float(static_cast<const T*>(a.logits)[row * a.stride + action]) : -INFINITY;
-      const bool live = row_counts(a, row, action, t, z_a, action_legal, rank == 0 && lane == 0);
-      if (a.log_probs) {
-        if (rank == 0 && lane == 0) a.log_probs[row] = live ? (z_a - t.peak) - logf(t.sum) : 0.f;
-      } else {
-        const RowGrad grad = finish_row(a, row, t, z_a, live, acc);
-        if (lane == 0) row_grad = grad, row_live = live, row_peak = t.peak;
-      }
-    }
-    if (a.grad) {
-      __syncthreads();
-      const RowGrad g = row_grad;
-      const float peak = row_peak;
-      const bool counts = row_live;
-      // Large coefficients could take a finite difference past the largest float: then a probability of zero is tested.
-      tested |= g.alpha > 0.5f || g.beta > 0.5f;
-      T* out = static_cast<T*>(a.grad) + row * a.grad_stride + lo;
-      const bool alike_out = ((reinterpret_cast<uintptr_t>(pz.from) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-      const int64_t at = action - lo;  // the action inside this slice
-      const Two from = two(-peak, -peak), scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
-      const Two inv_sum = two(g.inv_sum, g.inv_sum), alpha = two(g.alpha, g.alpha), beta = two(g.beta, g.beta),
-                constant = two(g.constant, g.constant);
-#pragma unroll 2
-      for (int u = tid; u < units; u += kWideThreads) {
-        const int j = head + u * kVec;
-        float vz[kVec], vr[kVec], v[kVec];
-        load_unit(z, j, true, vz);
-        if (kExact) load_unit(r, j, alike, vr);
-        if (!counts) {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) v[e] = 0.f;
-        } else if (tested) {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) v[e] = gradient_entry(g, peak, vz[e], kExact ? vr[e] : 0.f, kExact);
-        } else {
-#pragma unroll
-          for (int e = 0; e < kVec; e += 2) {
-            const Two zz = two(vz[e], vz[e + 1]);
-            const Two x = zz + from;
-            Two k = fma(alpha, x, constant);
-            if (kExact) k = fma(beta, fma(two(vr[e], vr[e + 1]), minus, zz), k);
-            const float2 f = apart_of(exp2_two(x * scale) * inv_sum * k);
-            v[e] = f.x, v[e + 1] = f.y;
-          }
-        }
-        if (counts && at >= j && at < j + kVec) {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            if (at == j + e) v[e] += g.action;
-        }
-        if (alike_out) {
-          *reinterpret_cast<uint4*>(out + j) = repack(v, T());
-        } else {
-#pragma unroll
-          for (int e = 0; e < kVec; ++e) put(out + j + e, v[e]);
-        }
-      }
-      if (tid < ends) {
-        const int j = end_entry(tid);
-        float v = counts ? gradient_entry(g, peak, as_float(z[j]), kExact ? as_float(r[j]) : 0.f, kExact) : 0.f;
-        if (counts && at == j) v += g.action;
-        put(out + j, v);
-      }
-    }
-    __syncthreads();  // the buffer may be overwritten
-    if (buffers == 1) issue(row + clusters, 0);
-  }
-  if (!a.log_probs && rank == 0 && tid == 0)
-    for (int k = 0; k < kTotals; ++k) a.partial[blockIdx.x / size * kTotals + k] = acc[k];
-  __syncwarp();
-  if (size > 1) tc::cluster_sync();  // no block leaves while another may still write to its shared memory
 }
 
-// ---- any width: one block per row, the row read once for its maxima, once for its sums, once for its gradient ---
-constexpr int kStreamThreads = 512;
-
-template <int kOp>  // 0: sum, 1: max
-__device__ __forceinline__ float block_reduce(float v, float* scratch) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float other = __shfl_xor_sync(0xffffffffu, v, o);
-    v = kOp ? max_nan(v, other) : v + other;
+// The mask bytes of a unit: one or two aligned words where they lie inside the row, else byte by byte.
+template <typename T>
+__device__ __forceinline__ uint2 mask_bytes(const Row<T>& row, int j) {
+  constexpr int kVec = kVector<T>;
+  const uint8_t* p = row.legal + j;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & (kVec - 1));
+  uint2 m = make_uint2(0, 0);
+  if (j - off >= 0 && j - off + 2 * kVec <= row.width) {
+    if constexpr (kVec == 8) {
+      const uint64_t* w = reinterpret_cast<const uint64_t*>(p - off);
+      uint64_t v = w[0];
+      if (off) v = v >> (8 * off) | w[1] << (64 - 8 * off);
+      m = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
+      m.x = off ? __funnelshift_r(w[0], w[1], 8 * off) : w[0];
+    }
+    return m;
   }
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) scratch[threadIdx.x >> 5] = v;
-  __syncthreads();
-  float out = scratch[0];
-  for (int w = 1; w < static_cast<int>(blockDim.x >> 5); ++w) out = kOp ? max_nan(out, scratch[w]) : out + scratch[w];
-  return out;
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    const uint32_t b = p[e];
+    if (e < 4)
+      m.x |= b << (8 * e);
+    else
+      m.y |= b << (8 * (e - 4));
+  }
+  return m;
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kStreamThreads) anchored_stream_kernel(const Args a) {
-  __shared__ float scratch[kStreamThreads / 32];
+__device__ __forceinline__ uint4 gather_unit(const T* p) {
+  T v[kVector<T>];
+#pragma unroll
+  for (int e = 0; e < kVector<T>; ++e) v[e] = p[e];
+  return *reinterpret_cast<const uint4*>(v);
+}
+
+// One unit of a row, what the mask hides at minus infinity; the number of legal entries is added to `count`.
+template <typename T, bool kExact>
+__device__ __forceinline__ void load_unit(const Row<T>& row, int j, uint4& z, uint4& r, float& count) {
+  z = *reinterpret_cast<const uint4*>(row.z + j);
+  if (kExact) r = row.alike ? *reinterpret_cast<const uint4*>(row.r + j) : gather_unit(row.r + j);
+  if (!row.legal) return;
+  const uint2 m = mask_bytes(row, j);
+  count += static_cast<float>((__popc(__vcmpne4(m.x, 0)) + __popc(__vcmpne4(m.y, 0))) >> 3);
+  hide<T>(z, m);
+  if (kExact) hide<T>(r, m);
+}
+
+// A batch's units, the first `n` of which exist, added to a part.
+template <typename T, bool kExact, int kUnits>
+__device__ __forceinline__ void add_units(Part& p, const uint4 (&z)[kUnits], const uint4 (&r)[kUnits], int n) {
+  constexpr int kVec = kVector<T>;
+  UnitMax<T> top_z, top_r;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (i >= n) continue;
+    top_z.take(z[i]);
+    if (kExact) top_r.take(r[i]);
+  }
+  lift<kExact>(p, top_z.value(), kExact ? top_r.value() : 0.f);
+  const float base = p.peak == -INFINITY ? 0.f : p.peak;
+  const float reference_base = p.reference_peak == -INFINITY ? 0.f : p.reference_peak;
+  const Two from = two(-base, -base), reference_from = two(-reference_base, -reference_base);
+  const Two scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
+  Two sum = two(0.f, 0.f), spread = sum, apart = sum, reference_sum = sum;
+#pragma unroll
+  for (int i = 0; i < kUnits; ++i) {
+    if (i >= n) continue;
+    float vz[kVec], vr[kVec];
+    unpack(z[i], vz, T());
+    if (kExact) unpack(r[i], vr, T());
+#pragma unroll
+    for (int e = 0; e < kVec; e += 2) {
+      const Two x = two(vz[e], vz[e + 1]) + from;
+      const Two e2 = exp2_two(x * scale);
+      sum = sum + e2;
+      spread = fma(e2, x, spread);
+      if (kExact) {
+        const Two y = two(vr[e], vr[e + 1]) + reference_from;
+        reference_sum = reference_sum + exp2_two(y * scale);
+        apart = fma(e2, fma(y, minus, x), apart);
+      }
+    }
+  }
+  float2 fs = apart_of(sum), fd = apart_of(spread), fa = apart_of(apart), fr = apart_of(reference_sum);
+  const float odd = (fd.x + fd.y) + (fa.x + fa.y);
+  if (isnan(odd)) {
+    p.tested = 1.f;
+    RowSums t = {};
+    t.peak = base, t.reference_peak = reference_base;
+#pragma unroll
+    for (int i = 0; i < kUnits; ++i) {
+      if (i >= n) continue;
+      float vz[kVec], vr[kVec];
+      unpack(z[i], vz, T());
+      if (kExact) unpack(r[i], vr, T());
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) add_entry(t, vz[e], kExact ? vr[e] : 0.f, kExact);
+    }
+    fs = make_float2(t.sum, 0.f), fd = make_float2(t.spread, 0.f), fa = make_float2(t.apart, 0.f);
+    fr = make_float2(t.reference_sum, 0.f);
+  }
+  p.sum += fs.x + fs.y, p.spread += fd.x + fd.y;
+  if (kExact) p.apart += fa.x + fa.y, p.reference_sum += fr.x + fr.y;
+}
+
+// An entry outside the units added to a part.
+template <typename T, bool kExact>
+__device__ __forceinline__ void add_end(Part& p, const Row<T>& row, int j) {
+  if (!row.in(j)) return;
+  const float z = as_float(row.z[j]), r = kExact ? as_float(row.r[j]) : 0.f;
+  lift<kExact>(p, z, r);
+  RowSums t = {};
+  t.peak = p.peak == -INFINITY ? 0.f : p.peak, t.reference_peak = p.reference_peak == -INFINITY ? 0.f : p.reference_peak;
+  add_entry(t, z, r, kExact);
+  p.sum += t.sum, p.spread += t.spread, p.count += 1.f;
+  if (kExact) p.apart += t.apart, p.reference_sum += t.reference_sum;
+}
+
+// The gradient of a unit.
+template <typename T, bool kExact>
+__device__ __forceinline__ uint4 gradient_unit(const RowGrad& g, float peak, bool tested, const uint4& z, const uint4& r,
+                                               int at) {
+  constexpr int kVec = kVector<T>;
+  float vz[kVec], vr[kVec], v[kVec];
+  unpack(z, vz, T());
+  if (kExact) unpack(r, vr, T());
+  if (tested) {
+#pragma unroll
+    for (int e = 0; e < kVec; ++e) v[e] = gradient_entry(g, peak, vz[e], kExact ? vr[e] : 0.f, kExact);
+  } else {
+    const Two from = two(-peak, -peak), scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
+    const Two inv_sum = two(g.inv_sum, g.inv_sum), alpha = two(g.alpha, g.alpha), beta = two(g.beta, g.beta),
+              constant = two(g.constant, g.constant);
+#pragma unroll
+    for (int e = 0; e < kVec; e += 2) {
+      const Two zz = two(vz[e], vz[e + 1]);
+      const Two x = zz + from;
+      Two k = fma(alpha, x, constant);
+      if (kExact) k = fma(beta, fma(two(vr[e], vr[e + 1]), minus, zz), k);
+      const float2 f = apart_of(exp2_two(x * scale) * inv_sum * k);
+      v[e] = f.x, v[e + 1] = f.y;
+    }
+  }
+  if (at >= 0) {  // the action's place in the unit
+#pragma unroll
+    for (int e = 0; e < kVec; ++e)
+      if (at == e) v[e] += g.action;
+  }
+  return repack(v, T());
+}
+
+// What a row's gradient needs, from the warp that finishes the row to the others.
+struct RowOut {
+  RowGrad grad;
+  float peak;
+  int live, tested;
+};
+
+template <typename T, bool kExact, int kThreads, bool kHeld>
+__global__ void __launch_bounds__(kThreads, (kThreads >= 512 ? 1024 : 768) / kThreads) anchored_row_kernel(const Args a) {
+  constexpr int kUnits = kThreads >= 512 ? 2 : 4, kWarps = kThreads / 32, kVec = kVector<T>;
+  __shared__ Part warp_parts[2][kWarps];
+  __shared__ RowOut row_out[2];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float acc[kTotals] = {};
-  const bool exact = a.reference != nullptr;
-  for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    const T* z = static_cast<const T*>(a.logits) + row * a.stride;
-    const T* r = exact ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
-    const uint8_t* legal = a.legal ? a.legal + row * a.legal_stride : nullptr;
-    const int64_t action = a.actions[row];
-    RowSums s = {};
-    float peak = -INFINITY, reference_peak = -INFINITY, count = 0.f;
-    for (int j = threadIdx.x; j < a.width; j += kStreamThreads) {
-      if (legal && !legal[j]) continue;
-      peak = max_nan(peak, as_float(z[j]));
-      if (exact) reference_peak = max_nan(reference_peak, as_float(r[j]));
-      count += 1.f;
+  int turn = 0;  // rows done: what the warps exchange alternates, so that two barriers a row are enough
+  for (int64_t index = blockIdx.x; index < a.rows; index += gridDim.x, turn ^= 1) {
+    const Row<T> row(a, index);
+    const bool masked = row.legal != nullptr;
+    const RowIn in = load_row(a, index);
+    bool action_legal = in.action >= 0 && in.action < a.width;
+    float z_a = -INFINITY;
+    uint4 z[kUnits], r[kUnits];
+    Part part = no_part();
+    constexpr int kBatch = kUnits * kThreads;  // units of a batch
+    // A batch's units, all in flight; returns how many this thread has.
+    auto load_batch = [&](int first) {
+      int n = 0;
+      if (!masked && row.alike && first + kBatch <= row.units) {
+        const T* from_z = row.z + row.unit_entry(first + tid);
+        const T* from_r = row.r + row.unit_entry(first + tid);
+#pragma unroll
+        for (int i = 0; i < kUnits; ++i) {
+          z[i] = *reinterpret_cast<const uint4*>(from_z + i * kThreads * kVec);
+          if (kExact) r[i] = *reinterpret_cast<const uint4*>(from_r + i * kThreads * kVec);
+        }
+        return kUnits;
+      }
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = first + tid + i * kThreads;
+        if (u >= row.units) continue;
+        load_unit<T, kExact>(row, row.unit_entry(u), z[i], r[i], part.count);
+        n = i + 1;
+      }
+      return n;
+    };
+    const int held = load_batch(0);
+    if (warp == 0 && action_legal) {
+      action_legal = row.in(static_cast<int>(in.action));
+      if (action_legal) z_a = as_float(row.z[in.action]);
     }
-    s.peak = block_reduce<1>(peak, scratch);
-    if (exact) s.reference_peak = block_reduce<1>(reference_peak, scratch);
-    s.count = block_reduce<0>(count, scratch);
-    // Nothing to exponentiate: every sum stays zero.
-    const bool any = s.peak != -INFINITY;
-    for (int j = threadIdx.x; any && j < a.width; j += kStreamThreads) {
-      if (legal && !legal[j]) continue;
-      add_entry(s, as_float(z[j]), exact ? as_float(r[j]) : 0.f, exact);
+    add_units<T, kExact, kUnits>(part, z, r, held);
+    if (!kHeld) {
+      for (int first = kBatch; first < row.units; first += kBatch) {
+        const int n = load_batch(first);
+        add_units<T, kExact, kUnits>(part, z, r, n);
+      }
     }
-    s.sum = block_reduce<0>(s.sum, scratch);
-    s.spread = block_reduce<0>(s.spread, scratch);
-    if (exact) {
-      s.reference_sum = block_reduce<0>(s.reference_sum, scratch);
-      s.apart = block_reduce<0>(s.apart, scratch);
+    if (tid < row.ends) add_end<T, kExact>(part, row, row.end_entry(tid));
+    join_lanes<kExact>(part, 32, masked);
+    if (lane == 0) warp_parts[turn][warp] = part;
+    __syncthreads();
+    if (warp == 0) {
+      part = lane < kWarps ? warp_parts[turn][lane] : no_part();
+      join_lanes<kExact>(part, kWarps, masked);
+      const RowSums s = {part.peak, part.sum, part.spread, part.apart, kExact ? part.reference_peak : 0.f, part.reference_sum,
+                         masked ? part.count : static_cast<float>(a.width)};
+      const bool live = row_counts(a, in, s, action_legal, lane == 0);
+      if (a.log_probs) {
+        if (lane == 0) a.log_probs[index] = live ? (z_a - s.peak) - logf(s.sum) : 0.f;
+      } else {
+        const RowGrad g = finish_row(a, in, s, z_a, live, acc);
+        // Large coefficients could take a finite difference past the largest float: then a probability of zero is tested.
+        if (lane == 0) row_out[turn] = {g, s.peak, live, part.tested != 0.f || g.alpha > 0.5f || g.beta > 0.5f};
+      }
     }
-    const bool inside = action >= 0 && action < a.width;
-    const bool action_legal = inside && (!legal || legal[action]);
-    const float z_a = action_legal ? as_float(z[action]) : -INFINITY;
-    const bool counts = row_counts(a, row, action, s, z_a, action_legal, threadIdx.x == 0);
-    if (a.log_probs) {
-      if (threadIdx.x == 0) a.log_probs[row] = counts ? (z_a - s.peak) - logf(s.sum) : 0.f;
-      continue;
-    }
-    const RowGrad g = finish_row(a, row, s, z_a, counts, acc);
     if (!a.grad) continue;
-    T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
-    for (int j = threadIdx.x; j < a.width; j += kStreamThreads) {
+    __syncthreads();
+    const RowOut o = row_out[turn];
+    T* out = static_cast<T*>(a.grad) + index * a.grad_stride;
+    const bool alike_out = ((reinterpret_cast<uintptr_t>(row.z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const int action_unit = in.action >= row.head ? (static_cast<int>(in.action) - row.head) / kVec : -1;
+    const int action_entry = (static_cast<int>(in.action) - row.head) % kVec;
+    auto store_batch = [&](int first) {
+      T* to = out + row.unit_entry(first + tid);
+      const bool whole = first + kBatch <= row.units;
+#pragma unroll
+      for (int i = 0; i < kUnits; ++i) {
+        const int u = first + tid + i * kThreads;
+        if (!whole && u >= row.units) continue;
+        const uint4 v = o.live ? gradient_unit<T, kExact>(o.grad, o.peak, o.tested, z[i], r[i], u == action_unit ? action_entry : -1)
+                               : make_uint4(0, 0, 0, 0);
+        if (alike_out) {
+          __stcs(reinterpret_cast<uint4*>(to + i * kThreads * kVec), v);
+        } else {
+          const T* e = reinterpret_cast<const T*>(&v);
+#pragma unroll
+          for (int k = 0; k < kVec; ++k) to[i * kThreads * kVec + k] = e[k];
+        }
+      }
+    };
+    if (kHeld) {
+      store_batch(0);
+    } else {
+      for (int first = 0; first < row.units; first += kBatch) {
+        load_batch(first);
+        store_batch(first);
+      }
+    }
+    if (tid < row.ends) {
+      const int j = row.end_entry(tid);
       float v = 0.f;
-      if (counts && !(legal && !legal[j])) {
-        v = gradient_entry(g, s.peak, as_float(z[j]), exact ? as_float(r[j]) : 0.f, exact);
-        if (j == action) v += g.action;
+      if (o.live && row.in(j)) {
+        v = gradient_entry(o.grad, o.peak, as_float(row.z[j]), kExact ? as_float(row.r[j]) : 0.f, kExact);
+        if (j == in.action) v += o.grad.action;
       }
       put(out + j, v);
     }
   }
-  if (!a.log_probs && threadIdx.x == 0)
+  if (!a.log_probs && tid == 0)
     for (int k = 0; k < kTotals; ++k) a.partial[blockIdx.x * kTotals + k] = acc[k];
 }
 
-// Warp k sums total k over the blocks: lane l the partials l, l + 32, ..., then a butterfly. The last total, the
-// objective, is written once more after them.
-__global__ void __launch_bounds__(kTotals * 32) anchored_totals_kernel(const double* partial, int count, float* totals) {
-  const int lane = threadIdx.x & 31, k = threadIdx.x >> 5;
+// Every total over the blocks: thread (g, k) takes total k of the blocks g, g + 112, ... in order, then one thread a total
+// the 112 sums in order. The last total, the objective, is written once more after them.
+constexpr int kTotalGroups = 112;
+
+__global__ void __launch_bounds__(1024) anchored_totals_kernel(const double* partial, int count, float* totals) {
+  __shared__ double sums[kTotalGroups][kTotals];
+  const int g = threadIdx.x / kTotals, k = threadIdx.x % kTotals;
   pdl_wait();
-  double total = 0;
+  if (g < kTotalGroups) {
+    double total = 0;
 #pragma unroll 8
-  for (int b = lane; b < count; b += 32) total += partial[b * kTotals + k];
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-  if (lane == 0) totals[k] = static_cast<float>(total);
-  if (lane == 0 && k == kTotals - 1) totals[kTotals] = static_cast<float>(total);
+    for (int b = g; b < count; b += kTotalGroups) total += partial[b * kTotals + k];
+    sums[g][k] = total;
+  }
+  __syncthreads();
+  if (threadIdx.x >= kTotals) return;
+  double total = 0;
+#pragma unroll 16
+  for (int i = 0; i < kTotalGroups; ++i) total += sums[i][k];
+  totals[k] = static_cast<float>(total);
+  if (k == kTotals - 1) totals[kTotals] = static_cast<float>(total);
 }
 
 // A gradient times the gradient of the objective. The usual one is 1, and then there is nothing to do.
@@ -914,61 +883,30 @@ int run_narrow(const Args& a, int* blocks, cudaStream_t s) {
   return check_launch("anchored_narrow_kernel");
 }
 
-constexpr int kSharedPerSm = 227 * 1024;
-constexpr int kSharedPerBlock = 224 * 1024;           // beside the static part
-constexpr int kSliceBytes = kSharedPerSm / 3 - 2048;  // three blocks an SM
-
-template <typename T, bool kExact>
-int run_wide(const Args& a, int* blocks, cudaStream_t s, bool* fits) {
-  auto kernel = anchored_wide_kernel<T, kExact>;
-  static const cudaError_t configured = [&] {
-    const cudaError_t rc = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedPerBlock);
-    return rc != cudaSuccess ? rc : cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  }();
-  if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "anchored_wide_kernel: %s", cudaGetErrorString(configured));
-  constexpr int kPlanes = kExact ? 2 : 1;
-  auto shared_of = [&](int slice) {  // a multiple of 16: slices are
-    return kPlanes * (slice * static_cast<int>(sizeof(T)) + 32) + (a.legal ? slice + 32 : 0);
-  };
-  int size = 1, slice = 0, shared = 0;
-  for (;; size *= 2) {
-    // Slices of whole units, so that every block's slice is aligned as the row is.
-    const int64_t each = (static_cast<int64_t>(a.width) + size - 1) / size;
-    if (each < (1 << 20)) {
-      slice = static_cast<int>((each + 15) / 16 * 16);
-      shared = shared_of(slice);
-      if (shared <= kSliceBytes) break;
-      if (size == kMaxCluster) break;
-    } else if (size == kMaxCluster) {
-      shared = kSharedPerBlock + 1;
-      break;
-    }
-  }
-  *fits = shared <= kSharedPerBlock;
-  if (!*fits) return CG_OK;
-  // Two buffers where three blocks an SM still fit.
-  const int buffers = 2 * shared <= kSliceBytes ? 2 : 1;
-  const int per_sm = std::max(1, std::min(3, kSharedPerSm / (buffers * shared + 2048)));
-  const int clusters = static_cast<int>(std::min<int64_t>(a.rows, std::max(1, per_sm * sm_count() / size)));
-  *blocks = clusters;  // one partial sum a cluster
-  cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(clusters * size));
-  config.blockDim = dim3(kWideThreads);
-  config.dynamicSmemBytes = buffers * shared;
-  config.stream = s;
-  cudaLaunchAttribute attribute[1];
-  attribute[0].id = cudaLaunchAttributeClusterDimension;
-  attribute[0].val.clusterDim.x = size;
-  attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
-  config.attrs = attribute;
-  config.numAttrs = 1;
-  const cudaError_t err = cudaLaunchKernelEx(&config, kernel, a, slice, clusters, shared, buffers);
-  if (err != cudaSuccess) return set_error(CG_ERR_CUDA, "anchored_wide_kernel launch: %s", cudaGetErrorString(err));
-  return check_launch("anchored_wide_kernel");
+template <typename T, bool kExact, int kThreads, bool kHeld>
+int run_row(const Args& a, int* blocks, cudaStream_t s) {
+  static const int resident = resident_blocks(anchored_row_kernel<T, kExact, kThreads, kHeld>, kThreads);
+  *blocks = static_cast<int>(std::min<int64_t>(a.rows, resident));
+  anchored_row_kernel<T, kExact, kThreads, kHeld><<<*blocks, kThreads, 0, s>>>(a);
+  return check_launch("anchored_row_kernel");
 }
 
-// A row goes where it fits: registers of four lanes (64 entries) or of a warp (1024), a cluster's shared memory, or nowhere
-// (it is streamed three times).
+// The smallest block that holds the row in its registers, else the smallest whose resident blocks' rows stay in L2
+// between their two readings (80 of its 126 MB, the rest for the gradient passing through).
+template <typename T, bool kExact>
+int run_wide(const Args& a, int* blocks, cudaStream_t s) {
+  constexpr int kHeldEntries = 4 * kVector<T>;  // a thread's
+  if (a.width <= 64 * kHeldEntries) return run_row<T, kExact, 64, true>(a, blocks, s);
+  if (a.width <= 128 * kHeldEntries) return run_row<T, kExact, 128, true>(a, blocks, s);
+  if (a.width <= 256 * kHeldEntries) return run_row<T, kExact, 256, true>(a, blocks, s);
+  const int64_t row_bytes = static_cast<int64_t>(a.width) * sizeof(T) * (kExact ? 2 : 1), room = int64_t{80} << 20;
+  if (!a.grad || 4 * sm_count() * row_bytes <= room) return run_row<T, kExact, 256, false>(a, blocks, s);
+  if (2 * sm_count() * row_bytes <= room) return run_row<T, kExact, 512, false>(a, blocks, s);
+  return run_row<T, kExact, 1024, false>(a, blocks, s);
+}
+
+// A row goes where it fits: registers of four lanes (64 entries), of a warp (1024) or of a block, or a block that reads it
+// twice.
 template <typename T>
 int run_typed(const Args& a, int* blocks, cudaStream_t s) {
   constexpr int kUnit = 8 / kVector<T>;  // vectors of eight entries
@@ -976,12 +914,7 @@ int run_typed(const Args& a, int* blocks, cudaStream_t s) {
   if (a.width <= 256) return run_narrow<T, 32, kUnit>(a, blocks, s);
   if (a.width <= 512) return run_narrow<T, 32, 2 * kUnit>(a, blocks, s);
   if (a.width <= 1024) return run_narrow<T, 32, 4 * kUnit>(a, blocks, s);
-  bool fits = false;
-  if (int rc = a.reference ? run_wide<T, true>(a, blocks, s, &fits) : run_wide<T, false>(a, blocks, s, &fits)) return rc;
-  if (fits) return CG_OK;
-  *blocks = static_cast<int>(std::min<int64_t>(a.rows, kPartials));
-  anchored_stream_kernel<T><<<*blocks, kStreamThreads, 0, s>>>(a);
-  return check_launch("anchored_stream_kernel");
+  return a.reference ? run_wide<T, true>(a, blocks, s) : run_wide<T, false>(a, blocks, s);
 }
 
 int run_rows(const Args& a, int dtype, int* blocks, cudaStream_t s) {
@@ -1026,7 +959,7 @@ extern "C" int cg_anchored_objective(const void* logits, int dtype, int64_t rows
                     clip_ratio, beta, alpha};
     if (int rc = run_rows(a, dtype, &blocks, s)) return rc;
   }
-  return launch_pdl("anchored_totals_kernel", anchored_totals_kernel, dim3(1), dim3(kTotals * 32), 0, s,
+  return launch_pdl("anchored_totals_kernel", anchored_totals_kernel, dim3(1), dim3(1024), 0, s,
                     static_cast<const double*>(partial), blocks, totals);
 }
 

@@ -262,7 +262,9 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
     grad_stride = stride if stride <= width + 64 else width
     grad = None
     if want_grad:
-        grad = torch.empty((rows, grad_stride), dtype=logits.dtype, device=logits.device)[:, :width]
+        grad = torch.empty((rows, grad_stride), dtype=logits.dtype, device=logits.device)
+        if grad_stride != width:
+            grad = grad[:, :width]
     sums = torch.empty(len(ANCHORED_KEYS) + 1, device=logits.device)  # the totals, and the objective once more
     need = nat.query("cg_anchored_objective_workspace_bytes", rows)
     with nat.on_device(logits.device):
