@@ -43,12 +43,6 @@ struct Args {
   float clip, beta, alpha;
 };
 
-__device__ __forceinline__ float exp2_fast(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // The larger value, a NaN if either is one (fmaxf would drop it, and a row of NaN would pass for an empty one).
 __device__ __forceinline__ float max_nan(float x, float y) {
   float m;
@@ -477,35 +471,6 @@ __device__ __forceinline__ void join_lanes(Part& p, int lanes, bool masked) {
   p.tested = __any_sync(0xffffffffu, p.tested != 0.f) ? 1.f : 0.f;
 }
 
-// Two fp32 values in one register pair, added, multiplied and combined in one instruction.
-struct Two {
-  uint64_t v;
-};
-__device__ __forceinline__ Two two(float lo, float hi) {
-  Two t;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(lo), "f"(hi));
-  return t;
-}
-__device__ __forceinline__ float2 apart_of(Two t) {
-  float2 f;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(t.v));
-  return f;
-}
-__device__ __forceinline__ Two operator+(Two a, Two b) {
-  Two t;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
-  return t;
-}
-__device__ __forceinline__ Two operator*(Two a, Two b) {
-  Two t;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
-  return t;
-}
-__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
-  Two t;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return t;
-}
 __device__ __forceinline__ Two exp2_two(Two x) {
   const float2 f = apart_of(x);
   return two(exp2_fast(f.x), exp2_fast(f.y));

@@ -96,11 +96,9 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const T* __restrict__ dy,
       for (int r = 0; r < kRows; ++r) {
         const int64_t i = i0 + 8 * r;
         if (i >= hi) continue;
+        if constexpr (kActivation != kActNone) times_slope<T, kActivation>(g[r], z[r]);
 #pragma unroll
-        for (int k = 0; k < kVec; ++k) {
-          if (kActivation != kActNone) g[r][k] *= activation_slope<T, kActivation>(z[r][k]);
-          sum[k] += g[r][k];
-        }
+        for (int k = 0; k < kVec; ++k) sum[k] += g[r][k];
         if (dpre) {
 #pragma unroll
           for (int k = 0; k < kVec; k += 4) {

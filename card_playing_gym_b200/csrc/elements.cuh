@@ -103,51 +103,99 @@ struct OperandOf<float> {
   using type = __nv_bfloat16;
 };
 
+// Two fp32 values in one register pair, added, multiplied and combined in one instruction.
+struct Two {
+  uint64_t v;
+};
+__device__ __forceinline__ Two two(float lo, float hi) {
+  Two t;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(t.v) : "f"(lo), "f"(hi));
+  return t;
+}
+__device__ __forceinline__ float2 apart_of(Two t) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(t.v));
+  return f;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+  Two t;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+  return t;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+  Two t;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(t.v) : "l"(a.v), "l"(b.v));
+  return t;
+}
+__device__ __forceinline__ Two fma(Two a, Two b, Two c) {
+  Two t;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return t;
+}
 // ---- activations ---------------------------------------------------------------------------------------------------
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ float reciprocal_fast(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
-// Phi(z) of the normal distribution and exp(-z^2 / 2), for 16-bit results: erfc by Abramowitz and Stegun 7.1.26,
-// t p(t) exp(-u^2) with u = |z| / sqrt 2, t = 1 / (1 + 0.3275911 u), within 1.5e-7 of erfc, a thousandth
-// of what the result's own rounding moves. One exponential serves the derivative too.
-__device__ __forceinline__ float normal_cumulative(float z, float* bell) {
-  const float t = reciprocal_fast(fmaf(0.3275911f * 0.70710678118654752f, fabsf(z), 1.f));
-  const float e = __expf(-0.5f * z * z);
-  float poly = fmaf(1.061405429f, t, -1.453152027f);
-  poly = fmaf(poly, t, 1.421413741f);
-  poly = fmaf(poly, t, -0.284496736f);
-  poly = fmaf(poly, t, 0.254829592f);
-  const float tail = 0.5f * poly * t * e;
+// Phi(z) of the normal distribution and exp(-z^2 / 2) for two z's, for 16-bit results: erfc by Abramowitz and
+// Stegun 7.1.26, t p(t) exp(-u^2) with u = |z| / sqrt 2, t = 1 / (1 + 0.3275911 u), within 1.5e-7 of erfc, a thousandth of
+// what the result's own rounding moves. One exponential serves the derivative too; the packed arithmetic halves
+// the rest.
+__device__ __forceinline__ Two normal_cumulative(Two z, Two* bell) {
+  const float2 f = apart_of(z);
+  const Two u = fma(two(fabsf(f.x), fabsf(f.y)), two(0.23164190f, 0.23164190f), two(1.f, 1.f));  // 0.3275911 / sqrt 2
+  const float2 fu = apart_of(u);
+  const Two t = two(reciprocal_fast(fu.x), reciprocal_fast(fu.y));
+  const float2 fe = apart_of(z * z * two(-0.72134752f, -0.72134752f));  // log2(e) / 2
+  const Two e = two(exp2_fast(fe.x), exp2_fast(fe.y));
+  Two poly = fma(two(0.5307027145f, 0.5307027145f), t, two(-0.7265760135f, -0.7265760135f));  // half of p's coefficients
+  poly = fma(poly, t, two(0.7107068705f, 0.7107068705f));
+  poly = fma(poly, t, two(-0.142248368f, -0.142248368f));
+  poly = fma(poly, t, two(0.127414796f, 0.127414796f));
+  const float2 tail = apart_of(poly * t * e);
   *bell = e;
-  return z < 0.f ? tail : 1.f - tail;
+  return two(f.x < 0.f ? tail.x : 1.f - tail.x, f.y < 0.f ? tail.y : 1.f - tail.y);
 }
 
 template <typename T, int kActivation>
 __device__ __forceinline__ float activate(float z) {
   if constexpr (kActivation == kActRelu) return z < 0.f ? 0.f : z;  // a NaN stays one
-  if constexpr (kActivation == kActGelu) {
-    if constexpr (sizeof(T) == 4) return gelu_erf(z);
-    float bell;
-    return z * normal_cumulative(z, &bell);
-  }
+  if constexpr (kActivation == kActGelu) return gelu_erf(z);
   if constexpr (kActivation == kActSilu) return __fdividef(z, 1.f + __expf(-z));
   return z;
+}
+
+// kCount (even) values at once.
+template <typename T, int kActivation, int kCount>
+__device__ __forceinline__ void activate4(float (&z)[kCount]) {
+  if constexpr (kActivation == kActGelu && sizeof(T) == 2) {
+#pragma unroll
+    for (int k = 0; k < kCount; k += 2) {
+      const Two v = two(z[k], z[k + 1]);
+      Two bell;
+      const float2 y = apart_of(v * normal_cumulative(v, &bell));
+      z[k] = y.x, z[k + 1] = y.y;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) z[k] = activate<T, kActivation>(z[k]);
+  }
 }
 
 template <typename T, int kActivation>
 __device__ __forceinline__ float activation_slope(float z) {
   if constexpr (kActivation == kActRelu) return z > 0.f ? 1.f : z == z ? 0.f : z;
   if constexpr (kActivation == kActGelu) {
-    float bell, cumulative;
-    if constexpr (sizeof(T) == 4) {
-      cumulative = 0.5f * (1.f + erff(z * 0.70710678118654752f));
-      bell = __expf(-0.5f * z * z);
-    } else {
-      cumulative = normal_cumulative(z, &bell);
-    }
+    const float cumulative = 0.5f * (1.f + erff(z * 0.70710678118654752f));
+    const float bell = __expf(-0.5f * z * z);
     return bell == 0.f ? cumulative : fmaf(z * 0.3989422804014327f, bell, cumulative);  // an infinity times zero
   }
   if constexpr (kActivation == kActSilu) {
@@ -155,6 +203,26 @@ __device__ __forceinline__ float activation_slope(float z) {
     return gate == 0.f ? 0.f : gate * fmaf(z, 1.f - gate, 1.f);
   }
   return 1.f;
+}
+
+// g *= act'(z) for kCount (even) values.
+template <typename T, int kActivation, int kCount>
+__device__ __forceinline__ void times_slope(float (&g)[kCount], const float (&z)[kCount]) {
+  if constexpr (kActivation == kActGelu && sizeof(T) == 2) {
+#pragma unroll
+    for (int k = 0; k < kCount; k += 2) {
+      // Past 14 the bell is zero, and an infinity times it is to be zero too.
+      const Two v = two(z[k], z[k + 1]);
+      const Two near = two(fminf(fmaxf(z[k], -14.f), 14.f), fminf(fmaxf(z[k + 1], -14.f), 14.f));
+      Two bell;
+      const Two cumulative = normal_cumulative(v, &bell);
+      const float2 y = apart_of(two(g[k], g[k + 1]) * fma(near * two(0.3989422804f, 0.3989422804f), bell, cumulative));
+      g[k] = y.x, g[k + 1] = y.y;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < kCount; ++k) g[k] *= activation_slope<T, kActivation>(z[k]);
+  }
 }
 
 // `body` with the activation as a constant.

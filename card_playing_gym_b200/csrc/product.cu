@@ -11,12 +11,14 @@
 //   warp 9     allocates tensor memory; in the even CTA lane 0 issues the MMAs
 // Loads of both CTAs complete on the even CTA's barriers; MMA completions are committed to both CTAs'.
 //
-// float32 operands are three bfloat16 parts each (8 bits of mantissa apiece, the parts exact): the six products of
-// parts that reach 2^-24 of the result run as one longer sum, the smallest first, at 6/1 of the bfloat16 work. The
-// tensor cores cut their running sum at each step (measured: 1.7e-8 of it, always toward zero), which a long
-// float32 sum would show: after kChunkBlocks blocks of k the epilogue takes the sum into registers, where it is
-// added with rounding, and the next chunk starts from zero in the other accumulator. 16-bit results keep one
-// running sum: at 8192 k's the cut is 9e-6 against their own rounding of 2^-11 or 2^-8.
+// float32 operands are three bfloat16 parts each (8 bits of mantissa apiece): the six products of parts that reach 2^-24 of
+// the result run from one stage that holds all three parts of both operands, at six times the bfloat16 work and
+// three times its traffic. The tensor cores cut their running sum at each step (measured: 1.7e-8 of it, always
+// toward zero), which a long float32 sum would show: the five small products have an accumulator of their own,
+// and after kChunkBlocks blocks of k the epilogue takes both sums into registers, where they are added with
+// rounding, and the next chunk starts from zero in the other pair of accumulators. tile_n is 128 for it, so that two
+// pairs fit tensor memory. 16-bit results keep one running sum: at 8192 k's the cut is 9e-6 against their own
+// rounding of 2^-11 or 2^-8.
 //
 // Where the tiles do not fill the chip's pairs, k is split: every split writes fp32 partial sums and
 // product_join_kernel adds them in order and applies the epilogue.
@@ -33,23 +35,27 @@ namespace cg {
 namespace {
 
 constexpr int kTileM = 256, kTileK = 64;  // a pair's rows; k's of a stage (128 bytes of 16-bit entries)
-constexpr int kStages = 6;
-constexpr int kHalfBytes = 128 * kTileK * 2;  // one CTA's A (or B at tile_n 256) of a stage
-constexpr int kStageBytes = 2 * kHalfBytes;
+constexpr int kHalfBytes = 128 * kTileK * 2;  // one CTA's rows of A (or of B at tile_n 256) of a stage
 constexpr int kEpilogueWarps = 8;
 constexpr int kLoadWarp = 8, kMmaWarp = 9;
 constexpr int kThreads = 10 * 32;
 constexpr int kSquareBytes = 32 * 32 * 4;
-constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSquareBytes + 1024;
-constexpr int kAccumulatorColumns = 256;
-constexpr int kBoxRows = 64;          // rows of a box of an operand stored across
-constexpr int kLeastSplitBlocks = 8;  // k blocks a split is worth: its partial tile costs 512 KB of traffic
-constexpr int kChunkBlocks = 4;       // k blocks (256 k's) of one running sum of a float32 product: 16 steps a part
-constexpr int kParts = 6;             // products of parts of a float32 product
+constexpr int kAccumulatorColumns = 256;  // of one of the two accumulators (float32: the main products' and the small ones')
+constexpr int kBoxRows = 64;              // rows of a box of an operand stored across
+constexpr int kLeastSplitBlocks = 8;      // k blocks a split is worth: its partial tile costs 512 KB of traffic
+constexpr int kChunkBlocks = 4;           // k blocks (256 k's) of one running sum of a float32 product: 16 steps
 
-// The pairs of parts of a float32 product, smallest first.
-__device__ __constant__ signed char kPartA[kParts] = {2, 0, 1, 1, 0, 0};
-__device__ __constant__ signed char kPartB[kParts] = {0, 2, 1, 0, 1, 0};
+// What a stage holds: one part of each operand, or a float32's three.
+template <typename T>
+struct Shape {
+  static constexpr bool kPromote = sizeof(T) == 4;
+  static constexpr int kParts = kPromote ? 3 : 1;
+  static constexpr int kTileN = kPromote ? 128 : 256;
+  static constexpr int kPartB = kTileN / 2 * kTileK * 2;  // bytes of one CTA's part of B at the widest tile
+  static constexpr int kStageBytes = kParts * (kHalfBytes + kPartB);
+  static constexpr int kStages = kPromote ? 2 : 6;
+  static constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kSquareBytes + 1024;
+};
 
 struct Params {
   int64_t rows, cols;
@@ -117,8 +123,7 @@ __device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int
 #pragma unroll
   for (int k = 0; k < 4; ++k) z[k] += bias[k];
   if (e.pre) store4(static_cast<T*>(e.pre) + i * cols + j, n, whole, z);
-#pragma unroll
-  for (int k = 0; k < 4; ++k) z[k] = activate<T, kActivation>(z[k]);
+  activate4<T, kActivation>(z);
   if (e.residual) {
     float r[4];
     load4(static_cast<const T*>(e.residual) + i * e.residual_stride + j, n, whole, r);
@@ -128,37 +133,46 @@ __device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int
   store4(static_cast<T*>(e.out) + i * e.out_stride + j, n, whole, z);
 }
 
-// A warp's square of 32 x 32 sums in shared memory (a row of eight four-column vectors, vector q of row r at q ^ (r & 7)) to
-// its place: four rows at a time, four columns a lane. 16-bit residual rows are all in flight before the
-// first result is stored (float32 ones would not fit beside a promoted sum).
-template <typename T, int kActivation>
-__device__ __forceinline__ void finish_square(const ProductEpilogue& e, const float4* square, int lane, int64_t i0, int64_t rows,
-                                              int64_t j, int64_t cols, bool aligned) {
+// What the epilogue of a warp's square reads from memory: a lane's four biases and its eight rows of residual.
+template <typename T>
+struct Ahead {
+  using Raw = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
+  Raw residual[8];
   float bias[4];
+  bool whole;  // the square lies inside the matrix and its rows are aligned
+  __device__ __forceinline__ Ahead() : whole(false) {}
+  __device__ __forceinline__ Ahead(const ProductEpilogue& e, int lane, int64_t i0, int64_t rows, int64_t j, int64_t cols,
+                                   bool aligned) {
+    whole = aligned && i0 + 32 <= rows && j - 4 * (lane & 7) + 32 <= cols;
+    load_bias<T>(e, j, cols, bias);
+    if (!whole || !e.residual) return;
+    const T* from = static_cast<const T*>(e.residual) + (i0 + (lane >> 3)) * e.residual_stride + j;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) residual[r] = *reinterpret_cast<const Raw*>(from + r * 4 * e.residual_stride);
+  }
+};
+
+// A warp's square of 32 x 32 sums in shared memory (a row of eight four-column vectors, vector q of row r at q ^ (r & 7)) to
+// its place: four rows at a time, four columns a lane.
+template <typename T, int kActivation>
+__device__ __forceinline__ void finish_square(const ProductEpilogue& e, const Ahead<T>& ahead, const float4* square, int lane,
+                                              int64_t i0, int64_t rows, int64_t j, int64_t cols, bool aligned) {
   const int q = lane & 7, first = lane >> 3;
-  if (aligned && i0 + 32 <= rows && j - 4 * q + 32 <= cols) {
+  if (ahead.whole) {
     const int64_t i = i0 + first;
     T* out = static_cast<T*>(e.out) + i * e.out_stride + j;
     T* pre = e.pre ? static_cast<T*>(e.pre) + i * cols + j : nullptr;
-    const int64_t out_step = 4 * e.out_stride, pre_step = 4 * cols, residual_step = 4 * e.residual_stride;
-    const T* from = static_cast<const T*>(e.residual) + i * e.residual_stride + j;
-    uint2 residual[8];
-    if (sizeof(T) == 2 && e.residual) {
-#pragma unroll
-      for (int r = 0; r < 8; ++r) residual[r] = *reinterpret_cast<const uint2*>(from + r * residual_step);
-    }
-    load_bias<T>(e, j, cols, bias);
+    const int64_t out_step = 4 * e.out_stride, pre_step = 4 * cols;
 #pragma unroll
     for (int r = 0; r < 8; ++r) {
       const int row = r * 4 + first;
       const float4 f = square[row * 8 + (q ^ (row & 7))];
-      float z[4] = {f.x + bias[0], f.y + bias[1], f.z + bias[2], f.w + bias[3]};
+      float z[4] = {f.x + ahead.bias[0], f.y + ahead.bias[1], f.z + ahead.bias[2], f.w + ahead.bias[3]};
       if (pre) store4(pre + r * pre_step, z);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) z[k] = activate<T, kActivation>(z[k]);
+      activate4<T, kActivation>(z);
       if (e.residual) {
         float add[4];
-        load4(sizeof(T) == 2 ? reinterpret_cast<const T*>(&residual[r]) : from + r * residual_step, add);
+        load4(reinterpret_cast<const T*>(&ahead.residual[r]), add);
 #pragma unroll
         for (int k = 0; k < 4; ++k) z[k] += add[k];
       }
@@ -167,13 +181,12 @@ __device__ __forceinline__ void finish_square(const ProductEpilogue& e, const fl
     return;
   }
   if (j >= cols) return;
-  load_bias<T>(e, j, cols, bias);
   for (int r = 0; r < 8; ++r) {
     const int row = r * 4 + first;
     if (i0 + row >= rows) return;
     const float4 f = square[row * 8 + (q ^ (row & 7))];
     float z[4] = {f.x, f.y, f.z, f.w};
-    finish4<T, kActivation>(e, i0 + row, j, cols, bias, aligned, z);
+    finish4<T, kActivation>(e, i0 + row, j, cols, ahead.bias, aligned, z);
   }
 }
 
@@ -187,13 +200,15 @@ template <typename T>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Params p) {
+  using S = Shape<T>;
+  constexpr bool kPromote = S::kPromote;
+  constexpr int kStages = S::kStages;
   extern __shared__ unsigned char smem_raw[];
   __shared__ __align__(8) uint64_t full[kStages], empty[kStages], acc_full[2], acc_empty[2];
   __shared__ uint32_t tmem_slot;
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = tc::cluster_ctarank();
-  constexpr bool kPromote = sizeof(T) == 4;
   if (threadIdx.x == 0) {
     for (int s = 0; s < kStages; ++s) {
       tc::bar_init(&full[s], 1);
@@ -221,7 +236,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
   if (warp == kLoadWarp) {
     if (lane == 0) {
-      const uint32_t bytes = kHalfBytes + half_n * kTileK * 2;
+      const uint32_t bytes = S::kParts * (kHalfBytes + half_n * kTileK * 2);
       int stage = 0;
       uint32_t lap = 0;
       for (int index = pair; index < items && ok; index += pairs) {
@@ -230,26 +245,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const int j0 = t.j * p.tile_n + static_cast<int>(rank) * half_n;
         for (int b = t.first; b < t.last; ++b) {
           if (lap > 0 && !(ok = tc::bar_wait(&empty[stage], (lap - 1) & 1u, 0x500))) break;
-          int k0 = b * kTileK, part_a = 0, part_b = 0;
-          if (kPromote) {
-            const int deep = p.chunk / kParts, chunk = b / p.chunk, inside = b - chunk * p.chunk;
-            const int segment = inside / deep;
-            k0 = (chunk * deep + inside - segment * deep) * kTileK;
-            part_a = kPartA[segment], part_b = kPartB[segment];
-          }
-          const uint32_t at = tc::smem_u32(smem + stage * kStageBytes);
+          const int k0 = b * kTileK;
+          const uint32_t at = tc::smem_u32(smem + stage * S::kStageBytes);
           const uint32_t barrier = tc::map_shared(tc::smem_u32(&full[stage]), 0);
           if (rank == 0) tc::bar_expect_tx(&full[stage], 2 * bytes);
-          if (p.across_a) {
-            for (int c = 0; c < 2; ++c) load_box(at + c * kBoxRows * 128, &map_a, i0 + c * 64, k0, part_a, barrier);
-          } else {
-            load_box(at, &map_a, k0, i0, part_a, barrier);
-          }
-          if (p.across_b) {
-            for (int c = 0; c < half_n / 64; ++c)
-              load_box(at + kHalfBytes + c * kBoxRows * 128, &map_b, j0 + c * 64, k0, part_b, barrier);
-          } else {
-            load_box(at + kHalfBytes, &map_b, k0, j0, part_b, barrier);
+#pragma unroll
+          for (int part = 0; part < S::kParts; ++part) {
+            const uint32_t to_a = at + part * kHalfBytes, to_b = at + S::kParts * kHalfBytes + part * S::kPartB;
+            if (p.across_a) {
+              for (int c = 0; c < 2; ++c) load_box(to_a + c * kBoxRows * 128, &map_a, i0 + c * 64, k0, part, barrier);
+            } else {
+              load_box(to_a, &map_a, k0, i0, part, barrier);
+            }
+            if (p.across_b) {
+              for (int c = 0; c < half_n / 64; ++c) load_box(to_b + c * kBoxRows * 128, &map_b, j0 + c * 64, k0, part, barrier);
+            } else {
+              load_box(to_b, &map_b, k0, j0, part, barrier);
+            }
           }
           if (++stage == kStages) {
             stage = 0;
@@ -278,14 +290,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           for (int b = first; b < last; ++b) {
             if (!(ok = tc::bar_wait_cluster(&full[stage], lap & 1u, 0x503))) break;
             tc::fence_after_sync();
-            const uint32_t at = tc::smem_u32(smem + stage * kStageBytes);
-            uint64_t da = operand_desc(at, p.across_a), db = operand_desc(at + kHalfBytes, p.across_b);
+            const uint32_t at = tc::smem_u32(smem + stage * S::kStageBytes);
+            // The product of part pa of A and part pb of B.
+            auto multiply = [&](int pa, int pb, uint32_t into, bool fresh) {
+              uint64_t da = operand_desc(at + pa * kHalfBytes, p.across_a);
+              uint64_t db = operand_desc(at + S::kParts * kHalfBytes + pb * S::kPartB, p.across_b);
 #pragma unroll
-            for (int k = 0; k < kTileK / 16; ++k) {
-              tc::mma_bf16_pair(accumulator, da, db, p.instruction, b > first || k > 0);
-              da += step_a;
-              db += step_b;
+              for (int k = 0; k < kTileK / 16; ++k) {
+                tc::mma_bf16_pair(into, da, db, p.instruction, !fresh || k > 0);
+                da += step_a;
+                db += step_b;
+              }
+            };
+            if constexpr (kPromote) {
+              const uint32_t small = accumulator + S::kTileN;
+              multiply(2, 0, small, b == first);
+              multiply(0, 2, small, false);
+              multiply(1, 1, small, false);
+              multiply(1, 0, small, false);
+              multiply(0, 1, small, false);
             }
+            multiply(0, 0, accumulator, b == first);
             tc::mma_commit_pair(&empty[stage]);
             if (++stage == kStages) {
               stage = 0;
@@ -297,7 +322,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    float4* square = reinterpret_cast<float4*>(smem + kStages * kStageBytes + warp * kSquareBytes);
+    float4* square = reinterpret_cast<float4*>(smem + kStages * S::kStageBytes + warp * kSquareBytes);
     const int quarter = warp & 3, half = warp >> 2;
     const bool aligned = epilogue_aligned<T>(p.e, p.cols);
     const int chunks = half_n / 32;  // 32-column chunks of this warp's half of the columns
@@ -309,8 +334,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       tc::fence_after_sync();
       return ok;
     };
-    auto read_sum = [&](int c, float (&v)[32]) {
-      tc::tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (done & 1) * kAccumulatorColumns +
+    auto read_sum = [&](int c, int column, float (&v)[32]) {
+      tc::tmem_ld32(tmem + (static_cast<uint32_t>(quarter * 32) << 16) + (done & 1) * kAccumulatorColumns + column +
                         (half * chunks + c) * 32,
                     v);
     };
@@ -325,11 +350,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       const Item t = item_of(p, index);
       const int64_t i0 = static_cast<int64_t>(t.i) * kTileM + rank * 128 + quarter * 32;
       const int64_t tile_j = static_cast<int64_t>(t.j) * p.tile_n;
+      auto column_of = [&](int c) { return tile_j + (half * chunks + c) * 32 + (lane & 7) * 4; };
+      auto outside = [&](int c) { return i0 >= p.rows || tile_j + (half * chunks + c) * 32 >= p.cols; };
+      // What a square's epilogue reads from memory, under way before its sums are.
+      auto ahead_of = [&](int c) {
+        return outside(c) || p.partial ? Ahead<T>() : Ahead<T>(p.e, lane, i0, p.rows, column_of(c), p.cols, aligned);
+      };
       // 32 rows by 32 columns of sums, a row a lane, to their place.
-      auto store_sums = [&](int c, const float (&v)[32]) {
-        const int column = (half * chunks + c) * 32;
-        const int64_t j = tile_j + column + (lane & 7) * 4;
-        if (i0 >= p.rows || tile_j + column >= p.cols) return;
+      auto store_sums = [&](int c, const float (&v)[32], const Ahead<T>& ahead) {
+        if (outside(c)) return;
+        const int64_t j = column_of(c);
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           square[lane * 8 + (q ^ (lane & 7))] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -344,36 +374,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         } else {
           with_activation(p.e.activation, [&](auto activation) {
-            finish_square<T, activation>(p.e, square, lane, i0, p.rows, j, p.cols, aligned);
+            finish_square<T, activation>(p.e, ahead, square, lane, i0, p.rows, j, p.cols, aligned);
           });
         }
         __syncwarp();
       };
       if constexpr (kPromote) {
-        float sums[4][32];
+        float sums[2][32];
         for (int first = t.first; first < t.last && ok; first += p.chunk) {
           if (!wait_sum()) break;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c >= chunks) continue;
+          for (int c = 0; c < 2; ++c) {
             float v[32];
-            read_sum(c, v);
+            read_sum(c, S::kTileN, v);
 #pragma unroll
             for (int k = 0; k < 32; ++k) sums[c][k] = first == t.first ? v[k] : sums[c][k] + v[k];
+            read_sum(c, 0, v);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) sums[c][k] += v[k];
           }
           release_sum();
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
-          if (c < chunks) store_sums(c, sums[c]);
+        for (int c = 0; c < 2; ++c) store_sums(c, sums[c], ahead_of(c));
       } else {
+        Ahead<T> ahead = ahead_of(0);
         if (!wait_sum()) break;
         for (int c = 0; c < chunks; ++c) {
           float v[32];
-          read_sum(c, v);
+          read_sum(c, 0, v);
           if (c == chunks - 1) release_sum();
-          store_sums(c, v);
+          store_sums(c, v, ahead);
+          if (c + 1 < chunks) ahead = ahead_of(c + 1);
         }
       }
     }
@@ -470,11 +503,11 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
     p.partial_stride = plan.partial_stride;
     p.e = e;
     static const cudaError_t configured =
-        cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmemBytes);
     if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel: %s", cudaGetErrorString(configured));
     const int items = plan.tiles_i * plan.tiles_j * plan.splits;
     const int pairs = std::min(items, sm_count() / 2);
-    product_kernel<T><<<2 * pairs, kThreads, kSmemBytes, stream>>>(map_a, map_b, p);
+    product_kernel<T><<<2 * pairs, kThreads, Shape<T>::kSmemBytes, stream>>>(map_a, map_b, p);
     if (int rc = check_launch("product_kernel")) return rc;
     if (plan.splits == 1) return CG_OK;
   }
@@ -488,22 +521,20 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
 
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
   ProductPlan plan = {};
-  plan.tile_n = cols > 128 ? 256 : 128;
+  plan.tile_n = dtype != CG_F32 && cols > 128 ? 256 : 128;
   plan.tiles_i = static_cast<int>((rows + kTileM - 1) / kTileM);
   plan.tiles_j = static_cast<int>((cols + plan.tile_n - 1) / plan.tile_n);
   const int64_t pairs = 74;  // the B200's 148 SMs
   const int64_t k_blocks = (depth + kTileK - 1) / kTileK, tiles = static_cast<int64_t>(plan.tiles_i) * plan.tiles_j;
-  // A split is a whole number of units: one k block, or a float32 chunk.
-  const int64_t unit_blocks = dtype == CG_F32 ? std::max<int64_t>(1, std::min<int64_t>(kChunkBlocks, k_blocks)) : 1;
-  const int64_t unit = unit_blocks * (dtype == CG_F32 ? kParts : 1), units = (k_blocks + unit_blocks - 1) / unit_blocks;
+  // A split is a whole number of units: kLeastSplitBlocks k blocks, or a float32 chunk.
+  const int64_t unit = dtype == CG_F32 ? kChunkBlocks : kLeastSplitBlocks, units = (k_blocks + unit - 1) / unit;
   int64_t splits = 1;
-  if (tiles > 0 && 2 * tiles <= pairs) splits = std::min(pairs / tiles, units * unit / kLeastSplitBlocks);
-  splits = std::max<int64_t>(1, std::min(splits, units));
+  if (tiles > 0 && 2 * tiles <= pairs) splits = std::max<int64_t>(1, std::min(pairs / tiles, units));
   const int64_t units_each = units > 0 ? (units + splits - 1) / splits : 1;
-  plan.blocks = static_cast<int>(units * unit);
+  plan.blocks = static_cast<int>(k_blocks);
   plan.per_split = static_cast<int>(units_each * unit);
   plan.splits = units > 0 ? static_cast<int>((units + units_each - 1) / units_each) : 1;
-  plan.chunk = dtype == CG_F32 ? static_cast<int>(unit) : std::max(1, plan.per_split);
+  plan.chunk = dtype == CG_F32 ? kChunkBlocks : plan.per_split;
   plan.partial_stride = (cols + 3) / 4 * 4;
   plan.partial_bytes = plan.splits > 1 ? plan.splits * rows * plan.partial_stride * 4 : 0;
   return plan;
