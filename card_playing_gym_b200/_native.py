@@ -92,8 +92,7 @@ class CardGridWeights(ctypes.Structure):
 
 class AdamWTensor(ctypes.Structure):
     _fields_ = [
-        ("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("numel", ctypes.c_int64), ("state", ctypes.c_int64),
-        ("group", ctypes.c_int32), ("reserved", ctypes.c_int32),
+        ("numel", ctypes.c_int64), ("state", ctypes.c_int64), ("group", ctypes.c_int32), ("reserved", ctypes.c_int32),
     ]
 
 
@@ -161,7 +160,7 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
                                   _p]),
     "cg_adamw_control_bytes": (_i64, []),
     "cg_adamw_workspace_bytes": (_i64, [_i32]),
-    "cg_adamw_step": (_i32, [_p, _i32, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p, _f32, _p, _p, _p, _i64, _p]),
+    "cg_adamw_step": (_i32, [_p, _p, _p, _i32, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p, _f32, _p, _p, _p, _i64, _p]),
 }
 
 

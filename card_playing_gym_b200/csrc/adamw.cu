@@ -19,7 +19,7 @@
 
 #include <algorithm>
 
-#include "common.cuh"
+#include "elements.cuh"
 
 namespace cg {
 namespace {
@@ -137,13 +137,6 @@ __device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
   *reinterpret_cast<uint4*>(p) = raw;
 }
 
-__device__ __forceinline__ float to_float(float v) { return v; }
-__device__ __forceinline__ float to_float(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_float(__nv_bfloat16 v) { return __bfloat162float(v); }
-__device__ __forceinline__ void from_float(float* p, float v) { *p = v; }
-__device__ __forceinline__ void from_float(__half* p, float v) { *p = __float2half_rn(v); }
-__device__ __forceinline__ void from_float(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-
 // Eight entries of a tensor from `at`; those at or past `numel` read as zero. `whole`: all eight are inside
 // and the address is aligned to eight entries.
 template <typename T>
@@ -153,7 +146,7 @@ __device__ __forceinline__ void load_entries(const T* base, int64_t at, int64_t 
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) v[i] = at + i < numel ? to_float(base[at + i]) : 0.f;
+  for (int i = 0; i < kPerLane; ++i) v[i] = at + i < numel ? as_float(base[at + i]) : 0.f;
 }
 
 template <typename T>
@@ -164,7 +157,7 @@ __device__ __forceinline__ void store_entries(T* base, int64_t at, int64_t numel
   }
 #pragma unroll
   for (int i = 0; i < kPerLane; ++i)
-    if (at + i < numel) from_float(base + at + i, v[i]);
+    if (at + i < numel) put(base + at + i, v[i]);
 }
 
 template <typename T>
@@ -191,13 +184,17 @@ __device__ __forceinline__ void encode8(uint8_t* codes, const float (&v)[8]) {
   *reinterpret_cast<uint2*>(codes) = raw;
 }
 
-// Square root and quotient within 2 units in the last place: the update they make is the learning rate's fraction
-// of a weight, and exact ones (some 30 instructions an entry) would cost more than the memory they hide behind.
+// Square root and reciprocal within 2 units in the last place: the update they make is the learning rate's fraction of a
+// weight, and exact ones (some 30 instructions an entry) would cost more than the memory they hide behind.
 __device__ __forceinline__ float root_fast(float v) {
   float r;
-  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+
+// Under the update's quotient at least: an entry without history does not divide zero by a zero eps, and its neighbours'
+// reciprocal is finite.
+constexpr float kLeastUnder = 1.2e-38f;
 
 // Largest of the warp's non-negative values; a NaN's bits compare above infinity's, so it is kept.
 __device__ __forceinline__ float warp_peak(float v) {
@@ -312,7 +309,6 @@ struct Loaded {
   float p[8], g[8], m[8], v[8];     // fp32 parts
   uint4 raw_g;                      // a 16-bit gradient
   uint2 codes_m, codes_v;           // 8-bit moments
-  float peak_m, peak_r;
   bool whole;
 };
 
@@ -335,8 +331,6 @@ __device__ __forceinline__ void load_block(Loaded<T, kBits>& l, const Entry& e, 
   if constexpr (kBits == 8) {
     l.codes_m = *reinterpret_cast<const uint2*>(static_cast<uint8_t*>(states.exp_avg) + held);
     l.codes_v = *reinterpret_cast<const uint2*>(static_cast<uint8_t*>(states.exp_avg_sq) + held);
-    l.peak_m = states.exp_avg_scale[held / kBlockEntries];
-    l.peak_r = states.exp_avg_sq_scale[held / kBlockEntries];
   } else {
     load8(static_cast<float*>(states.exp_avg) + held, l.m);
     load8(static_cast<float*>(states.exp_avg_sq) + held, l.v);
@@ -344,31 +338,40 @@ __device__ __forceinline__ void load_block(Loaded<T, kBits>& l, const Entry& e, 
 }
 
 template <typename T, int kBits>
-__device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e, const States& states, int64_t at, int lane,
-                                             const Factors& f, float clip) {
+__device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e, const States& states, int64_t at,
+                                             const Factors& f, float clip, float& scale_m, float& scale_r) {
   const int64_t held = e.state + at;
   if constexpr (sizeof(T) == 2) {
     if (l.whole) load8(reinterpret_cast<const T*>(&l.raw_g), l.g);
   }
   if constexpr (kBits == 8) {
-    decode8(l.codes_m, l.peak_m * (1.f / kE4m3Max), l.m);
-    decode8(l.codes_v, l.peak_r * (1.f / kE4m3Max), l.v);
+    decode8(l.codes_m, scale_m * (1.f / kE4m3Max), l.m);
+    decode8(l.codes_v, scale_r * (1.f / kE4m3Max), l.v);
 #pragma unroll
     for (int i = 0; i < kPerLane; ++i) l.v[i] *= l.v[i];
   }
   float peak_m = 0.f, peak_r = 0.f;
+  const Two beta1 = two(f.beta1, f.beta1), rest1 = two(f.rest1 * clip, f.rest1 * clip), beta2 = two(f.beta2, f.beta2),
+            rest2 = two(f.rest2, f.rest2), clips = two(clip, clip), decay = two(f.decay, f.decay),
+            step = two(-f.step, -f.step), unbias = two(f.root, f.root), eps = two(f.eps, f.eps);
 #pragma unroll
-  for (int i = 0; i < kPerLane; ++i) {
-    const float g = l.g[i] * clip;
-    l.m[i] = f.beta1 * l.m[i] + f.rest1 * g;
-    l.v[i] = f.beta2 * l.v[i] + f.rest2 * (g * g);
-    const float root = root_fast(l.v[i]);
-    l.p[i] = l.p[i] * f.decay - f.step * __fdividef(l.m[i], root * f.root + f.eps);
+  for (int i = 0; i < kPerLane; i += 2) {
+    const Two raw = two(l.g[i], l.g[i + 1]), g = raw * clips;
+    const Two m = fma(beta1, two(l.m[i], l.m[i + 1]), rest1 * raw);
+    const Two v = fma(beta2, two(l.v[i], l.v[i + 1]), rest2 * (g * g));
+    const float2 fv = apart_of(v), fm = apart_of(m);
+    const float2 root = make_float2(root_fast(fv.x), root_fast(fv.y));
+    const float2 under = apart_of(fma(two(root.x, root.y), unbias, eps));
+    const Two update = m * two(reciprocal_fast(fmaxf(under.x, kLeastUnder)), reciprocal_fast(fmaxf(under.y, kLeastUnder)));
+    const float2 p = apart_of(fma(step, update, two(l.p[i], l.p[i + 1]) * decay));
+    l.p[i] = p.x, l.p[i + 1] = p.y;
+    l.m[i] = fm.x, l.m[i + 1] = fm.y;
     if (kBits == 8) {
-      l.v[i] = root;
-      // Bits, not fmaxf, which would drop a NaN.
-      peak_m = __uint_as_float(max(__float_as_uint(peak_m), __float_as_uint(fabsf(l.m[i]))));
-      peak_r = __uint_as_float(max(__float_as_uint(peak_r), __float_as_uint(root)));
+      l.v[i] = root.x, l.v[i + 1] = root.y;
+      peak_m = max_nan(peak_m, max_nan(fabsf(fm.x), fabsf(fm.y)));
+      peak_r = max_nan(peak_r, max_nan(root.x, root.y));
+    } else {
+      l.v[i] = fv.x, l.v[i + 1] = fv.y;
     }
   }
   if (sizeof(T) == 2) store8(states.master + held, l.p);
@@ -376,67 +379,84 @@ __device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e
   if constexpr (kBits == 8) {
     peak_m = warp_peak(peak_m);
     peak_r = warp_peak(peak_r);
-    const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max / peak_m;
-    const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max / peak_r;
+    const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max * reciprocal_fast(peak_m);
+    const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max * reciprocal_fast(peak_r);
+    float least = kE4m3Least;
 #pragma unroll
-    for (int i = 0; i < kPerLane; ++i) {
-      l.m[i] *= to_m;
-      l.v[i] = l.v[i] > 0.f ? fmaxf(l.v[i] * to_r, kE4m3Least) : l.v[i] * to_r;
+    for (int i = 0; i < kPerLane; i += 2) {
+      const float2 m = apart_of(two(l.m[i], l.m[i + 1]) * two(to_m, to_m));
+      const float2 v = apart_of(two(l.v[i], l.v[i + 1]) * two(to_r, to_r));
+      l.m[i] = m.x, l.m[i + 1] = m.y, l.v[i] = v.x, l.v[i + 1] = v.y;
+      least = fminf(least, fminf(v.x, v.y));
+    }
+    if (least < kE4m3Least) {  // a root under the smallest code: it keeps that one unless it is zero
+#pragma unroll
+      for (int i = 0; i < kPerLane; ++i) l.v[i] = l.v[i] > 0.f ? fmaxf(l.v[i], kE4m3Least) : l.v[i];
     }
     encode8(static_cast<uint8_t*>(states.exp_avg) + held, l.m);
     encode8(static_cast<uint8_t*>(states.exp_avg_sq) + held, l.v);
-    if (lane == 0) {
-      states.exp_avg_scale[held / kBlockEntries] = peak_m;
-      states.exp_avg_sq_scale[held / kBlockEntries] = peak_r;
-    }
+    scale_m = peak_m, scale_r = peak_r;
   } else {
     store8(static_cast<float*>(states.exp_avg) + held, l.m);
     store8(static_cast<float*>(states.exp_avg_sq) + held, l.v);
   }
 }
 
-// A warp takes every eighth block of its chunk; the next block's loads are in flight while this one is computed and
-// stored. The first loads go out before the wait for the factors: nothing the kernel before this one writes is among
-// them.
+// A warp takes eight neighbouring blocks, whose scales are one 32-byte sector: its lanes read and write them at once. (Read
+// and written block by block, from sectors that eight warps were writing to, they were what the kernel waited for:
+// 134 M float32 weights with 8-bit moments 510 us, with whole sectors 360.) Three thread blocks an SM, with the registers
+// that leaves, do better than more (134 M bfloat16 weights, 8 bits: 376 us; four 400, five 472). The first loads go out before the wait for the factors: nothing
+// the kernel before this one writes is among them.
 template <typename T, int kBits, int kMax>
-__global__ void __launch_bounds__(kThreads, kBits == 8 ? 3 : 2) adamw_update_kernel(const __grid_constant__ Table<kMax> table,
-                                                                                    const States states, const Control* control) {
+__global__ void __launch_bounds__(kThreads, 3) adamw_update_kernel(const __grid_constant__ Table<kMax> table, const States states,
+                                                                   const Control* control) {
+  constexpr int kWarpBlocks = kChunk / kThreads * 32 / kBlockEntries;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const Entry& e = table.e[find_tensor(table, blockIdx.x)];
   const bool aligned = aligned8(static_cast<const T*>(e.param)) && aligned8(static_cast<const T*>(e.grad));
-  const int64_t start = static_cast<int64_t>(blockIdx.x - e.first_chunk) * kChunk;
-  const int64_t end = min(start + kChunk, e.numel);
-  constexpr int kStride = kThreads / 32 * kBlockEntries;
-  int64_t block = start + warp * kBlockEntries;
-  if (block >= end) return;
-  Loaded<T, kBits> now, next;
-  load_block(now, e, states, block + lane * kPerLane, aligned);
+  const int64_t first = static_cast<int64_t>(blockIdx.x - e.first_chunk) * kChunk + warp * kWarpBlocks * kBlockEntries;
+  if (first >= e.numel) return;
+  const int blocks = static_cast<int>(min(static_cast<int64_t>(kWarpBlocks), (e.numel - first + kBlockEntries - 1) / kBlockEntries));
+  Loaded<T, kBits> l;
+  load_block(l, e, states, first + lane * kPerLane, aligned);
+  const int64_t scale_at = (e.state + first) / kBlockEntries + lane;
+  float scales_m = 0.f, scales_r = 0.f;  // of this lane's block
+  if (kBits == 8 && lane < blocks) scales_m = states.exp_avg_scale[scale_at], scales_r = states.exp_avg_sq_scale[scale_at];
   pdl_wait();
   if (control->skip) return;  // a norm that is not finite: nothing moves
   const float clip = control->clip;
   const Factors f = control->groups[e.group];
-  for (;;) {
-    const int64_t after = block + kStride;
-    if (after < end) load_block(next, e, states, after + lane * kPerLane, aligned);
-    update_block(now, e, states, block + lane * kPerLane, lane, f, clip);
-    if (after >= end) break;
-    now = next;
-    block = after;
+  for (int i = 0; i < blocks; ++i) {
+    float scale_m = 0.f, scale_r = 0.f;
+    if (kBits == 8) scale_m = __shfl_sync(0xffffffffu, scales_m, i), scale_r = __shfl_sync(0xffffffffu, scales_r, i);
+    const int64_t at = first + i * kBlockEntries + lane * kPerLane;
+    if (i > 0) load_block(l, e, states, at, aligned);
+    update_block(l, e, states, at, f, clip, scale_m, scale_r);
+    if (kBits == 8 && lane == i) scales_m = scale_m, scales_r = scale_r;
   }
+  if (kBits == 8 && lane < blocks) states.exp_avg_scale[scale_at] = scales_m, states.exp_avg_sq_scale[scale_at] = scales_r;
 }
 
 constexpr int kFewTensors = 64, kManyTensors = 640;  // 2.6 and 25 KB of kernel parameters (32 KB is the limit)
 
 // The tensors from `next` on that fit one launch; those without a gradient or without entries are left out.
+struct Tensors {
+  const cg_adamw_tensor* extents;
+  void* const* params;
+  const void* const* grads;
+  int count;
+  bool live(int i) const { return grads[i] && extents[i].numel > 0; }
+};
+
 template <int kMax>
-void fill_table(const cg_adamw_tensor* tensors, int count, int& next, Table<kMax>& table) {
+void fill_table(const Tensors& tensors, int& next, Table<kMax>& table) {
   table.count = table.chunks = 0;
-  while (next < count && table.count < kMax) {
-    const cg_adamw_tensor& t = tensors[next];
-    if (t.grad && t.numel > 0) {
+  while (next < tensors.count && table.count < kMax) {
+    const cg_adamw_tensor& t = tensors.extents[next];
+    if (tensors.live(next)) {
       const int64_t chunks = (t.numel + kChunk - 1) / kChunk;
       if (table.count && table.chunks + chunks > INT32_MAX) break;
-      table.e[table.count++] = {t.param, t.grad, t.numel, t.state, table.chunks, t.group};
+      table.e[table.count++] = {tensors.params[next], tensors.grads[next], t.numel, t.state, table.chunks, t.group};
       table.chunks += static_cast<int>(chunks);
     }
     ++next;
@@ -444,18 +464,18 @@ void fill_table(const cg_adamw_tensor* tensors, int count, int& next, Table<kMax
 }
 
 template <typename T, int kMax>
-int run_step(const cg_adamw_tensor* tensors, int count, const Groups& groups, int bits, const States& states,
+int run_step(const Tensors& tensors, const Groups& groups, int bits, const States& states,
              int64_t* steps, float max_norm, float* norm_out, Control* control, double* partial, cudaStream_t s) {
   Table<kMax> table;
   if (max_norm > 0) {
     int partials = 0;
-    for (int next = 0; next < count;) {
-      fill_table(tensors, count, next, table);
+    for (int next = 0; next < tensors.count;) {
+      fill_table(tensors, next, table);
       partials += std::min(table.chunks, kNormBlocks);
     }
     int first = 0;
-    for (int next = 0; next < count;) {
-      fill_table(tensors, count, next, table);
+    for (int next = 0; next < tensors.count;) {
+      fill_table(tensors, next, table);
       if (!table.chunks) continue;
       const int blocks = std::min(table.chunks, kNormBlocks);
       adamw_norm_kernel<T, kMax><<<blocks, kThreads, 0, s>>>(table, groups, max_norm, first, partials, partial, steps,
@@ -467,8 +487,8 @@ int run_step(const cg_adamw_tensor* tensors, int count, const Groups& groups, in
     adamw_factors_kernel<<<1, 32, 0, s>>>(groups, steps, control);
     if (int rc = check_launch("adamw_factors_kernel")) return rc;
   }
-  for (int next = 0; next < count;) {
-    fill_table(tensors, count, next, table);
+  for (int next = 0; next < tensors.count;) {
+    fill_table(tensors, next, table);
     if (!table.chunks) continue;
     auto kernel = bits == 8 ? adamw_update_kernel<T, 8, kMax> : adamw_update_kernel<T, 32, kMax>;
     if (int rc = launch_pdl("adamw_update_kernel", kernel, dim3(table.chunks), dim3(kThreads), 0, s, table, states,
@@ -491,12 +511,12 @@ extern "C" int64_t cg_adamw_workspace_bytes(int count) {
   return (static_cast<int64_t>(count) / cg::kFewTensors + 1) * cg::kNormBlocks * static_cast<int64_t>(sizeof(double));
 }
 
-extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtype, const cg_adamw_group* groups,
+extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params, const void* const* grads, int count, int dtype, const cg_adamw_group* groups,
                              int group_count, int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq,
                              float* exp_avg_sq_scale, float* master, int64_t* steps, float max_norm, float* norm_out,
                              void* control, void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace cg;
-  CG_REQUIRE(count >= 0 && (count == 0 || tensors), "cg_adamw_step: bad tensor table");
+  CG_REQUIRE(count >= 0 && (count == 0 || (tensors && params && grads)), "cg_adamw_step: bad tensor table");
   CG_REQUIRE(valid_dtype(dtype), "cg_adamw_step: dtype must be float32, float16 or bfloat16");
   CG_REQUIRE(state_bits == 8 || state_bits == 32, "cg_adamw_step: state_bits must be 8 or 32");
   CG_REQUIRE(groups && group_count > 0 && group_count <= kMaxGroups, "cg_adamw_step: 1..%d groups", kMaxGroups);
@@ -514,14 +534,15 @@ extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtyp
     CG_REQUIRE(g.eps >= 0, "cg_adamw_step: eps must not be negative");
     table.g[k] = g;
   }
+  const Tensors all{tensors, params, grads, count};
   int live = 0;
   for (int i = 0; i < count; ++i) {
     const cg_adamw_tensor& t = tensors[i];
     CG_REQUIRE(t.numel >= 0 && t.state >= 0 && t.state % kBlockEntries == 0, "cg_adamw_step: tensor %d: bad extent", i);
     CG_REQUIRE(t.numel <= static_cast<int64_t>(INT32_MAX) * kChunk, "cg_adamw_step: tensor %d is too large", i);
     CG_REQUIRE(t.group >= 0 && t.group < group_count, "cg_adamw_step: tensor %d: no such group", i);
-    CG_REQUIRE(t.numel == 0 || !t.grad || t.param, "cg_adamw_step: tensor %d: NULL parameter", i);
-    live += t.grad && t.numel > 0;
+    CG_REQUIRE(t.numel == 0 || !grads[i] || params[i], "cg_adamw_step: tensor %d: NULL parameter", i);
+    live += all.live(i);
   }
   if (!live) return CG_OK;
   const States states{exp_avg, exp_avg_scale, exp_avg_sq, exp_avg_sq_scale, master};
@@ -531,8 +552,8 @@ extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtyp
   auto run = [&](auto sample) {
     using T = decltype(sample);
     return live <= kFewTensors
-               ? run_step<T, kFewTensors>(tensors, count, table, state_bits, states, steps, max_norm, norm_out, c, partial, s)
-               : run_step<T, kManyTensors>(tensors, count, table, state_bits, states, steps, max_norm, norm_out, c, partial, s);
+               ? run_step<T, kFewTensors>(all, table, state_bits, states, steps, max_norm, norm_out, c, partial, s)
+               : run_step<T, kManyTensors>(all, table, state_bits, states, steps, max_norm, norm_out, c, partial, s);
   };
   if (dtype == CG_F32) return run(float{});
   if (dtype == CG_F16) return run(__half{});

@@ -43,13 +43,6 @@ struct Args {
   float clip, beta, alpha;
 };
 
-// The larger value, a NaN if either is one (fmaxf would drop it, and a row of NaN would pass for an empty one).
-__device__ __forceinline__ float max_nan(float x, float y) {
-  float m;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
-  return m;
-}
-
 // A row's sums over its legal entries, relative to a base near the largest logit (every formula is the same for any
 // base; one within kLazy of the maximum keeps the exponentials in range).
 struct RowSums {

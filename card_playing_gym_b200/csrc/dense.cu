@@ -53,9 +53,14 @@ __global__ void __launch_bounds__(256) pack_kernel(const T* in, int64_t stride, 
 // ---- dpre and the bias gradient -----------------------------------------------------------------------------------
 // A block takes 32 sixteen-byte vectors of columns of one slice of the rows, a vector a lane, a row a warp at a time. Its
 // warps' column sums join in shared memory, the slices' in order in bias_sum_kernel. It is bound by memory once the
-// activation's slope costs one exponential: sixteen entries of each input a lane are in flight at a time.
+// activation's slope costs one exponential and rows are under way while others are computed.
 template <typename T>
 constexpr int kSlopeVector = 16 / static_cast<int>(sizeof(T));
+
+template <typename T>
+__device__ __forceinline__ bool aligned_vector(const void* base, int64_t stride) {
+  return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && stride % kSlopeVector<T> == 0;
+}
 
 // The first n entries of a vector at `p`; `whole`: all of them, aligned to four.
 template <typename T, int kVec>
@@ -74,39 +79,66 @@ __global__ void __launch_bounds__(256, 3) slope_kernel(const T* __restrict__ dy,
                                                        int64_t rows, int64_t cols, int64_t slice,
                                                        typename OperandOf<T>::type* __restrict__ dpre, int64_t dpre_stride,
                                                        float* __restrict__ partial) {
-  constexpr int kVec = kSlopeVector<T>, kRows = 16 / kVec;
+  constexpr int kVec = kSlopeVector<T>, kRows = 2;
   __shared__ float s[8][32 * kVec];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t j = (static_cast<int64_t>(blockIdx.x) * 32 + lane) * kVec;
   const int64_t lo = blockIdx.y * slice, hi = min(rows, lo + slice);
   const int n = static_cast<int>(max(int64_t{0}, min(static_cast<int64_t>(kVec), cols - j)));
-  const bool whole_dy = aligned4<T>(dy, dy_stride) && n == kVec, whole_pre = aligned4<T>(pre, cols) && n == kVec;
+  const bool whole_dy = aligned_vector<T>(dy, dy_stride) && n == kVec, whole_pre = aligned_vector<T>(pre, cols) && n == kVec;
   float sum[kVec] = {};
-  if (n > 0) {
-    for (int64_t i0 = lo + warp; i0 < hi; i0 += 8 * kRows) {
-      float g[kRows][kVec], z[kRows][kVec];
+  // One row's gradients, times the slopes, to their place and into the sums.
+  auto take_row = [&](int64_t i, float (&g)[kVec], const float (&z)[kVec]) {
+    if constexpr (kActivation != kActNone) times_slope<T, kActivation>(g, z);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int64_t i = i0 + 8 * r;
-        if (i >= hi) continue;
-        load_vector<T, kVec>(dy + i * dy_stride + j, n, whole_dy, g[r]);
-        if (kActivation != kActNone) load_vector<T, kVec>(pre + i * cols + j, n, whole_pre, z[r]);
+    for (int k = 0; k < kVec; ++k) sum[k] += g[k];
+    if (!dpre) return;
+#pragma unroll
+    for (int k = 0; k < kVec; k += 4) {
+      const float part[4] = {g[k], g[k + 1], g[k + 2], g[k + 3]};
+      if (k < n) store_operand<T>(dpre + i * dpre_stride + j + k, rows * dpre_stride, part);
+    }
+  };
+  if (whole_dy && (kActivation == kActNone || whole_pre)) {
+    // Two rows' vectors as they are in memory, the next two's under way while these are computed. Two sets of registers
+    // are taken in turn: a copy would wait for its loads.
+    struct Rows {
+      uint4 g[kRows], z[kRows];
+    } even, odd;
+    auto load = [&](Rows& r, int64_t i0) {
+#pragma unroll
+      for (int k = 0; k < kRows; ++k) {
+        const int64_t i = min(i0 + 8 * k, hi - 1);  // past the slice: a row that is not used
+        r.g[k] = *reinterpret_cast<const uint4*>(dy + i * dy_stride + j);
+        if (kActivation != kActNone) r.z[k] = *reinterpret_cast<const uint4*>(pre + i * cols + j);
       }
+    };
+    int64_t i0 = lo + warp;
+    auto step = [&](Rows& now, Rows& next) {
+      const int64_t after = i0 + 8 * kRows;
+      if (after < hi) load(next, after);
 #pragma unroll
-      for (int r = 0; r < kRows; ++r) {
-        const int64_t i = i0 + 8 * r;
-        if (i >= hi) continue;
-        if constexpr (kActivation != kActNone) times_slope<T, kActivation>(g[r], z[r]);
-#pragma unroll
-        for (int k = 0; k < kVec; ++k) sum[k] += g[r][k];
-        if (dpre) {
-#pragma unroll
-          for (int k = 0; k < kVec; k += 4) {
-            const float part[4] = {g[r][k], g[r][k + 1], g[r][k + 2], g[r][k + 3]};
-            if (k < n) store_operand<T>(dpre + i * dpre_stride + j + k, rows * dpre_stride, part);
-          }
-        }
+      for (int k = 0; k < kRows; ++k) {
+        if (i0 + 8 * k >= hi) continue;
+        float g[kVec], z[kVec];
+        load_vector<T, kVec>(reinterpret_cast<const T*>(&now.g[k]), kVec, true, g);
+        if (kActivation != kActNone) load_vector<T, kVec>(reinterpret_cast<const T*>(&now.z[k]), kVec, true, z);
+        take_row(i0 + 8 * k, g, z);
       }
+      i0 = after;
+      return after < hi;
+    };
+    if (i0 < hi) {
+      load(even, i0);
+      while (step(even, odd) && step(odd, even)) {
+      }
+    }
+  } else if (n > 0) {
+    for (int64_t i = lo + warp; i < hi; i += 8) {
+      float g[kVec], z[kVec];
+      load_vector<T, kVec>(dy + i * dy_stride + j, n, whole_dy, g);
+      if (kActivation != kActNone) load_vector<T, kVec>(pre + i * cols + j, n, whole_pre, z);
+      take_row(i, g, z);
     }
   }
   if (!partial) return;

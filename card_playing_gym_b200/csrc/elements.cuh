@@ -9,6 +9,13 @@
 
 namespace cg {
 
+// The larger value, a NaN if either is one (fmaxf would drop it).
+__device__ __forceinline__ float max_nan(float x, float y) {
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(x), "f"(y));
+  return m;
+}
+
 __device__ __forceinline__ float as_float(float v) { return v; }
 __device__ __forceinline__ float as_float(__half v) { return __half2float(v); }
 __device__ __forceinline__ float as_float(__nv_bfloat16 v) { return __bfloat162float(v); }

@@ -9,14 +9,14 @@ With ``weight_decay=0`` it is Adam. It is a ``torch.optim.Optimizer`` (parameter
 
 from __future__ import annotations
 
+from array import array
 from operator import attrgetter
 
-import numpy as np
 import torch
 
 from . import _native as nat
 
-_dtype_of, _layout_of = attrgetter("dtype"), attrgetter("layout")
+_dtype_of, _layout_of, _bytes_of = attrgetter("dtype"), attrgetter("layout"), attrgetter("nbytes")
 
 BLOCK = 256  # entries of one scale of the 8-bit moments; every parameter's state starts on a multiple of it
 
@@ -109,15 +109,16 @@ class AdamW(torch.optim.Optimizer):
             if "master" in views:
                 views["master"].copy_(p.detach())
             self.state[p] = views
-        # The host table of the step: extents and groups are fixed, addresses are filled in at every step.
+        # The host's side of the step: extents and groups are fixed, addresses are gathered at every step.
         self._table = (nat.AdamWTensor * len(self._parameters))()
-        self._addresses = np.frombuffer(self._table, dtype=np.dtype([("param", "u8"), ("grad", "u8"), ("rest", "V24")]))
         self._dtype = first.dtype
-        self._numels = [p.numel() for p in self._parameters]
+        self._bytes = [p.nbytes for p in self._parameters]
+        need = nat.query("cg_adamw_workspace_bytes", len(self._table)) if self.max_norm else 0
+        self._workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
         index = 0
         for number, group in enumerate(self.param_groups):
             for _ in group["params"]:
-                self._table[index].numel = self._numels[index]
+                self._table[index].numel = self._parameters[index].numel()
                 self._table[index].state = starts[index]
                 self._table[index].group = number
                 index += 1
@@ -150,22 +151,25 @@ class AdamW(torch.optim.Optimizer):
         self.steps.copy_(state_dict["steps"])
 
     # -- the step -----------------------------------------------------------------------------------------------------
-    def _check(self, params: list, grads: list, present: list) -> None:
-        """That the table still describes the parameters and gradients: one pass per property, for the host's sake."""
+    def _check(self, params: list, grads: list) -> None:
+        """That the table still describes the parameters and gradients: one pass per property, for the host's sake.
 
-        held = grads if all(present) else [g for g in grads if g is not None]
-        numels = self._numels if all(present) else [n for g, n in zip(grads, self._numels) if g is not None]
-        if (list(map(torch.Tensor.numel, params)) != self._numels or set(map(_dtype_of, params)) != {self._dtype}
+        torch holds a gradient to its parameter's shape, dtype and device when it is set; its size in bytes is checked
+        here again, since the parameter may have changed between."""
+
+        sizes, given = self._bytes, [g for g in grads if g is not None]
+        if len(given) != len(grads):
+            sizes = [n for g, n in zip(grads, sizes) if g is not None]
+            grads = given
+        if (list(map(_bytes_of, params)) != self._bytes or set(map(_dtype_of, params)) != {self._dtype}
                 or set(map(torch.Tensor.get_device, params)) != {self.steps.get_device()}
                 or not all(map(torch.Tensor.is_contiguous, params))):
             raise ValueError("a parameter has changed its size, dtype, device or layout since the optimizer was built")
-        if set(map(_layout_of, held)) - {torch.strided} or not all(map(torch.Tensor.is_contiguous, held)):
+        if set(map(_layout_of, grads)) - {torch.strided} or not all(map(torch.Tensor.is_contiguous, grads)):
             raise ValueError("a gradient is not dense and contiguous")
-        if (list(map(torch.Tensor.numel, held)) != numels or set(map(_dtype_of, held)) - {self._dtype}
-                or set(map(torch.Tensor.get_device, held)) - {self.steps.get_device()}):
-            raise ValueError("a gradient has not its parameter's size, dtype or device")
+        if list(map(_bytes_of, grads)) != sizes:
+            raise ValueError("a gradient has not its parameter's size")
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -174,20 +178,20 @@ class AdamW(torch.optim.Optimizer):
         flat, device = self.flat, self.steps.device
         params = self._parameters
         grads = [p.grad for p in params]
-        self._check(params, grads, [g is not None for g in grads])
-        self._addresses["param"] = list(map(torch.Tensor.data_ptr, params))
-        self._addresses["grad"] = [0 if g is None else g.data_ptr() for g in grads]
+        self._check(params, grads)
         table = self._table
+        from_params = array("Q", map(torch.Tensor.data_ptr, params))
+        from_grads = array("Q", [0 if g is None else g.data_ptr() for g in grads])
         for entry, group in zip(self._groups, self.param_groups):
             entry.lr, entry.eps, entry.weight_decay = group["lr"], group["eps"], group["weight_decay"]
             entry.beta1, entry.beta2 = group["betas"]
-        need = nat.query("cg_adamw_workspace_bytes", len(table)) if self.max_norm else 0
         second = flat["exp_avg_sq" if self.state_bits == 32 else "exp_avg_sq_root"]
+        workspace = self._workspace
         with nat.on_device(device):
-            workspace = torch.empty(need, dtype=torch.uint8, device=device) if need else None
-            nat.call("cg_adamw_step", table, len(table), nat.DTYPE_CODES[self._dtype], self._groups, len(self._groups),
-                     self.state_bits, nat.ptr(flat["exp_avg"]), nat.ptr(flat.get("exp_avg_scale")), nat.ptr(second),
+            nat.call("cg_adamw_step", table, from_params.buffer_info()[0], from_grads.buffer_info()[0], len(table),
+                     nat.DTYPE_CODES[self._dtype], self._groups, len(self._groups), self.state_bits,
+                     nat.ptr(flat["exp_avg"]), nat.ptr(flat.get("exp_avg_scale")), nat.ptr(second),
                      nat.ptr(flat.get("exp_avg_sq_root_scale")), nat.ptr(flat.get("master")), nat.ptr(self.steps),
                      float(self.max_norm or 0.0), nat.ptr(self.grad_norm), nat.ptr(self._control),
-                     nat.ptr(workspace), need, nat.stream_handle(device))
+                     nat.ptr(workspace), 0 if workspace is None else workspace.numel(), nat.stream_handle(device))
         return loss

@@ -431,14 +431,13 @@ int cg_center_zero_sum(const float* values, const int64_t* players, int64_t n, i
  * multiple of 256, padded with zeros to the next multiple: exp_avg and exp_avg_sq fp32
  * (state_bits 32), or e4m3 codes of m and of sqrt(v) with one fp32 scale per 256 entries
  * (the block's largest magnitude, code 448; state_bits 8); master fp32 copies of 16-bit
- * parameters (NULL for fp32 ones). A tensor with grad NULL is left as it is. steps int64 is
+ * parameters (NULL for fp32 ones). params and grads are host arrays of device addresses, contiguous
+ * tensors; one whose grad is NULL is left as it is. steps int64 is
  * t on the device, shared by all tensors, and counts up by one. With max_norm a norm that is
  * not finite leaves everything as it is (steps too); norm_out fp32 receives |g|.
  * control: cg_adamw_control_bytes(), zeroed before its first use and kept with the state.
  * ------------------------------------------------------------------------------- */
 typedef struct {
-  void* param;
-  const void* grad;
   int64_t numel, state;
   int32_t group, reserved;
 } cg_adamw_tensor;
@@ -447,8 +446,8 @@ typedef struct {
 } cg_adamw_group;
 int64_t cg_adamw_control_bytes(void);
 int64_t cg_adamw_workspace_bytes(int count);
-int cg_adamw_step(const cg_adamw_tensor* tensors, int count, int dtype, const cg_adamw_group* groups, int group_count,
-                  int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale,
+int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params, const void* const* grads, int count, int dtype,
+                  const cg_adamw_group* groups, int group_count, int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale,
                   float* master, int64_t* steps, float max_norm, float* norm_out, void* control, void* workspace,
                   int64_t workspace_bytes, void* stream);
 
