@@ -4,9 +4,9 @@ The reference registers its one native kernel as ``cardgym::decode_attention`` w
 kernel so that ``torch.compile`` and CUDA-graph capture can trace through it
 (cardgym/nn/cuda_decode.py:172-181). The same is done here for every entry point a traced caller
 needs: the ragged trunk decode (which writes the KV pool it is given), the fused heads + masked
-sampling, masked sampling alone, segmented GAE, the baseline's seat values, the PPO objective
-and the value loss. Each op calls the same C ABI as the Python wrappers in ``trunk``, ``plump``,
-``sampling`` and ``ppo``; its fake kernel only allocates outputs of the right shapes, so a trace
+sampling, masked sampling alone, segmented GAE, the baseline's seat values, the PPO objective,
+the value loss, the anchored objective, the actions' log-probabilities and the fused linear layer. Each op calls the same C ABI as the Python wrappers in ``trunk``, ``plump``,
+``sampling``, ``ppo`` and ``dense``; its fake kernel only allocates outputs of the right shapes, so a trace
 never runs a kernel. ``decode_attention`` is registered by ``cuda_decode``.
 
 Descriptors that are C structs in the ABI (trunk dimensions, the heads layout) are passed as int
@@ -193,3 +193,59 @@ def value_loss(prediction: torch.Tensor, players: torch.Tensor, targets: torch.T
 @value_loss.register_fake
 def _(prediction, players, targets, weights, reward_scale):
     return prediction.new_empty(prediction.shape, dtype=torch.float32), prediction.new_empty(4, dtype=torch.float64)
+
+
+# -- the update's training operators -----------------------------------------------------------------------------------
+@torch.library.custom_op("cardgym_b200::anchored_objective", mutates_args=())
+def anchored_objective(logits: torch.Tensor, reference_logits: torch.Tensor | None,
+                       reference_log_probs: torch.Tensor | None, legal: torch.Tensor | None, actions: torch.Tensor,
+                       old_log_probs: torch.Tensor, advantages: torch.Tensor, weights: torch.Tensor, clip_ratio: float,
+                       beta: float, alpha: float) -> tuple[torch.Tensor, torch.Tensor]:
+    """The anchored objective of ``ppo.anchored_objective``: (dL/dlogits in the logits' dtype, totals fp32 [9] in
+    ``ppo.ANCHORED_KEYS`` order)."""
+
+    from .ppo import anchored_objective as run
+
+    leaf = logits.detach().requires_grad_()
+    with torch.enable_grad():
+        objective, totals = run(leaf, actions, old_log_probs, advantages, weights, clip_ratio=clip_ratio, beta=beta,
+                                alpha=alpha, reference_logits=reference_logits, reference_log_probs=reference_log_probs,
+                                legal=legal)
+    (grad,) = torch.autograd.grad(objective, leaf)
+    return grad.contiguous(), totals.clone()
+
+
+@anchored_objective.register_fake
+def _(logits, reference_logits, reference_log_probs, legal, actions, old_log_probs, advantages, weights, clip_ratio, beta,
+      alpha):
+    return logits.new_empty(logits.shape), logits.new_empty(9, dtype=torch.float32)
+
+
+@torch.library.custom_op("cardgym_b200::action_log_probs", mutates_args=())
+def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, legal: torch.Tensor | None) -> torch.Tensor:
+    """log pi(action) per row, fp32 [N] (``ppo.action_log_probs``)."""
+
+    from .ppo import action_log_probs as run
+
+    return run(logits, actions, legal=legal)
+
+
+@action_log_probs.register_fake
+def _(logits, actions, legal):
+    return logits.new_empty(logits.shape[0], dtype=torch.float32)
+
+
+@torch.library.custom_op("cardgym_b200::linear", mutates_args=())
+def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None, residual: torch.Tensor | None,
+           activation: str) -> torch.Tensor:
+    """activation(x @ weight.T + bias) + residual (``dense.linear``, forward)."""
+
+    from .dense import linear as run
+
+    with torch.no_grad():
+        return run(x, weight, bias, residual, activation=activation)
+
+
+@linear.register_fake
+def _(x, weight, bias, residual, activation):
+    return x.new_empty((*x.shape[:-1], weight.shape[0]))
