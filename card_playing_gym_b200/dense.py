@@ -8,6 +8,7 @@
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -62,6 +63,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         dx = dweight = dbias = None
         needs_x, needs_weight, needs_bias, needs_residual, _ = ctx.needs_input_grad

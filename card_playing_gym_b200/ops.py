@@ -5,9 +5,10 @@ kernel so that ``torch.compile`` and CUDA-graph capture can trace through it
 (cardgym/nn/cuda_decode.py:172-181). The same is done here for every entry point a traced caller
 needs: the ragged trunk decode (which writes the KV pool it is given), the fused heads + masked
 sampling, masked sampling alone, segmented GAE, the baseline's seat values, the PPO objective,
-the value loss, the anchored objective, the actions' log-probabilities and the fused linear layer. Each op calls the same C ABI as the Python wrappers in ``trunk``, ``plump``,
-``sampling``, ``ppo`` and ``dense``; its fake kernel only allocates outputs of the right shapes, so a trace
-never runs a kernel. ``decode_attention`` is registered by ``cuda_decode``.
+the value loss, the anchored objective, the actions' log-probabilities and the fused linear layer.
+Each op calls the same C ABI as the Python wrappers in ``trunk``, ``plump``, ``sampling``, ``ppo`` and
+``dense``; its fake kernel only allocates outputs of the right shapes, so a trace never runs a
+kernel. ``decode_attention`` is registered by ``cuda_decode``.
 
 Descriptors that are C structs in the ABI (trunk dimensions, the heads layout) are passed as int
 lists in their field order.
@@ -204,15 +205,11 @@ def anchored_objective(logits: torch.Tensor, reference_logits: torch.Tensor | No
     """The anchored objective of ``ppo.anchored_objective``: (dL/dlogits in the logits' dtype, totals fp32 [9] in
     ``ppo.ANCHORED_KEYS`` order)."""
 
-    from .ppo import anchored_objective as run
+    from .ppo import _anchored_inputs, _run_anchored
 
-    leaf = logits.detach().requires_grad_()
-    with torch.enable_grad():
-        objective, totals = run(leaf, actions, old_log_probs, advantages, weights, clip_ratio=clip_ratio, beta=beta,
-                                alpha=alpha, reference_logits=reference_logits, reference_log_probs=reference_log_probs,
-                                legal=legal)
-    (grad,) = torch.autograd.grad(objective, leaf)
-    return grad.contiguous(), totals.clone()
+    grad, sums = _run_anchored(*_anchored_inputs(logits, actions, old_log_probs, advantages, weights, clip_ratio, beta,
+                                                 alpha, reference_logits, reference_log_probs, legal))
+    return grad.contiguous(), sums[:-1].clone()
 
 
 @anchored_objective.register_fake

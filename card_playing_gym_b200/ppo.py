@@ -18,8 +18,10 @@ from __future__ import annotations
 
 import math
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -225,6 +227,11 @@ def _plane_of(name: str, tensor: torch.Tensor, like: torch.Tensor) -> torch.Tens
     return _unit_rows(tensor)
 
 
+@lru_cache(maxsize=1024)
+def _anchored_workspace_bytes(rows: int) -> int:
+    return nat.query("cg_anchored_objective_workspace_bytes", rows)
+
+
 def _unit_rows(plane: torch.Tensor) -> torch.Tensor:
     """The plane with adjacent row entries and rows that do not overlap (a copy only where it has neither)."""
 
@@ -266,7 +273,7 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
         if grad_stride != width:
             grad = grad[:, :width]
     sums = torch.empty(len(ANCHORED_KEYS) + 1, device=logits.device)  # the totals, and the objective once more
-    need = nat.query("cg_anchored_objective_workspace_bytes", rows)
+    need = _anchored_workspace_bytes(rows)
     with nat.on_device(logits.device):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
         nat.call("cg_anchored_objective", nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], rows, width, stride,
@@ -278,29 +285,59 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
 
 
 class _AnchoredObjective(torch.autograd.Function):
+    """``rest`` is one argument, not ten: autograd handles every argument of a function on the host."""
+
     @staticmethod
-    def forward(ctx, logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights, clip,
-                beta, alpha):
-        inputs = (logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights)
-        ctx.scalars = (clip, beta, alpha)
+    def forward(ctx, logits, rest):
         ctx.set_materialize_grads(False)  # the totals have no gradient to make zeros for
-        ctx.gradient, sums = _run_anchored(*inputs, *ctx.scalars)
-        ctx.save_for_backward(*inputs)  # a second backward computes the gradient again
+        ctx.gradient, sums = _run_anchored(logits, *rest)
+        # A second backward computes the gradient again, from inputs that must not have changed.
+        ctx.save_for_backward(logits)
+        ctx.rest, ctx.versions = rest, [t._version for t in rest if isinstance(t, torch.Tensor)]
         totals = sums[:-1]
         ctx.mark_non_differentiable(totals)
         return sums[-1], totals
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_objective, _grad_totals):
         if grad_objective is None:
-            return (None,) * 11
+            return None, None
         gradient, ctx.gradient = ctx.gradient, None
         if gradient is None:
-            gradient, _ = _run_anchored(*ctx.saved_tensors, *ctx.scalars)
+            (logits,) = ctx.saved_tensors
+            if ctx.versions != [t._version for t in ctx.rest if isinstance(t, torch.Tensor)]:
+                raise RuntimeError("an input of anchored_objective was modified in place before its second backward")
+            gradient, _ = _run_anchored(logits, *ctx.rest)
         with nat.on_device(gradient.device):
             nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
                      _row_stride(gradient), nat.ptr(grad_objective.contiguous()), nat.stream_handle(gradient.device))
-        return (gradient, *(None,) * 10)
+        return gradient, None
+
+
+def _anchored_inputs(logits, actions, old_log_probs, advantages, weights, clip_ratio, beta, alpha, reference_logits,
+                     reference_log_probs, legal) -> tuple:
+    """``_run_anchored``'s arguments, checked, in the types and layouts the kernels take."""
+
+    if beta and (reference_logits is None) == (reference_log_probs is None):
+        raise ValueError("a KL term takes reference_logits or reference_log_probs, one of the two")
+    if reference_logits is not None and reference_log_probs is not None:
+        raise ValueError("give reference_logits or reference_log_probs, not both")
+    if clip_ratio < 0:
+        raise ValueError("clip_ratio must not be negative")
+    logits, actions, legal = _logits_and_mask(logits, actions, legal)
+    rows, device = logits.shape[0], logits.device
+    if reference_logits is not None:
+        if reference_logits.dtype != logits.dtype:
+            raise ValueError(f"reference_logits must be {logits.dtype}, not {reference_logits.dtype}")
+        reference_logits = _plane_of("reference_logits", reference_logits, logits)
+    if reference_log_probs is not None:
+        reference_log_probs = _rows_of("reference_log_probs", reference_log_probs, rows, device, torch.float32)
+    rest = (_rows_of("old_log_probs", old_log_probs, rows, device, torch.float32),
+            _rows_of("advantages", advantages, rows, device, torch.float32),
+            _rows_of("weights", weights, rows, device, torch.float32))
+    return (logits, reference_logits, reference_log_probs, legal, actions, *rest, float(clip_ratio), float(beta),
+            float(alpha))
 
 
 def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_probs: torch.Tensor,
@@ -323,27 +360,10 @@ def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_prob
     (``_native.fault_status``).
     """
 
-    if beta and (reference_logits is None) == (reference_log_probs is None):
-        raise ValueError("a KL term takes reference_logits or reference_log_probs, one of the two")
-    if reference_logits is not None and reference_log_probs is not None:
-        raise ValueError("give reference_logits or reference_log_probs, not both")
-    if clip_ratio < 0:
-        raise ValueError("clip_ratio must not be negative")
-    logits, actions, legal = _logits_and_mask(logits, actions, legal)
-    rows, device = logits.shape[0], logits.device
-    if reference_logits is not None:
-        if reference_logits.dtype != logits.dtype:
-            raise ValueError(f"reference_logits must be {logits.dtype}, not {reference_logits.dtype}")
-        reference_logits = _plane_of("reference_logits", reference_logits, logits)
-    if reference_log_probs is not None:
-        reference_log_probs = _rows_of("reference_log_probs", reference_log_probs, rows, device, torch.float32)
-    rest = (_rows_of("old_log_probs", old_log_probs, rows, device, torch.float32),
-            _rows_of("advantages", advantages, rows, device, torch.float32),
-            _rows_of("weights", weights, rows, device, torch.float32))
-    inputs = (logits, reference_logits, reference_log_probs, legal, actions, *rest, float(clip_ratio), float(beta),
-              float(alpha))
-    if torch.is_grad_enabled() and logits.requires_grad:
-        return _AnchoredObjective.apply(*inputs)
+    inputs = _anchored_inputs(logits, actions, old_log_probs, advantages, weights, clip_ratio, beta, alpha,
+                              reference_logits, reference_log_probs, legal)
+    if torch.is_grad_enabled() and inputs[0].requires_grad:
+        return _AnchoredObjective.apply(inputs[0], inputs[1:])
     _, sums = _run_anchored(*inputs, want_grad=False)
     return sums[-1], sums[:-1]
 
