@@ -20,8 +20,9 @@
 // pairs fit tensor memory. 16-bit results keep one running sum: at 8192 k's the cut is 9e-6 against their own
 // rounding of 2^-11 or 2^-8.
 //
-// Where the tiles do not fill the chip's pairs, k is split: every split writes fp32 partial sums and
-// product_join_kernel adds them in order and applies the epilogue.
+// Where the last round of tiles leaves half the pairs idle, k is split for the tiles of that round: every split writes
+// fp32 partial sums and product_join_kernel adds them in order and applies the epilogue (8192 k's of 4096 x 4096: 256
+// tiles are three rounds of 74 and 34 tiles in two halves).
 #include "product.h"
 
 #include <cuda.h>
@@ -59,33 +60,38 @@ struct Shape {
 
 struct Params {
   int64_t rows, cols;
-  int tile_n, tiles_i, tiles_j, blocks, splits, per_split;
+  int tile_n, tiles_i, tiles_j, blocks, whole, splits, per_split;  // tiles from `whole` on are split
   int chunk;  // blocks of one running sum; for float32 its k blocks times the parts
   uint32_t instruction;
   int across_a, across_b;
-  float* partial;
-  int64_t partial_stride;
+  float* partial;  // [split tile][split][256][tile_n]
   ProductEpilogue e;
 };
 
 struct Item {
-  int i, j, split, first, last;
+  int i, j, slot, first, last;  // slot: of its partial sums, or -1
 };
 
 // Tiles go in groups of eight columns, down the rows inside a group, so that the pairs working at one time share
 // their operands in L2.
+__device__ __forceinline__ void place_tile(int tile, int tiles_i, int tiles_j, int* i, int* j) {
+  const int group = tile / (8 * tiles_i);
+  const int width = min(8, tiles_j - group * 8);
+  const int inside = tile - group * 8 * tiles_i;
+  *i = inside / width;
+  *j = group * 8 + inside % width;
+}
+
 __device__ __forceinline__ Item item_of(const Params& p, int index) {
-  Item t;
-  const int tiles = p.tiles_i * p.tiles_j;
-  t.split = index / tiles;
-  const int tile = index % tiles;
-  const int group = tile / (8 * p.tiles_i);
-  const int width = min(8, p.tiles_j - group * 8);
-  const int inside = tile - group * 8 * p.tiles_i;
-  t.i = inside / width;
-  t.j = group * 8 + inside % width;
-  t.first = t.split * p.per_split;
-  t.last = min(t.first + p.per_split, p.blocks);
+  Item t = {0, 0, -1, 0, p.blocks};
+  int tile = index;
+  if (index >= p.whole) {
+    t.slot = index - p.whole;
+    tile = p.whole + t.slot / p.splits;
+    t.first = t.slot % p.splits * p.per_split;
+    t.last = min(t.first + p.per_split, p.blocks);
+  }
+  place_tile(tile, p.tiles_i, p.tiles_j, &t.i, &t.j);
   return t;
 }
 
@@ -229,7 +235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   tc::cluster_sync();  // barriers and tensor memory are ready in both CTAs
   tc::fence_after_sync();
   const uint32_t tmem = tmem_slot;
-  const int items = p.tiles_i * p.tiles_j * p.splits;
+  const int items = p.whole + (p.tiles_i * p.tiles_j - p.whole) * p.splits;
   const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
   const int half_n = p.tile_n / 2;
   bool ok = true;
@@ -354,7 +360,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       auto outside = [&](int c) { return i0 >= p.rows || tile_j + (half * chunks + c) * 32 >= p.cols; };
       // What a square's epilogue reads from memory, under way before its sums are.
       auto ahead_of = [&](int c) {
-        return outside(c) || p.partial ? Ahead<T>() : Ahead<T>(p.e, lane, i0, p.rows, column_of(c), p.cols, aligned);
+        return outside(c) || t.slot >= 0 ? Ahead<T>() : Ahead<T>(p.e, lane, i0, p.rows, column_of(c), p.cols, aligned);
       };
       // 32 rows by 32 columns of sums, a row a lane, to their place.
       auto store_sums = [&](int c, const float (&v)[32], const Ahead<T>& ahead) {
@@ -364,13 +370,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int q = 0; q < 8; ++q)
           square[lane * 8 + (q ^ (lane & 7))] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
         __syncwarp();
-        if (p.partial) {
-          float* to = p.partial + (t.split * p.rows + i0 + (lane >> 3)) * p.partial_stride + j;
+        if (t.slot >= 0) {
+          const int64_t row0 = static_cast<int64_t>(t.slot) * kTileM + rank * 128 + quarter * 32 + (lane >> 3);
+          float* to = p.partial + row0 * p.tile_n + (half * chunks + c) * 32 + (lane & 7) * 4;
 #pragma unroll
           for (int r = 0; r < 8; ++r) {
             const int row = r * 4 + (lane >> 3);
-            if (i0 + row < p.rows && j < p.cols)
-              *reinterpret_cast<float4*>(to + r * 4 * p.partial_stride) = square[row * 8 + ((lane & 7) ^ (row & 7))];
+            *reinterpret_cast<float4*>(to + r * 4 * p.tile_n) = square[row * 8 + ((lane & 7) ^ (row & 7))];
           }
         } else {
           with_activation(p.e.activation, [&](auto activation) {
@@ -425,16 +431,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
   if (warp == kMmaWarp) tc::tmem_dealloc_pair(tmem, 512);
 }
 
+// The split tiles' sums, from `whole` on, to their place. splits is zero for a product of no depth.
 template <typename T>
-__global__ void __launch_bounds__(256) product_join_kernel(const float* partial, int64_t partial_stride, int splits, int64_t rows,
-                                                           int64_t cols, const ProductEpilogue e) {
+__global__ void __launch_bounds__(256) product_join_kernel(const float* partial, int whole, int splits, int tile_n, int tiles_i,
+                                                           int tiles_j, int64_t rows, int64_t cols, const ProductEpilogue e) {
   const bool aligned = epilogue_aligned<T>(e, cols);
-  const int64_t quads = (cols + 3) / 4, total = rows * quads;
+  const int quads = tile_n / 4;
+  const int64_t total = static_cast<int64_t>(tiles_i * tiles_j - whole) * kTileM * quads;
   for (int64_t index = blockIdx.x * 256ll + threadIdx.x; index < total; index += gridDim.x * 256ll) {
-    const int64_t i = index / quads, j = (index - i * quads) * 4;
+    const int64_t line = index / quads;
+    const int q = static_cast<int>(index - line * quads), tile = static_cast<int>(line / kTileM), row = static_cast<int>(line % kTileM);
+    int ti, tj;
+    place_tile(whole + tile, tiles_i, tiles_j, &ti, &tj);
+    const int64_t i = static_cast<int64_t>(ti) * kTileM + row, j = static_cast<int64_t>(tj) * tile_n + q * 4;
+    if (i >= rows || j >= cols) continue;
     float z[4] = {0.f, 0.f, 0.f, 0.f};
+    const float* from = partial + (static_cast<int64_t>(tile) * splits * kTileM + row) * tile_n + q * 4;
     for (int s = 0; s < splits; ++s) {
-      const float4 f = *reinterpret_cast<const float4*>(partial + (s * rows + i) * partial_stride + j);
+      const float4 f = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(s) * kTileM * tile_n);
       z[0] += f.x, z[1] += f.y, z[2] += f.z, z[3] += f.w;
     }
     float bias[4];
@@ -494,26 +508,26 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
     Params p;
     p.rows = rows, p.cols = cols;
     p.tile_n = plan.tile_n, p.tiles_i = plan.tiles_i, p.tiles_j = plan.tiles_j;
-    p.blocks = plan.blocks, p.splits = plan.splits, p.per_split = plan.per_split, p.chunk = plan.chunk;
+    p.blocks = plan.blocks, p.whole = plan.whole, p.splits = plan.splits, p.per_split = plan.per_split, p.chunk = plan.chunk;
     p.across_a = a.across, p.across_b = b.across;
     // fp32 accumulator; A and B both float16 or both bfloat16; the transpose bits say "across".
     p.instruction = (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (a.across ? 1u << 15 : 0u) | (b.across ? 1u << 16 : 0u) |
                     (static_cast<uint32_t>(plan.tile_n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
-    p.partial = plan.splits > 1 ? partial : nullptr;
-    p.partial_stride = plan.partial_stride;
+    p.partial = partial;
     p.e = e;
     static const cudaError_t configured =
         cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmemBytes);
     if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel: %s", cudaGetErrorString(configured));
-    const int items = plan.tiles_i * plan.tiles_j * plan.splits;
+    const int items = plan.whole + (plan.tiles_i * plan.tiles_j - plan.whole) * plan.splits;
     const int pairs = std::min(items, sm_count() / 2);
     product_kernel<T><<<2 * pairs, kThreads, Shape<T>::kSmemBytes, stream>>>(map_a, map_b, p);
     if (int rc = check_launch("product_kernel")) return rc;
-    if (plan.splits == 1) return CG_OK;
+    if (plan.whole == plan.tiles_i * plan.tiles_j) return CG_OK;
   }
-  const int64_t quads = rows * ((cols + 3) / 4);
+  const int64_t quads = static_cast<int64_t>(plan.tiles_i * plan.tiles_j - plan.whole) * kTileM * (plan.tile_n / 4);
   const int blocks = static_cast<int>(std::min<int64_t>((quads + 255) / 256, 16 * sm_count()));
-  product_join_kernel<T><<<blocks, 256, 0, stream>>>(partial, plan.partial_stride, plan.blocks > 0 ? plan.splits : 0, rows, cols, e);
+  product_join_kernel<T><<<blocks, 256, 0, stream>>>(partial, plan.whole, plan.splits, plan.tile_n, plan.tiles_i, plan.tiles_j, rows,
+                                                     cols, e);
   return check_launch("product_join_kernel");
 }
 
@@ -528,15 +542,17 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
   const int64_t k_blocks = (depth + kTileK - 1) / kTileK, tiles = static_cast<int64_t>(plan.tiles_i) * plan.tiles_j;
   // A split is a whole number of units: kLeastSplitBlocks k blocks, or a float32 chunk.
   const int64_t unit = dtype == CG_F32 ? kChunkBlocks : kLeastSplitBlocks, units = (k_blocks + unit - 1) / unit;
+  const int64_t last_round = tiles % pairs;  // tiles that would not fill a round of pairs
   int64_t splits = 1;
-  if (tiles > 0 && 2 * tiles <= pairs) splits = std::max<int64_t>(1, std::min(pairs / tiles, units));
+  if (last_round > 0 && 2 * last_round <= pairs) splits = std::max<int64_t>(1, std::min(pairs / last_round, units));
   const int64_t units_each = units > 0 ? (units + splits - 1) / splits : 1;
+  splits = units > 0 ? (units + units_each - 1) / units_each : 0;
   plan.blocks = static_cast<int>(k_blocks);
   plan.per_split = static_cast<int>(units_each * unit);
-  plan.splits = units > 0 ? static_cast<int>((units + units_each - 1) / units_each) : 1;
-  plan.chunk = dtype == CG_F32 ? kChunkBlocks : plan.per_split;
-  plan.partial_stride = (cols + 3) / 4 * 4;
-  plan.partial_bytes = plan.splits > 1 ? plan.splits * rows * plan.partial_stride * 4 : 0;
+  plan.splits = static_cast<int>(splits);
+  plan.whole = static_cast<int>(splits == 1 ? tiles : splits == 0 ? 0 : tiles - last_round);
+  plan.chunk = dtype == CG_F32 ? kChunkBlocks : std::max(1, plan.blocks);
+  plan.partial_bytes = (tiles - plan.whole) * splits * kTileM * plan.tile_n * 4;
   return plan;
 }
 

@@ -27,8 +27,8 @@ struct ProductOperand {
 
 // The product's plan: a function of the sizes alone.
 struct ProductPlan {
-  int tile_n, tiles_i, tiles_j, blocks, splits, per_split, chunk;
-  int64_t partial_stride, partial_bytes;
+  int tile_n, tiles_i, tiles_j, blocks, whole, splits, per_split, chunk;
+  int64_t partial_bytes;
 };
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype);
 
