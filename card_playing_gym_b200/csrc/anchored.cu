@@ -108,7 +108,7 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, const RowIn& in, co
   }
   g.alpha = w * a.alpha * norm;
   g.action = w * slope;
-  g.constant = -g.action + g.alpha * (entropy - log_sum) - g.beta * (kl + log_apart + (s.peak - s.reference_peak));
+  g.constant = -g.action + g.alpha * (entropy - log_sum) - g.beta * (kl + log_apart);
   const float objective = surrogate + a.beta * kl - a.alpha * norm * entropy;
   acc[0] += w * surrogate;
   acc[1] += w;
@@ -218,180 +218,301 @@ struct UnitMax<float> {
   __device__ __forceinline__ float value() const { return top; }
 };
 
-// Whether every row of a plane starts on sixteen bytes.
-template <typename T>
-__device__ __forceinline__ bool aligned_rows(const void* base, int64_t stride, int64_t rows) {
-  return (reinterpret_cast<uintptr_t>(base) & 15) == 0 && (rows == 1 || stride * static_cast<int64_t>(sizeof(T)) % 16 == 0);
+__device__ __forceinline__ Two exp2_two(Two x) {
+  const float2 f = apart_of(x);
+  return two(exp2_fast(f.x), exp2_fast(f.y));
 }
 
-// ---- up to 1024 entries: a row in the registers of four lanes or of a warp --------------------------------------------
-// A row has some 300 instructions of its own (reductions, logarithms, the ratio) beside 30 an entry, so rows of up to 64
-// entries take four lanes, eight rows a warp. The row is read once and written once,
-// and the grid is one resident wave of warps. Aligned rows move in vectors of sixteen bytes, a lane holding every
-// kLanes-th vector; others entry by entry, a lane holding every kLanes-th entry, so that both are coalesced.
-template <typename T, int kLanes, int kVectors>
+// Minus infinity in the entries of a unit whose byte of `keep` is zero; the others are 255.
+template <typename T>
+__device__ __forceinline__ void hide(uint4& unit, uint2 keep) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&unit);
+  constexpr uint32_t kInf = sizeof(T) == 4 ? 0xff800000u : std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    const uint32_t mask = sizeof(T) == 4 ? __byte_perm(keep.x, 0, 0x1111 * e)
+                                         : __byte_perm(e < 2 ? keep.x : keep.y, 0, e & 1 ? 0x3322 : 0x1100);
+    w[e] = (w[e] & mask) | (kInf & ~mask);
+  }
+}
+
+// A row's planes, and where its units and the entries outside them are.
+template <typename T>
+struct Row {
+  const T* z;
+  const T* r;
+  const uint8_t* legal;
+  int width, lead, head, units, ends;  // lead: entries from the aligned address at or before the row to it
+  bool alike;
+  __device__ __forceinline__ Row(const Args& a, int64_t row) {
+    z = static_cast<const T*>(a.logits) + row * a.stride;
+    r = a.reference ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
+    legal = a.legal ? a.legal + row * a.legal_stride : nullptr;
+    width = a.width;
+    lead = static_cast<int>((reinterpret_cast<uintptr_t>(z) & 15) / sizeof(T));
+    head = min((kVector<T> - lead) % kVector<T>, width);
+    units = (width - head) / kVector<T>;
+    ends = width - units * kVector<T>;
+    alike = !r || ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(r)) & 15) == 0;
+  }
+  __device__ __forceinline__ int unit_entry(int unit) const { return head + unit * kVector<T>; }
+  __device__ __forceinline__ int end_entry(int k) const { return k < head ? k : k + units * kVector<T>; }
+  __device__ __forceinline__ bool in(int j) const { return !legal || legal[j]; }
+};
+
+// The mask bytes of a unit: one or two aligned words where they lie inside the row, else byte by byte.
+template <typename T>
+__device__ __forceinline__ uint2 mask_bytes(const Row<T>& row, int j) {
+  constexpr int kVec = kVector<T>;
+  const uint8_t* p = row.legal + j;
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & (kVec - 1));
+  uint2 m = make_uint2(0, 0);
+  if (off == 0 || (j - off >= 0 && j - off + 2 * kVec <= row.width)) {
+    if constexpr (kVec == 8) {
+      const uint64_t* w = reinterpret_cast<const uint64_t*>(p - off);
+      uint64_t v = w[0];
+      if (off) v = v >> (8 * off) | w[1] << (64 - 8 * off);
+      m = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
+      m.x = off ? __funnelshift_r(w[0], w[1], 8 * off) : w[0];
+    }
+    return m;
+  }
+#pragma unroll
+  for (int e = 0; e < kVec; ++e) {
+    const uint32_t b = p[e];
+    if (e < 4)
+      m.x |= b << (8 * e);
+    else
+      m.y |= b << (8 * (e - 4));
+  }
+  return m;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 gather_unit(const T* p) {
+  T v[kVector<T>];
+#pragma unroll
+  for (int e = 0; e < kVector<T>; ++e) v[e] = p[e];
+  return *reinterpret_cast<const uint4*>(v);
+}
+
+// ---- up to 1024 entries: a row in the registers of a few lanes ----------------------------------------------------------
+// A row has some 300 instructions of its own (reductions, logarithms, the ratio) beside 25 an entry, so as few lanes as hold
+// it, sixteen entries each, take a row, and a warp takes up to sixteen rows at a time. The row is read once and written
+// once, and the grid is one resident wave of warps. A lane holds every kLanes-th unit of sixteen bytes from the aligned
+// address at or before the row's start; the units that the row only partly fills, and planes aligned differently
+// from the logits', go entry by entry.
+//
+// An entry whose exponential is zero counts for nothing. So that no test is needed, its distance from the maximum is
+// held to kFar, where the exponential is zero too, and its distance from the reference is set to zero.
+constexpr float kFar = -1e4f;
+
+template <typename T, bool kExact, int kLanes, int kPer>
 __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
-  constexpr int kVec = kVector<T>, kPer = kVec * kVectors, kGroups = 32 / kLanes;
+  constexpr int kVec = kVector<T>, kVectors = kPer / kVec, kGroups = 32 / kLanes;
   __shared__ double scratch[8][kTotals];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = lane / kLanes, l = lane % kLanes;
-  const uint32_t group_mask = kLanes == 32 ? 0xffffffffu : ((1u << (kLanes & 31)) - 1u) << (group * kLanes);
-  const bool exact = a.reference != nullptr;
-  const bool vectors = aligned_rows<T>(a.logits, a.stride, a.rows) &&
-                       (!exact || aligned_rows<T>(a.reference, a.reference_stride, a.rows)) &&
-                       (!a.grad || aligned_rows<T>(a.grad, a.grad_stride, a.rows)) &&
-                       (!a.legal || ((reinterpret_cast<uintptr_t>(a.legal) & (kVec - 1)) == 0 &&
-                                     (a.rows == 1 || a.legal_stride % kVec == 0)));
+  auto whole = [&](const void* base, int64_t stride, int size) {
+    return ((reinterpret_cast<uintptr_t>(base) | (a.rows > 1 ? stride * size : 0)) & (size * kVec - 1)) == 0;
+  };
+  const bool plain_planes = whole(a.logits, a.stride, sizeof(T)) && (!kExact || whole(a.reference, a.reference_stride, sizeof(T))) &&
+                            (!a.legal || whole(a.legal, a.legal_stride, 1));
+  const Two scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
   float acc[kTotals] = {};
-  // The entry of slot (v, e).
-  auto entry = [&](int v, int e) { return vectors ? (l + kLanes * v) * kVec + e : l + kLanes * (v * kVec + e); };
-  auto reduce = [&](float v, bool largest) {
+  auto total = [&](float v) {
 #pragma unroll
-    for (int o = kLanes / 2; o > 0; o >>= 1) {
-      const float other = __shfl_xor_sync(0xffffffffu, v, o);
-      v = largest ? max_nan(v, other) : v + other;
-    }
+    for (int o = kLanes / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+  };
+  auto largest = [&](float v) {
+#pragma unroll
+    for (int o = kLanes / 2; o > 0; o >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
   };
   const int64_t step = static_cast<int64_t>(gridDim.x) * 8 * kGroups;
   const int64_t warp_first = (static_cast<int64_t>(blockIdx.x) * 8 + warp) * kGroups;
   // Every group of a warp runs the same iterations, so that the shuffles stay converged.
-  for (int64_t base = warp_first; base < a.rows; base += step) {
-    const int64_t row = base + group;
+  for (int64_t first = warp_first; first < a.rows; first += step) {
+    const int64_t row = first + group;
     const bool live = row < a.rows;
-    const T* gz = static_cast<const T*>(a.logits) + row * a.stride;
-    const T* gr = exact ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
-    const uint8_t* gl = a.legal ? a.legal + row * a.legal_stride : nullptr;
-    RowIn in_row = {-1, 0.f, 0.f, 0.f, 0.f};
-    if (live) in_row = load_row(a, row);
-    const int64_t action = in_row.action;
-    // Illegal entries, and those past the row, are minus infinity.
-    float z[kPer], r[kPer], z_a = 0.f, count = 0.f;
-    bool mine = false;
-    if (vectors) {
-      uint4 raw_z[kVectors], raw_r[kVectors];
-      uint2 raw_l[kVectors];
+    const Row<T> planes(a, row);
+    const int lead = planes.lead;
+    RowIn in = {-1, 0.f, 0.f, 0.f, 0.f};
+    if (live) in = load_row(a, row);
+    // Illegal entries, and those outside the row, are minus infinity.
+    float z[kPer], r[kPer];
+    uint4 raw_z[kVectors], raw_r[kVectors];
+    uint2 keep[kVectors];
+    // The planes alike, the mask's words whole: no branch between the loads, which wait together.
+    auto fetch = [&](auto which) {
+      constexpr bool plain = decltype(which)::value;
 #pragma unroll
       for (int v = 0; v < kVectors; ++v) {
-        const int j = (l + kLanes * v) * kVec;
+        const int j = (l + kLanes * v) * kVec - (plain ? 0 : lead);
         raw_z[v] = raw_r[v] = make_uint4(0, 0, 0, 0);
-        raw_l[v] = make_uint2(0x01010101u, 0x01010101u);
-        if (!live || j + kVec > a.width) continue;
-        raw_z[v] = *reinterpret_cast<const uint4*>(gz + j);
-        if (exact) raw_r[v] = *reinterpret_cast<const uint4*>(gr + j);
-        if (gl) {
-          if constexpr (kVec == 4)
-            raw_l[v].x = *reinterpret_cast<const uint32_t*>(gl + j);
-          else
-            raw_l[v] = *reinterpret_cast<const uint2*>(gl + j);
-        }
-      }
-#pragma unroll
-      for (int v = 0; v < kVectors; ++v) {
-        const int j = (l + kLanes * v) * kVec;
-        float t[kVec], u[kVec];
-        uint32_t in[kVec];
-        if (live && j < a.width && j + kVec > a.width) {  // the row's last entries, fewer than a vector
+        keep[v] = make_uint2(0, 0);
+        if (!live || j >= a.width) continue;
+        if ((plain || j >= 0) && j + kVec <= a.width) {
+          raw_z[v] = *reinterpret_cast<const uint4*>(planes.z + j);
+          if (kExact)
+            raw_r[v] = plain || planes.alike ? *reinterpret_cast<const uint4*>(planes.r + j) : gather_unit(planes.r + j);
+          keep[v] = make_uint2(~0u, ~0u);
+          if (planes.legal) {
+            if constexpr (!plain)
+              keep[v] = mask_bytes(planes, j);
+            else if constexpr (kVec == 4)
+              keep[v].x = *reinterpret_cast<const uint32_t*>(planes.legal + j);
+            else
+              keep[v] = *reinterpret_cast<const uint2*>(planes.legal + j);
+          }
+        } else {  // a unit that the row fills in part
+          T tz[kVec], tr[kVec];
 #pragma unroll
           for (int e = 0; e < kVec; ++e) {
-            const bool inside = j + e < a.width;
-            t[e] = inside ? as_float(gz[j + e]) : 0.f;
-            u[e] = inside && exact ? as_float(gr[j + e]) : 0.f;
-            in[e] = inside ? (gl ? gl[j + e] : 1u) : 0u;
+            const bool inside = j + e >= 0 && j + e < a.width;
+            put(&tz[e], 0.f), put(&tr[e], 0.f);
+            if (inside) tz[e] = planes.z[j + e];
+            if (inside && kExact) tr[e] = planes.r[j + e];
+            const uint32_t byte = !inside ? 0u : planes.legal ? planes.legal[j + e] : 1u;
+            (e < 4 ? keep[v].x : keep[v].y) |= byte << (8 * (e & 3));
           }
-        } else {
-          unpack(raw_z[v], t, T());
-          unpack(raw_r[v], u, T());
-#pragma unroll
-          for (int e = 0; e < kVec; ++e)
-            in[e] = live && j < a.width ? (e < 4 ? raw_l[v].x : raw_l[v].y) >> (8 * (e & 3)) & 255u : 0u;
-        }
-#pragma unroll
-        for (int e = 0; e < kVec; ++e) {
-          const int k = v * kVec + e;
-          z[k] = in[e] ? t[e] : -INFINITY;
-          r[k] = in[e] ? u[e] : -INFINITY;
-          count += in[e] ? 1.f : 0.f;
-          if (in[e] && j + e == action) z_a = z[k], mine = true;
+          raw_z[v] = *reinterpret_cast<const uint4*>(tz), raw_r[v] = *reinterpret_cast<const uint4*>(tr);
         }
       }
-    } else {
+    };
+    if (plain_planes)
+      fetch(std::true_type());
+    else
+      fetch(std::false_type());
+    int bits = 0;
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) {
-        const int j = l + kLanes * k;
-        const bool in = live && j < a.width && (!gl || gl[j]);
-        z[k] = in ? as_float(gz[j]) : -INFINITY;
-        r[k] = in && exact ? as_float(gr[j]) : -INFINITY;
-        count += in ? 1.f : 0.f;
-        if (in && j == action) z_a = z[k], mine = true;
+    for (int v = 0; v < kVectors; ++v) {
+      uint2 k = make_uint2(__vcmpne4(keep[v].x, 0), 0u);
+      if constexpr (kVec == 8) k.y = __vcmpne4(keep[v].y, 0);
+      bits += __popc(k.x) + __popc(k.y);
+      hide<T>(raw_z[v], k);
+      float t[kVec];
+      unpack(raw_z[v], t, T());
+#pragma unroll
+      for (int e = 0; e < kVec; ++e) z[v * kVec + e] = t[e];
+      if (kExact) {
+        hide<T>(raw_r[v], k);
+        unpack(raw_r[v], t, T());
+#pragma unroll
+        for (int e = 0; e < kVec; ++e) r[v * kVec + e] = t[e];
       }
     }
+    const float count = static_cast<float>(bits >> 3);
+    const bool action_legal = in.action >= 0 && in.action < a.width && planes.in(static_cast<int>(in.action));
+    const float z_a = action_legal ? as_float(planes.z[in.action]) : -INFINITY;
+    const float r_a = kExact && action_legal ? as_float(planes.r[in.action]) : -INFINITY;
     RowSums s = {};
-    float peak = -INFINITY, reference_peak = -INFINITY;
+    float peak = z[0], reference_peak = kExact ? r[0] : 0.f;
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) {
+    for (int k = 1; k < kPer; ++k) {
       peak = max_nan(peak, z[k]);
-      if (exact) reference_peak = max_nan(reference_peak, r[k]);
+      if (kExact) reference_peak = max_nan(reference_peak, r[k]);
     }
-    s.peak = reduce(peak, true);
-    if (exact) s.reference_peak = reduce(reference_peak, true);
-    s.count = reduce(count, false);
-    const bool action_legal = (__ballot_sync(0xffffffffu, mine) & group_mask) != 0;
-    z_a = reduce(z_a, false);  // one lane holds it
-    if (!action_legal) z_a = -INFINITY;
-    if (s.peak != -INFINITY) {
+    s.peak = largest(peak);
+    if (kExact) s.reference_peak = largest(reference_peak);
+    s.count = total(count);
+    const float base = s.peak == -INFINITY ? 0.f : s.peak;
+    Two x[kPer / 2], e[kPer / 2], d[kPer / 2], sum = two(0.f, 0.f), spread = sum, apart = sum, reference_sum = sum;
+    // An entry's distance from the maximum, its exponential, and its distance from the reference's.
+    auto measure = [&](Two zz, Two rr, Two* xx, Two* ee, Two* dd, Two* reference_e) {
+      const float2 far = apart_of(zz + two(-base, -base));
+      *xx = two(max_nan(far.x, kFar), max_nan(far.y, kFar));
+      *ee = exp2_two(*xx * scale);
+      if (kExact) {
+        const Two y = rr + two(-s.reference_peak, -s.reference_peak);
+        *reference_e = exp2_two(y * scale);
+        const float2 g = apart_of(fma(y, minus, *xx)), f = apart_of(*ee);
+        *dd = two(f.x == 0.f ? 0.f : g.x, f.y == 0.f ? 0.f : g.y);
+      }
+    };
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) add_entry(s, z[k], exact ? r[k] : 0.f, exact);
+    for (int k = 0; k < kPer / 2; ++k) {
+      Two reference_e;
+      measure(two(z[2 * k], z[2 * k + 1]), kExact ? two(r[2 * k], r[2 * k + 1]) : sum, &x[k], &e[k], &d[k], &reference_e);
+      sum = sum + e[k];
+      spread = fma(e[k], x[k], spread);
+      if (kExact) {
+        reference_sum = reference_sum + reference_e;
+        apart = fma(e[k], d[k], apart);
+      }
     }
-    s.sum = reduce(s.sum, false);
-    if (!a.log_probs) s.spread = reduce(s.spread, false);
-    if (exact) {
-      s.reference_sum = reduce(s.reference_sum, false);
-      s.apart = reduce(s.apart, false);
+    const float2 fs = apart_of(sum), fd = apart_of(spread), fa = apart_of(apart), fr = apart_of(reference_sum);
+    s.sum = total(fs.x + fs.y);
+    if (!a.log_probs) s.spread = total(fd.x + fd.y);
+    if (kExact) {
+      s.reference_sum = total(fr.x + fr.y);
+      s.apart = total(fa.x + fa.y);
     }
-    const bool counts = row_counts(a, in_row, s, action_legal, l == 0);
+    const bool counts = row_counts(a, in, s, action_legal, l == 0);
     if (a.log_probs) {
       if (live && l == 0) a.log_probs[row] = counts ? (z_a - s.peak) - logf(s.sum) : 0.f;
       continue;
     }
-    const RowGrad g = finish_row(a, in_row, s, z_a, counts, acc);  // every lane of the group keeps the same totals
+    const RowGrad g = finish_row(a, in, s, z_a, counts, acc);  // every lane of the group keeps the same totals
     if (!a.grad || !live) continue;
     T* out = static_cast<T*>(a.grad) + row * a.grad_stride;
+    const bool alike_out = ((reinterpret_cast<uintptr_t>(planes.z) ^ reinterpret_cast<uintptr_t>(out)) & 15) == 0;
+    const Two inv_sum = two(g.inv_sum, g.inv_sum), alpha = two(g.alpha, g.alpha), beta = two(g.beta, g.beta),
+              constant = two(g.constant, g.constant);
+    const bool plain = counts && isfinite(g.constant);
+    auto gradient = [&](Two xx, Two ee, Two dd) {
+      const Two p = ee * inv_sum;
+      Two k = fma(alpha, xx, constant);
+      if (kExact) k = fma(beta, dd, k);
+      const float2 v = apart_of(p * k), f = apart_of(ee);
+      if (plain) return v;
+      // No gradient where the row does not count or the probability is zero, whatever it is multiplied by.
+      return make_float2(counts && f.x != 0.f ? v.x : 0.f, counts && f.y != 0.f ? v.y : 0.f);
+    };
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) {
       float t[kVec];
 #pragma unroll
-      for (int e = 0; e < kVec; ++e) {
-        const int k = v * kVec + e;
-        t[e] = counts ? gradient_entry(g, s.peak, z[k], exact ? r[k] : 0.f, exact) : 0.f;
-        if (counts && entry(v, e) == action) t[e] += g.action;
+      for (int k = 0; k < kVec; k += 2) {
+        const int at = (v * kVec + k) / 2;
+        const float2 f = gradient(x[at], e[at], d[at]);
+        t[k] = f.x, t[k + 1] = f.y;
       }
-      const int j = (l + kLanes * v) * kVec;
-      if (vectors && j + kVec <= a.width) {
+      const int j = (l + kLanes * v) * kVec - lead;
+      if (alike_out && j >= 0 && j + kVec <= a.width) {
         *reinterpret_cast<uint4*>(out + j) = repack(t, T());
       } else {
 #pragma unroll
-        for (int e = 0; e < kVec; ++e)
-          if (entry(v, e) < a.width) put(out + entry(v, e), t[e]);
+        for (int k = 0; k < kVec; ++k)
+          if (j + k >= 0 && j + k < a.width) put(out + j + k, t[k]);
       }
+    }
+    // The action's entry, once more by the lane that has just written it.
+    if (counts && l == (static_cast<int>(in.action) + lead) / kVec % kLanes) {
+      Two xx, ee, dd, reference_e;
+      measure(two(z_a, z_a), two(r_a, r_a), &xx, &ee, &dd, &reference_e);
+      put(out + in.action, gradient(xx, ee, dd).x + g.action);
     }
   }
   if (a.log_probs) return;
   // The groups' leaders in order, then the warps.
 #pragma unroll
   for (int k = 0; k < kTotals; ++k) {
-    double total = acc[k];
+    double sum = acc[k];
 #pragma unroll
     for (int other = 1; other < kGroups; ++other) {
-      total += __shfl_sync(0xffffffffu, acc[k], other * kLanes);
+      sum += __shfl_sync(0xffffffffu, acc[k], other * kLanes);
     }
-    if (lane == 0) scratch[warp][k] = total;
+    if (lane == 0) scratch[warp][k] = sum;
   }
   __syncthreads();
   if (threadIdx.x < kTotals) {
-    double total = 0;
-    for (int w = 0; w < 8; ++w) total += scratch[w][threadIdx.x];
-    a.partial[blockIdx.x * kTotals + threadIdx.x] = total;
+    double sum = 0;
+    for (int w = 0; w < 8; ++w) sum += scratch[w][threadIdx.x];
+    a.partial[blockIdx.x * kTotals + threadIdx.x] = sum;
   }
 }
 
@@ -464,99 +585,15 @@ __device__ __forceinline__ void join_lanes(Part& p, int lanes, bool masked) {
   p.tested = __any_sync(0xffffffffu, p.tested != 0.f) ? 1.f : 0.f;
 }
 
-__device__ __forceinline__ Two exp2_two(Two x) {
-  const float2 f = apart_of(x);
-  return two(exp2_fast(f.x), exp2_fast(f.y));
-}
-
-// A row's planes, and where its units and the entries outside them are.
-template <typename T>
-struct Row {
-  const T* z;
-  const T* r;
-  const uint8_t* legal;
-  int width, head, units, ends;
-  bool alike;
-  __device__ __forceinline__ Row(const Args& a, int64_t row) {
-    z = static_cast<const T*>(a.logits) + row * a.stride;
-    r = a.reference ? static_cast<const T*>(a.reference) + row * a.reference_stride : nullptr;
-    legal = a.legal ? a.legal + row * a.legal_stride : nullptr;
-    width = a.width;
-    const uintptr_t lead = (16 - (reinterpret_cast<uintptr_t>(z) & 15)) & 15;
-    head = min(static_cast<int>(lead / sizeof(T)), width);
-    units = (width - head) / kVector<T>;
-    ends = width - units * kVector<T>;
-    alike = !r || ((reinterpret_cast<uintptr_t>(z) ^ reinterpret_cast<uintptr_t>(r)) & 15) == 0;
-  }
-  __device__ __forceinline__ int unit_entry(int unit) const { return head + unit * kVector<T>; }
-  __device__ __forceinline__ int end_entry(int k) const { return k < head ? k : k + units * kVector<T>; }
-  __device__ __forceinline__ bool in(int j) const { return !legal || legal[j]; }
-};
-
-// Minus infinity in the entries of a unit whose mask byte is zero.
-template <typename T>
-__device__ __forceinline__ void hide(uint4& unit, uint2 mask) {
-  uint32_t* w = reinterpret_cast<uint32_t*>(&unit);
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) w[e] = mask.x >> (8 * e) & 255u ? w[e] : 0xff800000u;
-  } else {
-    constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0xfc00fc00u : 0xff80ff80u;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const uint32_t bytes = (e < 2 ? mask.x : mask.y) >> (16 * (e & 1));
-      const uint32_t keep = (bytes & 0xffu ? 0x0000ffffu : 0u) | (bytes & 0xff00u ? 0xffff0000u : 0u);
-      w[e] = (w[e] & keep) | (kInf & ~keep);
-    }
-  }
-}
-
-// The mask bytes of a unit: one or two aligned words where they lie inside the row, else byte by byte.
-template <typename T>
-__device__ __forceinline__ uint2 mask_bytes(const Row<T>& row, int j) {
-  constexpr int kVec = kVector<T>;
-  const uint8_t* p = row.legal + j;
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & (kVec - 1));
-  uint2 m = make_uint2(0, 0);
-  if (j - off >= 0 && j - off + 2 * kVec <= row.width) {
-    if constexpr (kVec == 8) {
-      const uint64_t* w = reinterpret_cast<const uint64_t*>(p - off);
-      uint64_t v = w[0];
-      if (off) v = v >> (8 * off) | w[1] << (64 - 8 * off);
-      m = make_uint2(static_cast<uint32_t>(v), static_cast<uint32_t>(v >> 32));
-    } else {
-      const uint32_t* w = reinterpret_cast<const uint32_t*>(p - off);
-      m.x = off ? __funnelshift_r(w[0], w[1], 8 * off) : w[0];
-    }
-    return m;
-  }
-#pragma unroll
-  for (int e = 0; e < kVec; ++e) {
-    const uint32_t b = p[e];
-    if (e < 4)
-      m.x |= b << (8 * e);
-    else
-      m.y |= b << (8 * (e - 4));
-  }
-  return m;
-}
-
-template <typename T>
-__device__ __forceinline__ uint4 gather_unit(const T* p) {
-  T v[kVector<T>];
-#pragma unroll
-  for (int e = 0; e < kVector<T>; ++e) v[e] = p[e];
-  return *reinterpret_cast<const uint4*>(v);
-}
-
 // One unit of a row, what the mask hides at minus infinity; the number of legal entries is added to `count`.
 template <typename T, bool kExact>
 __device__ __forceinline__ void load_unit(const Row<T>& row, int j, uint4& z, uint4& r, float& count) {
   z = *reinterpret_cast<const uint4*>(row.z + j);
   if (kExact) r = row.alike ? *reinterpret_cast<const uint4*>(row.r + j) : gather_unit(row.r + j);
   if (!row.legal) return;
-  const uint2 m = mask_bytes(row, j);
-  count += static_cast<float>((__popc(__vcmpne4(m.x, 0)) + __popc(__vcmpne4(m.y, 0))) >> 3);
+  uint2 m = mask_bytes(row, j);
+  m = make_uint2(__vcmpne4(m.x, 0), __vcmpne4(m.y, 0));
+  count += static_cast<float>((__popc(m.x) + __popc(m.y)) >> 3);
   hide<T>(z, m);
   if (kExact) hide<T>(r, m);
 }
@@ -736,7 +773,8 @@ __global__ void __launch_bounds__(kThreads, (kThreads >= 512 ? 1024 : 768) / kTh
       if (a.log_probs) {
         if (lane == 0) a.log_probs[index] = live ? (z_a - s.peak) - logf(s.sum) : 0.f;
       } else {
-        const RowGrad g = finish_row(a, in, s, z_a, live, acc);
+        RowGrad g = finish_row(a, in, s, z_a, live, acc);
+        if (kExact) g.constant -= g.beta * (s.peak - s.reference_peak);  // the entries' own differences are z - r here
         // Large coefficients could take a finite difference past the largest float: then a probability of zero is tested.
         if (lane == 0) row_out[turn] = {g, s.peak, live, part.tested != 0.f || g.alpha > 0.5f || g.beta > 0.5f};
       }
@@ -832,12 +870,12 @@ int resident_blocks(K kernel, int threads) {
   return std::min(per_sm * sm_count(), kPartials);
 }
 
-template <typename T, int kLanes, int kVectors>
+template <typename T, bool kExact, int kLanes, int kPer>
 int run_narrow(const Args& a, int* blocks, cudaStream_t s) {
-  static const int resident = resident_blocks(anchored_narrow_kernel<T, kLanes, kVectors>, 256);
+  static const int resident = resident_blocks(anchored_narrow_kernel<T, kExact, kLanes, kPer>, 256);
   constexpr int kRows = 8 * (32 / kLanes);
   *blocks = static_cast<int>(std::min<int64_t>((a.rows + kRows - 1) / kRows, resident));
-  anchored_narrow_kernel<T, kLanes, kVectors><<<*blocks, 256, 0, s>>>(a);
+  anchored_narrow_kernel<T, kExact, kLanes, kPer><<<*blocks, 256, 0, s>>>(a);
   return check_launch("anchored_narrow_kernel");
 }
 
@@ -849,30 +887,40 @@ int run_row(const Args& a, int* blocks, cudaStream_t s) {
   return check_launch("anchored_row_kernel");
 }
 
-// The smallest block that holds the row in its registers, else the smallest whose resident blocks' rows stay in L2
-// between their two readings (80 of its 126 MB, the rest for the gradient passing through).
+// The smallest block that holds the row in its registers. Longer rows: 16-bit ones, bound by their arithmetic, take 256
+// threads; so do float32 ones whose resident blocks' rows stay in L2 between their two readings (80 of its 126 MB, the rest
+// for the gradient passing through), else 1024 threads, which have fewer rows in work.
 template <typename T, bool kExact>
 int run_wide(const Args& a, int* blocks, cudaStream_t s) {
   constexpr int kHeldEntries = 4 * kVector<T>;  // a thread's
   if (a.width <= 64 * kHeldEntries) return run_row<T, kExact, 64, true>(a, blocks, s);
   if (a.width <= 128 * kHeldEntries) return run_row<T, kExact, 128, true>(a, blocks, s);
   if (a.width <= 256 * kHeldEntries) return run_row<T, kExact, 256, true>(a, blocks, s);
-  const int64_t row_bytes = static_cast<int64_t>(a.width) * sizeof(T) * (kExact ? 2 : 1), room = int64_t{80} << 20;
-  if (!a.grad || 4 * sm_count() * row_bytes <= room) return run_row<T, kExact, 256, false>(a, blocks, s);
-  if (2 * sm_count() * row_bytes <= room) return run_row<T, kExact, 512, false>(a, blocks, s);
-  return run_row<T, kExact, 1024, false>(a, blocks, s);
+  if constexpr (sizeof(T) == 4) {
+    const int64_t row_bytes = static_cast<int64_t>(a.width) * sizeof(T) * (kExact ? 2 : 1);
+    if (a.grad && 3 * sm_count() * row_bytes > int64_t{80} << 20) return run_row<T, kExact, 1024, false>(a, blocks, s);
+  }
+  return run_row<T, kExact, 256, false>(a, blocks, s);
 }
 
-// A row goes where it fits: registers of four lanes (64 entries), of a warp (1024) or of a block, or a block that reads it
-// twice.
+// A row goes where it fits: registers of two lanes (32 entries) to a warp (1024) or of a block, or a block that reads it
+// twice. An unaligned row takes up to a unit more.
+template <typename T, bool kExact>
+int run_typed(const Args& a, int* blocks, cudaStream_t s) {
+  const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && (a.rows == 1 || a.stride % kVector<T> == 0);
+  const int64_t span = static_cast<int64_t>(a.width) + (aligned ? 0 : kVector<T> - 1);
+  if (span <= 32) return run_narrow<T, kExact, 2, 16>(a, blocks, s);
+  if (span <= 64) return run_narrow<T, kExact, 4, 16>(a, blocks, s);
+  if (span <= 128) return run_narrow<T, kExact, 8, 16>(a, blocks, s);
+  if (span <= 256) return run_narrow<T, kExact, 16, 16>(a, blocks, s);
+  if (span <= 512) return run_narrow<T, kExact, 32, 16>(a, blocks, s);
+  if (span <= 1024) return run_narrow<T, kExact, 32, 32>(a, blocks, s);
+  return run_wide<T, kExact>(a, blocks, s);
+}
+
 template <typename T>
 int run_typed(const Args& a, int* blocks, cudaStream_t s) {
-  constexpr int kUnit = 8 / kVector<T>;  // vectors of eight entries
-  if (a.width <= 64) return run_narrow<T, 4, 2 * kUnit>(a, blocks, s);
-  if (a.width <= 256) return run_narrow<T, 32, kUnit>(a, blocks, s);
-  if (a.width <= 512) return run_narrow<T, 32, 2 * kUnit>(a, blocks, s);
-  if (a.width <= 1024) return run_narrow<T, 32, 4 * kUnit>(a, blocks, s);
-  return a.reference ? run_wide<T, true>(a, blocks, s) : run_wide<T, false>(a, blocks, s);
+  return a.reference ? run_typed<T, true>(a, blocks, s) : run_typed<T, false>(a, blocks, s);
 }
 
 int run_rows(const Args& a, int dtype, int* blocks, cudaStream_t s) {
