@@ -4,8 +4,8 @@
 // CTA's own 128 rows of A and its half of B's tile_n rows from its own shared memory, so a stage of 64 k's is 32 KB per
 // SM for 2 x 256 x 256 x 64 FMAs, and each CTA's tensor memory receives its own 128 rows. The kernel is persistent: tensor
 // memory holds two accumulators, and the epilogue of one tile runs while the next is multiplied.
-//   warps 0-7  epilogue: tensor memory -> registers -> a 4 KB shared-memory square per warp -> rows of four columns a lane,
-//              so that bias, residual and results move in whole sectors whatever the strides
+//   warps 0-7  epilogue: 32 columns of a row a lane from tensor memory to registers and, where rows are aligned, from there to
+//              their place in whole sectors; else through a 4 KB shared-memory square per warp, four columns a lane
 //   warp 8     lane 0 fills the ring of six stages by TMA (128-byte swizzle; both operand orders, so neither product of
 //              the backward pass transposes anything in memory)
 //   warp 9     allocates tensor memory; in the even CTA lane 0 issues the MMAs
@@ -139,60 +139,97 @@ __device__ __forceinline__ void finish4(const ProductEpilogue& e, int64_t i, int
   store4(static_cast<T*>(e.out) + i * e.out_stride + j, n, whole, z);
 }
 
-// What the epilogue of a warp's square reads from memory: a lane's four biases and its eight rows of residual.
+// Thirty-two entries of a row in memory, as they are: 16-byte aligned, `sectors`: to 32 bytes too, which then move whole.
 template <typename T>
-struct Ahead {
-  using Raw = typename std::conditional<sizeof(T) == 4, uint4, uint2>::type;
-  Raw residual[8];
-  float bias[4];
-  bool whole;  // the square lies inside the matrix and its rows are aligned
-  __device__ __forceinline__ Ahead() : whole(false) {}
-  __device__ __forceinline__ Ahead(const ProductEpilogue& e, int lane, int64_t i0, int64_t rows, int64_t j, int64_t cols,
-                                   bool aligned) {
-    whole = aligned && i0 + 32 <= rows && j - 4 * (lane & 7) + 32 <= cols;
-    load_bias<T>(e, j, cols, bias);
-    if (!whole || !e.residual) return;
-    const T* from = static_cast<const T*>(e.residual) + (i0 + (lane >> 3)) * e.residual_stride + j;
+struct RowOf32 {
+  static constexpr int kWords = static_cast<int>(sizeof(T)) * 8;
+  uint32_t w[kWords];
+  __device__ __forceinline__ void load(const T* p, bool sectors) {
+    const char* from = reinterpret_cast<const char*>(p);
+    if (sectors) {
 #pragma unroll
-    for (int r = 0; r < 8; ++r) residual[r] = *reinterpret_cast<const Raw*>(from + r * 4 * e.residual_stride);
+      for (int k = 0; k < kWords; k += 8)
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(w[k]), "=r"(w[k + 1]), "=r"(w[k + 2]), "=r"(w[k + 3]), "=r"(w[k + 4]), "=r"(w[k + 5]),
+                       "=r"(w[k + 6]), "=r"(w[k + 7])
+                     : "l"(from + 4 * k));
+    } else {
+#pragma unroll
+      for (int k = 0; k < kWords; k += 4) *reinterpret_cast<uint4*>(w + k) = *reinterpret_cast<const uint4*>(from + 4 * k);
+    }
+  }
+  __device__ __forceinline__ void store(T* p, bool sectors) const {
+    char* to = reinterpret_cast<char*>(p);
+    if (sectors) {
+#pragma unroll
+      for (int k = 0; k < kWords; k += 8)
+        asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(w[k]), "r"(w[k + 1]), "r"(w[k + 2]),
+                     "r"(w[k + 3]), "r"(w[k + 4]), "r"(w[k + 5]), "r"(w[k + 6]), "r"(w[k + 7]), "l"(to + 4 * k)
+                     : "memory");
+    } else {
+#pragma unroll
+      for (int k = 0; k < kWords; k += 4)
+        *reinterpret_cast<uint4*>(to + 4 * k) = make_uint4(w[k], w[k + 1], w[k + 2], w[k + 3]);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&z)[32]) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) w[k] = __float_as_uint(z[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) pair_from(*reinterpret_cast<typename PairOf<T>::type*>(&w[k]), z[2 * k], z[2 * k + 1]);
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&z)[32]) const {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < 32; ++k) z[k] += __uint_as_float(w[k]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float2 f = pair_float(*reinterpret_cast<const typename PairOf<T>::type*>(&w[k]));
+        z[2 * k] += f.x, z[2 * k + 1] += f.y;
+      }
+    }
   }
 };
 
-// A warp's square of 32 x 32 sums in shared memory (a row of eight four-column vectors, vector q of row r at q ^ (r & 7)) to
-// its place: four rows at a time, four columns a lane.
+// Row i's 32 sums from column j on, all inside the matrix, to their place. A lane a row, without a detour through shared
+// memory: every 32-byte sector moves whole all the same (8192 x 1024 x 4096 bfloat16 with GELU 70 us, through squares 82).
 template <typename T, int kActivation>
-__device__ __forceinline__ void finish_square(const ProductEpilogue& e, const Ahead<T>& ahead, const float4* square, int lane,
-                                              int64_t i0, int64_t rows, int64_t j, int64_t cols, bool aligned) {
-  const int q = lane & 7, first = lane >> 3;
-  if (ahead.whole) {
-    const int64_t i = i0 + first;
-    T* out = static_cast<T*>(e.out) + i * e.out_stride + j;
-    T* pre = e.pre ? static_cast<T*>(e.pre) + i * cols + j : nullptr;
-    const int64_t out_step = 4 * e.out_stride, pre_step = 4 * cols;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-      const int row = r * 4 + first;
-      const float4 f = square[row * 8 + (q ^ (row & 7))];
-      float z[4] = {f.x + ahead.bias[0], f.y + ahead.bias[1], f.z + ahead.bias[2], f.w + ahead.bias[3]};
-      if (pre) store4(pre + r * pre_step, z);
-      activate4<T, kActivation>(z);
-      if (e.residual) {
-        float add[4];
-        load4(reinterpret_cast<const T*>(&ahead.residual[r]), add);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) z[k] += add[k];
-      }
-      store4(out + r * out_step, z);
-    }
-    return;
+__device__ __forceinline__ void finish_row32(const ProductEpilogue& e, const RowOf32<T>& residual, int64_t i, int64_t j,
+                                             int64_t cols, bool inside, bool sectors, float (&z)[32]) {
+  RowOf32<T> row;
+  if (e.bias) {
+    row.load(static_cast<const T*>(e.bias) + j, false);
+    row.add_to(z);
   }
+  if (e.pre) {
+    row.set(z);
+    if (inside) row.store(static_cast<T*>(e.pre) + i * cols + j, sectors);
+  }
+  activate4<T, kActivation>(z);
+  if (e.residual) residual.add_to(z);
+  row.set(z);
+  if (inside) row.store(static_cast<T*>(e.out) + i * e.out_stride + j, sectors);
+}
+
+// The same for a square of 32 x 32 sums in shared memory (a row of eight four-column vectors, vector q of row r at
+// q ^ (r & 7)) that the matrix's edge cuts or whose rows are not aligned: four rows at a time, four columns a lane.
+template <typename T, int kActivation>
+__device__ __forceinline__ void finish_square(const ProductEpilogue& e, const float4* square, int lane, int64_t i0, int64_t rows,
+                                              int64_t j, int64_t cols, bool aligned) {
+  const int q = lane & 7, first = lane >> 3;
   if (j >= cols) return;
+  float bias[4];
+  load_bias<T>(e, j, cols, bias);
   for (int r = 0; r < 8; ++r) {
     const int row = r * 4 + first;
     if (i0 + row >= rows) return;
     const float4 f = square[row * 8 + (q ^ (row & 7))];
     float z[4] = {f.x, f.y, f.z, f.w};
-    finish4<T, kActivation>(e, i0 + row, j, cols, ahead.bias, aligned, z);
+    finish4<T, kActivation>(e, i0 + row, j, cols, bias, aligned, z);
   }
 }
 
@@ -352,20 +389,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
       if (lane == 0) tc::bar_arrive_cluster(tc::map_shared(tc::smem_u32(&acc_empty[done & 1]), 0));
       ++done;
     };
+    // Every plane's rows start on a multiple of `bytes`.
+    auto rows_start_on = [&](int bytes) {
+      auto on = [&](const void* base, int64_t stride) {
+        return !base || ((reinterpret_cast<uintptr_t>(base) | (stride * sizeof(T))) & (bytes - 1)) == 0;
+      };
+      return on(p.e.out, p.e.out_stride) && on(p.e.residual, p.e.residual_stride) && on(p.e.pre, p.cols) && on(p.e.bias, 0);
+    };
+    const bool direct = rows_start_on(16), sectors = rows_start_on(32);
     for (int index = pair; index < items && ok; index += pairs) {
       const Item t = item_of(p, index);
-      const int64_t i0 = static_cast<int64_t>(t.i) * kTileM + rank * 128 + quarter * 32;
-      const int64_t tile_j = static_cast<int64_t>(t.j) * p.tile_n;
-      auto column_of = [&](int c) { return tile_j + (half * chunks + c) * 32 + (lane & 7) * 4; };
-      auto outside = [&](int c) { return i0 >= p.rows || tile_j + (half * chunks + c) * 32 >= p.cols; };
-      // What a square's epilogue reads from memory, under way before its sums are.
-      auto ahead_of = [&](int c) {
-        return outside(c) || t.slot >= 0 ? Ahead<T>() : Ahead<T>(p.e, lane, i0, p.rows, column_of(c), p.cols, aligned);
+      const int64_t i0 = static_cast<int64_t>(t.i) * kTileM + rank * 128 + quarter * 32, i = i0 + lane;
+      auto first_column = [&](int c) { return static_cast<int64_t>(t.j) * p.tile_n + (half * chunks + c) * 32; };
+      auto row_at_once = [&](int c) { return direct && t.slot < 0 && first_column(c) + 32 <= p.cols; };
+      // A row's residual, under way before its sums are.
+      auto residual_of = [&](int c) {
+        RowOf32<T> r;
+        if (p.e.residual && i < p.rows && row_at_once(c))
+          r.load(static_cast<const T*>(p.e.residual) + i * p.e.residual_stride + first_column(c), sectors);
+        return r;
       };
       // 32 rows by 32 columns of sums, a row a lane, to their place.
-      auto store_sums = [&](int c, const float (&v)[32], const Ahead<T>& ahead) {
-        if (outside(c)) return;
-        const int64_t j = column_of(c);
+      auto store_sums = [&](int c, float (&v)[32], const RowOf32<T>& residual) {
+        const int64_t j0 = first_column(c);
+        if (i0 >= p.rows || j0 >= p.cols) return;
+        if (row_at_once(c)) {
+          with_activation(p.e.activation, [&](auto activation) {
+            finish_row32<T, activation>(p.e, residual, i, j0, p.cols, i < p.rows, sectors, v);
+          });
+          return;
+        }
 #pragma unroll
         for (int q = 0; q < 8; ++q)
           square[lane * 8 + (q ^ (lane & 7))] = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
@@ -380,7 +433,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           }
         } else {
           with_activation(p.e.activation, [&](auto activation) {
-            finish_square<T, activation>(p.e, ahead, square, lane, i0, p.rows, j, p.cols, aligned);
+            finish_square<T, activation>(p.e, square, lane, i0, p.rows, j0 + (lane & 7) * 4, p.cols, aligned);
           });
         }
         __syncwarp();
@@ -403,16 +456,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         if (!ok) break;
 #pragma unroll
-        for (int c = 0; c < 2; ++c) store_sums(c, sums[c], ahead_of(c));
+        for (int c = 0; c < 2; ++c) store_sums(c, sums[c], residual_of(c));
       } else {
-        Ahead<T> ahead = ahead_of(0);
+        RowOf32<T> residual = residual_of(0);
         if (!wait_sum()) break;
         for (int c = 0; c < chunks; ++c) {
           float v[32];
           read_sum(c, 0, v);
           if (c == chunks - 1) release_sum();
-          store_sums(c, v, ahead);
-          if (c + 1 < chunks) ahead = ahead_of(c + 1);
+          store_sums(c, v, residual);
+          if (c + 1 < chunks) residual = residual_of(c + 1);
         }
       }
     }
@@ -436,17 +489,17 @@ template <typename T>
 __global__ void __launch_bounds__(256) product_join_kernel(const float* partial, int whole, int splits, int tile_n, int tiles_i,
                                                            int tiles_j, int64_t rows, int64_t cols, const ProductEpilogue e) {
   const bool aligned = epilogue_aligned<T>(e, cols);
-  const int quads = tile_n / 4;
-  const int64_t total = static_cast<int64_t>(tiles_i * tiles_j - whole) * kTileM * quads;
-  for (int64_t index = blockIdx.x * 256ll + threadIdx.x; index < total; index += gridDim.x * 256ll) {
-    const int64_t line = index / quads;
-    const int q = static_cast<int>(index - line * quads), tile = static_cast<int>(line / kTileM), row = static_cast<int>(line % kTileM);
+  const int shift = tile_n == 256 ? 6 : 5;  // vectors of four columns in a tile's row
+  const int total = (tiles_i * tiles_j - whole) * kTileM << shift;  // at most 37 tiles
+  for (int index = blockIdx.x * 256 + threadIdx.x; index < total; index += gridDim.x * 256) {
+    const int line = index >> shift, q = index & ((1 << shift) - 1), tile = line / kTileM, row = line % kTileM;
     int ti, tj;
     place_tile(whole + tile, tiles_i, tiles_j, &ti, &tj);
     const int64_t i = static_cast<int64_t>(ti) * kTileM + row, j = static_cast<int64_t>(tj) * tile_n + q * 4;
     if (i >= rows || j >= cols) continue;
     float z[4] = {0.f, 0.f, 0.f, 0.f};
     const float* from = partial + (static_cast<int64_t>(tile) * splits * kTileM + row) * tile_n + q * 4;
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) {
       const float4 f = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(s) * kTileM * tile_n);
       z[0] += f.x, z[1] += f.y, z[2] += f.z, z[3] += f.w;
@@ -535,10 +588,13 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
 
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
   ProductPlan plan = {};
-  plan.tile_n = dtype != CG_F32 && cols > 128 ? 256 : 128;
+  const int64_t pairs = 74;  // the B200's 148 SMs
+  auto tiles_of = [&](int tile_n) { return (rows + kTileM - 1) / kTileM * ((cols + tile_n - 1) / tile_n); };
+  // 16-bit operands: half tiles where they fill more than half the pairs in one round and whole ones would be split
+  // (2048 x 1024 x 1024: 18 us against 25; 512 x 4096 x 4096: equal).
+  plan.tile_n = dtype == CG_F32 || cols <= 128 || (tiles_of(128) <= pairs && 2 * tiles_of(128) > pairs) ? 128 : 256;
   plan.tiles_i = static_cast<int>((rows + kTileM - 1) / kTileM);
   plan.tiles_j = static_cast<int>((cols + plan.tile_n - 1) / plan.tile_n);
-  const int64_t pairs = 74;  // the B200's 148 SMs
   const int64_t k_blocks = (depth + kTileK - 1) / kTileK, tiles = static_cast<int64_t>(plan.tiles_i) * plan.tiles_j;
   // A split is a whole number of units: kLeastSplitBlocks k blocks, or a float32 chunk.
   const int64_t unit = dtype == CG_F32 ? kChunkBlocks : kLeastSplitBlocks, units = (k_blocks + unit - 1) / unit;
