@@ -83,26 +83,26 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, const RowIn& in, co
   RowGrad g = {0.f, 0.f, 0.f, 0.f, 0.f};
   if (!counts) return g;
   const float w = in.weight, advantage = in.advantage;
-  const float log_sum = __logf(s.sum);
+  const float log_sum = logf(s.sum);
   const float lp = (z_a - s.peak) - log_sum;
   const float log_ratio = lp - in.old_log_prob;
-  const float ratio = __expf(log_ratio);
+  const float ratio = expf(log_ratio);
   const float free = ratio * advantage;
   const float bounded = fminf(fmaxf(ratio, 1.f - a.clip), 1.f + a.clip) * advantage;
   const bool held = free > bounded;
   const float surrogate = -(held ? bounded : free);
   float slope = held ? 0.f : -advantage * ratio;
-  g.inv_sum = __fdividef(1.f, s.sum);
+  g.inv_sum = 1.f / s.sum;
   const float entropy = log_sum - s.spread * g.inv_sum;
   const bool eligible = s.count > 1.f;
-  const float norm = eligible ? __fdividef(1.f, __logf(s.count)) : 0.f;
+  const float norm = eligible ? 1.f / logf(s.count) : 0.f;
   float kl = 0.f, log_apart = 0.f;
   if (a.reference) {
-    log_apart = log_sum - __logf(s.reference_sum);
+    log_apart = log_sum - logf(s.reference_sum);
     kl = s.apart * g.inv_sum - log_apart;
     g.beta = w * a.beta;
   } else if (a.reference_action) {
-    const float u = in.reference_log_prob - lp, grown = __expf(u);
+    const float u = in.reference_log_prob - lp, grown = expf(u);
     kl = grown - u - 1.f;
     slope += a.beta * (1.f - grown);
   }
