@@ -7,6 +7,8 @@
 
 from __future__ import annotations
 
+import functools
+
 import torch
 from torch.autograd.function import once_differentiable
 
@@ -29,11 +31,22 @@ def _row_stride(matrix: torch.Tensor) -> int:
     return max(matrix.stride(0), matrix.shape[1]) if matrix.shape[0] > 1 else matrix.shape[1]
 
 
+@functools.lru_cache(maxsize=4096)
+def _workspace_bytes(*layout: int) -> int:
+    return nat.query("cg_linear_workspace_bytes", *layout)
+
+
 def _workspace(x, weight, dy, activation: int) -> torch.Tensor | None:
-    need = nat.query("cg_linear_workspace_bytes", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight),
-                     nat.ptr(dy), 0 if dy is None else _row_stride(dy), nat.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1],
-                     weight.shape[0], activation, 0 if dy is None else 1)
+    # Of the addresses only their places within sixteen bytes count.
+    need = _workspace_bytes(nat.ptr(x) & 15, _row_stride(x), nat.ptr(weight) & 15, _row_stride(weight),
+                            0 if dy is None else nat.ptr(dy) & 15, 0 if dy is None else _row_stride(dy),
+                            nat.DTYPE_CODES[x.dtype], x.shape[0], x.shape[1], weight.shape[0], activation,
+                            0 if dy is None else 1)
     return torch.empty(need, dtype=torch.uint8, device=x.device) if need else None
+
+
+def _empty(matrix: torch.Tensor) -> torch.Tensor:
+    return torch.empty_like(matrix) if matrix.is_contiguous() else matrix.new_empty(matrix.shape)
 
 
 def _forward(x, weight, bias, residual, activation: int, keep: bool):
@@ -42,7 +55,7 @@ def _forward(x, weight, bias, residual, activation: int, keep: bool):
     rows, inner = x.shape
     outer = weight.shape[0]
     with nat.on_device(x.device):
-        y = torch.empty((rows, outer), dtype=x.dtype, device=x.device)
+        y = x.new_empty((rows, outer))
         pre = torch.empty_like(y) if keep else None
         workspace = _workspace(x, weight, None, activation)
         nat.call("cg_linear_forward", nat.ptr(x), _row_stride(x), nat.ptr(weight), _row_stride(weight), nat.ptr(bias),
@@ -73,9 +86,9 @@ class _Linear(torch.autograd.Function):
             outer = weight.shape[0]
             g = _unit_rows(dy)
             with nat.on_device(x.device):
-                dx = torch.empty((rows, inner), dtype=x.dtype, device=x.device) if needs_x else None
-                dweight = torch.empty((outer, inner), dtype=x.dtype, device=x.device) if needs_weight else None
-                dbias = torch.empty(outer, dtype=x.dtype, device=x.device) if needs_bias else None
+                dx = _empty(x) if needs_x else None
+                dweight = _empty(weight) if needs_weight else None
+                dbias = x.new_empty(outer) if needs_bias else None
                 workspace = _workspace(x, weight, g, ctx.activation)
                 nat.call("cg_linear_backward", nat.ptr(g), _row_stride(g), nat.ptr(pre), nat.ptr(x), _row_stride(x),
                          nat.ptr(weight), _row_stride(weight), nat.DTYPE_CODES[x.dtype], rows, inner, outer,
