@@ -299,11 +299,15 @@ __device__ __forceinline__ uint4 gather_unit(const T* p) {
 }
 
 // ---- up to 1024 entries: a row in the registers of a few lanes ----------------------------------------------------------
-// A row has some 300 instructions of its own (reductions, logarithms, the ratio) beside 25 an entry, so as few lanes as hold
-// it, sixteen entries each, take a row, and a warp takes up to sixteen rows at a time. The row is read once and written
-// once, and the grid is one resident wave of warps. A lane holds every kLanes-th unit of sixteen bytes from the aligned
+// A row has some 350 instructions of its own (reductions, logarithms, the ratio) beside 25 an entry, so as few lanes as hold
+// it, sixteen entries each, take a row, and a warp takes up to sixteen rows at a time (100,000 x 100: 50 us; with eight
+// entries a lane 62). The row is read once and written once, and the grid is one resident wave of warps, two blocks an SM
+// (with three the registers spill: 262,144 x 52 73 us instead of 61). A lane holds every kLanes-th unit of sixteen bytes from the aligned
 // address at or before the row's start; the units that the row only partly fills, and planes aligned differently
 // from the logits', go entry by entry.
+//
+// What bounds it is the issue of those instructions: 262,144 masked float32 rows of 52 with a reference take 61 us (164 MB, 41%
+// of the copy bandwidth), 40,000 rows of 1000 113 us (65%).
 //
 // An entry whose exponential is zero counts for nothing. So that no test is needed, its distance from the maximum is
 // held to kFar, where the exponential is zero too, and its distance from the reference is set to zero.
@@ -520,11 +524,12 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
 // A thread holds its share of the row, or of a batch of it, in registers as it is in memory: up to four units of sixteen
 // bytes of each plane in flight at a time. It sums a batch relative to the batch's own maxima and merges the result into
 // its running sums, so the row's maxima are never waited for; the block joins its threads once a row.
-// A row of one batch (kHeld) is read once and its gradient computed from the registers. A longer one is read again for
-// the gradient, out of L2: the blocks are made so large that the rows in work at one time fit there (see run_wide).
+// A row of one batch (kHeld) is read once and its gradient computed from the registers (16,384 x 4096 bfloat16: 124 us, read
+// twice 230). A longer one is read again for the gradient, out of L2 where the rows in work at one time fit (see run_wide).
 //
-// What bounds it is instruction issue beside memory: three exponentials an entry and, in packed fp32 pairs, some 20
-// instructions. Entries at minus infinity, which the packed sums turn into NaN, are found by that and summed again
+// What bounds it is instruction issue beside memory: three exponentials an entry and, in packed fp32 pairs, some 25
+// instructions at 2.2 a cycle and SM. 4096 x 131072 bfloat16 with a reference: 860 us for 3.2 GB, 57% of the copy bandwidth;
+// 4000 x 32000 float32 361 us, 65%; log-probabilities of 1500 x 50,021 float16 42 us, 55%. Entries at minus infinity, which the packed sums turn into NaN, are found by that and summed again
 // with tests. Units start where the logits' row is aligned; the few entries before and after them go one a
 // thread, and planes aligned differently from the logits' are read entry by entry.
 
@@ -888,8 +893,9 @@ int run_row(const Args& a, int* blocks, cudaStream_t s) {
 }
 
 // The smallest block that holds the row in its registers. Longer rows: 16-bit ones, bound by their arithmetic, take 256
-// threads; so do float32 ones whose resident blocks' rows stay in L2 between their two readings (80 of its 126 MB, the rest
-// for the gradient passing through), else 1024 threads, which have fewer rows in work.
+// threads (131,072 entries: 859 us, with 1024 threads 878; 32,000: 220 against 264). So do float32 ones whose resident
+// blocks' rows stay in L2 between their two readings (80 of its 126 MB, the rest for the gradient passing through:
+// 10,000 entries 123 us against 185), else 1024 threads, which have fewer rows in work (32,000: 361 against 411).
 template <typename T, bool kExact>
 int run_wide(const Args& a, int* blocks, cudaStream_t s) {
   constexpr int kHeldEntries = 4 * kVector<T>;  // a thread's
@@ -903,8 +909,8 @@ int run_wide(const Args& a, int* blocks, cudaStream_t s) {
   return run_row<T, kExact, 256, false>(a, blocks, s);
 }
 
-// A row goes where it fits: registers of two lanes (32 entries) to a warp (1024) or of a block, or a block that reads it
-// twice. An unaligned row takes up to a unit more.
+// A row goes where it fits: registers of two lanes (32 entries) to a warp (1024; 40,000 x 1000 float32: 113 us, by the next
+// rule's blocks 170) or of a block, or a block that reads it twice. An unaligned row takes up to a unit more.
 template <typename T, bool kExact>
 int run_typed(const Args& a, int* blocks, cudaStream_t s) {
   const bool aligned = (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0 && (a.rows == 1 || a.stride % kVector<T> == 0);

@@ -36,7 +36,8 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype);
 int run_product(const ProductOperand& a, const ProductOperand& b, int64_t rows, int64_t cols, int64_t depth, int dtype,
                 const ProductEpilogue& e, void* partial, cudaStream_t stream);
 
-// The forward layer of at most kFewRows rows, its weights read once.
+// The forward layer of at most kFewRows rows, its weights read once. (4096 x 8192, 24 tokens: bfloat16 20 us, by run_product
+// 33; float32 139 against 165. 32 tokens: 22 against 32, and 172 against 166; 2048 x 512 float32 10 against 27.)
 constexpr int kFewRows = 32;
 int run_few_rows(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t rows, int64_t inner,
                  int64_t outer, int dtype, const ProductEpilogue& e, cudaStream_t stream);
