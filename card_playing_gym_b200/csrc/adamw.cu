@@ -351,13 +351,13 @@ __device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e
     for (int i = 0; i < kPerLane; ++i) l.v[i] *= l.v[i];
   }
   float peak_m = 0.f, peak_r = 0.f;
-  const Two beta1 = two(f.beta1, f.beta1), rest1 = two(f.rest1 * clip, f.rest1 * clip), beta2 = two(f.beta2, f.beta2),
+  const Two beta1 = two(f.beta1, f.beta1), rest1 = two(f.rest1, f.rest1), beta2 = two(f.beta2, f.beta2),
             rest2 = two(f.rest2, f.rest2), clips = two(clip, clip), decay = two(f.decay, f.decay),
             step = two(-f.step, -f.step), unbias = two(f.root, f.root), eps = two(f.eps, f.eps);
 #pragma unroll
   for (int i = 0; i < kPerLane; i += 2) {
     const Two raw = two(l.g[i], l.g[i + 1]), g = raw * clips;
-    const Two m = fma(beta1, two(l.m[i], l.m[i + 1]), rest1 * raw);
+    const Two m = beta1 * two(l.m[i], l.m[i + 1]) + rest1 * g;
     const Two v = fma(beta2, two(l.v[i], l.v[i + 1]), rest2 * (g * g));
     const float2 fv = apart_of(v), fm = apart_of(m);
     const float2 root = make_float2(root_fast(fv.x), root_fast(fv.y));
@@ -512,10 +512,11 @@ extern "C" int64_t cg_adamw_workspace_bytes(int count) {
   return (static_cast<int64_t>(count) / cg::kFewTensors + 1) * cg::kNormBlocks * static_cast<int64_t>(sizeof(double));
 }
 
-extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params, const void* const* grads, int count, int dtype, const cg_adamw_group* groups,
-                             int group_count, int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq,
-                             float* exp_avg_sq_scale, float* master, int64_t* steps, float max_norm, float* norm_out,
-                             void* control, void* workspace, int64_t workspace_bytes, void* stream) {
+extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params, const void* const* grads, int count,
+                             int dtype, const cg_adamw_group* groups, int group_count, int state_bits, void* exp_avg,
+                             float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale, float* master, int64_t* steps,
+                             float max_norm, float* norm_out, void* control, void* workspace, int64_t workspace_bytes,
+                             void* stream) {
   using namespace cg;
   CG_REQUIRE(count >= 0 && (count == 0 || (tensors && params && grads)), "cg_adamw_step: bad tensor table");
   CG_REQUIRE(valid_dtype(dtype), "cg_adamw_step: dtype must be float32, float16 or bfloat16");

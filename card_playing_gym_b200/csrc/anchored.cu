@@ -302,9 +302,9 @@ __device__ __forceinline__ uint4 gather_unit(const T* p) {
 // A row has some 350 instructions of its own (reductions, logarithms, the ratio) beside 25 an entry, so as few lanes as hold
 // it, sixteen entries each, take a row, and a warp takes up to sixteen rows at a time (100,000 x 100: 50 us; with eight
 // entries a lane 62). The row is read once and written once, and the grid is one resident wave of warps, two blocks an SM
-// (with three the registers spill: 262,144 x 52 73 us instead of 61). A lane holds every kLanes-th unit of sixteen bytes from the aligned
-// address at or before the row's start; the units that the row only partly fills, and planes aligned differently
-// from the logits', go entry by entry.
+// (with three the registers spill: 262,144 x 52 73 us instead of 61). A lane holds every kLanes-th unit of sixteen bytes from
+// the aligned address at or before the row's start; the units that the row only partly fills, and planes aligned
+// differently from the logits', go entry by entry.
 //
 // What bounds it is the issue of those instructions: 262,144 masked float32 rows of 52 with a reference take 61 us (164 MB, 41%
 // of the copy bandwidth), 40,000 rows of 1000 113 us (65%).
@@ -322,7 +322,8 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
   auto whole = [&](const void* base, int64_t stride, int size) {
     return ((reinterpret_cast<uintptr_t>(base) | (a.rows > 1 ? stride * size : 0)) & (size * kVec - 1)) == 0;
   };
-  const bool plain_planes = whole(a.logits, a.stride, sizeof(T)) && (!kExact || whole(a.reference, a.reference_stride, sizeof(T))) &&
+  const bool plain_planes = whole(a.logits, a.stride, sizeof(T)) &&
+                            (!kExact || whole(a.reference, a.reference_stride, sizeof(T))) &&
                             (!a.legal || whole(a.legal, a.legal_stride, 1));
   const Two scale = two(kLog2e, kLog2e), minus = two(-1.f, -1.f);
   float acc[kTotals] = {};
@@ -529,9 +530,11 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
 //
 // What bounds it is instruction issue beside memory: three exponentials an entry and, in packed fp32 pairs, some 25
 // instructions at 2.2 a cycle and SM. 4096 x 131072 bfloat16 with a reference: 860 us for 3.2 GB, 57% of the copy bandwidth;
-// 4000 x 32000 float32 361 us, 65%; log-probabilities of 1500 x 50,021 float16 42 us, 55%. Entries at minus infinity, which the packed sums turn into NaN, are found by that and summed again
-// with tests. Units start where the logits' row is aligned; the few entries before and after them go one a
-// thread, and planes aligned differently from the logits' are read entry by entry.
+// 4000 x 32000 float32 361 us, 65%; log-probabilities of 1500 x 50,021 float16 42 us, 55%.
+//
+// Entries at minus infinity, which the packed sums turn into NaN, are found by that and summed again with tests. Units
+// start where the logits' row is aligned; the few entries before and after them go one a thread, and planes aligned
+// differently from the logits' are read entry by entry.
 
 // Partial results over some entries, each relative to their own maxima. `tested`: minus infinity was among them.
 struct Part {

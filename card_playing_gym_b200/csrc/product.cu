@@ -582,15 +582,15 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
     if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel: %s", cudaGetErrorString(configured));
     const int items = plan.whole + (plan.tiles_i * plan.tiles_j - plan.whole) * plan.splits;
     const int pairs = std::min(items, sm_count() / 2);
-    if (int rc = launch_pdl("product_kernel", product_kernel<T>, dim3(2 * pairs), dim3(kThreads), Shape<T>::kSmemBytes, stream, map_a,
-                            map_b, p))
+    if (int rc = launch_pdl("product_kernel", product_kernel<T>, dim3(2 * pairs), dim3(kThreads), Shape<T>::kSmemBytes, stream,
+                            map_a, map_b, p))
       return rc;
     if (plan.whole == plan.tiles_i * plan.tiles_j) return CG_OK;
   }
   const int64_t quads = static_cast<int64_t>(plan.tiles_i * plan.tiles_j - plan.whole) * kTileM * (plan.tile_n / 4);
   const int blocks = static_cast<int>(std::min<int64_t>((quads + 255) / 256, 16 * sm_count()));
-  return launch_pdl("product_join_kernel", product_join_kernel<T>, dim3(blocks), dim3(256), 0, stream, partial, plan.whole, plan.splits,
-                    plan.tile_n, plan.tiles_i, plan.tiles_j, rows, cols, e);
+  return launch_pdl("product_join_kernel", product_join_kernel<T>, dim3(blocks), dim3(256), 0, stream, partial, plan.whole,
+                    plan.splits, plan.tile_n, plan.tiles_i, plan.tiles_j, rows, cols, e);
 }
 
 }  // namespace
