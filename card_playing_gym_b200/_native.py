@@ -8,10 +8,11 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
-from functools import lru_cache
+from functools import lru_cache, wraps
 from pathlib import Path
 
 import torch
+from torch.autograd.function import once_differentiable
 
 LIBRARY = Path(__file__).resolve().parent / "libcg_b200.so"
 
@@ -261,6 +262,19 @@ def on_device(device: torch.device):
 def stream_handle(device: torch.device | None = None) -> int:
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def backward_once(backward):
+    """``once_differentiable`` for an autograd function's backward, at its cost (some 6 us) only where a graph of the
+    backward pass itself is being made."""
+
+    refusing = once_differentiable(backward)
+
+    @wraps(backward)
+    def either(ctx, *grads):
+        return refusing(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return either
 
 
 class Workspace:

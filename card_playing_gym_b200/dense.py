@@ -7,10 +7,9 @@
 
 from __future__ import annotations
 
-import functools
+from functools import lru_cache
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -31,7 +30,7 @@ def _row_stride(matrix: torch.Tensor) -> int:
     return max(matrix.stride(0), matrix.shape[1]) if matrix.shape[0] > 1 else matrix.shape[1]
 
 
-@functools.lru_cache(maxsize=4096)
+@lru_cache(maxsize=4096)
 def _workspace_bytes(*layout: int) -> int:
     return nat.query("cg_linear_workspace_bytes", *layout)
 
@@ -76,7 +75,7 @@ class _Linear(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @nat.backward_once
     def backward(ctx, dy):
         dx = dweight = dbias = None
         needs_x, needs_weight, needs_bias, needs_residual, _ = ctx.needs_input_grad

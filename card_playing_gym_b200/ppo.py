@@ -21,7 +21,6 @@ from dataclasses import dataclass
 from functools import lru_cache
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _native as nat
 
@@ -299,7 +298,7 @@ class _AnchoredObjective(torch.autograd.Function):
         return sums[-1], totals
 
     @staticmethod
-    @once_differentiable
+    @nat.backward_once
     def backward(ctx, grad_objective, _grad_totals):
         if grad_objective is None:
             return None, None
