@@ -408,3 +408,27 @@ def test_the_library_refuses_bad_arguments():
     with pytest.raises(nat.NativeError, match="totals"):
         nat.call("cg_anchored_objective", None, 0, 0, 4, 4, None, 0, None, None, 0, None, None, None, None, 0.2, 0.0,
                  0.0, None, 4, None, None, 0, None)
+
+
+def _moved(plane, before, after):
+    """The plane as columns of a wider store: its rows start `before` entries in."""
+
+    store = torch.zeros((plane.shape[0], before + plane.shape[1] + after), dtype=plane.dtype, device=plane.device)
+    store[:, before:before + plane.shape[1]] = plane
+    return store[:, before:before + plane.shape[1]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("legal", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [2, 17, 31, 32, 33, 61, 64, 65, 125, 128, 129, 250, 256, 257, 509, 512, 513, 777, 1017, 1018,
+                                   1024, 1025])
+def test_the_edges_of_a_rows_registers_at_any_alignment(width, dtype, legal):
+    data = inputs(70, width, TYPES[dtype], legal=legal, seed=width)
+    check(data)
+    data["logits"] = _moved(data["logits"], 1, 2)
+    data["reference_logits"] = _moved(data["reference_logits"], 3, 1)
+    if legal:
+        data["legal"] = _moved(data["legal"], 1, 0)
+    check(data)
+    assert nat.fault_status() == 0

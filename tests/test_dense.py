@@ -253,3 +253,23 @@ def test_refusals_without_a_gpu():
         nat.call("cg_linear_forward", None, 8, None, 8, None, None, 0, 0, 4, 8, 6, 9, None, None, None, 0, None)
     with pytest.raises(nat.NativeError, match="shape"):
         nat.query("cg_linear_workspace_bytes", None, 8, None, 8, None, 0, 0, -1, 8, 8, 0, 0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(4800, 520, 1000), (4800, 520, 500), (2000, 300, 1000), (5000, 100, 1001), (700, 720, 240)])
+def test_rounds_of_tiles_that_do_not_fill_the_chip(shape, dtype):
+    check(case(*shape, TYPES[dtype]), "gelu")
+    assert nat.fault_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("outer", [36, 40, 68, 72, 100, 160])
+def test_results_whose_rows_start_off_a_sector(outer, dtype):
+    data = case(300, 64, outer, TYPES[dtype])
+    check(data, "silu")
+    wide = torch.zeros((300, outer + 12), dtype=TYPES[dtype], device="cuda")
+    for offset in (1, 4, 8):
+        wide[:, offset:offset + outer] = data["residual"]
+        check({**data, "residual": wide[:, offset:offset + outer]}, "relu")
