@@ -577,9 +577,15 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
                     (static_cast<uint32_t>(plan.tile_n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
     p.partial = partial;
     p.e = e;
-    static const cudaError_t configured =
-        cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmemBytes);
-    if (configured != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel: %s", cudaGetErrorString(configured));
+    static bool configured[64] = {false};
+    int device = 0;
+    cudaGetDevice(&device);
+    if (!configured[device & 63]) {
+      cudaError_t err =
+          cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmemBytes);
+      if (err != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel smem: %s", cudaGetErrorString(err));
+      configured[device & 63] = true;
+    }
     const int items = plan.whole + (plan.tiles_i * plan.tiles_j - plan.whole) * plan.splits;
     const int pairs = std::min(items, sm_count() / 2);
     if (int rc = launch_pdl("product_kernel", product_kernel<T>, dim3(2 * pairs), dim3(kThreads), Shape<T>::kSmemBytes, stream,

@@ -9,6 +9,7 @@ backward pass and the gradient entering its products round once more each."""
 from __future__ import annotations
 
 import math
+from pathlib import Path
 
 import pytest
 import torch
@@ -273,3 +274,25 @@ def test_results_whose_rows_start_off_a_sector(outer, dtype):
     for offset in (1, 4, 8):
         wide[:, offset:offset + outer] = data["residual"]
         check({**data, "residual": wide[:, offset:offset + outer]}, "relu")
+
+
+def test_every_kernel_with_large_shared_memory_is_set_up_on_each_device():
+    """The permission for more than 48 KB of dynamic shared memory belongs to a device: a host function that asks for it
+    keeps its record of having asked by device."""
+
+    for path in sorted((Path(dense.__file__).parent / "csrc").glob("*.cu")):
+        lines = path.read_text().splitlines()
+        for at, line in enumerate(lines):
+            if "cudaFuncSetAttribute(" in line:
+                assert any("[device & 63]" in before for before in lines[at - 4:at]), f"{path.name}:{at + 1}"
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_a_second_device_of_the_process(dtype):
+    data = case(300, 64, 96, TYPES[dtype])
+    want = dense.linear(data["x"], data["weight"], data["bias"], data["residual"], activation="gelu")
+    other = {name: value.to("cuda:1") for name, value in data.items()}
+    got = dense.linear(other["x"], other["weight"], other["bias"], other["residual"], activation="gelu")
+    assert torch.equal(got.to("cuda:0"), want)
