@@ -207,9 +207,9 @@ def anchored_objective(logits: torch.Tensor, reference_logits: torch.Tensor | No
 
     from .ppo import _anchored_inputs, _run_anchored
 
-    grad, sums = _run_anchored(*_anchored_inputs(logits, actions, old_log_probs, advantages, weights, clip_ratio, beta,
-                                                 alpha, reference_logits, reference_log_probs, legal))
-    return grad.contiguous(), sums[:-1].clone()
+    grad, _, totals = _run_anchored(*_anchored_inputs(logits, actions, old_log_probs, advantages, weights, clip_ratio,
+                                                      beta, alpha, reference_logits, reference_log_probs, legal))
+    return grad.contiguous(), totals.clone()
 
 
 @anchored_objective.register_fake

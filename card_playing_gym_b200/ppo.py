@@ -272,6 +272,9 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
         if grad_stride != width:
             grad = grad[:, :width]
     sums = torch.empty(len(ANCHORED_KEYS) + 1, device=logits.device)  # the totals, and the objective once more
+    # The objective is a tensor of its own on the sums' last place: a caller may add to it in place, which autograd refuses
+    # for a view made inside its function.
+    objective = sums.new_empty(0).set_(sums.untyped_storage(), len(ANCHORED_KEYS), (), ())
     need = _anchored_workspace_bytes(rows)
     with nat.on_device(logits.device):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
@@ -280,7 +283,7 @@ def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions,
                  nat.ptr(reference_log_probs), nat.ptr(legal), 0 if legal is None else _row_stride(legal),
                  nat.ptr(actions), nat.ptr(old), nat.ptr(advantages), nat.ptr(weights), clip, beta, alpha,
                  nat.ptr(grad), grad_stride, nat.ptr(sums), nat.ptr(workspace), need, nat.stream_handle(logits.device))
-    return grad, sums
+    return grad, objective, sums[:-1]
 
 
 class _AnchoredObjective(torch.autograd.Function):
@@ -289,13 +292,12 @@ class _AnchoredObjective(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, rest):
         ctx.set_materialize_grads(False)  # the totals have no gradient to make zeros for
-        ctx.gradient, sums = _run_anchored(logits, *rest)
+        ctx.gradient, objective, totals = _run_anchored(logits, *rest)
         # A second backward computes the gradient again, from inputs that must not have changed.
         ctx.save_for_backward(logits)
         ctx.rest, ctx.versions = rest, [t._version for t in rest if isinstance(t, torch.Tensor)]
-        totals = sums[:-1]
         ctx.mark_non_differentiable(totals)
-        return sums[-1], totals
+        return objective, totals
 
     @staticmethod
     @nat.backward_once
@@ -307,7 +309,7 @@ class _AnchoredObjective(torch.autograd.Function):
             (logits,) = ctx.saved_tensors
             if ctx.versions != [t._version for t in ctx.rest if isinstance(t, torch.Tensor)]:
                 raise RuntimeError("an input of anchored_objective was modified in place before its second backward")
-            gradient, _ = _run_anchored(logits, *ctx.rest)
+            gradient, _, _ = _run_anchored(logits, *ctx.rest)
         with nat.on_device(gradient.device):
             nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
                      _row_stride(gradient), nat.ptr(grad_objective.contiguous()), nat.stream_handle(gradient.device))
@@ -363,8 +365,8 @@ def anchored_objective(logits: torch.Tensor, actions: torch.Tensor, old_log_prob
                               reference_logits, reference_log_probs, legal)
     if torch.is_grad_enabled() and inputs[0].requires_grad:
         return _AnchoredObjective.apply(inputs[0], inputs[1:])
-    _, sums = _run_anchored(*inputs, want_grad=False)
-    return sums[-1], sums[:-1]
+    _, objective, totals = _run_anchored(*inputs, want_grad=False)
+    return objective, totals
 
 
 def action_log_probs(logits: torch.Tensor, actions: torch.Tensor, *, legal: torch.Tensor | None = None) -> torch.Tensor:

@@ -432,3 +432,27 @@ def test_the_edges_of_a_rows_registers_at_any_alignment(width, dtype, legal):
         data["legal"] = _moved(data["legal"], 1, 0)
     check(data)
     assert nat.fault_status() == 0
+
+
+@pytest.mark.gpu
+def test_the_objective_may_be_added_to_in_place():
+    """As other losses are: autograd takes it as a tensor of its own, and the totals keep their values."""
+
+    data = inputs(16, 300, torch.float32)
+    _, want_totals, once = run(data)
+    logits = data["logits"].detach().requires_grad_()
+    other = torch.ones(3, device="cuda", requires_grad=True)
+    objective, totals = ppo.anchored_objective(logits, data["actions"], data["old"], data["advantages"], data["weights"],
+                                               clip_ratio=CLIP, beta=BETA, alpha=ALPHA,
+                                               reference_logits=data["reference_logits"])
+    objective += 5.0 * other.sum()
+    objective /= 4.0
+    objective.backward()
+    assert torch.equal(logits.grad, 0.25 * once) and torch.equal(other.grad, torch.full_like(other, 1.25))
+    assert torch.equal(totals, want_totals)
+    with torch.no_grad():
+        value, totals = ppo.anchored_objective(logits, data["actions"], data["old"], data["advantages"], data["weights"],
+                                               clip_ratio=CLIP, beta=BETA, alpha=ALPHA,
+                                               reference_logits=data["reference_logits"])
+        value += 1.0
+    assert torch.equal(totals, want_totals)
