@@ -783,8 +783,9 @@ __global__ void __launch_bounds__(kThreads, (kThreads >= 512 ? 1024 : 768) / kTh
       } else {
         RowGrad g = finish_row(a, in, s, z_a, live, acc);
         if (kExact) g.constant -= g.beta * (s.peak - s.reference_peak);  // the entries' own differences are z - r here
-        // Large coefficients could take a finite difference past the largest float: then a probability of zero is tested.
-        if (lane == 0) row_out[turn] = {g, s.peak, live, part.tested != 0.f || g.alpha > 0.5f || g.beta > 0.5f};
+        // Large coefficients, of either sign, could take a finite difference past the largest float: then a probability of
+        // zero is tested.
+        if (lane == 0) row_out[turn] = {g, s.peak, live, part.tested != 0.f || fabsf(g.alpha) > 0.5f || fabsf(g.beta) > 0.5f};
       }
     }
     if (!a.grad) continue;

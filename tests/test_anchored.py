@@ -456,3 +456,19 @@ def test_the_objective_may_be_added_to_in_place():
                                                reference_logits=data["reference_logits"])
         value += 1.0
     assert torch.equal(totals, want_totals)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weight,beta,alpha", [(4.0, 1.0, 0.0), (-4.0, 1.0, 0.0), (1.0, -4.0, 0.0), (1.0, 0.1, 40.0),
+                                               (1.0, 0.1, -40.0), (-3.0, 0.3, 2.0)])
+@pytest.mark.parametrize("width", [52, 2000, 30000])
+def test_the_lowest_logit_has_no_gradient_under_large_coefficients_of_either_sign(width, weight, beta, alpha):
+    """A probability of zero times a coefficient times the lowest logit's distance, which passes the largest float."""
+
+    data = inputs(8, width, torch.float32, legal=True)
+    hide = ~data["legal"]
+    data["weights"][:] = weight
+    filled = dict(data, legal=None, logits=data["logits"].masked_fill(hide, torch.finfo(torch.float32).min),
+                  reference_logits=data["reference_logits"].masked_fill(hide, -1e5))
+    objective, totals, gradient = run(filled, beta=beta, alpha=alpha)
+    assert torch.isfinite(gradient).all() and not gradient[hide].any()
