@@ -293,9 +293,10 @@ class _AnchoredObjective(torch.autograd.Function):
     def forward(ctx, logits, rest):
         ctx.set_materialize_grads(False)  # the totals have no gradient to make zeros for
         ctx.gradient, objective, totals = _run_anchored(logits, *rest)
-        # A second backward computes the gradient again, from inputs that must not have changed.
-        ctx.save_for_backward(logits)
-        ctx.rest, ctx.versions = rest, [t._version for t in rest if isinstance(t, torch.Tensor)]
+        # A second backward computes the gradient again. Autograd holds the inputs for it (released with the graph, seen by
+        # saved-tensor hooks, refused if one has changed in place by then).
+        ctx.save_for_backward(logits, *rest[:-3])
+        ctx.scalars = rest[-3:]
         ctx.mark_non_differentiable(totals)
         return objective, totals
 
@@ -306,10 +307,7 @@ class _AnchoredObjective(torch.autograd.Function):
             return None, None
         gradient, ctx.gradient = ctx.gradient, None
         if gradient is None:
-            (logits,) = ctx.saved_tensors
-            if ctx.versions != [t._version for t in ctx.rest if isinstance(t, torch.Tensor)]:
-                raise RuntimeError("an input of anchored_objective was modified in place before its second backward")
-            gradient, _, _ = _run_anchored(logits, *ctx.rest)
+            gradient, _, _ = _run_anchored(*ctx.saved_tensors, *ctx.scalars)
         with nat.on_device(gradient.device):
             nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
                      _row_stride(gradient), nat.ptr(grad_objective.contiguous()), nat.stream_handle(gradient.device))

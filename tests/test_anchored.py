@@ -472,3 +472,33 @@ def test_the_lowest_logit_has_no_gradient_under_large_coefficients_of_either_sig
                   reference_logits=data["reference_logits"].masked_fill(hide, -1e5))
     objective, totals, gradient = run(filled, beta=beta, alpha=alpha)
     assert torch.isfinite(gradient).all() and not gradient[hide].any()
+
+
+@pytest.mark.gpu
+def test_the_inputs_are_released_with_the_graph():
+    """What the backward pass may need is held by autograd: hooks see it, and the first backward lets go of it."""
+
+    data = inputs(64, 5000, torch.float32, legal=True)
+    logits = data["logits"].detach().requires_grad_()
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.shape) or t, lambda t: t):
+        objective, _ = ppo.anchored_objective(logits, data["actions"], data["old"], data["advantages"], data["weights"],
+                                              clip_ratio=CLIP, beta=BETA, alpha=ALPHA,
+                                              reference_logits=data["reference_logits"], legal=data["legal"])
+    assert seen.count(torch.Size([64, 5000])) == 3  # logits, reference, mask
+    objective.backward()
+    held = torch.cuda.memory_allocated()
+    del data["reference_logits"], data["legal"]
+    assert torch.cuda.memory_allocated() <= held - 64 * 5000 * 5 and objective.grad_fn is not None
+
+
+@pytest.mark.gpu
+def test_a_second_backward_refuses_inputs_that_have_changed():
+    data = inputs(8, 300, torch.float32)
+    logits = data["logits"].detach().requires_grad_()
+    objective, _ = ppo.anchored_objective(logits, data["actions"], data["old"], data["advantages"], data["weights"],
+                                          clip_ratio=CLIP, beta=BETA, reference_logits=data["reference_logits"])
+    objective.backward(retain_graph=True)
+    data["advantages"].add_(1.0)
+    with pytest.raises(RuntimeError, match="modified"):
+        objective.backward()
