@@ -153,6 +153,8 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
     "cg_anchored_objective_workspace_bytes": (_i64, [_i64]),
     "cg_anchored_objective": (_i32, [_p, _i32, _i64, _i32, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p, _f32, _f32,
                                      _f32, _p, _i64, _p, _p, _i64, _p]),
+    "cg_anchored_gradient": (_i32, [_p, _i32, _i64, _i32, _i64, _p, _i64, _p, _p, _i64, _p, _p, _p, _p, _f32, _f32,
+                                    _f32, _p, _i32, _p, _i64, _p]),
     "cg_anchored_scale": (_i32, [_p, _i32, _i64, _i32, _i64, _p, _p]),
     "cg_action_log_probs": (_i32, [_p, _i32, _i64, _i32, _i64, _p, _i64, _p, _p, _p]),
     "cg_linear_workspace_bytes": (_i64, [_p, _i64, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _i32, _i32]),

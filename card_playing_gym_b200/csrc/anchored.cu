@@ -37,10 +37,15 @@ struct Args {
   const float* weights;
   void* grad;                      // or null: the totals alone
   float* log_probs;                // or null: the actions' log-probabilities and nothing else
-  double* partial;
+  double* partial;                 // or null: no totals
   int64_t rows, stride, reference_stride, legal_stride, grad_stride;
   int width;
   float clip, beta, alpha;
+  const float* scale;              // of the gradient, or null for 1
+  bool given;                      // grad holds the gradient for a scale of 1 already
+
+  // Nothing to do: the gradient of the usual scale is there. (Every thread reads the same word.)
+  __device__ __forceinline__ bool done() const { return given && *scale == 1.f; }
 };
 
 // A row's sums over its legal entries, relative to a base near the largest logit (every formula is the same for any
@@ -83,6 +88,7 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, const RowIn& in, co
   RowGrad g = {0.f, 0.f, 0.f, 0.f, 0.f};
   if (!counts) return g;
   const float w = in.weight, advantage = in.advantage;
+  const float grad_w = a.scale ? w * *a.scale : w;  // scaled before the gradient is rounded to its type
   const float log_sum = logf(s.sum);
   const float lp = (z_a - s.peak) - log_sum;
   const float log_ratio = lp - in.old_log_prob;
@@ -100,14 +106,14 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, const RowIn& in, co
   if (a.reference) {
     log_apart = log_sum - logf(s.reference_sum);
     kl = s.apart * g.inv_sum - log_apart;
-    g.beta = w * a.beta;
+    g.beta = grad_w * a.beta;
   } else if (a.reference_action) {
     const float u = in.reference_log_prob - lp, grown = expf(u);
     kl = grown - u - 1.f;
     slope += a.beta * (1.f - grown);
   }
-  g.alpha = w * a.alpha * norm;
-  g.action = w * slope;
+  g.alpha = grad_w * a.alpha * norm;
+  g.action = grad_w * slope;
   g.constant = -g.action + g.alpha * (entropy - log_sum) - g.beta * (kl + log_apart);
   const float objective = surrogate + a.beta * kl - a.alpha * norm * entropy;
   acc[0] += w * surrogate;
@@ -123,7 +129,7 @@ __device__ __forceinline__ RowGrad finish_row(const Args& a, const RowIn& in, co
 }
 
 // Whether a row counts: it has an action inside the vocabulary and something legal, and for the objective its
-// weight is not zero and its action is legal. Bad actions set the fault word.
+// weight is not zero and its action is legal. Bad actions set the fault word (once: not again for the gradient alone).
 __device__ __forceinline__ bool row_counts(const Args& a, const RowIn& in, const RowSums& s, bool action_legal, bool report) {
   if (in.action < 0) return false;
   if (in.action >= a.width) {
@@ -317,6 +323,7 @@ template <typename T, bool kExact, int kLanes, int kPer>
 __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
   constexpr int kVec = kVector<T>, kVectors = kPer / kVec, kGroups = 32 / kLanes;
   __shared__ double scratch[8][kTotals];
+  if (a.done()) return;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int group = lane / kLanes, l = lane % kLanes;
   auto whole = [&](const void* base, int64_t stride, int size) {
@@ -456,7 +463,7 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
       s.reference_sum = total(fr.x + fr.y);
       s.apart = total(fa.x + fa.y);
     }
-    const bool counts = row_counts(a, in, s, action_legal, l == 0);
+    const bool counts = row_counts(a, in, s, action_legal, l == 0 && !a.scale);
     if (a.log_probs) {
       if (live && l == 0) a.log_probs[row] = counts ? (z_a - s.peak) - logf(s.sum) : 0.f;
       continue;
@@ -502,7 +509,7 @@ __global__ void __launch_bounds__(256, 2) anchored_narrow_kernel(const Args a) {
       put(out + in.action, gradient(xx, ee, dd).x + g.action);
     }
   }
-  if (a.log_probs) return;
+  if (!a.partial) return;
   // The groups' leaders in order, then the warps.
 #pragma unroll
   for (int k = 0; k < kTotals; ++k) {
@@ -722,6 +729,7 @@ __global__ void __launch_bounds__(kThreads, (kThreads >= 512 ? 1024 : 768) / kTh
   constexpr int kUnits = kThreads >= 512 ? 2 : 4, kWarps = kThreads / 32, kVec = kVector<T>;
   __shared__ Part warp_parts[2][kWarps];
   __shared__ RowOut row_out[2];
+  if (a.done()) return;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   float acc[kTotals] = {};
   int turn = 0;  // rows done: what the warps exchange alternates, so that two barriers a row are enough
@@ -777,7 +785,7 @@ __global__ void __launch_bounds__(kThreads, (kThreads >= 512 ? 1024 : 768) / kTh
       join_lanes<kExact>(part, kWarps, masked);
       const RowSums s = {part.peak, part.sum, part.spread, part.apart, kExact ? part.reference_peak : 0.f, part.reference_sum,
                          masked ? part.count : static_cast<float>(a.width)};
-      const bool live = row_counts(a, in, s, action_legal, lane == 0);
+      const bool live = row_counts(a, in, s, action_legal, lane == 0 && !a.scale);
       if (a.log_probs) {
         if (lane == 0) a.log_probs[index] = live ? (z_a - s.peak) - logf(s.sum) : 0.f;
       } else {
@@ -831,7 +839,7 @@ __global__ void __launch_bounds__(kThreads, (kThreads >= 512 ? 1024 : 768) / kTh
       put(out + j, v);
     }
   }
-  if (!a.log_probs && tid == 0)
+  if (a.partial && tid == 0)
     for (int k = 0; k < kTotals; ++k) a.partial[blockIdx.x * kTotals + k] = acc[k];
 }
 
@@ -942,6 +950,26 @@ int run_rows(const Args& a, int dtype, int* blocks, cudaStream_t s) {
 }  // namespace
 }  // namespace cg
 
+namespace cg {
+namespace {
+
+// The checks that the objective and its gradient share.
+int check_rows(const char* name, const Args& a, int dtype) {
+  CG_REQUIRE(valid_dtype(dtype), "%s: dtype must be float32, float16 or bfloat16", name);
+  CG_REQUIRE(a.rows >= 0 && a.width > 0, "%s: bad shape", name);
+  CG_REQUIRE(a.stride >= a.width && (!a.grad || a.grad_stride >= a.width) &&
+                 (!a.reference || a.reference_stride >= a.width) && (!a.legal || a.legal_stride >= a.width),
+             "%s: stride < width", name);
+  CG_REQUIRE(!(a.reference && a.reference_action), "%s: one reference at most", name);
+  CG_REQUIRE(a.clip >= 0, "%s: clip_ratio must not be negative", name);
+  CG_REQUIRE(a.rows == 0 || (a.logits && a.actions && a.old_log_probs && a.advantages && a.weights), "%s: NULL pointer",
+             name);
+  return CG_OK;
+}
+
+}  // namespace
+}  // namespace cg
+
 extern "C" int64_t cg_anchored_objective_workspace_bytes(int64_t rows) {
   return std::min<int64_t>(std::max<int64_t>(rows, 1), cg::kPartials) * cg::kTotals * static_cast<int64_t>(sizeof(double));
 }
@@ -954,29 +982,38 @@ extern "C" int cg_anchored_objective(const void* logits, int dtype, int64_t rows
                                      int64_t grad_stride, float* totals, void* workspace, int64_t workspace_bytes,
                                      void* stream) {
   using namespace cg;
-  CG_REQUIRE(valid_dtype(dtype), "cg_anchored_objective: dtype must be float32, float16 or bfloat16");
-  CG_REQUIRE(rows >= 0 && width > 0, "cg_anchored_objective: bad shape");
-  CG_REQUIRE(stride >= width && (!grad || grad_stride >= width) && (!reference_logits || reference_stride >= width) &&
-                 (!legal || legal_stride >= width),
-             "cg_anchored_objective: stride < width");
-  CG_REQUIRE(!(reference_logits && reference_log_probs), "cg_anchored_objective: one reference at most");
-  CG_REQUIRE(clip_ratio >= 0, "cg_anchored_objective: clip_ratio must not be negative");
+  auto* partial = static_cast<double*>(workspace);
+  const Args a = {logits, reference_logits, reference_log_probs, legal, actions, old_log_probs, advantages, weights,
+                  grad, nullptr, partial, rows, stride, reference_stride, legal_stride, grad_stride, width,
+                  clip_ratio, beta, alpha, nullptr, false};
+  if (int rc = check_rows("cg_anchored_objective", a, dtype)) return rc;
   CG_REQUIRE(totals, "cg_anchored_objective: NULL totals");
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   int blocks = 0;
-  auto* partial = static_cast<double*>(workspace);
   if (rows > 0) {
-    CG_REQUIRE(logits && actions && old_log_probs && advantages && weights,
-               "cg_anchored_objective: NULL pointer");
     if (!workspace || workspace_bytes < cg_anchored_objective_workspace_bytes(rows))
       return set_error(CG_ERR_WORKSPACE, "cg_anchored_objective: workspace too small");
-    const Args a = {logits, reference_logits, reference_log_probs, legal, actions, old_log_probs, advantages, weights,
-                    grad, nullptr, partial, rows, stride, reference_stride, legal_stride, grad_stride, width,
-                    clip_ratio, beta, alpha};
     if (int rc = run_rows(a, dtype, &blocks, s)) return rc;
   }
   return launch_pdl("anchored_totals_kernel", anchored_totals_kernel, dim3(1), dim3(1024), 0, s,
                     static_cast<const double*>(partial), blocks, totals);
+}
+
+extern "C" int cg_anchored_gradient(const void* logits, int dtype, int64_t rows, int width, int64_t stride,
+                                    const void* reference_logits, int64_t reference_stride,
+                                    const float* reference_log_probs, const uint8_t* legal, int64_t legal_stride,
+                                    const int64_t* actions, const float* old_log_probs, const float* advantages,
+                                    const float* weights, float clip_ratio, float beta, float alpha, const float* scale,
+                                    int given, void* grad, int64_t grad_stride, void* stream) {
+  using namespace cg;
+  const Args a = {logits, reference_logits, reference_log_probs, legal, actions, old_log_probs, advantages, weights,
+                  grad, nullptr, nullptr, rows, stride, reference_stride, legal_stride, grad_stride, width,
+                  clip_ratio, beta, alpha, scale, given != 0};
+  if (int rc = check_rows("cg_anchored_gradient", a, dtype)) return rc;
+  if (rows == 0) return CG_OK;
+  CG_REQUIRE(grad && scale, "cg_anchored_gradient: NULL pointer");
+  int blocks = 0;
+  return run_rows(a, dtype, &blocks, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int cg_anchored_scale(void* grad, int dtype, int64_t rows, int width, int64_t stride, const float* scale,

@@ -260,29 +260,39 @@ def _logits_and_mask(logits: torch.Tensor, actions: torch.Tensor, legal: torch.T
     return _unit_rows(logits), _rows_of("actions", actions, logits.shape[0], logits.device, torch.int64), legal
 
 
-def _run_anchored(logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights, clip, beta,
-                  alpha, want_grad: bool = True):
+def _row_arguments(logits, reference_logits, reference_log_probs, legal, actions, old, advantages, weights, clip, beta,
+                   alpha) -> tuple:
+    """What ``cg_anchored_objective`` and ``cg_anchored_gradient`` begin with."""
+
+    return (nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], *logits.shape, _row_stride(logits), nat.ptr(reference_logits),
+            0 if reference_logits is None else _row_stride(reference_logits), nat.ptr(reference_log_probs),
+            nat.ptr(legal), 0 if legal is None else _row_stride(legal), nat.ptr(actions), nat.ptr(old),
+            nat.ptr(advantages), nat.ptr(weights), clip, beta, alpha)
+
+
+def _gradient_like(logits: torch.Tensor) -> torch.Tensor:
+    """Room for the gradient, in the logits' row stride where that only pads the row, so that both rows align alike."""
+
     rows, width = logits.shape
-    # The gradient takes the logits' row stride where that only pads the row, so that both rows align alike.
     stride = _row_stride(logits)
-    grad_stride = stride if stride <= width + 64 else width
-    grad = None
-    if want_grad:
-        grad = torch.empty((rows, grad_stride), dtype=logits.dtype, device=logits.device)
-        if grad_stride != width:
-            grad = grad[:, :width]
+    if stride > width + 64:
+        stride = width
+    grad = torch.empty((rows, stride), dtype=logits.dtype, device=logits.device)
+    return grad if stride == width else grad[:, :width]
+
+
+def _run_anchored(logits, *rest, want_grad: bool = True):
+    grad = _gradient_like(logits) if want_grad else None
     sums = torch.empty(len(ANCHORED_KEYS) + 1, device=logits.device)  # the totals, and the objective once more
     # The objective is a tensor of its own on the sums' last place: a caller may add to it in place, which autograd refuses
     # for a view made inside its function.
     objective = sums.new_empty(0).set_(sums.untyped_storage(), len(ANCHORED_KEYS), (), ())
-    need = _anchored_workspace_bytes(rows)
+    need = _anchored_workspace_bytes(logits.shape[0])
     with nat.on_device(logits.device):
         workspace = torch.empty(need, dtype=torch.uint8, device=logits.device)
-        nat.call("cg_anchored_objective", nat.ptr(logits), nat.DTYPE_CODES[logits.dtype], rows, width, stride,
-                 nat.ptr(reference_logits), 0 if reference_logits is None else _row_stride(reference_logits),
-                 nat.ptr(reference_log_probs), nat.ptr(legal), 0 if legal is None else _row_stride(legal),
-                 nat.ptr(actions), nat.ptr(old), nat.ptr(advantages), nat.ptr(weights), clip, beta, alpha,
-                 nat.ptr(grad), grad_stride, nat.ptr(sums), nat.ptr(workspace), need, nat.stream_handle(logits.device))
+        nat.call("cg_anchored_objective", *_row_arguments(logits, *rest), nat.ptr(grad),
+                 0 if grad is None else _row_stride(grad), nat.ptr(sums), nat.ptr(workspace), need,
+                 nat.stream_handle(logits.device))
     return grad, objective, sums[:-1]
 
 
@@ -293,8 +303,8 @@ class _AnchoredObjective(torch.autograd.Function):
     def forward(ctx, logits, rest):
         ctx.set_materialize_grads(False)  # the totals have no gradient to make zeros for
         ctx.gradient, objective, totals = _run_anchored(logits, *rest)
-        # A second backward computes the gradient again. Autograd holds the inputs for it (released with the graph, seen by
-        # saved-tensor hooks, refused if one has changed in place by then).
+        # Autograd holds the inputs for the backward pass (released with the graph, seen by saved-tensor hooks, refused if
+        # one has changed in place by then).
         ctx.save_for_backward(logits, *rest[:-3])
         ctx.scalars = rest[-3:]
         ctx.mark_non_differentiable(totals)
@@ -303,14 +313,26 @@ class _AnchoredObjective(torch.autograd.Function):
     @staticmethod
     @nat.backward_once
     def backward(ctx, grad_objective, _grad_totals):
+        """The gradient made with the objective, times ``grad_objective``, which only the device knows.
+
+        Where it is not 1, a float32 gradient is multiplied in place. A 16-bit one was rounded for a factor of 1 (a loss
+        scale could not bring back what became zero), so its kernel runs again, as it does in a second backward."""
+
         if grad_objective is None:
             return None, None
         gradient, ctx.gradient = ctx.gradient, None
-        if gradient is None:
-            gradient, _, _ = _run_anchored(*ctx.saved_tensors, *ctx.scalars)
+        scale = grad_objective.contiguous()
+        if gradient is not None and gradient.dtype is torch.float32:
+            with nat.on_device(gradient.device):
+                nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
+                         _row_stride(gradient), nat.ptr(scale), nat.stream_handle(gradient.device))
+            return gradient, None
+        inputs, given = ctx.saved_tensors, gradient is not None
+        if not given:
+            gradient = _gradient_like(inputs[0])
         with nat.on_device(gradient.device):
-            nat.call("cg_anchored_scale", nat.ptr(gradient), nat.DTYPE_CODES[gradient.dtype], *gradient.shape,
-                     _row_stride(gradient), nat.ptr(grad_objective.contiguous()), nat.stream_handle(gradient.device))
+            nat.call("cg_anchored_gradient", *_row_arguments(*inputs, *ctx.scalars), nat.ptr(scale), given,
+                     nat.ptr(gradient), _row_stride(gradient), nat.stream_handle(gradient.device))
         return gradient, None
 
 

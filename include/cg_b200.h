@@ -396,7 +396,16 @@ int cg_anchored_objective(const void* logits, int dtype, int64_t rows, int width
                           const float* old_log_probs, const float* advantages, const float* weights, float clip_ratio,
                           float beta, float alpha, void* grad, int64_t grad_stride, float* totals, void* workspace,
                           int64_t workspace_bytes, void* stream);
-/* grad *= *scale in place (scale on the device): the chain rule for the gradient above; returns at once
+/* The gradient alone times *scale (on the device), scaled in fp32 before it is rounded to its type: the chain
+ * rule for 16-bit gradients, whose small entries a factor after the rounding could not bring back. given != 0:
+ * grad holds the gradient for a scale of 1 already, and the kernel returns at once where *scale is 1. */
+int cg_anchored_gradient(const void* logits, int dtype, int64_t rows, int width, int64_t stride,
+                         const void* reference_logits, int64_t reference_stride, const float* reference_log_probs,
+                         const uint8_t* legal, int64_t legal_stride, const int64_t* actions,
+                         const float* old_log_probs, const float* advantages, const float* weights, float clip_ratio,
+                         float beta, float alpha, const float* scale, int given, void* grad, int64_t grad_stride,
+                         void* stream);
+/* grad *= *scale in place (scale on the device): the chain rule for fp32 gradients; returns at once
  * where *scale is 1. */
 int cg_anchored_scale(void* grad, int dtype, int64_t rows, int width, int64_t stride, const float* scale, void* stream);
 /* lp[action] alone, fp32 [rows] (the behaviour's or the reference's log-probabilities for the

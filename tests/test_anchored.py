@@ -502,3 +502,58 @@ def test_a_second_backward_refuses_inputs_that_have_changed():
     data["advantages"].add_(1.0)
     with pytest.raises(RuntimeError, match="modified"):
         objective.backward()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("factor_of_loss", [65536.0, 3.0, 0.37])
+@pytest.mark.parametrize("legal", [False, True])
+@pytest.mark.parametrize("reference", ["logits", "log-probs"])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("width", [52, 700, 3000, 20000])
+def test_a_loss_scale_comes_before_the_gradients_rounding(width, dtype, reference, legal, factor_of_loss):
+    """With weights of a mean over many rows a 16-bit gradient is small: (factor * objective).backward() is the scaled
+    objective's gradient rounded once, not the factor times a gradient that was rounded, to zero in part, before it."""
+
+    data = inputs(24, width, TYPES[dtype], reference=reference, legal=legal)
+    data["weights"] = data["weights"] / 2.0 ** 18
+    _, _, want, scale, _ = formula(data)
+    logits = data["logits"].detach().requires_grad_()
+    extra = {k: data[k] for k in ("reference_logits", "reference_log_probs") if k in data}
+    objective, totals = ppo.anchored_objective(logits, data["actions"], data["old"], data["advantages"], data["weights"],
+                                               clip_ratio=CLIP, beta=BETA, alpha=ALPHA, legal=data["legal"], **extra)
+    before = totals.clone()
+    (got,) = torch.autograd.grad(factor_of_loss * objective, logits, retain_graph=True)
+    k = factor(width)
+    for by, gradient in ((factor_of_loss, got), (0.5, torch.autograd.grad(0.5 * objective, logits)[0])):
+        bound = by * (k * scale[:, None] + (1 + 2 * k) * HALF_STEP[TYPES[dtype]] * want.abs())
+        if TYPES[dtype] == torch.float16:
+            bound = bound + 2.0 ** -25
+        assert gradient.dtype == TYPES[dtype]
+        assert ((gradient.double() - by * want).abs() <= bound).all()
+    assert torch.equal(totals, before) and nat.fault_status() == 0
+
+
+@pytest.mark.gpu
+def test_a_gradient_scaler_trains_half_precision_logits():
+    """GradScaler's scale reaches the gradient before its rounding, and its unscaled gradient is the formula's."""
+
+    data = inputs(64, 52, torch.float16, legal=True)
+    data["weights"] = data["weights"] / 2.0 ** 20
+    _, _, want, scale, _ = formula(data)
+    logits = data["logits"].detach().requires_grad_()
+    objective, _ = ppo.anchored_objective(logits, data["actions"], data["old"], data["advantages"], data["weights"],
+                                          clip_ratio=CLIP, beta=BETA, alpha=ALPHA, legal=data["legal"],
+                                          reference_logits=data["reference_logits"])
+    scaler = torch.amp.GradScaler("cuda", init_scale=2.0 ** 20)
+    scaler.scale(objective).backward()
+    k = factor(52)
+    bound = 2.0 ** 20 * (k * scale[:, None] + (1 + 2 * k) * 2.0 ** -11 * want.abs()) + 2.0 ** -25
+    assert ((logits.grad.double() - 2.0 ** 20 * want).abs() <= bound).all()
+
+
+def test_the_library_refuses_a_gradient_without_its_scale():
+    fill = [None, 0, 0, 4, 4, None, 0, None, None, 0, None, None, None, None, 0.2, 0.0, 0.0]
+    with pytest.raises(nat.NativeError, match="NULL pointer"):
+        nat.call("cg_anchored_gradient", None, 0, 1, *fill[3:], None, 0, None, 4, None)
+    with pytest.raises(nat.NativeError, match="dtype"):
+        nat.call("cg_anchored_gradient", None, 9, *fill[2:], None, 0, None, 4, None)
