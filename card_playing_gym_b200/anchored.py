@@ -61,16 +61,26 @@ class Decisions:
 
 
 class AnchoredUpdate:
-    """One update of ``head`` per call, anchored to a frozen copy of it taken here (or to ``reference``)."""
+    """One update of ``head`` per call, anchored to a frozen copy of it taken here (or to ``reference``).
+
+    ``loss_scale`` multiplies the objective for the backward pass, None: 1024 for a float16 head (whose gradients of a mean
+    over many rows would fall below float16's least step) and 1 for the others. AdamW's step is the same for scaled
+    gradients with ``eps`` and ``max_norm`` scaled alike, so nothing is scaled back: the optimizer's moments and
+    ``grad_norm`` are those of the scaled objective.
+    """
 
     def __init__(self, head: PolicyHead, *, reference: PolicyHead | None = None, lr: float = 1e-3,
                  weight_decay: float = 0.0, state_bits: int = 32, max_norm: float = 1.0, clip_ratio: float = 0.2,
-                 beta: float = 0.05, alpha: float = 0.01) -> None:
+                 beta: float = 0.05, alpha: float = 0.01, loss_scale: float | None = None) -> None:
         self.head = head
         self.reference = copy.deepcopy(head) if reference is None else reference
         self.reference.requires_grad_(False)
-        self.optimizer = AdamW(head.parameters(), lr=lr, weight_decay=weight_decay, state_bits=state_bits,
-                               max_norm=max_norm)
+        if loss_scale is None:
+            loss_scale = 1024.0 if head.up.dtype is torch.float16 else 1.0
+        self.loss_scale = loss_scale
+        self._scale = torch.full((), loss_scale, device=head.up.device)
+        self.optimizer = AdamW(head.parameters(), lr=lr, eps=1e-8 * loss_scale, weight_decay=weight_decay,
+                               state_bits=state_bits, max_norm=max_norm * loss_scale)
         self.clip_ratio, self.beta, self.alpha = clip_ratio, beta, alpha
 
     def __call__(self, batch: Decisions) -> torch.Tensor:
@@ -82,7 +92,7 @@ class AnchoredUpdate:
         objective, totals = ppo.anchored_objective(
             self.head(batch.hidden), batch.actions, batch.old_log_probs, batch.advantages, batch.weights,
             clip_ratio=self.clip_ratio, beta=self.beta, alpha=self.alpha, reference_logits=reference, legal=batch.legal)
-        objective.backward()
+        objective.backward(self._scale)
         self.optimizer.step()
         return totals
 

@@ -91,3 +91,39 @@ def test_updates_lower_the_objective(dtype, bits):
 def test_the_command_runs(capsys):
     assert anchored.main(["--rows", "256", "--steps", "2", "--state-bits", "8"]) == 0
     assert capsys.readouterr().out.count("objective") == 2
+
+
+@pytest.mark.gpu
+def test_half_precision_gradients_of_a_mean_over_many_rows_keep_their_small_entries():
+    """A power of two on the weights only moves float16 exponents, so the first moment of an update with weights of 2^-18 is
+    2^-12 of that with weights of 2^-6, but for the entries that either loses below float16's least step: together less
+    than a rounding of the whole, 2^-11 of its size. (Unscaled, three quarters of the logits' gradient are zero.)"""
+
+    moments = []
+    for weight in (2.0 ** -18, 2.0 ** -6):
+        head = anchored.PolicyHead(dtype=torch.float16, generator=torch.Generator(device="cuda").manual_seed(0))
+        batch = anchored.synthetic_decisions(head, 4096)
+        batch.weights = torch.full_like(batch.weights, weight)
+        reference = anchored.PolicyHead(dtype=torch.float16, generator=torch.Generator(device="cuda").manual_seed(3))
+        update = anchored.AnchoredUpdate(head, reference=reference, max_norm=1e6)
+        update(batch)
+        assert int(update.optimizer.steps) == 1
+        moments.append(update.optimizer.flat["exp_avg"].double() / (weight * update.loss_scale))
+    assert (moments[0] - moments[1]).norm() <= 2.0 ** -11 * moments[1].norm()
+
+
+@pytest.mark.gpu
+def test_a_loss_scale_leaves_the_update_as_it_is():
+    """In float32 a power of two on the objective changes exponents alone: eps and the clip move with it, all but the
+    1e-6 beside the norm (2^-20 of the clip's factor at a norm of 1)."""
+
+    heads = []
+    for scale in (1.0, 256.0):
+        head = anchored.PolicyHead(generator=torch.Generator(device="cuda").manual_seed(0))
+        batch = anchored.synthetic_decisions(head, 500)
+        update = anchored.AnchoredUpdate(head, lr=1e-2, max_norm=1e-3, loss_scale=scale)
+        for _ in range(2):
+            update(batch)
+        heads.append(head)
+    for p, q in zip(*(h.parameters() for h in heads)):
+        assert (p - q).abs().max() <= 1e-2 * 1e-2
