@@ -16,8 +16,9 @@
 // three times its traffic. The tensor cores cut their running sum at each step (measured: 1.7e-8 of it, always
 // toward zero), which a long float32 sum would show: the five small products have an accumulator of their own,
 // and after kChunkBlocks blocks of k the epilogue takes both sums into registers, where they are added with
-// rounding, and the next chunk starts from zero in the other pair of accumulators. tile_n is 128 for it, so that two
-// pairs fit tensor memory. 16-bit results keep one running sum: at 8192 k's the cut is 9e-6 against their own
+// rounding, and the next chunk starts from zero in the other pair of accumulators. An infinity or NaN is its own first
+// part, so the product of first parts is the float32 one; what it makes of the small products (an infinity times parts of
+// either sign, or of zero) is left out. tile_n is 128 for float32, so that two pairs fit tensor memory. 16-bit results keep one running sum: at 8192 k's the cut is 9e-6 against their own
 // rounding of 2^-11 or 2^-8.
 //
 // Where the last round of tiles leaves half the pairs idle, k is split for the tiles of that round: every split writes
@@ -454,7 +455,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             float v[32];
             read_sum(c, S::kTileN, v);
 #pragma unroll
-            for (int k = 0; k < 32; ++k) sums[c][k] = first == t.first ? v[k] : sums[c][k] + v[k];
+            for (int k = 0; k < 32; ++k) {
+              const float small = fabsf(v[k]) < INFINITY ? v[k] : 0.f;
+              sums[c][k] = first == t.first ? small : sums[c][k] + small;
+            }
             read_sum(c, 0, v);
 #pragma unroll
             for (int k = 0; k < 32; ++k) sums[c][k] += v[k];

@@ -296,3 +296,47 @@ def test_a_second_device_of_the_process(dtype):
     other = {name: value.to("cuda:1") for name, value in data.items()}
     got = dense.linear(other["x"], other["weight"], other["bias"], other["residual"], activation="gelu")
     assert torch.equal(got.to("cuda:0"), want)
+
+
+def same_kind(got, want):
+    """Both NaN, both an infinity of one sign, or both finite."""
+
+    return (torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isposinf(got), torch.isposinf(want))
+            and torch.equal(torch.isneginf(got), torch.isneginf(want)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("activation", list(ACT))
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows,inner,outer", [(20, 64, 96), (32, 300, 100), (33, 64, 96), (140, 64, 96), (140, 700, 131),
+                                              (64, 4000, 72)])
+def test_an_infinity_is_one_whatever_the_row_count(rows, inner, outer, dtype, activation):
+    """One infinity in a row makes every sum of it an infinity of the weight's sign, two of them a NaN where the signs
+    differ, in the formula as in the layer."""
+
+    data = case(rows, inner, outer, TYPES[dtype], residual=False)
+    data["x"][7, 5] = math.inf
+    data["x"][9] = 0.0
+    data["x"][9, 5] = -math.inf
+    data["x"][11, 3], data["x"][11, inner - 1] = math.inf, -math.inf
+    data["weight"][4, 2] = math.inf
+    data["x"][13, 2] = 0.0
+    got = dense.linear(data["x"], data["weight"], data["bias"], activation=activation)
+    want = ACT[activation](data["x"].double() @ data["weight"].double().t() + data["bias"].double())
+    assert torch.isinf(want[7]).sum() >= outer // 4 and torch.isnan(want[13, 4])
+    assert same_kind(got.double(), want)
+    assert nat.fault_status() == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("rows", [20, 140, 3000])
+def test_an_infinity_in_the_backward_pass(rows, dtype):
+    data = case(rows, 72, 100, TYPES[dtype], residual=False)
+    data["dy"][3, 8] = math.inf
+    data["x"][6, 2] = -math.inf
+    leaves = {k: data[k].detach().requires_grad_() for k in ("x", "weight", "bias")}
+    grads = torch.autograd.grad(dense.linear(*leaves.values()), list(leaves.values()), data["dy"])
+    dy = data["dy"].double()
+    for got, want in zip(grads, (dy @ data["weight"].double(), dy.t() @ data["x"].double(), dy.sum(0))):
+        assert torch.isinf(want).any() and same_kind(got.double(), want)
