@@ -194,4 +194,6 @@ class AdamW(torch.optim.Optimizer):
                      nat.ptr(flat.get("exp_avg_sq_root_scale")), nat.ptr(flat.get("master")), nat.ptr(self.steps),
                      float(self.max_norm or 0.0), nat.ptr(self.grad_norm), nat.ptr(self._control),
                      nat.ptr(workspace), 0 if workspace is None else workspace.numel(), nat.stream_handle(device))
+        # The kernel writes through addresses: autograd learns here that a graph's saved weights have changed.
+        torch.autograd.graph.increment_version([p for p, g in zip(params, from_grads) if g] if 0 in from_grads else params)
         return loss

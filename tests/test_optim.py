@@ -13,7 +13,7 @@ import math
 import pytest
 import torch
 
-from card_playing_gym_b200 import optim
+from card_playing_gym_b200 import dense, optim
 
 EPS32 = 2.0 ** -24
 TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
@@ -292,3 +292,22 @@ def test_refusals_without_a_gpu():
         optim.AdamW([p], betas=(0.9, 1.0))
     with pytest.raises(ValueError, match="negative"):
         optim.AdamW([p], lr=-1.0)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_backward_pass_through_stepped_weights_is_refused(bits):
+    """As with torch's optimizers: a graph from before the step has saved the weights, which the step has changed."""
+
+    weight, still = (torch.nn.Parameter(torch.randn(40, 24, device="cuda")) for _ in range(2))
+    x = torch.randn(50, 24, device="cuda", requires_grad=True)
+    opt = optim.AdamW([weight, still], state_bits=bits)
+    loss = dense.linear(x, weight).square().sum()
+    loss.backward(retain_graph=True)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    assert still._version == 0  # no gradient: the step left it as it was
+    loss = dense.linear(x, weight).square().sum()
+    loss.backward()
+    opt.step()
