@@ -187,14 +187,14 @@ __device__ __forceinline__ void encode8(uint8_t* codes, const float (&v)[8]) {
 // Square root and reciprocal within 2 units in the last place: the update they make is the learning rate's fraction of a
 // weight, and exact ones (some 30 instructions an entry) would cost more than the memory they hide behind.
 __device__ __forceinline__ float root_fast(float v) {
-  float r;
-  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  float r;  // of a subnormal v too, which is what a gradient of 1e-18 leaves
+  asm("sqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 
-// Under the update's quotient at least: an entry without history does not divide zero by a zero eps, and its neighbours'
-// reciprocal is finite.
-constexpr float kLeastUnder = 1.2e-38f;
+// Under the update's quotient at least, 2^-75: the root of any v above zero is larger, an entry without history does not
+// divide zero by a zero eps, and one whose v has become zero below float32's range is updated as if it had the least one.
+constexpr float kLeastUnder = 2.6469780e-23f;
 
 // Largest of the warp's non-negative values; a NaN's bits compare above infinity's, so it is kept.
 __device__ __forceinline__ float warp_peak(float v) {

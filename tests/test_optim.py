@@ -311,3 +311,32 @@ def test_a_backward_pass_through_stepped_weights_is_refused(bits):
     loss = dense.linear(x, weight).square().sum()
     loss.backward()
     opt.step()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("size", [1e-18, 3e-19])
+def test_a_second_moment_below_the_normal_range_counts_without_eps(size, bits):
+    """v = 1e-3 g^2 is subnormal here, within 2^-150 of its value (1e-5 of it at least); the first step moves by lr all the same."""
+
+    p = torch.nn.Parameter(torch.zeros(700, device="cuda"))
+    sign = torch.where(torch.arange(700, device="cuda") % 3 == 0, -1.0, 1.0)
+    p.grad = size * sign
+    opt = optim.AdamW([p], lr=1e-2, eps=0.0, weight_decay=0.0, state_bits=bits)
+    opt.step()
+    assert (p.detach() + 1e-2 * sign).abs().max() <= 1e-2 * 1e-4
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [8, 32])
+@pytest.mark.parametrize("size", [1e-20, 1e-22, 1e-24, 1e-30, 1e-38, 0.0])
+def test_without_eps_a_vanishing_gradient_moves_a_weight_by_a_few_learning_rates_at_most(size, bits):
+    """Adam's update is at most about (1 - b1) / sqrt(1 - b2) learning rates, 3.2, before the bias correction by 1 / (1 - b1)
+    of a first step, 32 in all; a v that float32 cannot hold must not make more of it."""
+
+    p = torch.nn.Parameter(torch.zeros(700, device="cuda"))
+    p.grad = torch.full_like(p, size)
+    opt = optim.AdamW([p], lr=1e-2, eps=0.0, weight_decay=0.0, state_bits=bits)
+    for _ in range(3):
+        opt.step()
+        assert torch.isfinite(p).all() and p.detach().abs().max() <= 3 * 33 * 1e-2
