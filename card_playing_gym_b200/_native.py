@@ -161,7 +161,7 @@ _SIGNATURES: dict[str, tuple[type, list]] = {
     "cg_linear_forward": (_i32, [_p, _i64, _p, _i64, _p, _p, _i64, _i32, _i64, _i64, _i64, _i32, _p, _p, _p, _i64, _p]),
     "cg_linear_backward": (_i32, [_p, _i64, _p, _p, _i64, _p, _i64, _i32, _i64, _i64, _i64, _i32, _p, _p, _p, _p, _i64,
                                   _p]),
-    "cg_adamw_control_bytes": (_i64, []),
+    "cg_adamw_control_bytes": (_i64, [_i32]),
     "cg_adamw_workspace_bytes": (_i64, [_i32]),
     "cg_adamw_step": (_i32, [_p, _p, _p, _i32, _i32, _p, _i32, _i32, _p, _p, _p, _p, _p, _p, _f32, _p, _p, _p, _i64, _p]),
 }

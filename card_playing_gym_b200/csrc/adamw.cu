@@ -28,7 +28,7 @@ constexpr int kBlockEntries = 256;  // entries of one scale; every tensor's stat
 constexpr int kPerLane = 8;
 constexpr int kThreads = 256;
 constexpr int kChunk = 16384;  // entries of a thread block: eight 256-entry blocks a warp
-constexpr int kMaxGroups = 16;
+constexpr int kGroupsAtOnce = 16;  // groups of a launch's parameters; more of them take launches of their own
 constexpr int kNormBlocks = 1184;  // partial sums of the norm: one fixed order of addition
 constexpr float kE4m3Max = 448.f;
 constexpr float kE4m3Least = 0.001953125f;  // 2^-9
@@ -38,18 +38,21 @@ struct Factors {
   float decay, step, root, eps, beta1, rest1, beta2, rest2;
 };
 
-// Zeroed before the first step; what the norm kernel leaves for the update.
+// Zeroed before the first step; what the norm kernel leaves for the update. Every group's factors follow it.
 struct Control {
   unsigned ticket;
   int skip;
   float clip;
   int reserved;
-  Factors groups[kMaxGroups];
 };
+__device__ __forceinline__ Factors* factors_of(Control* control) { return reinterpret_cast<Factors*>(control + 1); }
+__device__ __forceinline__ const Factors* factors_of(const Control* control) {
+  return reinterpret_cast<const Factors*>(control + 1);
+}
 
 struct Groups {
-  int count;
-  cg_adamw_group g[kMaxGroups];
+  int first, count;
+  cg_adamw_group g[kGroupsAtOnce];
 };
 
 struct Entry {
@@ -202,15 +205,8 @@ __device__ __forceinline__ float warp_peak(float v) {
 }
 
 // ---- the global norm and the step's factors ----------------------------------------------------------
-// One thread per group, in double: 1 - b2^t loses half its digits in fp32.
-__device__ void make_factors(const Groups& groups, int64_t* steps, bool finite, float clip, Control* control) {
-  const int64_t t = *steps + 1;
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    control->clip = clip;
-    control->skip = finite ? 0 : 1;
-    if (finite) *steps = t;
-  }
+// One thread per group, in double: 1 - b2^t loses half its digits in fp32. t: the step being made.
+__device__ void make_factors(const Groups& groups, int64_t t, Control* control) {
   for (int k = threadIdx.x; k < groups.count; k += blockDim.x) {
     const cg_adamw_group g = groups.g[k];
     Factors f;
@@ -222,14 +218,30 @@ __device__ void make_factors(const Groups& groups, int64_t* steps, bool finite, 
     f.rest1 = static_cast<float>(1.0 - g.beta1);
     f.beta2 = static_cast<float>(g.beta2);
     f.rest2 = static_cast<float>(1.0 - g.beta2);
-    control->groups[k] = f;
+    factors_of(control)[groups.first + k] = f;
   }
 }
 
+// The first groups' factors, the clip and the step's count.
+__device__ void begin_step(const Groups& groups, int64_t* steps, bool finite, float clip, Control* control) {
+  const int64_t t = *steps + 1;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    control->clip = clip;
+    control->skip = finite ? 0 : 1;
+    if (finite) *steps = t;
+  }
+  make_factors(groups, t, control);
+}
+
+// Without a clip, or for the groups past the first ones: the step has been counted by then.
 __global__ void __launch_bounds__(32) adamw_factors_kernel(const __grid_constant__ Groups groups, int64_t* steps,
                                                            Control* control) {
   pdl_trigger();
-  make_factors(groups, steps, true, 1.f, control);
+  if (groups.first == 0)
+    begin_step(groups, steps, true, 1.f, control);
+  else
+    make_factors(groups, *steps, control);
 }
 
 // Squares are summed in fp32 over a thread's eight entries and in double from there on.
@@ -299,7 +311,7 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
   for (int w = 0; w < kThreads / 32; ++w) total += s[w];
   const double norm = sqrt(total);
   if (threadIdx.x == 0) *norm_out = static_cast<float>(norm);
-  make_factors(groups, steps, isfinite(norm), static_cast<float>(fmin(1.0, max_norm / (norm + 1e-6))), control);
+  begin_step(groups, steps, isfinite(norm), static_cast<float>(fmin(1.0, max_norm / (norm + 1e-6))), control);
 }
 
 // ---- the update -----------------------------------------------------------------------------------------
@@ -426,7 +438,7 @@ __global__ void __launch_bounds__(kThreads, 3) adamw_update_kernel(const __grid_
   pdl_wait();
   if (control->skip) return;  // a norm that is not finite: nothing moves
   const float clip = control->clip;
-  const Factors f = control->groups[e.group];
+  const Factors f = factors_of(control)[e.group];
   for (int i = 0; i < blocks; ++i) {
     float scale_m = 0.f, scale_r = 0.f;
     if (kBits == 8) scale_m = __shfl_sync(0xffffffffu, scales_m, i), scale_r = __shfl_sync(0xffffffffu, scales_r, i);
@@ -464,10 +476,19 @@ void fill_table(const Tensors& tensors, int& next, Table<kMax>& table) {
   }
 }
 
+Groups groups_from(const cg_adamw_group* all, int count, int first) {
+  Groups groups;
+  groups.first = first;
+  groups.count = std::min(count - first, kGroupsAtOnce);
+  for (int k = 0; k < groups.count; ++k) groups.g[k] = all[first + k];
+  return groups;
+}
+
 template <typename T, int kMax>
-int run_step(const Tensors& tensors, const Groups& groups, int bits, const States& states,
+int run_step(const Tensors& tensors, const cg_adamw_group* all_groups, int group_count, int bits, const States& states,
              int64_t* steps, float max_norm, float* norm_out, Control* control, double* partial, cudaStream_t s) {
   Table<kMax> table;
+  const Groups groups = groups_from(all_groups, group_count, 0);
   if (max_norm > 0) {
     int partials = 0;
     for (int next = 0; next < tensors.count;) {
@@ -488,6 +509,10 @@ int run_step(const Tensors& tensors, const Groups& groups, int bits, const State
     adamw_factors_kernel<<<1, 32, 0, s>>>(groups, steps, control);
     if (int rc = check_launch("adamw_factors_kernel")) return rc;
   }
+  for (int more = kGroupsAtOnce; more < group_count; more += kGroupsAtOnce) {
+    adamw_factors_kernel<<<1, 32, 0, s>>>(groups_from(all_groups, group_count, more), steps, control);
+    if (int rc = check_launch("adamw_factors_kernel")) return rc;
+  }
   for (int next = 0; next < tensors.count;) {
     fill_table(tensors, next, table);
     if (!table.chunks) continue;
@@ -502,7 +527,13 @@ int run_step(const Tensors& tensors, const Groups& groups, int bits, const State
 }  // namespace
 }  // namespace cg
 
-extern "C" int64_t cg_adamw_control_bytes(void) { return sizeof(cg::Control); }
+extern "C" int64_t cg_adamw_control_bytes(int groups) {
+  if (groups < 1) {
+    cg::set_error(CG_ERR_ARGUMENT, "cg_adamw_control_bytes: no groups");
+    return -1;
+  }
+  return static_cast<int64_t>(sizeof(cg::Control)) + groups * static_cast<int64_t>(sizeof(cg::Factors));
+}
 
 extern "C" int64_t cg_adamw_workspace_bytes(int count) {
   if (count < 0) {
@@ -521,20 +552,17 @@ extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params
   CG_REQUIRE(count >= 0 && (count == 0 || (tensors && params && grads)), "cg_adamw_step: bad tensor table");
   CG_REQUIRE(valid_dtype(dtype), "cg_adamw_step: dtype must be float32, float16 or bfloat16");
   CG_REQUIRE(state_bits == 8 || state_bits == 32, "cg_adamw_step: state_bits must be 8 or 32");
-  CG_REQUIRE(groups && group_count > 0 && group_count <= kMaxGroups, "cg_adamw_step: 1..%d groups", kMaxGroups);
+  CG_REQUIRE(groups && group_count > 0, "cg_adamw_step: no groups");
   CG_REQUIRE(exp_avg && exp_avg_sq && steps && control, "cg_adamw_step: NULL state");
   CG_REQUIRE(state_bits == 32 || (exp_avg_scale && exp_avg_sq_scale), "cg_adamw_step: 8-bit states need scales");
   CG_REQUIRE(dtype == CG_F32 || master, "cg_adamw_step: 16-bit parameters need fp32 master copies");
   CG_REQUIRE(!(max_norm > 0) || norm_out, "cg_adamw_step: max_norm needs norm_out");
   if (max_norm > 0 && (!workspace || workspace_bytes < cg_adamw_workspace_bytes(count)))
     return set_error(CG_ERR_WORKSPACE, "cg_adamw_step: workspace too small");
-  Groups table;
-  table.count = group_count;
   for (int k = 0; k < group_count; ++k) {
     const cg_adamw_group& g = groups[k];
     CG_REQUIRE(g.beta1 >= 0 && g.beta1 < 1 && g.beta2 >= 0 && g.beta2 < 1, "cg_adamw_step: betas must lie in [0, 1)");
     CG_REQUIRE(g.eps >= 0, "cg_adamw_step: eps must not be negative");
-    table.g[k] = g;
   }
   const Tensors all{tensors, params, grads, count};
   int live = 0;
@@ -554,8 +582,8 @@ extern "C" int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params
   auto run = [&](auto sample) {
     using T = decltype(sample);
     return live <= kFewTensors
-               ? run_step<T, kFewTensors>(all, table, state_bits, states, steps, max_norm, norm_out, c, partial, s)
-               : run_step<T, kManyTensors>(all, table, state_bits, states, steps, max_norm, norm_out, c, partial, s);
+               ? run_step<T, kFewTensors>(all, groups, group_count, state_bits, states, steps, max_norm, norm_out, c, partial, s)
+               : run_step<T, kManyTensors>(all, groups, group_count, state_bits, states, steps, max_norm, norm_out, c, partial, s);
   };
   if (dtype == CG_F32) return run(float{});
   if (dtype == CG_F16) return run(__half{});

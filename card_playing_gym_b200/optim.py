@@ -97,7 +97,8 @@ class AdamW(torch.optim.Optimizer):
         self.flat = flat
         self.steps = torch.zeros((), dtype=torch.int64, device=device)
         self.grad_norm = torch.zeros((), device=device)
-        self._control = torch.zeros(nat.query("cg_adamw_control_bytes"), dtype=torch.uint8, device=device)
+        self._control = torch.zeros(nat.query("cg_adamw_control_bytes", len(self.param_groups)), dtype=torch.uint8,
+                                    device=device)
         for p, start in zip(self._parameters, starts):
             size = p.numel()
             views = {}

@@ -444,7 +444,7 @@ int cg_center_zero_sum(const float* values, const int64_t* players, int64_t n, i
  * tensors; one whose grad is NULL is left as it is. steps int64 is
  * t on the device, shared by all tensors, and counts up by one. With max_norm a norm that is
  * not finite leaves everything as it is (steps too); norm_out fp32 receives |g|.
- * control: cg_adamw_control_bytes(), zeroed before its first use and kept with the state.
+ * control: cg_adamw_control_bytes(groups), zeroed before its first use and kept with the state.
  * ------------------------------------------------------------------------------- */
 typedef struct {
   int64_t numel, state;
@@ -453,7 +453,7 @@ typedef struct {
 typedef struct {
   double lr, beta1, beta2, eps, weight_decay;
 } cg_adamw_group;
-int64_t cg_adamw_control_bytes(void);
+int64_t cg_adamw_control_bytes(int groups);
 int64_t cg_adamw_workspace_bytes(int count);
 int cg_adamw_step(const cg_adamw_tensor* tensors, void* const* params, const void* const* grads, int count, int dtype,
                   const cg_adamw_group* groups, int group_count, int state_bits, void* exp_avg, float* exp_avg_scale, void* exp_avg_sq, float* exp_avg_sq_scale,

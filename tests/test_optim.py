@@ -340,3 +340,26 @@ def test_without_eps_a_vanishing_gradient_moves_a_weight_by_a_few_learning_rates
     for _ in range(3):
         opt.step()
         assert torch.isfinite(p).all() and p.detach().abs().max() <= 3 * 33 * 1e-2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("max_norm", [None, 0.5])
+@pytest.mark.parametrize("count", [1, 16, 17, 32, 33, 70, 700])
+def test_any_number_of_groups(count, max_norm):
+    """Learning rates by layer: each group's own hyperparameters at every step, past one launch's share of them."""
+
+    params = parameters([(40 + i % 7,) for i in range(count)], torch.float32)
+    groups = [dict(params=[p], lr=1e-3 * (1 + i % 40), betas=(0.8 + 0.001 * (i % 90), 0.99), eps=1e-8, weight_decay=0.01 * (i % 3))
+              for i, p in enumerate(params)]
+    clip = 1.0
+    if max_norm is not None:
+        clip = min(1.0, max_norm / (math.sqrt(sum(float((p.grad.double() ** 2).sum()) for p in params)) + 1e-6))
+    want = [Formula([p], g["lr"], g["betas"], g["eps"], g["weight_decay"], None) for p, g in zip(params, groups)]
+    opt = optim.AdamW(groups, max_norm=max_norm)
+    for _ in range(2):
+        opt.step()
+        for w, p in zip(want, params):
+            w.step([p.grad.double() * clip])
+    assert int(opt.steps) == 2
+    for w, p in zip(want, params):
+        assert (p.detach().double() - w.p[0]).abs().max() <= 2 * 20 * EPS32 * (w.p[0].abs().max() + 0.4)
