@@ -340,3 +340,26 @@ def test_an_infinity_in_the_backward_pass(rows, dtype):
     dy = data["dy"].double()
     for got, want in zip(grads, (dy @ data["weight"].double(), dy.t() @ data["x"].double(), dy.sum(0))):
         assert torch.isinf(want).any() and same_kind(got.double(), want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 24, 32, 33, 4096])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_gelu_left_of_zero_is_rounded_once(dtype, rows):
+    """Products by one are exact, so a 16-bit GELU is its value's nearest one, but for 3% of the spacing there (1e-5 of the
+    value is 2% of float16's), down to z = -13; the slope too, with 2^-20 where its terms cancel. Few rows or many."""
+
+    kind = TYPES[dtype]
+    x = torch.linspace(-13, 4, 8192, device="cuda").to(kind).view(-1, 1)[:: 8192 // rows][:rows] if rows > 1 else \
+        torch.full((1, 1), -4.0, dtype=kind, device="cuda")
+    x = x.contiguous().requires_grad_()
+    one = torch.ones((1, 1), dtype=kind, device="cuda")
+    y = dense.linear(x, one, activation="gelu")
+    (slope,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = x.detach().double()
+    cumulative = 0.5 * torch.special.erfc(-z / math.sqrt(2))
+    least = torch.finfo(kind).smallest_normal
+    for got, want, extra in ((y, z * cumulative, 0.0),
+                             (slope, cumulative + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), 2.0 ** -20)):
+        spacing = 2.0 ** torch.floor(torch.log2(want.abs().clamp(min=least))) * 2 * HALF_STEP[kind]
+        assert ((got.double() - want).abs() <= 0.53 * spacing + extra).all()
