@@ -557,3 +557,30 @@ def test_the_library_refuses_a_gradient_without_its_scale():
         nat.call("cg_anchored_gradient", None, 0, 1, *fill[3:], None, 0, None, 4, None)
     with pytest.raises(nat.NativeError, match="dtype"):
         nat.call("cg_anchored_gradient", None, 9, *fill[2:], None, 0, None, 4, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("apart", [0.0, 1e-4, -1e-3, 0.01, 0.3, -0.49, 0.51, -1.0, 2.0])
+@pytest.mark.parametrize("width", [2, 52, 700, 2000])
+def test_the_sampled_divergences_do_not_cancel_near_the_reference(width, apart):
+    """exp(u) - u - 1 is u^2 / 2 near zero, far below the rounding of 1. Of uniform logits log pi = -log(width) is off by
+    2^-21 at most (4 units in the last place of 7.6), which moves the estimate by |exp(u) - 1| times it; its own
+    arithmetic takes 2^-20 of itself, and past the series 2^-22 of exp(u) + |u| + 1."""
+
+    rows = 40
+    logits = torch.zeros((rows, width), device="cuda", requires_grad=True)
+    level = -math.log(width)
+    log_probs = torch.full((rows,), level + apart, device="cuda")
+    ones = torch.ones(rows, device="cuda")
+    actions = torch.arange(rows, device="cuda") % width
+    objective, totals = ppo.anchored_objective(logits, actions, log_probs, 0.0 * ones, ones, clip_ratio=CLIP, beta=1.0,
+                                               reference_log_probs=log_probs)
+    objective.backward()
+    u = float(log_probs[0].double()) - level
+    for key, v in (("reference_kl", u), ("behavior_kl", -u)):
+        want = math.expm1(v) - v
+        bound = abs(math.expm1(v)) * 2.0 ** -21 + 2.0 ** -20 * want + (2.0 ** -22 * (math.exp(v) + abs(v) + 1) if abs(v) >= 0.49 else 0)
+        got = float(totals[ppo.ANCHORED_KEYS.index(key)]) / rows
+        assert abs(got - want) <= bound + 2.0 ** -42, key
+    slope = -math.expm1(u) * (1.0 - 1.0 / width)  # d KL / d logit of the action
+    assert abs(float(logits.grad[0, 0]) - slope) <= 2.0 ** -20 * abs(slope) + 2.0 ** -20 * math.exp(u)
