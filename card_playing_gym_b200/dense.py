@@ -7,6 +7,7 @@
 
 from __future__ import annotations
 
+import math
 from functools import lru_cache
 
 import torch
@@ -125,8 +126,9 @@ def linear(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = No
             raise ValueError(f"{name} must be {x.dtype} on {x.device}, as x is, not {tensor.dtype} on {tensor.device}")
     nat.ptr(x)  # refuses CPU tensors
     if x.dim() != 2:
-        x = x.reshape(-1, x.shape[-1]) if x.shape[-1] else x.new_empty((shape[:-1].numel(), 0))
-        residual = None if residual is None else residual.reshape(x.shape[0], outer)
+        rows = math.prod(shape[:-1])  # -1 is ambiguous where a row has no entries
+        x = x.reshape(rows, x.shape[-1])
+        residual = None if residual is None else residual.reshape(rows, outer)
     inputs = (_unit_rows(x), _unit_rows(weight), None if bias is None else bias.contiguous(),
               None if residual is None else _unit_rows(residual))
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in inputs):

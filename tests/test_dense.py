@@ -363,3 +363,22 @@ def test_gelu_left_of_zero_is_rounded_once(dtype, rows):
                              (slope, cumulative + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi), 2.0 ** -20)):
         spacing = 2.0 ** torch.floor(torch.log2(want.abs().clamp(min=least))) * 2 * HALF_STEP[kind]
         assert ((got.double() - want).abs() <= 0.53 * spacing + extra).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", [(2, 3, 0), (0,), (0, 4, 0), (2, 0, 5), (3, 1, 0)])
+def test_leading_dimensions_of_empty_extents(shape, dtype):
+    kind = TYPES[dtype]
+    x = torch.zeros(shape, dtype=kind, device="cuda", requires_grad=True)
+    weight = torch.ones((6, shape[-1]), dtype=kind, device="cuda", requires_grad=True)
+    bias = normal((6,), kind, 3).requires_grad_()
+    residual = normal((*shape[:-1], 6), kind, 4).requires_grad_()
+    y = dense.linear(x, weight, bias, residual, activation="relu")
+    want = torch.relu(bias.double()) + residual.double()
+    assert y.shape == (*shape[:-1], 6)
+    assert ((y.double() - want).abs() <= 2 * HALF_STEP[kind] * (want.abs() + 1)).all()
+    grads = torch.autograd.grad(y, (x, weight, bias, residual), torch.ones_like(y))
+    rows = math.prod(shape[:-1])
+    assert [g.shape for g in grads] == [x.shape, weight.shape, bias.shape, residual.shape]
+    assert torch.equal(grads[2].double(), rows * (bias > 0).double()) and torch.equal(grads[3], torch.ones_like(residual))
