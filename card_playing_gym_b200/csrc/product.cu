@@ -503,9 +503,11 @@ __global__ void __launch_bounds__(256) product_join_kernel(const float* partial,
   pdl_trigger();
   const bool aligned = epilogue_aligned<T>(e, cols);
   const int shift = tile_n == 256 ? 6 : 5;  // vectors of four columns in a tile's row
-  const int total = (tiles_i * tiles_j - whole) * kTileM << shift;  // at most 37 tiles
-  for (int index = blockIdx.x * 256 + threadIdx.x; index < total; index += gridDim.x * 256) {
-    const int line = index >> shift, q = index & ((1 << shift) - 1), tile = line / kTileM, row = line % kTileM;
+  // At most 37 split tiles, but every tile of a product of no depth.
+  const int64_t total = static_cast<int64_t>(tiles_i * tiles_j - whole) * kTileM << shift;
+  for (int64_t index = blockIdx.x * 256 + threadIdx.x; index < total; index += gridDim.x * 256) {
+    const int tile = static_cast<int>((index >> shift) / kTileM), row = static_cast<int>((index >> shift) % kTileM);
+    const int q = static_cast<int>(index) & ((1 << shift) - 1);
     int ti, tj;
     place_tile(whole + tile, tiles_i, tiles_j, &ti, &tj);
     const int64_t i = static_cast<int64_t>(ti) * kTileM + row, j = static_cast<int64_t>(tj) * tile_n + q * 4;

@@ -382,3 +382,14 @@ def test_leading_dimensions_of_empty_extents(shape, dtype):
     rows = math.prod(shape[:-1])
     assert [g.shape for g in grads] == [x.shape, weight.shape, bias.shape, residual.shape]
     assert torch.equal(grads[2].double(), rows * (bias > 0).double()) and torch.equal(grads[3], torch.ones_like(residual))
+
+
+@pytest.mark.gpu
+def test_a_product_of_no_depth_past_32_bits_of_entries():
+    """2^33 outputs (17 GB), all of them the bias."""
+
+    x = torch.zeros((1 << 20, 0), dtype=torch.bfloat16, device="cuda")
+    bias = normal((8192,), torch.bfloat16, 1)
+    torch.full((1 << 33,), math.nan, dtype=torch.bfloat16, device="cuda")  # what the output's memory may hold
+    y = dense.linear(x, torch.zeros((8192, 0), dtype=torch.bfloat16, device="cuda"), bias)
+    assert all(torch.equal(piece, bias.expand_as(piece)) for piece in y.split(1 << 16))
