@@ -244,7 +244,19 @@ __global__ void __launch_bounds__(32) adamw_factors_kernel(const __grid_constant
     make_factors(groups, *steps, control);
 }
 
-// Squares are summed in fp32 over a thread's eight entries and in double from there on.
+// Squares are summed in fp32 over a thread's eight entries and in double from there on. Entries past 1.8e19, whose squares
+// fp32 does not hold, are summed in double throughout: the norm of finite gradients is finite unless it passes fp32 itself.
+__device__ __forceinline__ double sum_of_squares(const float (&g)[8]) {
+  float sum = 0.f;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) sum = fmaf(g[i], g[i], sum);
+  if (sum < INFINITY) return sum;
+  double wide = 0;
+#pragma unroll
+  for (int i = 0; i < kPerLane; ++i) wide += static_cast<double>(g[i]) * g[i];
+  return wide;
+}
+
 template <typename T, int kMax>
 __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_constant__ Table<kMax> table,
                                                               const __grid_constant__ Groups groups, float max_norm,
@@ -269,23 +281,16 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
 #pragma unroll
         for (int c = 0; c < kAtOnce; ++c) load8(grad + start + ((b + c) * kThreads + threadIdx.x) * kPerLane, g[c]);
 #pragma unroll
-        for (int c = 0; c < kAtOnce; ++c) {
-          float sum = 0.f;
-#pragma unroll
-          for (int i = 0; i < kPerLane; ++i) sum = fmaf(g[c][i], g[c][i], sum);
-          total += sum;
-        }
+        for (int c = 0; c < kAtOnce; ++c) total += sum_of_squares(g[c]);
       }
       continue;
     }
     for (int b = 0; b < kSteps; ++b) {
       const int64_t at = start + (b * kThreads + threadIdx.x) * kPerLane;
       if (at >= e.numel) break;
-      float g[8], sum = 0.f;
+      float g[8];
       load_entries(grad, at, e.numel, aligned && at + kPerLane <= e.numel, g);
-#pragma unroll
-      for (int i = 0; i < kPerLane; ++i) sum = fmaf(g[i], g[i], sum);
-      total += sum;
+      total += sum_of_squares(g);
     }
   }
 #pragma unroll
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(kThreads) adamw_norm_kernel(const __grid_const
   for (int w = 0; w < kThreads / 32; ++w) total += s[w];
   const double norm = sqrt(total);
   if (threadIdx.x == 0) *norm_out = static_cast<float>(norm);
-  begin_step(groups, steps, isfinite(norm), static_cast<float>(fmin(1.0, max_norm / (norm + 1e-6))), control);
+  begin_step(groups, steps, isfinite(static_cast<float>(norm)), static_cast<float>(fmin(1.0, max_norm / (norm + 1e-6))), control);
 }
 
 // ---- the update -----------------------------------------------------------------------------------------

@@ -363,3 +363,35 @@ def test_any_number_of_groups(count, max_norm):
     assert int(opt.steps) == 2
     for w, p in zip(want, params):
         assert (p.detach().double() - w.p[0]).abs().max() <= 2 * 20 * EPS32 * (w.p[0].abs().max() + 0.4)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("offset", [0, 3])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("bits", [8, 32])
+def test_gradients_whose_squares_pass_the_largest_float_are_clipped(bits, dtype, offset):
+    """Entries of 1e25: the norm is finite, so the step is taken, with gradients of 1e25 times the clip's 1e-27."""
+
+    params = parameters([(20000,), (77,)], TYPES[dtype], offset)
+    for p in params:
+        p.grad.mul_(1e27)
+    norm = math.sqrt(sum(float((p.grad.double() ** 2).sum()) for p in params))
+    opt = optim.AdamW(params, lr=1e-2, weight_decay=0.0, max_norm=1.0, state_bits=bits)
+    before = [p.detach().float().clone() for p in params]
+    opt.step()
+    assert int(opt.steps) == 1 and float(opt.grad_norm) == pytest.approx(norm, rel=8 * EPS32)
+    for p, old in zip(params, before):
+        held = (opt.state[p]["master"] if dtype != "fp32" else p.detach()).double()
+        g = p.grad.double() / norm
+        want = old.double() - 1e-2 * g / (g.abs() + 1e-8)
+        assert (held - want).abs().max() <= 1e-2 * 1e-4 + 20 * EPS32
+
+
+@pytest.mark.gpu
+def test_a_norm_past_the_largest_float_skips_the_step():
+    params = parameters([(300,)], torch.float32)
+    params[0].grad.fill_(3e38)
+    before = params[0].detach().clone()
+    opt = optim.AdamW(params, max_norm=1.0)
+    opt.step()
+    assert int(opt.steps) == 0 and float(opt.grad_norm) == math.inf and torch.equal(params[0].detach(), before)
