@@ -25,7 +25,9 @@ class AdamW(torch.optim.Optimizer):
     """AdamW(params, lr, betas, eps, weight_decay, state_bits=32 | 8, max_norm=None).
 
     Parameters are contiguous CUDA tensors of one dtype (float32, float16 or bfloat16) on one device. 16-bit
-    parameters keep float32 master copies in the state, which the step updates and rounds once into the parameter.
+    parameters keep float32 master copies in the state, which the step updates and rounds once into the parameter. Where a
+    parameter has been written to since (a checkpoint loaded into the model, an in-place edit), the next step takes
+    its values over into the master copy.
 
     ``state_bits=8`` holds m and sqrt(v) as e4m3 codes scaled by the largest magnitude of each block of 256
     entries. ``max_norm`` clips the gradients' global norm, coefficient min(1, max_norm / (norm + 1e-6)); where the
@@ -110,6 +112,9 @@ class AdamW(torch.optim.Optimizer):
             if "master" in views:
                 views["master"].copy_(p.detach())
             self.state[p] = views
+        # What the master copies were last known to follow.
+        self._versions = [p._version for p in self._parameters]
+        self._addresses = array("Q", map(torch.Tensor.data_ptr, self._parameters))
         # The host's side of the step: extents and groups are fixed, addresses are gathered at every step.
         self._table = (nat.AdamWTensor * len(self._parameters))()
         self._dtype = first.dtype
@@ -171,6 +176,17 @@ class AdamW(torch.optim.Optimizer):
         if list(map(_bytes_of, grads)) != sizes:
             raise ValueError("a gradient has not its parameter's size")
 
+    def _follow(self, params: list, addresses: array) -> None:
+        """Takes parameters that something else has written to into their master copies. An entry that is its master
+        rounded keeps the master's low bits, so that a checkpoint's parameters and masters load in either order."""
+
+        moved = addresses != self._addresses
+        for p, known in zip(params, self._versions):
+            if moved or p._version != known:
+                master, value = self.state[p]["master"], p.detach()
+                master.copy_(torch.where(master.to(value.dtype) == value, master, value.float()))
+        self._addresses = addresses
+
     def step(self, closure=None):
         loss = None
         if closure is not None:
@@ -183,6 +199,8 @@ class AdamW(torch.optim.Optimizer):
         table = self._table
         from_params = array("Q", map(torch.Tensor.data_ptr, params))
         from_grads = array("Q", [0 if g is None else g.data_ptr() for g in grads])
+        if "master" in flat and ([p._version for p in params] != self._versions or from_params != self._addresses):
+            self._follow(params, from_params)
         for entry, group in zip(self._groups, self.param_groups):
             entry.lr, entry.eps, entry.weight_decay = group["lr"], group["eps"], group["weight_decay"]
             entry.beta1, entry.beta2 = group["betas"]
@@ -197,4 +215,6 @@ class AdamW(torch.optim.Optimizer):
                      nat.ptr(workspace), 0 if workspace is None else workspace.numel(), nat.stream_handle(device))
         # The kernel writes through addresses: autograd learns here that a graph's saved weights have changed.
         torch.autograd.graph.increment_version([p for p, g in zip(params, from_grads) if g] if 0 in from_grads else params)
+        if "master" in flat:
+            self._versions = [p._version for p in params]
         return loss

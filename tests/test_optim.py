@@ -395,3 +395,49 @@ def test_a_norm_past_the_largest_float_skips_the_step():
     opt = optim.AdamW(params, max_norm=1.0)
     opt.step()
     assert int(opt.steps) == 0 and float(opt.grad_norm) == math.inf and torch.equal(params[0].detach(), before)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_weights_loaded_after_the_optimizer_was_made_are_the_ones_that_step(dtype):
+    """A checkpoint loaded into the model, an edit in place, another tensor under the parameter: 16-bit masters follow."""
+
+    kind = TYPES[dtype]
+    params = parameters([(300,), (9, 33)], kind)
+    opt = optim.AdamW(params, lr=1e-3)
+    opt.step()
+    fresh = parameters([(300,), (9, 33)], kind, seed=5)
+    model = torch.nn.ParameterList(params)
+    model.load_state_dict(torch.nn.ParameterList(fresh).state_dict())
+    for edit in (None, lambda p: p.mul_(0.5), lambda p: p.add_(1.0)):
+        if edit is not None:
+            with torch.no_grad():
+                edit(params[1])
+        before = [p.detach().double() for p in params]
+        opt.step()
+        for p, old in zip(params, before):
+            moved = (p.detach().double() - old).abs()
+            assert moved.max() <= 4e-3 + 2.0 ** -7 * old.abs().max() and (dtype != "fp32" or moved.max() > 0)
+    params[0].data = torch.full_like(params[0].data, 3.0)
+    opt.step()
+    assert (params[0].detach().double() - 3.0).abs().max() <= 4e-3 + 2.0 ** -7 * 3
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("model_first", [False, True])
+def test_masters_keep_their_low_bits_when_a_checkpoint_is_loaded(model_first):
+    params = parameters([(700,)], torch.bfloat16)
+    opt = optim.AdamW(params, lr=1e-4, max_norm=1.0)
+    for _ in range(3):
+        opt.step()
+    others = parameters([(700,)], torch.bfloat16, seed=7)
+    others[0].grad.copy_(params[0].grad)
+    again = optim.AdamW(others, lr=1e-4, max_norm=1.0)
+    loads = [lambda: again.load_state_dict(opt.state_dict()),
+             lambda: torch.nn.ParameterList(others).load_state_dict(torch.nn.ParameterList(params).state_dict())]
+    for load in reversed(loads) if model_first else loads:
+        load()
+    for _ in range(3):
+        opt.step()
+        again.step()
+    assert torch.equal(opt.flat["master"], again.flat["master"]) and torch.equal(params[0], others[0])
