@@ -393,3 +393,19 @@ def test_a_product_of_no_depth_past_32_bits_of_entries():
     torch.full((1 << 33,), math.nan, dtype=torch.bfloat16, device="cuda")  # what the output's memory may hold
     y = dense.linear(x, torch.zeros((8192, 0), dtype=torch.bfloat16, device="cuda"), bias)
     assert all(torch.equal(piece, bias.expand_as(piece)) for piece in y.split(1 << 16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [1, 20, 32, 33, 5000])
+def test_float32_silu_in_full_precision(rows):
+    """Products by one are exact. An exponential, a sum and a quotient of at most two units in the last place each: 2^-21 of
+    the value, and for the slope of its larger term, g and z g (1 - g)."""
+
+    x = torch.linspace(-80, 20, 5000, device="cuda")[:: 5000 // rows][:rows].reshape(-1, 1).requires_grad_()
+    one = torch.ones((1, 1), device="cuda")
+    y = dense.linear(x, one, activation="silu")
+    (slope,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    z = x.detach().double()
+    gate = 1 / (1 + torch.exp(-z))
+    assert ((y.double() - z * gate).abs() <= 2.0 ** -21 * (z * gate).abs()).all()
+    assert ((slope.double() - gate * (1 + z * (1 - gate))).abs() <= 2.0 ** -21 * gate * (1 + z.abs())).all()
