@@ -552,10 +552,18 @@ int make_map(CUtensorMap* map, const ProductOperand& o, int64_t inner, int64_t o
   const cuuint64_t strides[2] = {(row_bytes + 15) & ~cuuint64_t{15},
                                  parts > 1 ? static_cast<cuuint64_t>(o.part) * 2 : (row_bytes + 15) & ~cuuint64_t{15}};
   const cuuint32_t boxes[3] = {64, static_cast<cuuint32_t>(box), 1}, steps[3] = {1, 1, 1};
-  const CUresult rc = encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
-                             const_cast<void*>(o.base), dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto make = [&] {
+    return encode(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.base),
+                  dims, strides, boxes, steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult rc = make();
+  if (rc == CUDA_ERROR_INVALID_CONTEXT) {
+    // The thread's first CUDA call (an autograd worker's, whose memory came from torch's cache): the driver call needs a
+    // current context, which the runtime sets at its own calls only.
+    int device = 0;
+    if (cudaGetDevice(&device) == cudaSuccess && cudaSetDevice(device) == cudaSuccess) rc = make();
+  }
   if (rc != CUDA_SUCCESS) return set_error(CG_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", static_cast<int>(rc));
   return CG_OK;
 }

@@ -9,6 +9,9 @@ backward pass and the gradient entering its products round once more each."""
 from __future__ import annotations
 
 import math
+import subprocess
+import sys
+from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
 import pytest
@@ -409,3 +412,30 @@ def test_float32_silu_in_full_precision(rows):
     gate = 1 / (1 + torch.exp(-z))
     assert ((y.double() - z * gate).abs() <= 2.0 ** -21 * (z * gate).abs()).all()
     assert ((slope.double() - gate * (1 + z * (1 - gate))).abs() <= 2.0 ** -21 * gate * (1 + z.abs())).all()
+
+
+@pytest.mark.gpu
+def test_a_threads_first_cuda_call_may_be_a_product():
+    """Memory from torch's cache leaves a new thread without a current context until its first launch, and a 16-bit layer
+    begins with a tensor map, a driver call that needs one."""
+
+    data = case(64, 64, 64, torch.bfloat16, bias=False, residual=False)
+    with torch.no_grad():
+        want = dense.linear(data["x"], data["weight"])
+        torch.cuda.synchronize()
+        with ThreadPoolExecutor(1) as pool:
+            got = pool.submit(lambda: dense.linear(data["x"], data["weight"])).result()
+    assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_a_programs_first_backward_pass_may_be_a_product():
+    """The autograd worker's first call, with neither a bias nor an activation to launch anything before it."""
+
+    code = ("import torch; from card_playing_gym_b200 import dense\n"
+            "x, w, dy = (torch.ones(64, 64, dtype=torch.bfloat16, device='cuda') for _ in range(3))\n"
+            "w.requires_grad_()\n"
+            "torch.autograd.grad(dense.linear(x, w), w, dy); grad, = torch.autograd.grad(dense.linear(x, w), w, dy)\n"
+            "assert (grad == 64).all()")
+    done = subprocess.run([sys.executable, "-c", code], cwd=Path(dense.__file__).parents[1], capture_output=True, text=True)
+    assert done.returncode == 0, done.stderr[-2000:]
