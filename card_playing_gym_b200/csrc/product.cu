@@ -13,13 +13,16 @@
 //
 // float32 operands are three bfloat16 parts each (8 bits of mantissa apiece): the six products of parts that reach 2^-24 of
 // the result run from one stage that holds all three parts of both operands, at six times the bfloat16 work and
-// three times its traffic. The tensor cores cut their running sum at each step (measured: 1.7e-8 of it, always
-// toward zero), which a long float32 sum would show: the five small products have an accumulator of their own,
+// three times its traffic. The tensor cores cut their running sum at each step
+// (measured on terms of one sign: by 1.7e-7 of it every 16 k's, always toward zero; of random signs a tenth of that), which
+// a long float32 sum would show: the five small products have an accumulator of their own,
 // and after kChunkBlocks blocks of k the epilogue takes both sums into registers, where they are added with
 // rounding, and the next chunk starts from zero in the other pair of accumulators. An infinity or NaN is its own first
 // part, so the product of first parts is the float32 one; what it makes of the small products (an infinity times parts of
-// either sign, or of zero) is left out. tile_n is 128 for float32, so that two pairs fit tensor memory. 16-bit results keep one running sum: at 8192 k's the cut is 9e-6 against their own
-// rounding of 2^-11 or 2^-8.
+// either sign, or of zero) is left out. tile_n is 128 for float32, so that two pairs fit tensor memory. 16-bit results keep one running sum as far as its cuts stay well
+// inside their own rounding: 16,384 k's of float16 (9e-5 of the sum at most, against 4.9e-4) and 65,536 of bfloat16 (3.9e-4
+// against 3.9e-3). Deeper products, the weight gradients of long batches, are split and the sums joined in fp32 with rounding
+// (262,144 rows of float16 in one sum: 1.5e-3 short, for 2304 x 2304 at 2270 us instead of 2440).
 //
 // Where the last round of tiles leaves half the pairs idle, k is split for the tiles of that round: every split writes
 // fp32 partial sums and product_join_kernel adds them in order and applies the epilogue (8192 k's of 4096 x 4096: 256
@@ -50,6 +53,8 @@ constexpr int kSquareBytes = 32 * 32 * 4;
 constexpr int kAccumulatorColumns = 256;  // of one of the two accumulators (float32: the main products' and the small ones')
 constexpr int kBoxRows = 64;              // rows of a box of an operand stored across
 constexpr int kLeastSplitBlocks = 4;      // k blocks a split is worth (100 x 1024 x 1024: 16 us, with 8 or 16 19)
+constexpr int kLongestHalfSum = 256;      // k blocks (16,384 k's) of one running sum of a float16 product
+constexpr int kLongestBfloatSum = 1024;   // and of a bfloat16 one (65,536 k's)
 constexpr int kChunkBlocks = 4;           // k blocks (256 k's) of one running sum of a float32 product: 16 steps
 
 // What a stage holds: one part of each operand, or a float32's three.
@@ -70,7 +75,7 @@ struct Params {
   int chunk;  // blocks of one running sum; for float32 its k blocks times the parts
   uint32_t instruction;
   int across_a, across_b;
-  float* partial;  // [split tile][split][256][tile_n]
+  float* partial;  // [split][split tile][256][tile_n]
   ProductEpilogue e;
 };
 
@@ -91,10 +96,11 @@ __device__ __forceinline__ void place_tile(int tile, int tiles_i, int tiles_j, i
 __device__ __forceinline__ Item item_of(const Params& p, int index) {
   Item t = {0, 0, -1, 0, p.blocks};
   int tile = index;
-  if (index >= p.whole) {
+  if (index >= p.whole) {  // split by split, so that the tiles in work at one time share their operands in L2
+    const int tiles = p.tiles_i * p.tiles_j - p.whole;
     t.slot = index - p.whole;
-    tile = p.whole + t.slot / p.splits;
-    t.first = t.slot % p.splits * p.per_split;
+    tile = p.whole + t.slot % tiles;
+    t.first = t.slot / tiles * p.per_split;
     t.last = min(t.first + p.per_split, p.blocks);
   }
   place_tile(tile, p.tiles_i, p.tiles_j, &t.i, &t.j);
@@ -503,7 +509,7 @@ __global__ void __launch_bounds__(256) product_join_kernel(const float* partial,
   pdl_trigger();
   const bool aligned = epilogue_aligned<T>(e, cols);
   const int shift = tile_n == 256 ? 6 : 5;  // vectors of four columns in a tile's row
-  // At most 37 split tiles, but every tile of a product of no depth.
+  // At most 37 split tiles, but every tile of a product of no depth or of a very great one.
   const int64_t total = static_cast<int64_t>(tiles_i * tiles_j - whole) * kTileM << shift;
   for (int64_t index = blockIdx.x * 256 + threadIdx.x; index < total; index += gridDim.x * 256) {
     const int tile = static_cast<int>((index >> shift) / kTileM), row = static_cast<int>((index >> shift) % kTileM);
@@ -513,10 +519,10 @@ __global__ void __launch_bounds__(256) product_join_kernel(const float* partial,
     const int64_t i = static_cast<int64_t>(ti) * kTileM + row, j = static_cast<int64_t>(tj) * tile_n + q * 4;
     if (i >= rows || j >= cols) continue;
     float z[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* from = partial + (static_cast<int64_t>(tile) * splits * kTileM + row) * tile_n + q * 4;
+    const float* from = partial + (static_cast<int64_t>(tile) * kTileM + row) * tile_n + q * 4;
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-      const float4 f = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(s) * kTileM * tile_n);
+      const float4 f = *reinterpret_cast<const float4*>(from + s * (total << 2));
       z[0] += f.x, z[1] += f.y, z[2] += f.z, z[3] += f.w;
     }
     float bias[4];
@@ -630,12 +636,19 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
   const int64_t last_round = tiles % pairs;  // tiles that would not fill a round of pairs
   int64_t splits = 1;
   if (last_round > 0 && 2 * last_round <= pairs) splits = std::max<int64_t>(1, std::min(pairs / last_round, units));
+  int64_t whole_tiles = tiles - last_round;
+  const int64_t longest = dtype == CG_F16 ? kLongestHalfSum : kLongestBfloatSum;
+  const int64_t sums = dtype == CG_F32 ? 1 : (k_blocks + longest - 1) / longest;
+  if (sums > splits || (sums > 1 && whole_tiles > 0)) {  // every tile is split for its sums' sake
+    splits = whole_tiles > 0 ? sums : std::max(splits, sums);
+    whole_tiles = 0;
+  }
   const int64_t units_each = units > 0 ? (units + splits - 1) / splits : 1;
   splits = units > 0 ? (units + units_each - 1) / units_each : 0;
   plan.blocks = static_cast<int>(k_blocks);
   plan.per_split = static_cast<int>(units_each * unit);
   plan.splits = static_cast<int>(splits);
-  plan.whole = static_cast<int>(splits == 1 ? tiles : splits == 0 ? 0 : tiles - last_round);
+  plan.whole = static_cast<int>(splits == 1 ? tiles : splits == 0 ? 0 : whole_tiles);
   plan.chunk = dtype == CG_F32 ? kChunkBlocks : std::max(1, plan.blocks);
   plan.partial_bytes = (tiles - plan.whole) * splits * kTileM * plan.tile_n * 4;
   return plan;

@@ -439,3 +439,27 @@ def test_a_programs_first_backward_pass_may_be_a_product():
             "assert (grad == 64).all()")
     done = subprocess.run([sys.executable, "-c", code], cwd=Path(dense.__file__).parents[1], capture_output=True, text=True)
     assert done.returncode == 0, done.stderr[-2000:]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("inner,outer", [(2304, 2304), (300, 200)])
+def test_the_weight_gradient_of_a_long_batch(inner, outer, dtype):
+    """The tensor cores cut a running sum toward zero, by some 1.7e-7 of it every 16 rows where its terms have one sign, which
+    moves the whole gradient: over 262,144 rows in one sum by 1.5e-3. Sums of 16,384 rows (float16) and 65,536 (bfloat16)
+    leave 9e-5 and 3.9e-4 of it; the bounds are 2^-13 and 2^-11. Factors of 1 to 2 a column spread the entries over a
+    binade, so that their own rounding averages out."""
+
+    rows, kind = 1 << 18, TYPES[dtype]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    uniform = lambda *shape: torch.rand(shape, generator=g, device="cuda")  # noqa: E731
+    x = (uniform(rows, inner).add_(0.5) * torch.exp2(uniform(inner))).to(kind)
+    dy = (uniform(rows, outer).add_(0.5) * torch.exp2(uniform(outer) - 6)).to(kind)
+    weight = torch.zeros((outer, inner), dtype=kind, device="cuda", requires_grad=True)
+    (got,) = torch.autograd.grad(dense.linear(x, weight), weight, dy)
+    some = list(range(0, outer, outer // 8))
+    want = torch.stack([(dy[:, j:j + 1].double() * x.double()).sum(0) for j in some])
+    off = got[some].double() / want - 1
+    shift = 2.0 ** -13 if dtype == "fp16" else 2.0 ** -11
+    assert abs(float(off.mean())) <= shift + HALF_STEP[kind] / off.numel() ** 0.5
+    assert float(off.abs().max()) <= HALF_STEP[kind] + 1.5 * shift
