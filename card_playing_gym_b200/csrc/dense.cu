@@ -221,7 +221,7 @@ Layout plan_layout(const void* x, int64_t x_stride, const void* weight, int64_t 
     l.sums = take(l.slices * outer * static_cast<int64_t>(sizeof(float)));
     if (activation != kActNone || needs_pack(dy, dy_stride, rows, dtype)) l.dpre = take(packed_bytes(rows, outer, dtype));
   }
-  if (!backward && rows <= kFewRows) return l;
+  if (!backward && few_rows(rows, inner, outer, dtype)) return l;
   if (needs_pack(x, x_stride, rows, dtype)) l.x = take(packed_bytes(rows, inner, dtype));
   if (needs_pack(weight, weight_stride, outer, dtype)) l.weight = take(packed_bytes(outer, inner, dtype));
   const int64_t partial = backward ? std::max(plan_product(rows, inner, outer, dtype).partial_bytes,
@@ -343,7 +343,7 @@ extern "C" int cg_linear_forward(const void* x, int64_t x_stride, const void* we
   const ProductEpilogue e = {bias, residual, pre, y, residual_stride, outer, activation};
   char* w = static_cast<char*>(workspace);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (rows <= kFewRows) return run_few_rows(x, x_stride, weight, weight_stride, rows, inner, outer, dtype, e, s);
+  if (few_rows(rows, inner, outer, dtype)) return run_few_rows(x, x_stride, weight, weight_stride, rows, inner, outer, dtype, e, s);
   if (dtype == CG_F32) return forward<float>(l, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, e, w, s);
   if (dtype == CG_F16) return forward<__half>(l, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, e, w, s);
   return forward<__nv_bfloat16>(l, x, x_stride, weight, weight_stride, dtype, rows, inner, outer, e, w, s);

@@ -1,4 +1,4 @@
-// The linear layer for a few tokens: y = act(x W^T + b) + residual with at most 32 rows of x.
+// The linear layer for a few tokens: y = act(x W^T + b) + residual with at most 32 rows of x (few_rows in product.h).
 //
 // W is read once and is all there is to read; it passes L1 by, which keeps the tokens.
 //
@@ -13,7 +13,8 @@
 //
 // 4096 x 8192, floor 10.3 us for 16-bit W: bfloat16 17 us for one token and 20 for 24 (bound by the latency of W's loads
 // and the launch). float32, floor 20.5: 33 us for one token, 41 for 8, 78 for 16, 172 for 32 (bound by the tokens' loads out
-// of L1 and L2, a vector for 16 products; in tensor-core parts 60, 60, 105 and 188).
+// of L1 and L2, a vector for 16 products; in tensor-core parts 60, 60, 105 and 188;
+// such a layer goes to run_product from 25 tokens on).
 #include "elements.cuh"
 
 namespace cg {

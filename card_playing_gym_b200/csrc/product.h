@@ -36,9 +36,14 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype);
 int run_product(const ProductOperand& a, const ProductOperand& b, int64_t rows, int64_t cols, int64_t depth, int dtype,
                 const ProductEpilogue& e, void* partial, cudaStream_t stream);
 
-// The forward layer of at most kFewRows rows, its weights read once. (4096 x 8192, 24 tokens: bfloat16 20 us, by run_product
-// 33; float32 139 against 165. 32 tokens: 22 against 32, and 172 against 166; 2048 x 512 float32 10 against 27.)
-constexpr int kFewRows = 32;
+// The forward layer of at most kFewRows rows, its weights read once: bfloat16 4096 x 8192 with 24 tokens 20 us, by run_product
+// 33, with 32 tokens 22 against 32. float32 pays for each token, 4096 x 8192 with 16 tokens 117 us against 165, with 24 174
+// against 165 and with 32 218 against 167, so more than 24 tokens of a large layer go to run_product: from 2^23 weights on
+// (8000 x 1000 with 32 tokens 54 us against 52, 4096 x 512 20 against 28).
+constexpr int kFewRows = 32, kFewRowsOfLarge32 = 24;
+inline bool few_rows(int64_t rows, int64_t inner, int64_t outer, int dtype) {
+  return rows <= (dtype == CG_F32 && inner * outer >= 1 << 23 ? kFewRowsOfLarge32 : kFewRows);
+}
 int run_few_rows(const void* x, int64_t x_stride, const void* weight, int64_t weight_stride, int64_t rows, int64_t inner,
                  int64_t outer, int dtype, const ProductEpilogue& e, cudaStream_t stream);
 

@@ -463,3 +463,24 @@ def test_the_weight_gradient_of_a_long_batch(inner, outer, dtype):
     shift = 2.0 ** -13 if dtype == "fp16" else 2.0 ** -11
     assert abs(float(off.mean())) <= shift + HALF_STEP[kind] / off.numel() ** 0.5
     assert float(off.abs().max()) <= HALF_STEP[kind] + 1.5 * shift
+
+
+def test_float32_tokens_go_where_they_are_faster():
+    """Up to 24 tokens the weights are read in place; more of them through a large float32 layer are packed for the tensor
+    cores, which takes a workspace."""
+
+    def workspace(rows, inner, outer, dtype):
+        return nat.query("cg_linear_workspace_bytes", None, inner, None, inner, None, 0, nat.DTYPE_CODES[dtype], rows, inner,
+                         outer, 0, 0)
+
+    for rows in (1, 24):
+        assert workspace(rows, 8192, 4096, torch.float32) == 0
+    assert workspace(25, 8192, 4096, torch.float32) > 0 and workspace(32, 1 << 16, 128, torch.float32) > 0
+    assert workspace(32, 512, 4096, torch.float32) == 0 and workspace(33, 512, 4096, torch.float32) > 0
+    assert workspace(32, 8192, 4096, torch.bfloat16) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [24, 25, 32, 33])
+def test_many_float32_tokens_through_a_large_layer(rows):
+    check(case(rows, 2048, 4100, torch.float32), "gelu")
