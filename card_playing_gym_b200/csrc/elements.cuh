@@ -223,7 +223,7 @@ __device__ __forceinline__ float activation_slope(float z) {
   }
   if constexpr (kActivation == kActSilu) {
     const float gate = sizeof(T) == 2 ? __fdividef(1.f, silu_under<T>(z)) : 1.f / silu_under<T>(z);
-    return gate == 0.f ? 0.f : gate * fmaf(z, 1.f - gate, 1.f);
+    return gate == 0.f || gate == 1.f ? gate : gate * fmaf(z, 1.f - gate, 1.f);  // an infinity times zero
   }
   return 1.f;
 }

@@ -484,3 +484,21 @@ def test_float32_tokens_go_where_they_are_faster():
 @pytest.mark.parametrize("rows", [24, 25, 32, 33])
 def test_many_float32_tokens_through_a_large_layer(rows):
     check(case(rows, 2048, 4100, torch.float32), "gelu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("activation", ["relu", "gelu", "silu"])
+def test_slopes_at_infinite_sums_are_their_limits(activation, dtype):
+    """A float16 sum past 65,504 is kept as an infinity for the backward pass: its slope is 1 (or 0 on the left), not a NaN."""
+
+    kind = TYPES[dtype]
+    big = math.inf if dtype != "fp16" else 60000.0
+    x = torch.full((40, 1), big, dtype=kind, device="cuda")
+    x[20:] = -big
+    x.requires_grad_()
+    two = torch.full((1, 1), 2.0, dtype=kind, device="cuda")
+    bias = torch.zeros(1, dtype=kind, device="cuda", requires_grad=True)
+    y = dense.linear(x, two, bias, activation=activation)
+    dx, dbias = torch.autograd.grad(y, (x, bias), torch.ones_like(y))
+    assert torch.equal(dx[:20], torch.full_like(dx[:20], 2.0)) and not dx[20:].any() and float(dbias) == 20.0
