@@ -24,6 +24,7 @@ namespace {
 
 constexpr int kTotals = 9;
 constexpr int kPartials = 4736;  // the grid's upper bound: a fixed order of addition for a given row count
+constexpr int kMostEntries = 1 << 30;  // of a row, counted in 32 bits with room for a batch past its end
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct Args {
@@ -969,7 +970,7 @@ namespace {
 // The checks that the objective and its gradient share.
 int check_rows(const char* name, const Args& a, int dtype) {
   CG_REQUIRE(valid_dtype(dtype), "%s: dtype must be float32, float16 or bfloat16", name);
-  CG_REQUIRE(a.rows >= 0 && a.width > 0, "%s: bad shape", name);
+  CG_REQUIRE(a.rows >= 0 && a.width > 0 && a.width <= kMostEntries, "%s: bad shape", name);
   CG_REQUIRE(a.stride >= a.width && (!a.grad || a.grad_stride >= a.width) &&
                  (!a.reference || a.reference_stride >= a.width) && (!a.legal || a.legal_stride >= a.width),
              "%s: stride < width", name);
@@ -1052,7 +1053,7 @@ extern "C" int cg_action_log_probs(const void* logits, int dtype, int64_t rows, 
                                    float* log_probs, void* stream) {
   using namespace cg;
   CG_REQUIRE(valid_dtype(dtype), "cg_action_log_probs: dtype must be float32, float16 or bfloat16");
-  CG_REQUIRE(rows >= 0 && width > 0, "cg_action_log_probs: bad shape");
+  CG_REQUIRE(rows >= 0 && width > 0 && width <= kMostEntries, "cg_action_log_probs: bad shape");
   CG_REQUIRE(stride >= width && (!legal || legal_stride >= width), "cg_action_log_probs: stride < width");
   if (rows == 0) return CG_OK;
   CG_REQUIRE(logits && actions && log_probs, "cg_action_log_probs: NULL pointer");

@@ -210,6 +210,7 @@ def ppo_terms(logits: torch.Tensor, old_probs: torch.Tensor, actions: torch.Tens
 # -- the anchored objective ------------------------------------------------------------------------
 ANCHORED_KEYS = ("policy_loss", "row_weight", "entropy_raw", "entropy", "entropy_weight", "clip", "behavior_kl",
                  "reference_kl", "objective")
+MOST_ENTRIES = 1 << 30  # of a row: the kernels count them in 32 bits
 
 
 def _rows_of(name: str, tensor: torch.Tensor, rows: int, device: torch.device, dtype: torch.dtype) -> torch.Tensor:
@@ -248,6 +249,8 @@ def _row_stride(plane: torch.Tensor) -> int:
 def _logits_and_mask(logits: torch.Tensor, actions: torch.Tensor, legal: torch.Tensor | None):
     if logits.dim() != 2 or logits.shape[1] == 0:
         raise ValueError(f"logits must be [rows, width] with a width, not {tuple(logits.shape)}")
+    if logits.shape[1] > MOST_ENTRIES:
+        raise ValueError(f"logits must have a width of at most {MOST_ENTRIES}, not {logits.shape[1]}")
     if logits.dtype not in nat.DTYPE_CODES:
         raise ValueError(f"logits must be float32, float16 or bfloat16, not {logits.dtype}")
     if actions.is_floating_point():

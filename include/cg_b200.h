@@ -388,7 +388,8 @@ int cg_value_loss(const float* prediction, const float* targets, const int32_t* 
  * (surr, 1, H, H / log |S|, [|S| > 1], [|ratio - 1| > clip], ratio - 1 - log ratio, KL), then L twice (one
  * to keep as the objective), summed in a fixed order. A row counts for nothing, with a zero gradient, where its action is negative, its
  * weight 0 or nothing in it is legal (a mask that is all zero, logits that are all minus infinity).
- * An action >= width or outside the legal set does the same and sets the fault word (0x420 / 0x421). */
+ * An action >= width or outside the legal set does the same and sets the fault word (0x420 / 0x421).
+ * width is at most 2^30. */
 int64_t cg_anchored_objective_workspace_bytes(int64_t rows);
 int cg_anchored_objective(const void* logits, int dtype, int64_t rows, int width, int64_t stride,
                           const void* reference_logits, int64_t reference_stride, const float* reference_log_probs,

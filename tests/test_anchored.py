@@ -584,3 +584,16 @@ def test_the_sampled_divergences_do_not_cancel_near_the_reference(width, apart):
         assert abs(got - want) <= bound + 2.0 ** -42, key
     slope = -math.expm1(u) * (1.0 - 1.0 / width)  # d KL / d logit of the action
     assert abs(float(logits.grad[0, 0]) - slope) <= 2.0 ** -20 * abs(slope) + 2.0 ** -20 * math.exp(u)
+
+
+def test_rows_past_32_bits_are_refused():
+    """By the wrapper, which would hand the library a width cut to 32 bits, and by the library."""
+
+    wide = torch.zeros((1, 1)).expand(1, (1 << 32) + 52)
+    with pytest.raises(ValueError, match="width of at most"):
+        ppo.action_log_probs(wide, torch.zeros(1, dtype=torch.int64))
+    one = torch.zeros(1)
+    with pytest.raises(ValueError, match="width of at most"):
+        ppo.anchored_objective(wide, torch.zeros(1, dtype=torch.int64), one, one, one, clip_ratio=CLIP, beta=0.0)
+    with pytest.raises(nat.NativeError, match="bad shape"):
+        nat.call("cg_action_log_probs", None, 0, 1, (1 << 30) + 1, (1 << 30) + 1, None, 0, None, None, None)
