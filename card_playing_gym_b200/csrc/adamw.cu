@@ -195,6 +195,12 @@ __device__ __forceinline__ float root_fast(float v) {
   return r;
 }
 
+// The reciprocal to its last bit, but for the rarest rounding cases: one step of Newton's method on the fast one.
+__device__ __forceinline__ float reciprocal_near(float x) {
+  const float r = reciprocal_fast(x);
+  return fmaf(r, fmaf(-x, r, 1.f), r);
+}
+
 // Under the update's quotient at least, 2^-75: the root of any v above zero is larger, an entry without history does not
 // divide zero by a zero eps, and one whose v has become zero below float32's range is updated as if it had the least one.
 constexpr float kLeastUnder = 2.6469780e-23f;
@@ -374,7 +380,10 @@ __device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e
 #pragma unroll
   for (int i = 0; i < kPerLane; i += 2) {
     const Two raw = two(l.g[i], l.g[i + 1]), g = raw * clips;
-    const Two m = beta1 * two(l.m[i], l.m[i + 1]) + rest1 * g;
+    // The products are rounded before their sum (packed ones are fused with a packed sum): an 8-bit code then is that of the
+    // formula's own fp32 arithmetic, not of a neighbouring value at its edge.
+    const float2 kept = apart_of(beta1 * two(l.m[i], l.m[i + 1])), added = apart_of(rest1 * g);
+    const Two m = two(__fadd_rn(kept.x, added.x), __fadd_rn(kept.y, added.y));
     const Two v = fma(beta2, two(l.v[i], l.v[i + 1]), rest2 * (g * g));
     const float2 fv = apart_of(v), fm = apart_of(m);
     const float2 root = make_float2(root_fast(fv.x), root_fast(fv.y));
@@ -396,8 +405,8 @@ __device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e
   if constexpr (kBits == 8) {
     peak_m = warp_peak(peak_m);
     peak_r = warp_peak(peak_r);
-    const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max * reciprocal_fast(peak_m);
-    const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max * reciprocal_fast(peak_r);
+    const float to_m = peak_m < kLeastPeak ? 0.f : kE4m3Max * reciprocal_near(peak_m);
+    const float to_r = peak_r < kLeastPeak ? 0.f : kE4m3Max * reciprocal_near(peak_r);
     float least = kE4m3Least;
 #pragma unroll
     for (int i = 0; i < kPerLane; i += 2) {

@@ -441,3 +441,27 @@ def test_masters_keep_their_low_bits_when_a_checkpoint_is_loaded(model_first):
         opt.step()
         again.step()
     assert torch.equal(opt.flat["master"], again.flat["master"]) and torch.equal(params[0], others[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_the_8_bit_first_moment_is_the_formulas_own_in_fp32(dtype):
+    """b1 m + (1 - b1) g with every operation rounded to fp32, over the block's largest magnitude: the same scales and the same
+    codes, step after step. (A product fused with the sum gives neighbouring codes at an edge, and a scale that follows
+    such a code is off by a code's step later.)"""
+
+    n = 1 << 21
+    params = parameters([(n,)], TYPES[dtype])
+    opt = optim.AdamW(params, lr=1e-3, betas=(0.9, 0.999), state_bits=8)
+    codes = torch.zeros(n // optim.BLOCK, optim.BLOCK, device="cuda")
+    scale = torch.zeros(n // optim.BLOCK, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    for _ in range(4):
+        params[0].grad.copy_(1e-2 * torch.randn(n, generator=g, device="cuda"))
+        grad = params[0].grad.float().view(-1, optim.BLOCK)
+        first = 0.9 * (codes * (scale * torch.tensor(1.0 / 448.0, device="cuda"))[:, None]) + (1 - 0.9) * grad
+        scale = first.abs().amax(dim=1)
+        codes = (first * (448.0 * (1.0 / scale))[:, None]).to(torch.float8_e4m3fn).float()
+        opt.step()
+        assert torch.equal(opt.flat["exp_avg_scale"], scale)
+        assert torch.equal(opt.flat["exp_avg"].float().view(-1, optim.BLOCK), codes)
