@@ -11,8 +11,9 @@
 //
 // 8-bit moments: m and sqrt(v) as e4m3, scaled by the largest magnitude of each block of 256 entries of a
 // tensor (fp32). The root halves the exponent range that v needs; a root that is not zero keeps at least the
-// smallest code, so that no entry with history divides by eps alone. A block's scale is exact, so the block
-// follows its largest entry through changes smaller than a code's step. The update itself uses the new fp32
+// smallest code, so that no entry with history divides by eps alone. A block's scale is held in fp32 (m's as the
+// formula gives it, the root's within 2 units in the last place), so the block follows its largest entry through changes
+// smaller than a code's step. The update itself uses the new fp32
 // moments, before they are rounded. A block is one warp's eight entries a lane, so its maximum is one
 // warp reduction.
 #include <cuda_fp8.h>
@@ -432,8 +433,9 @@ __device__ __forceinline__ void update_block(Loaded<T, kBits>& l, const Entry& e
 // and written block by block, from sectors that eight warps were writing to, they were what the kernel waited for:
 // 134 M float32 weights with 8-bit moments 510 us, with whole sectors 360.) Three thread blocks an SM, with the registers
 // that leaves, do better than more (134 M bfloat16 weights, 8 bits: 376 us; four 400, five 472). The first loads go out
-// before the wait for the factors: nothing the kernel before this one writes is among them. 32-bit moments move 6.3 TB/s,
-// 96% of the copy bandwidth; 8-bit ones 5.95 (float32 weights) and 5.7 (bfloat16), short of it by their codes' arithmetic.
+// before the wait for the factors: nothing the kernel before this one writes is among them. Without a clip,
+// 134 M weights: 32-bit moments 571 us (float32, 6.6 TB/s) and 586 (bfloat16, 6.4), the copy bandwidth; 8-bit ones 338 (6.4)
+// and 356 (6.0), short of it by their codes' arithmetic.
 template <typename T, int kBits, int kMax>
 __global__ void __launch_bounds__(kThreads, 3) adamw_update_kernel(const __grid_constant__ Table<kMax> table, const States states,
                                                                    const Control* control) {

@@ -4,7 +4,7 @@
 // Row i over its legal set S, logits z, reference logits r, lp = z - lse_S(z), lr = r - lse_S(r), p = exp(lp):
 //   ratio = exp(lp_a - old), surr = -min(ratio A, clip(ratio) A), H = -sum p lp
 //   KL = sum p (lp - lr)                       with the reference's logits, or
-//   KL = exp(u) - u - 1, u = lr_a - lp_a       with the reference's log-probability of the action alone
+//   KL = exp(u) - u - 1, u = lr_a - lp_a       with the reference's log-probability of the action alone (excess())
 //   L = sum_i w (surr + beta KL - alpha [|S| > 1] H / log |S|)
 //   dL/dz_j = p_j (K0 + w beta (z_j - r_j) + w alpha' (z_j - max z)) + [j = a] w c
 // with c = d surr / d ratio * ratio (+ beta (1 - exp(u))), alpha' = alpha / log |S| and
@@ -13,8 +13,11 @@
 // sums of small terms, from cancelling against the large log-sum-exps. An illegal entry acts as a logit of minus
 // infinity, whatever it holds.
 //
-// All row arithmetic is fp32. The totals are summed in fp32 over the rows of one thread (some tens) and in double
-// from there on, in a fixed order.
+// All row arithmetic is fp32. The totals are summed in fp32 over the rows of one thread (rows over the resident groups of
+// lanes, or over the resident blocks for wide rows: 14 of 262,144 rows of 52, 150 to 600 of as many wide ones) and in double
+// from there on, in a fixed order. The entries' exponentials are ex2.approx, off by 2^-22 and by 2^-24 of
+// the exponent's size, since kernels that wait for issue would pay for every instruction of a full-precision one: against 64
+// bits the float32 gradient of 262,144 rows of 52 is 6.1e-7 off, by plain fp32 operations 1.1e-6.
 #include <algorithm>
 
 #include "elements.cuh"
@@ -918,8 +921,8 @@ int run_row(const Args& a, int* blocks, cudaStream_t s) {
   return check_launch("anchored_row_kernel");
 }
 
-// The smallest block that holds the row in its registers. Longer rows: 16-bit ones, bound by their arithmetic, take 256
-// threads (131,072 entries: 859 us, with 1024 threads 878; 32,000: 220 against 264). So do float32 ones whose resident
+// The smallest block that holds the row in its registers. Longer rows: 16-bit ones take 256 threads, whether or not the
+// rows in work fit L2 (131,072 entries, which do not: 859 us, with 1024 threads 878; 32,000: 220 against 264). So do float32 ones whose resident
 // blocks' rows stay in L2 between their two readings (80 of its 126 MB, the rest for the gradient passing through:
 // 10,000 entries 123 us against 185), else 1024 threads, which have fewer rows in work (32,000: 361 against 411).
 template <typename T, bool kExact>
