@@ -224,9 +224,9 @@ Layout plan_layout(const void* x, int64_t x_stride, const void* weight, int64_t 
   if (!backward && few_rows(rows, inner, outer, dtype)) return l;
   if (needs_pack(x, x_stride, rows, dtype)) l.x = take(packed_bytes(rows, inner, dtype));
   if (needs_pack(weight, weight_stride, outer, dtype)) l.weight = take(packed_bytes(outer, inner, dtype));
-  const int64_t partial = backward ? std::max(plan_product(rows, inner, outer, dtype).partial_bytes,
-                                              plan_product(outer, inner, rows, dtype).partial_bytes)
-                                   : plan_product(rows, outer, inner, dtype).partial_bytes;
+  const int64_t partial = backward ? std::max(plan_product(rows, inner, outer, dtype).bytes(),
+                                              plan_product(outer, inner, rows, dtype).bytes())
+                                   : plan_product(rows, outer, inner, dtype).bytes();
   l.partial = take(partial);
   return l;
 }

@@ -11,18 +11,20 @@
 //   warp 9     allocates tensor memory; in the even CTA lane 0 issues the MMAs
 // Loads of both CTAs complete on the even CTA's barriers; MMA completions are committed to both CTAs'.
 //
-// float32 operands are three bfloat16 parts each (8 bits of mantissa apiece): the six products of parts that reach 2^-24 of
-// the result run from one stage that holds all three parts of both operands, at six times the bfloat16 work and
-// three times its traffic. The tensor cores cut their running sum at each step
-// (measured on terms of one sign: by 1.7e-7 of it every 16 k's, always toward zero; of random signs a tenth of that), which
-// a long float32 sum would show: the five small products have an accumulator of their own,
-// and after kChunkBlocks blocks of k the epilogue takes both sums into registers, where they are added with
-// rounding, and the next chunk starts from zero in the other pair of accumulators. An infinity or NaN is its own first
-// part, so the product of first parts is the float32 one; what it makes of the small products (an infinity times parts of
-// either sign, or of zero) is left out. tile_n is 128 for float32, so that two pairs fit tensor memory. 16-bit results keep one running sum as far as its cuts stay well
-// inside their own rounding: 16,384 k's of float16 (9e-5 of the sum at most, against 4.9e-4) and 65,536 of bfloat16 (3.9e-4
-// against 3.9e-3). Deeper products, the weight gradients of long batches, are split and the sums joined in fp32 with rounding
-// (262,144 rows of float16 in one sum: 1.5e-3 short, for 2304 x 2304 at 2270 us instead of 2440).
+// float32 operands are three bfloat16 parts each (8 bits of mantissa apiece): the six products of parts that reach
+// 2^-24 of the result run from one stage that holds all three parts of both operands, at six times the bfloat16 work
+// and three times its traffic. The tensor cores cut their running sum at each step (measured on terms of one sign: by
+// 1.7e-7 of it every 16 k's, always toward zero; of random signs a tenth of that), which a long float32 sum would show:
+// the five small products have an accumulator of their own, and after kChunkBlocks blocks of k the epilogue takes both
+// sums into registers, where they are added with rounding, and the next chunk starts from zero in the other pair of
+// accumulators. An infinity or NaN is its own first part, so the product of first parts is the float32 one; what it
+// makes of the small products (an infinity times parts of either sign, or of zero) is left out. tile_n is 128 for
+// float32, so that two pairs fit tensor memory.
+//
+// 16-bit results keep one running sum as far as its cuts stay well inside their own rounding: 16,384 k's of float16
+// (9e-5 of the sum at most, against 4.9e-4) and 65,536 of bfloat16 (3.9e-4 against 3.9e-3). Deeper products, the weight
+// gradients of long batches, add such sums with rounding, in a place of each lane's own that stays in L2 (262,144 rows
+// of float16 in one sum: 1.5e-3 short).
 //
 // Where the last round of tiles leaves half the pairs idle, k is split for the tiles of that round: every split writes
 // fp32 partial sums and product_join_kernel adds them in order and applies the epilogue (8192 k's of 4096 x 4096: 256
@@ -44,6 +46,7 @@
 namespace cg {
 namespace {
 
+constexpr int kPairs = 74;  // of the B200's 148 SMs
 constexpr int kTileM = 256, kTileK = 64;  // a pair's rows; k's of a stage (128 bytes of 16-bit entries)
 constexpr int kHalfBytes = 128 * kTileK * 2;  // one CTA's rows of A (or of B at tile_n 256) of a stage
 constexpr int kEpilogueWarps = 8;
@@ -55,6 +58,7 @@ constexpr int kBoxRows = 64;              // rows of a box of an operand stored 
 constexpr int kLeastSplitBlocks = 4;      // k blocks a split is worth (100 x 1024 x 1024: 16 us, with 8 or 16 19)
 constexpr int kLongestHalfSum = 256;      // k blocks (16,384 k's) of one running sum of a float16 product
 constexpr int kLongestBfloatSum = 1024;   // and of a bfloat16 one (65,536 k's)
+constexpr int kRunningFloats = kEpilogueWarps * 4 * 32 * 32;  // of one CTA: 128 rows by 256 columns
 constexpr int kChunkBlocks = 4;           // k blocks (256 k's) of one running sum of a float32 product: 16 steps
 
 // What a stage holds: one part of each operand, or a float32's three.
@@ -75,7 +79,8 @@ struct Params {
   int chunk;  // blocks of one running sum; for float32 its k blocks times the parts
   uint32_t instruction;
   int across_a, across_b;
-  float* partial;  // [split][split tile][256][tile_n]
+  float* partial;  // [split tile][split][256][tile_n]
+  float* running;  // sums of 16-bit products between chunks: [CTA][warp][chunk of columns][column][lane]
   ProductEpilogue e;
 };
 
@@ -96,11 +101,10 @@ __device__ __forceinline__ void place_tile(int tile, int tiles_i, int tiles_j, i
 __device__ __forceinline__ Item item_of(const Params& p, int index) {
   Item t = {0, 0, -1, 0, p.blocks};
   int tile = index;
-  if (index >= p.whole) {  // split by split, so that the tiles in work at one time share their operands in L2
-    const int tiles = p.tiles_i * p.tiles_j - p.whole;
+  if (index >= p.whole) {
     t.slot = index - p.whole;
-    tile = p.whole + t.slot % tiles;
-    t.first = t.slot / tiles * p.per_split;
+    tile = p.whole + t.slot / p.splits;
+    t.first = t.slot % p.splits * p.per_split;
     t.last = min(t.first + p.per_split, p.blocks);
   }
   place_tile(tile, p.tiles_i, p.tiles_j, &t.i, &t.j);
@@ -251,7 +255,8 @@ __device__ __forceinline__ bool epilogue_aligned(const ProductEpilogue& e, int64
          (!e.pre || aligned4<T>(e.pre, cols));
 }
 
-template <typename T>
+// kDeep: a 16-bit product of more than one running sum (a kernel of its own: the others' epilogues are 5% slower with it).
+template <typename T, bool kDeep>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     product_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const __grid_constant__ Params p) {
@@ -475,12 +480,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int c = 0; c < 2; ++c) store_sums(c, sums[c], residual_of(c));
       } else {
+        // Between the chunks of a deep product its sums wait in a place of this lane's own.
+        auto running = [&](int c) { return p.running + (((blockIdx.x * kEpilogueWarps + warp) * 4 + c) * 32) * 32 + lane; };
+        auto add_running = [&](int c, float (&v)[32]) {
+#pragma unroll
+          for (int k = 0; k < 32; ++k) v[k] += __ldcg(running(c) + k * 32);
+        };
+        int first = t.first;
+        if constexpr (kDeep) {
+          for (; first + p.chunk < t.last && wait_sum(); first += p.chunk) {
+            for (int c = 0; c < chunks; ++c) {
+              float v[32];
+              read_sum(c, 0, v);
+              if (c == chunks - 1) release_sum();
+              if (first > t.first) add_running(c, v);
+#pragma unroll
+              for (int k = 0; k < 32; ++k) __stcg(running(c) + k * 32, v[k]);
+            }
+          }
+          if (!ok) break;
+        }
         RowOf32<T> residual = residual_of(0);
         if (!wait_sum()) break;
         for (int c = 0; c < chunks; ++c) {
           float v[32];
           read_sum(c, 0, v);
           if (c == chunks - 1) release_sum();
+          if (kDeep && first > t.first) add_running(c, v);
           store_sums(c, v, residual);
           if (c + 1 < chunks) residual = residual_of(c + 1);
         }
@@ -509,7 +535,7 @@ __global__ void __launch_bounds__(256) product_join_kernel(const float* partial,
   pdl_trigger();
   const bool aligned = epilogue_aligned<T>(e, cols);
   const int shift = tile_n == 256 ? 6 : 5;  // vectors of four columns in a tile's row
-  // At most 37 split tiles, but every tile of a product of no depth or of a very great one.
+  // At most 37 split tiles, but every tile of a product of no depth.
   const int64_t total = static_cast<int64_t>(tiles_i * tiles_j - whole) * kTileM << shift;
   for (int64_t index = blockIdx.x * 256 + threadIdx.x; index < total; index += gridDim.x * 256) {
     const int tile = static_cast<int>((index >> shift) / kTileM), row = static_cast<int>((index >> shift) % kTileM);
@@ -519,10 +545,10 @@ __global__ void __launch_bounds__(256) product_join_kernel(const float* partial,
     const int64_t i = static_cast<int64_t>(ti) * kTileM + row, j = static_cast<int64_t>(tj) * tile_n + q * 4;
     if (i >= rows || j >= cols) continue;
     float z[4] = {0.f, 0.f, 0.f, 0.f};
-    const float* from = partial + (static_cast<int64_t>(tile) * kTileM + row) * tile_n + q * 4;
+    const float* from = partial + (static_cast<int64_t>(tile) * splits * kTileM + row) * tile_n + q * 4;
 #pragma unroll 4
     for (int s = 0; s < splits; ++s) {
-      const float4 f = *reinterpret_cast<const float4*>(from + s * (total << 2));
+      const float4 f = *reinterpret_cast<const float4*>(from + static_cast<int64_t>(s) * kTileM * tile_n);
       z[0] += f.x, z[1] += f.y, z[2] += f.z, z[3] += f.w;
     }
     float bias[4];
@@ -596,19 +622,22 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
     p.instruction = (1u << 4) | (half ? 0u : (1u << 7) | (1u << 10)) | (a.across ? 1u << 15 : 0u) | (b.across ? 1u << 16 : 0u) |
                     (static_cast<uint32_t>(plan.tile_n >> 3) << 17) | (static_cast<uint32_t>(kTileM >> 4) << 24);
     p.partial = partial;
+    p.running = partial + plan.partial_bytes / 4;
     p.e = e;
+    auto kernel = sizeof(T) == 2 && plan.blocks > plan.chunk ? product_kernel<T, sizeof(T) == 2> : product_kernel<T, false>;
     static bool configured[64] = {false};
     int device = 0;
     cudaGetDevice(&device);
     if (!configured[device & 63]) {
-      cudaError_t err =
-          cudaFuncSetAttribute(product_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmemBytes);
-      if (err != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel smem: %s", cudaGetErrorString(err));
+      for (auto each : {product_kernel<T, sizeof(T) == 2>, product_kernel<T, false>}) {
+        cudaError_t err = cudaFuncSetAttribute(each, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape<T>::kSmemBytes);
+        if (err != cudaSuccess) return set_error(CG_ERR_CUDA, "product_kernel smem: %s", cudaGetErrorString(err));
+      }
       configured[device & 63] = true;
     }
     const int items = plan.whole + (plan.tiles_i * plan.tiles_j - plan.whole) * plan.splits;
-    const int pairs = std::min(items, sm_count() / 2);
-    if (int rc = launch_pdl("product_kernel", product_kernel<T>, dim3(2 * pairs), dim3(kThreads), Shape<T>::kSmemBytes, stream,
+    const int pairs = std::min({items, sm_count() / 2, kPairs});
+    if (int rc = launch_pdl("product_kernel", kernel, dim3(2 * pairs), dim3(kThreads), Shape<T>::kSmemBytes, stream,
                             map_a, map_b, p))
       return rc;
     if (plan.whole == plan.tiles_i * plan.tiles_j) return CG_OK;
@@ -623,7 +652,7 @@ int run_typed(const ProductOperand& a, const ProductOperand& b, int64_t rows, in
 
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
   ProductPlan plan = {};
-  const int64_t pairs = 74;  // the B200's 148 SMs
+  const int64_t pairs = kPairs;
   auto tiles_of = [&](int tile_n) { return (rows + kTileM - 1) / kTileM * ((cols + tile_n - 1) / tile_n); };
   // 16-bit operands: half tiles where they fill more than half the pairs in one round and whole ones would be split
   // (2048 x 1024 x 1024: 18 us against 25; 512 x 4096 x 4096: equal).
@@ -636,21 +665,15 @@ ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype) {
   const int64_t last_round = tiles % pairs;  // tiles that would not fill a round of pairs
   int64_t splits = 1;
   if (last_round > 0 && 2 * last_round <= pairs) splits = std::max<int64_t>(1, std::min(pairs / last_round, units));
-  int64_t whole_tiles = tiles - last_round;
-  const int64_t longest = dtype == CG_F16 ? kLongestHalfSum : kLongestBfloatSum;
-  const int64_t sums = dtype == CG_F32 ? 1 : (k_blocks + longest - 1) / longest;
-  if (sums > splits || (sums > 1 && whole_tiles > 0)) {  // every tile is split for its sums' sake
-    splits = whole_tiles > 0 ? sums : std::max(splits, sums);
-    whole_tiles = 0;
-  }
   const int64_t units_each = units > 0 ? (units + splits - 1) / splits : 1;
   splits = units > 0 ? (units + units_each - 1) / units_each : 0;
   plan.blocks = static_cast<int>(k_blocks);
   plan.per_split = static_cast<int>(units_each * unit);
   plan.splits = static_cast<int>(splits);
-  plan.whole = static_cast<int>(splits == 1 ? tiles : splits == 0 ? 0 : whole_tiles);
-  plan.chunk = dtype == CG_F32 ? kChunkBlocks : std::max(1, plan.blocks);
+  plan.whole = static_cast<int>(splits == 1 ? tiles : splits == 0 ? 0 : tiles - last_round);
+  plan.chunk = dtype == CG_F32 ? kChunkBlocks : dtype == CG_F16 ? kLongestHalfSum : kLongestBfloatSum;
   plan.partial_bytes = (tiles - plan.whole) * splits * kTileM * plan.tile_n * 4;
+  plan.running_bytes = dtype != CG_F32 && plan.blocks > plan.chunk ? 2 * pairs * kRunningFloats * 4 : 0;
   return plan;
 }
 

@@ -28,7 +28,8 @@ struct ProductOperand {
 // The product's plan: a function of the sizes alone.
 struct ProductPlan {
   int tile_n, tiles_i, tiles_j, blocks, whole, splits, per_split, chunk;
-  int64_t partial_bytes;
+  int64_t partial_bytes, running_bytes;  // of the workspace: split tiles' sums, then sums between chunks
+  int64_t bytes() const { return partial_bytes + running_bytes; }
 };
 ProductPlan plan_product(int64_t rows, int64_t cols, int64_t depth, int dtype);
 
