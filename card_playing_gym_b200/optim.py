@@ -27,7 +27,8 @@ class AdamW(torch.optim.Optimizer):
     Parameters are contiguous CUDA tensors of one dtype (float32, float16 or bfloat16) on one device. 16-bit
     parameters keep float32 master copies in the state, which the step updates and rounds once into the parameter. Where a
     parameter has been written to since (a checkpoint loaded into the model, an in-place edit), the next step takes
-    its values over into the master copy.
+    its values over into the master copy; it sees writes that count the parameter's version up or give it another
+    address, which writes through ``.data`` do not.
 
     ``state_bits=8`` holds m and sqrt(v) as e4m3 codes scaled by the largest magnitude of each block of 256
     entries. ``max_norm`` clips the gradients' global norm, coefficient min(1, max_norm / (norm + 1e-6)); where the
