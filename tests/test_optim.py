@@ -13,7 +13,8 @@ import math
 import pytest
 import torch
 
-from card_playing_gym_b200 import dense, optim
+from card_playing_gym_b200 import dense
+from card_playing_gym_b200 import optim
 
 EPS32 = 2.0 ** -24
 TYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
